@@ -9,11 +9,13 @@ Public surface
 * ``attn_fwd(q, k, v, causal=False, ...) -> (O, L)``, ``attn_bwd_prep`` / ``attn_bwd`` / ``dq_shuffle`` (the
   backward pass), ``paged_decode(...) -> (O, L)`` and ``paged_kv_append(...)``: torch-tensor front ends over
   the C ABI (ctypes).
+* ``qk_norm_rotary(...)`` and ``qk_norm_rotary_bwd(...)``: RMS norm of every head of q and k with the rotation of its position.
 * ``load_tk_kernel(causal)`` / ``load_tk_kernel_fwd(causal)`` / ``load_tk_kernel_bkwd(causal)`` /
   ``load_tk_kernel_bkwd_prep(causal)``: the reference's extension modules (``tk_kernel.dispatch_micro``,
   ``tk_kernel_fwd.dispatch_fwd``, ``tk_kernel_bkwd.dispatch_bwd_combined``, ``tk_kernel_bkwd_prep.dispatch_prep``
   and ``.dispatch_dq_shuffle``) built for B200.
-* ``HipAttnFunction`` in :mod:`hipkittens_b200.attention`: the reference's autograd-function forward.
+* ``HipAttnFunction`` in :mod:`hipkittens_b200.attention`: the reference's autograd-function forward; ``QkNormRotary`` there:
+  the module over ``qk_norm_rotary``.
 """
 from ._native import (  # noqa: F401
     HK_DQ_BHND,
@@ -36,6 +38,8 @@ from ._native import (  # noqa: F401
     attn_fwd_paged,
     paged_kv_append,
     paged_kv_append_rotary,
+    qk_norm_rotary,
+    qk_norm_rotary_bwd,
     rotary,
     rotary_bnhd,
 )
@@ -61,6 +65,8 @@ __all__ = [
     "paged_kv_append",
     "paged_kv_append_rotary",
     "paged_decode_workspace_bytes",
+    "qk_norm_rotary",
+    "qk_norm_rotary_bwd",
     "rotary",
     "rotary_bnhd",
 ]

@@ -17,7 +17,7 @@ import torch
 _PKG = os.path.dirname(os.path.abspath(__file__))
 _LIB = os.path.join(_PKG, "lib", "libhk_attn.so")
 
-HK_OK, HK_EINVAL, HK_EUNSUPPORTED, HK_ECUDA, HK_ETIMEOUT, HK_EWORKSPACE, HK_EBADPAGE, HK_EBADLEN = 0, -1, -2, -3, -4, -5, -6, -7
+HK_OK, HK_EINVAL, HK_EUNSUPPORTED, HK_ECUDA, HK_ETIMEOUT, HK_EWORKSPACE, HK_EBADPAGE, HK_EBADLEN, HK_EBADPOS = 0, -1, -2, -3, -4, -5, -6, -7, -8
 
 # Every symbol declared in include/hk_attn.h.
 EXPORTED_SYMBOLS = (
@@ -36,6 +36,9 @@ EXPORTED_SYMBOLS = (
     "hk_rotary",
     "hk_rotary_bnhd",
     "hk_paged_kv_append_rotary",
+    "hk_qk_norm_rotary",
+    "hk_qk_norm_rotary_bwd",
+    "hk_qk_norm_rotary_bwd_workspace_bytes",
     "hk_attn_paged_decode_workspace_bytes",
     "hk_attn_paged_decode",
     "hk_attn_paged_decode_static",
@@ -113,6 +116,13 @@ def capi() -> ctypes.CDLL:
     lib.hk_rotary_bnhd.restype = ci
     lib.hk_paged_kv_append_rotary.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, ci, ci, ci, ci, ci, ci, ci, ci, ci, ci, vp]
     lib.hk_paged_kv_append_rotary.restype = ci
+    lib.hk_qk_norm_rotary.argtypes = [vp] * 8 + [ci] * 7 + [ll3] * 2 + [vp, ci, cf, ci, ci, vp]
+    lib.hk_qk_norm_rotary.restype = ci
+    lib.hk_qk_norm_rotary_bwd_workspace_bytes.argtypes = [ci]
+    lib.hk_qk_norm_rotary_bwd_workspace_bytes.restype = ctypes.c_size_t
+    lib.hk_qk_norm_rotary_bwd.argtypes = ([vp] * 12 + [ci] * 7 + [ll3] * 2 +
+                                          [vp, ci, cf, ci, vp, ctypes.c_size_t, ci, vp])
+    lib.hk_qk_norm_rotary_bwd.restype = ci
     lib.hk_attn_paged_decode_workspace_bytes.argtypes = [ci, ci, ci, ci, ci]
     lib.hk_attn_paged_decode_workspace_bytes.restype = ctypes.c_size_t
     lib.hk_attn_paged_decode.argtypes = [vp, vp, vp, vp, vp, vp, vp, ci, ci, ci, ci, ci, ci, ci, cf, vp,
@@ -506,6 +516,152 @@ def rotary_bnhd(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, out: Opti
     _check(capi().hk_rotary_bnhd(x.data_ptr(), out.data_ptr(), sin.data_ptr(), cos.data_ptr(), b, n, h, d,
                                  2 * cos.shape[1], int(pos_offset), x.device.index, s.cuda_stream), "hk_rotary_bnhd")
     return out
+
+
+HK_QKN_INTERLEAVED, HK_QKN_TABLE_F32, HK_QKN_WEIGHT_F32 = 1, 2, 4
+
+
+def _qkn_check(q, k, q_weight, k_weight, cos, sin, positions, pos_offset, eps):
+    """What the norm and rotation and its gradients have in common: checked shapes, and the flags that say the types."""
+    for name, t in (("q", q), ("k", k)):
+        if not isinstance(t, torch.Tensor) or t.device.type != "cuda" or t.dim() != 4:
+            raise RuntimeError(f"{name} must be a 4-D CUDA tensor")
+        if t.dtype != torch.bfloat16:
+            raise RuntimeError(f"{name} must be torch.bfloat16")
+        if t.numel() and t.stride(3) != 1:
+            raise RuntimeError(f"{name}: the last dimension must be contiguous")
+    b, n, h, d = q.shape
+    if k.shape[:2] != q.shape[:2] or k.shape[3] != d:
+        raise RuntimeError("q must be [B,N,H,D] and k [B,N,H_KV,D]")
+    flags = 0
+    for name, t in (("cos", cos), ("sin", sin)):
+        if not isinstance(t, torch.Tensor) or t.dim() != 2 or not t.is_contiguous() or t.dtype not in (torch.bfloat16, torch.float32):
+            raise RuntimeError(f"{name} must be a contiguous bf16 or fp32 tensor [rows, R/2]")
+    if cos.shape != sin.shape or cos.dtype != sin.dtype:
+        raise RuntimeError("cos and sin must have the same shape and type")
+    if cos.dtype == torch.float32:
+        flags |= HK_QKN_TABLE_F32
+    weights = [t for t in (q_weight, k_weight) if t is not None]
+    for t in weights:
+        if not isinstance(t, torch.Tensor) or t.shape != (d,) or not t.is_contiguous() or t.dtype not in (torch.bfloat16, torch.float32):
+            raise RuntimeError("q_weight and k_weight must be contiguous bf16 or fp32 tensors [D]")
+    if len({t.dtype for t in weights}) > 1:
+        raise RuntimeError("q_weight and k_weight must have the same type")
+    if weights and weights[0].dtype == torch.float32:
+        flags |= HK_QKN_WEIGHT_F32
+    if positions is None:
+        if pos_offset < 0 or cos.shape[0] < n + pos_offset:
+            raise RuntimeError("cos/sin must have N + pos_offset rows")
+    elif pos_offset != 0:
+        raise RuntimeError("positions and pos_offset exclude each other")
+    elif (not isinstance(positions, torch.Tensor) or positions.dtype != torch.int32 or positions.shape != (b, n)
+          or not positions.is_contiguous()):
+        raise RuntimeError("positions must be a contiguous int32 tensor [B, N]")
+    if not eps >= 0:
+        raise RuntimeError("eps must not be negative")
+    _require_same_device(q, k=k, q_weight=q_weight, k_weight=k_weight, cos=cos, sin=sin, positions=positions)
+    return flags
+
+
+def _qkn_strides(t):
+    # a dimension of size 1 has no stride that matters: give it one the library takes
+    return (ctypes.c_longlong * 3)(*(st if n > 1 else t.shape[3] for st, n in zip(t.stride()[:3], t.shape[:3])))
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def qk_norm_rotary(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    q_weight: Optional[torch.Tensor],
+    k_weight: Optional[torch.Tensor],
+    cos: torch.Tensor,
+    sin: torch.Tensor,
+    positions: Optional[torch.Tensor] = None,
+    pos_offset: int = 0,
+    eps: float = 1e-6,
+    interleaved: bool = False,
+    q_out: Optional[torch.Tensor] = None,
+    k_out: Optional[torch.Tensor] = None,
+    stream: Optional[torch.cuda.Stream] = None,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """RMS norm of every head of q and k, times a weight [D], and the rotation of its position, in one pass: what models that
+    normalise queries and keys do in front of attention.
+
+    q [B,N,H,D], k [B,N,H_KV,D] bf16, contiguous or views with a contiguous last dimension and other strides that are multiples of 8
+    (slices of a packed projection); weights bf16 or fp32 (None: ones); cos, sin [rows, R/2] bf16 or fp32, R <= D (the rest
+    of a head is normalised and not rotated). Token n of every sequence takes row n + pos_offset of the tables, or row
+    `positions[b, n]` (int32 [B, N]; the rows of a position outside the tables come back as zeros and are reported as
+    HK_EBADPOS). `interleaved` rotates the pairs (2i, 2i+1) instead of (i, i + R/2). fp32 throughout, rounded once. Returns
+    new contiguous tensors, or `q_out` and `k_out`, which may be q and k themselves. Asynchronous on `stream` (default: torch's
+    current stream)."""
+    if stream is None:
+        r = _front().qk_norm_rotary(q, k, q_weight, k_weight, cos, sin, positions, pos_offset, eps, interleaved, q_out, k_out)
+        if r is not None:
+            return _done(r, "hk_qk_norm_rotary")
+    flags = _qkn_check(q, k, q_weight, k_weight, cos, sin, positions, pos_offset, eps)
+    b, n, h, d = q.shape
+    outs = []
+    for name, t, o in (("q_out", q, q_out), ("k_out", k, k_out)):
+        if o is None:
+            o = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        if not isinstance(o, torch.Tensor) or o.shape != t.shape or o.dtype != t.dtype or not o.is_contiguous():
+            raise RuntimeError(f"{name} must be a contiguous bf16 tensor of its input's shape")
+        _require_same_device(q, **{name: o})
+        outs.append(o)
+    s = stream if stream is not None else torch.cuda.current_stream(q.device)
+    _check(capi().hk_qk_norm_rotary(q.data_ptr(), k.data_ptr(), _ptr(q_weight), _ptr(k_weight), cos.data_ptr(), sin.data_ptr(),
+                                    outs[0].data_ptr(), outs[1].data_ptr(), b, n, h, k.shape[2], d, 2 * cos.shape[1],
+                                    cos.shape[0], _qkn_strides(q), _qkn_strides(k), _ptr(positions), int(pos_offset), float(eps),
+                                    flags | (HK_QKN_INTERLEAVED if interleaved else 0), q.device.index, s.cuda_stream),
+           "hk_qk_norm_rotary")
+    return outs[0], outs[1]
+
+
+def qk_norm_rotary_bwd(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    q_weight: Optional[torch.Tensor],
+    k_weight: Optional[torch.Tensor],
+    cos: torch.Tensor,
+    sin: torch.Tensor,
+    dq_out: torch.Tensor,
+    dk_out: torch.Tensor,
+    positions: Optional[torch.Tensor] = None,
+    pos_offset: int = 0,
+    eps: float = 1e-6,
+    interleaved: bool = False,
+    weight_grads: bool = True,
+    stream: Optional[torch.cuda.Stream] = None,
+) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """Gradients of `qk_norm_rotary` with respect to q, k and the weights (None for a weight that is None, or without
+    `weight_grads`), from those of its outputs (contiguous bf16). q and k are its inputs."""
+    if stream is None:
+        r = _front().qk_norm_rotary_bwd(q, k, q_weight, k_weight, cos, sin, dq_out, dk_out, positions, pos_offset, eps,
+                                        interleaved, weight_grads)
+        if r is not None:
+            return _done(r, "hk_qk_norm_rotary_bwd")
+    flags = _qkn_check(q, k, q_weight, k_weight, cos, sin, positions, pos_offset, eps)
+    b, n, h, d = q.shape
+    for name, t, g in (("dq_out", q, dq_out), ("dk_out", k, dk_out)):
+        if not isinstance(g, torch.Tensor) or g.shape != t.shape or g.dtype != t.dtype or not g.is_contiguous():
+            raise RuntimeError(f"{name} must be a contiguous bf16 tensor of its output's shape")
+    _require_same_device(q, dq_out=dq_out, dk_out=dk_out)
+    dq, dk = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
+    dws = [torch.empty_like(w) if weight_grads and w is not None else None for w in (q_weight, k_weight)]
+    s = stream if stream is not None else torch.cuda.current_stream(q.device)
+    need = int(capi().hk_qk_norm_rotary_bwd_workspace_bytes(d))
+    with torch.cuda.stream(s):  # the workspace goes back to the pool of the stream that uses it
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if any(w is not None for w in dws) else None
+    _check(capi().hk_qk_norm_rotary_bwd(q.data_ptr(), k.data_ptr(), _ptr(q_weight), _ptr(k_weight), cos.data_ptr(), sin.data_ptr(),
+                                        dq_out.data_ptr(), dk_out.data_ptr(), dq.data_ptr(), dk.data_ptr(), _ptr(dws[0]),
+                                        _ptr(dws[1]), b, n, h, k.shape[2], d, 2 * cos.shape[1], cos.shape[0], _qkn_strides(q),
+                                        _qkn_strides(k), _ptr(positions), int(pos_offset), float(eps),
+                                        flags | (HK_QKN_INTERLEAVED if interleaved else 0), _ptr(ws), need, q.device.index,
+                                        s.cuda_stream), "hk_qk_norm_rotary_bwd")
+    return dq, dk, dws[0], dws[1]
 
 
 def paged_decode_workspace_bytes(s: int, h: int, d: int, max_pages: int, page_size: int = 16) -> int:

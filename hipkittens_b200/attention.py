@@ -23,8 +23,9 @@ from __future__ import annotations
 import torch
 import torch.nn as nn
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
-from ._native import attn_bwd_strided, attn_fwd, device_status, key_padding_lens
+from ._native import attn_bwd_strided, attn_fwd, device_status, key_padding_lens, qk_norm_rotary, qk_norm_rotary_bwd
 
 
 def _tma_viewable(t: torch.Tensor) -> bool:
@@ -204,3 +205,42 @@ class HipCrossAttention(nn.Module):
         causal = self.causal if causal is None else causal
         assert kv.shape[0] == batch_size and kv.shape[4] == q.shape[3]
         return _attend(q, kv, causal, self.softmax_scale, key_padding_mask)
+
+
+class QkNormRotaryFunction(Function):
+    """``qk_norm_rotary`` with gradients of q, k and the weights. The tables are constants. Asynchronous in both directions, as
+    the call itself is."""
+
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions=None, pos_offset=0, eps=1e-6, interleaved=False):
+        if ctx.needs_input_grad[4] or ctx.needs_input_grad[5]:
+            raise RuntimeError("cos and sin have no gradients: pass tensors that do not require them")
+        ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
+        ctx.rest = pos_offset, eps, interleaved
+        return qk_norm_rotary(q, k, q_weight, k_weight, cos, sin, positions, pos_offset, eps, interleaved)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq_out, dk_out):
+        *saved, positions = ctx.saved_tensors
+        dy = (t.to(torch.bfloat16).contiguous() for t in (dq_out, dk_out))
+        wanted = ctx.needs_input_grad[2] or ctx.needs_input_grad[3]
+        grads = qk_norm_rotary_bwd(*saved, *dy, positions, *ctx.rest, weight_grads=wanted)
+        return (*grads, None, None, None, None, None, None)
+
+
+class QkNormRotary(nn.Module):
+    """RMS norm of every head of q and k with a learned weight each, and the rotation of its position:
+    q [B,N,H,D], k [B,N,H_KV,D] -> the same, ready for attention (``qk_norm_rotary`` says what `cos`, `sin`, `positions` and
+    `pos_offset` are)."""
+
+    def __init__(self, head_dim, eps=1e-6, interleaved=False, device=None, dtype=None):
+        super().__init__()
+        self.eps = eps
+        self.interleaved = interleaved
+        self.q_weight = nn.Parameter(torch.ones(head_dim, device=device, dtype=dtype))
+        self.k_weight = nn.Parameter(torch.ones(head_dim, device=device, dtype=dtype))
+
+    def forward(self, q, k, cos, sin, positions=None, pos_offset=0):
+        return QkNormRotaryFunction.apply(q, k, self.q_weight, self.k_weight, cos, sin, positions, pos_offset, self.eps,
+                                          self.interleaved)

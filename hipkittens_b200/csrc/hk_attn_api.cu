@@ -8,6 +8,7 @@
 #include <cstdio>
 #include <cstring>
 #include <mutex>
+#include <type_traits>
 
 #include "../../include/hk_attn.h"
 #include "attn_bwd_sm100.cuh"
@@ -16,6 +17,7 @@
 #include "key_padding_sm100.cuh"
 #include "paged_decode_sm100.cuh"
 #include "paged_kv_append_sm100.cuh"
+#include "qk_norm_rotary_sm100.cuh"
 #include "rotary_sm100.cuh"
 
 namespace {
@@ -219,6 +221,7 @@ int status_to_code(int word) {
     case hk::kStatusSmemAlign: return HK_EUNSUPPORTED;
     case hk::kStatusBadPage: return HK_EBADPAGE;
     case hk::kStatusBadLen: return HK_EBADLEN;
+    case hk::kStatusBadPos: return HK_EBADPOS;
     default: return HK_ETIMEOUT;
   }
 }
@@ -529,6 +532,19 @@ int launch_bwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& 
                                hk::BwdSmem<D>::kDynBytes, stream, tq, tk, tv, tdo, p));
   g_launches.fetch_add(1, std::memory_order_relaxed);
   return HK_OK;
+}
+
+// The kernel for D and the flags: fn.template operator()<LPR, INTER, TF32>().
+template <typename Fn>
+int qkn_pick(int D, int flags, const Fn& fn) {
+  const bool inter = flags & HK_QKN_INTERLEAVED, f32 = flags & HK_QKN_TABLE_F32;
+  auto tables = [&](auto lpr, auto in) {
+    return f32 ? fn(lpr, in, std::true_type{}) : fn(lpr, in, std::false_type{});
+  };
+  auto layout = [&](auto lpr) { return inter ? tables(lpr, std::true_type{}) : tables(lpr, std::false_type{}); };
+  if (D <= 64) return layout(std::integral_constant<int, 4>{});
+  if (D <= 128) return layout(std::integral_constant<int, 8>{});
+  return layout(std::integral_constant<int, 16>{});
 }
 
 }  // namespace
@@ -923,6 +939,134 @@ int hk_rotary_bnhd(const void* x, void* o, const void* sin, const void* cos, int
                        cuda_stream);
 }
 
+// Shared head of the two entries: everything but the outputs, the gradients and how rows are dealt to blocks.
+static int qkn_params(hk::QknParams& p, const void* q, const void* k, const void* q_weight, const void* k_weight,
+                      const void* cos, const void* sin, int B, int N, int H, int H_KV, int D, int rotary_dim, int table_rows,
+                      const long long* q_strides, const long long* k_strides, const int32_t* positions, int pos_offset,
+                      float eps, int flags) {
+  if (!q || !k || !cos || !sin || !q_strides || !k_strides) return HK_EINVAL;
+  if (B <= 0 || N <= 0 || H <= 0 || H_KV <= 0 || D <= 0 || table_rows <= 0 || pos_offset < 0) return HK_EINVAL;
+  if (flags & ~(HK_QKN_INTERLEAVED | HK_QKN_TABLE_F32 | HK_QKN_WEIGHT_F32)) return HK_EINVAL;
+  if (!(eps >= 0.f)) return HK_EINVAL;
+  if (rotary_dim <= 0) rotary_dim = D;
+  if (D % 16 != 0 || D > hk::kQknMaxD || rotary_dim % 16 != 0 || rotary_dim > D) return HK_EUNSUPPORTED;
+  if (!positions && 1ll * N + pos_offset > table_rows) return HK_EINVAL;
+  for (const void* ptr : {q, k, q_weight, k_weight, cos, sin})
+    if (!aligned16(ptr)) return HK_EINVAL;
+  if (reinterpret_cast<uintptr_t>(positions) & 3) return HK_EINVAL;
+  p = {};
+  for (int i = 0; i < 2; ++i) {
+    const long long* st = i ? k_strides : q_strides;
+    for (int d = 0; d < 3; ++d)
+      if (st[d] <= 0 || st[d] % 8 != 0 || st[d] >= (1ll << 39)) return HK_EINVAL;
+    const long long rows = 1ll * B * N * (i ? H_KV : H);
+    if (rows > 0x7ff00000ll) return HK_EINVAL;  // rows are indexed with int, some thousand beyond the last as well
+    hk::QknSide& s = p.side[i];
+    s.x = static_cast<const __nv_bfloat16*>(i ? k : q);
+    s.w = i ? k_weight : q_weight;
+    s.stride_b = st[0], s.stride_n = st[1], s.stride_h = st[2];
+    s.rows = int(rows);
+    s.heads = i ? H_KV : H;
+    s.fd_heads = hk::FastDiv(s.heads);
+  }
+  p.cos = cos;
+  p.sin = sin;
+  p.positions = positions;
+  p.N = N, p.D = D, p.R = rotary_dim, p.table_rows = table_rows, p.pos0 = pos_offset;
+  p.weight_f32 = (flags & HK_QKN_WEIGHT_F32) != 0;
+  p.eps = eps;
+  p.fd_n = hk::FastDiv(N);
+  return HK_OK;
+}
+
+int hk_qk_norm_rotary(const void* q, const void* k, const void* q_weight, const void* k_weight, const void* cos,
+                      const void* sin, void* q_out, void* k_out, int B, int N, int H, int H_KV, int D, int rotary_dim,
+                      int table_rows, const long long* q_strides, const long long* k_strides, const int32_t* positions,
+                      int pos_offset, float eps, int flags, int device, void* cuda_stream) {
+  hk::QknParams p;
+  int rc = qkn_params(p, q, k, q_weight, k_weight, cos, sin, B, N, H, H_KV, D, rotary_dim, table_rows, q_strides, k_strides,
+                      positions, pos_offset, eps, flags);
+  if (rc != HK_OK) return rc;
+  if (!q_out || !k_out || !aligned16(q_out) || !aligned16(k_out)) return HK_EINVAL;
+  DeviceState* st = nullptr;
+  DeviceScope scope;
+  if ((rc = scope.enter(device, &st)) != HK_OK) return rc;
+  p.side[0].out = static_cast<__nv_bfloat16*>(q_out);
+  p.side[1].out = static_cast<__nv_bfloat16*>(k_out);
+  p.status = st->status;
+  return qkn_pick(D, flags, [&](auto lpr, auto inter, auto f32) {
+    constexpr int kRows = hk::kQknThreads / decltype(lpr)::value;
+    auto blocks = [&](int i, int un) { return (p.side[i].rows + kRows * un - 1) / (kRows * un); };
+    const bool few = blocks(0, 4) + blocks(1, 4) < 4 * st->sm_count;
+    auto* fn = few ? hk::qk_norm_rotary_kernel<decltype(lpr)::value, decltype(inter)::value, decltype(f32)::value, 1>
+                   : hk::qk_norm_rotary_kernel<decltype(lpr)::value, decltype(inter)::value, decltype(f32)::value, 4>;
+    p.blocks0 = blocks(0, few ? 1 : 4);
+    HK_CUDA(hk::launch_dependent(true, fn, unsigned(p.blocks0 + blocks(1, few ? 1 : 4)), hk::kQknThreads, 0,
+                                 static_cast<cudaStream_t>(cuda_stream), p));
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    return HK_OK;
+  });
+}
+
+size_t hk_qk_norm_rotary_bwd_workspace_bytes(int D) {
+  return D > 0 && D % 16 == 0 && D <= hk::kQknMaxD ? size_t(hk::kQknMaxBlocks) * D * sizeof(float) : 0;
+}
+
+int hk_qk_norm_rotary_bwd(const void* q, const void* k, const void* q_weight, const void* k_weight, const void* cos,
+                          const void* sin, const void* dq_out, const void* dk_out, void* dq, void* dk, void* dq_weight,
+                          void* dk_weight, int B, int N, int H, int H_KV, int D, int rotary_dim, int table_rows,
+                          const long long* q_strides, const long long* k_strides, const int32_t* positions, int pos_offset,
+                          float eps, int flags, void* workspace, size_t workspace_bytes, int device, void* cuda_stream) {
+  hk::QknParams p;
+  int rc = qkn_params(p, q, k, q_weight, k_weight, cos, sin, B, N, H, H_KV, D, rotary_dim, table_rows, q_strides, k_strides,
+                      positions, pos_offset, eps, flags);
+  if (rc != HK_OK) return rc;
+  if (!dq_out || !dk_out || !dq || !dk) return HK_EINVAL;
+  for (const void* ptr : {dq_out, dk_out, static_cast<const void*>(dq), static_cast<const void*>(dk)})
+    if (!aligned16(ptr)) return HK_EINVAL;
+  if ((dq_weight && !q_weight) || (dk_weight && !k_weight)) return HK_EINVAL;
+  for (const void* ptr : {dq_weight, dk_weight})
+    if (reinterpret_cast<uintptr_t>(ptr) & 3) return HK_EINVAL;
+  const bool sums = dq_weight || dk_weight;
+  if (sums && (!workspace || workspace_bytes < hk_qk_norm_rotary_bwd_workspace_bytes(D) || !aligned16(workspace)))
+    return HK_EWORKSPACE;
+  DeviceState* st = nullptr;
+  DeviceScope scope;
+  if ((rc = scope.enter(device, &st)) != HK_OK) return rc;
+  const void* dy[2] = {dq_out, dk_out};
+  void* dx[2] = {dq, dk};
+  void* dw[2] = {dq_weight, dk_weight};
+  for (int i = 0; i < 2; ++i) {
+    p.side[i].dy = static_cast<const __nv_bfloat16*>(dy[i]);
+    p.side[i].out = static_cast<__nv_bfloat16*>(dx[i]);
+    p.side[i].dw = dw[i];
+  }
+  p.partial = sums ? static_cast<float*>(workspace) : nullptr;
+  p.status = st->status;
+  cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
+  return qkn_pick(D, flags, [&](auto lpr, auto inter, auto f32) {
+    constexpr int kRows = 2 * hk::kQknThreads / decltype(lpr)::value;
+    // as many blocks as the GPU holds, shared between q and k by their rows
+    const int most = std::min(hk::kQknMaxBlocks, 4 * st->sm_count);
+    int blocks[2];
+    for (int i = 0; i < 2; ++i) {
+      const int need = (p.side[i].rows + kRows - 1) / kRows;
+      const double share = double(p.side[i].rows) / (double(p.side[0].rows) + p.side[1].rows);
+      blocks[i] = std::max(1, std::min(need, int(share * most)));
+    }
+    p.blocks0 = blocks[0];
+    const int grid = blocks[0] + blocks[1];
+    auto* fn = hk::qk_norm_rotary_bwd_kernel<decltype(lpr)::value, decltype(inter)::value, decltype(f32)::value>;
+    HK_CUDA(hk::launch_dependent(true, fn, unsigned(grid), hk::kQknThreads, 0, stream, p));
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    if (sums) {
+      HK_CUDA(hk::launch_dependent(true, hk::qk_norm_rotary_dw_kernel, dim3((D + 31) / 32, 2), 1024, 0, stream, p, grid));
+      g_launches.fetch_add(1, std::memory_order_relaxed);
+    }
+    return HK_OK;
+  });
+}
+
 size_t hk_attn_paged_decode_workspace_bytes(int S, int H, int D, int max_pages_per_seq, int page_size) {
   return hk::decode_workspace_bytes(S, H, D, max_pages_per_seq, page_size);
 }
@@ -1146,6 +1290,7 @@ const char* hk_strerror(int code) {
     case HK_EWORKSPACE: return "workspace missing, misaligned or too small";
     case HK_EBADPAGE: return "block-table entry outside the page pool";
     case HK_EBADLEN: return "context length beyond the block table's capacity (clamped)";
+    case HK_EBADPOS: return "position outside the rotary tables (its rows are zeros)";
     default: return "unknown error code";
   }
 }

@@ -200,6 +200,128 @@ PyObject* rotary_bnhd(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
+// What the norm and rotation of q and k and its gradients share; `arg` holds q, k, q_weight, k_weight, cos, sin.
+struct Qkn {
+  const Tensor *q, *k, *w[2], *cos, *sin, *positions;
+  long long qs[3], ks[3];
+  int flags = 0, pos_offset;
+  float eps;
+  const void *q_ptr, *k_ptr, *w_ptr[2], *cos_ptr, *sin_ptr;
+  const int32_t* pos_ptr;
+  int b, n, h, hkv, d, r, rows, device;
+  bool take(PyObject* const* arg, PyObject* pos, PyObject* offset, PyObject* eps_arg, PyObject* interleaved) {
+    q = plain(arg[0]), k = plain(arg[1]), cos = plain(arg[4]), sin = plain(arg[5]);
+    if (!is(q, at::kBFloat16, 4) || !is(k, at::kBFloat16, 4) || !PyBool_Check(interleaved) || !PyFloat_CheckExact(eps_arg) ||
+        !PyLong_CheckExact(offset))
+      return false;
+    if (k->size(0) != q->size(0) || k->size(1) != q->size(1) || k->size(3) != q->size(3) || !q->numel() || !k->numel()) return false;
+    const bool q_ok = tma_strides(*q, qs), k_ok = tma_strides(*k, ks);
+    if (!q_ok || !k_ok) return false;
+    if (!(dense(cos, at::kBFloat16, 2) && dense(sin, at::kBFloat16, 2))) {
+      if (!(dense(cos, at::kFloat, 2) && dense(sin, at::kFloat, 2))) return false;
+      flags |= HK_QKN_TABLE_F32;
+    }
+    if (cos->sizes() != sin->sizes() || !same_device(*q, {k, cos, sin})) return false;
+    bool f32 = false, b16 = false;
+    for (int i = 0; i < 2; ++i) {
+      w[i] = nullptr;
+      if (arg[2 + i] == Py_None) continue;
+      w[i] = plain(arg[2 + i]);
+      if (!w[i] || w[i]->dim() != 1 || w[i]->size(0) != q->size(3) || !w[i]->is_contiguous() || w[i]->device() != q->device())
+        return false;
+      f32 |= w[i]->scalar_type() == at::kFloat, b16 |= w[i]->scalar_type() == at::kBFloat16;
+      if (w[i]->scalar_type() != at::kFloat && w[i]->scalar_type() != at::kBFloat16) return false;
+    }
+    if (f32 && b16) return false;
+    if (f32) flags |= HK_QKN_WEIGHT_F32;
+    int overflow = 0;
+    const long off = PyLong_AsLongAndOverflow(offset, &overflow);
+    if (overflow || off < 0 || !fits({off, cos->size(0), 2 * cos->size(1)})) return false;
+    for (int64_t v : q->sizes())
+      if (!fits({v})) return false;
+    positions = nullptr;
+    if (pos != Py_None) {
+      positions = plain(pos);
+      if (!dense(positions, at::kInt, 2) || positions->size(0) != q->size(0) || positions->size(1) != q->size(1) ||
+          positions->device() != q->device() || off != 0)
+        return false;
+    } else if (cos->size(0) < q->size(1) + off) {
+      return false;
+    }
+    eps = static_cast<float>(PyFloat_AS_DOUBLE(eps_arg));
+    if (!(eps >= 0.f)) return false;
+    if (interleaved == Py_True) flags |= HK_QKN_INTERLEAVED;
+    pos_offset = i32(off);
+    b = i32(q->size(0)), n = i32(q->size(1)), h = i32(q->size(2)), d = i32(q->size(3)), hkv = i32(k->size(2));
+    r = i32(2 * cos->size(1)), rows = i32(cos->size(0)), device = q->device().index();
+    return true;
+  }
+  void read() {
+    q_ptr = ptr(*q), k_ptr = ptr(*k), cos_ptr = ptr(*cos), sin_ptr = ptr(*sin);
+    for (int i = 0; i < 2; ++i) w_ptr[i] = w[i] ? ptr(*w[i]) : nullptr;
+    pos_ptr = positions ? ptr<int32_t>(*positions) : nullptr;
+  }
+};
+
+// qk_norm_rotary(q, k, q_weight, k_weight, cos, sin, positions, pos_offset, eps, interleaved, q_out, k_out)
+PyObject* qk_norm_rotary(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  Qkn p;
+  if (n_args != 12 || !p.take(a, a[6], a[7], a[8], a[9])) Py_RETURN_NONE;
+  Tensor qo, ko;
+  if (!output(a[10], *p.q, p.q->sizes(), at::kBFloat16, qo) || !output(a[11], *p.q, p.k->sizes(), at::kBFloat16, ko))
+    Py_RETURN_NONE;
+  void* st = stream_of(*p.q);
+  p.read();
+  void *qop = ptr(qo), *kop = ptr(ko);
+  const int rc = unlocked([&] {
+    return hk_qk_norm_rotary(p.q_ptr, p.k_ptr, p.w_ptr[0], p.w_ptr[1], p.cos_ptr, p.sin_ptr, qop, kop, p.b, p.n, p.h, p.hkv,
+                             p.d, p.r, p.rows, p.qs, p.ks, p.pos_ptr, p.pos_offset, p.eps, p.flags, p.device, st);
+  });
+  return result(rc, qo, ko);
+  END_HANDLE_TH_ERRORS
+}
+
+// qk_norm_rotary_bwd(q, k, q_weight, k_weight, cos, sin, dq_out, dk_out, positions, pos_offset, eps, interleaved, weight_grads)
+PyObject* qk_norm_rotary_bwd(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  Qkn p;
+  if (n_args != 13 || !PyBool_Check(a[12]) || !p.take(a, a[8], a[9], a[10], a[11])) Py_RETURN_NONE;
+  const Tensor* dy[2] = {plain(a[6]), plain(a[7])};
+  const Tensor* x[2] = {p.q, p.k};
+  Tensor dx[2], dw[2], ws;
+  bool sums = false;
+  for (int i = 0; i < 2; ++i) {
+    if (!dense(dy[i], at::kBFloat16, 4) || dy[i]->sizes() != x[i]->sizes() || dy[i]->device() != p.q->device() ||
+        !output(Py_None, *p.q, x[i]->sizes(), at::kBFloat16, dx[i]))
+      Py_RETURN_NONE;
+    if (a[12] == Py_True && p.w[i]) {
+      if (!output(Py_None, *p.w[i], p.w[i]->sizes(), p.w[i]->scalar_type(), dw[i])) Py_RETURN_NONE;
+      sums = true;
+    }
+  }
+  const size_t need = sums ? hk_qk_norm_rotary_bwd_workspace_bytes(p.d) : 0;
+  if (need && !output(Py_None, *p.q, {int64_t(need)}, at::kByte, ws)) Py_RETURN_NONE;
+  void* st = stream_of(*p.q);
+  p.read();
+  const void *dqo = ptr(*dy[0]), *dko = ptr(*dy[1]);
+  void *dq = ptr(dx[0]), *dk = ptr(dx[1]), *dqw = dw[0].defined() ? ptr(dw[0]) : nullptr,
+       *dkw = dw[1].defined() ? ptr(dw[1]) : nullptr, *wsp = need ? ptr(ws) : nullptr;
+  const int rc = unlocked([&] {
+    return hk_qk_norm_rotary_bwd(p.q_ptr, p.k_ptr, p.w_ptr[0], p.w_ptr[1], p.cos_ptr, p.sin_ptr, dqo, dko, dq, dk, dqw, dkw,
+                                 p.b, p.n, p.h, p.hkv, p.d, p.r, p.rows, p.qs, p.ks, p.pos_ptr, p.pos_offset, p.eps,
+                                 p.flags, wsp, need, p.device, st);
+  });
+  if (rc != HK_OK) return PyLong_FromLong(rc);
+  auto wrapped = [](const Tensor& t) {
+    if (t.defined()) return THPVariable_Wrap(t);
+    Py_INCREF(Py_None);
+    return Py_None;
+  };
+  return Py_BuildValue("(NNNN)", THPVariable_Wrap(dx[0]), THPVariable_Wrap(dx[1]), wrapped(dw[0]), wrapped(dw[1]));
+  END_HANDLE_TH_ERRORS
+}
+
 // What the paged entries share: q [S,T,H,D], pools [P,page,H_KV,D], block_table [S,max_pages], lengths [S].
 struct Paged {
   const Tensor *q, *kp, *vp, *table, *lens;
@@ -318,6 +440,7 @@ PyObject* paged_kv_append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
 #define HK_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {HK_METHOD(attn_fwd),       HK_METHOD(attn_bwd_strided), HK_METHOD(rotary_bnhd),
                          HK_METHOD(paged_decode),   HK_METHOD(attn_fwd_paged),   HK_METHOD(paged_kv_append),
+                         HK_METHOD(qk_norm_rotary), HK_METHOD(qk_norm_rotary_bwd),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_front", "Native tensor front ends of hipkittens_b200", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};

@@ -28,6 +28,7 @@ extern "C" {
 #define HK_EWORKSPACE (-5)   /* workspace missing or too small */
 #define HK_EBADPAGE (-6)     /* a block-table entry outside [0, num_pages) was met; it was not dereferenced */
 #define HK_EBADLEN (-7)      /* a context length beyond max_pages_per_seq * page_size was met; it was clamped */
+#define HK_EBADPOS (-8)      /* a position outside the rotary tables was met; its rows came back as zeros */
 
 /* Attention forward.
  * Replaces dispatch_micro<D>(attn_globals<D>) (kernels/attn/gqa/kernel.cpp:93-100,576-581, causal twin
@@ -205,6 +206,41 @@ int hk_rotary(const void* x, void* o, const void* sin, const void* cos, int B, i
  * Same arithmetic as hk_rotary (bit-identical results); x and o may be the same buffer. */
 int hk_rotary_bnhd(const void* x, void* o, const void* sin, const void* cos, int B, int N, int H, int D,
                    int rotary_dim, int pos_offset, int device, void* cuda_stream);
+
+/* RMS norm of every head of q and k and the rotation of its position, in one pass: the step in front of attention in models
+ * that normalise queries and keys. The reference has the rotation alone (kernels/rotary/kernel.cpp:44-98).
+ *   y = x / sqrt(mean(x^2) + eps) * w over the D values of a head, then the rotation of hk_rotary by row `pos` of the tables;
+ *   fp32 throughout, rounded once.
+ *   q, k           : bf16 [B, N, H, D] and [B, N, H_KV, D], through element strides of batch, sequence and head (HOST arrays,
+ *                    positive multiples of 8; the last dimension is contiguous), e.g. views of a packed projection
+ *   q_out, k_out   : bf16, contiguous; may be q and k themselves where those are contiguous
+ *   q_weight, k_weight : [D] bf16, or fp32 with HK_QKN_WEIGHT_F32; NULL = ones
+ *   cos, sin       : [table_rows, rotary_dim / 2] bf16, or fp32 with HK_QKN_TABLE_F32
+ *   positions      : DEVICE int32 [B, N], the row of the tables for each token; NULL: token n of every sequence has row
+ *                    n + pos_offset (N + pos_offset <= table_rows). A position outside [0, table_rows) is not
+ *                    looked up: its rows come back as zeros, and hk_last_device_status reports HK_EBADPOS.
+ *   flags          : HK_QKN_INTERLEAVED rotates the pairs (2i, 2i + 1) instead of (i, i + rotary_dim / 2)
+ *   D and rotary_dim multiples of 16, rotary_dim <= D <= 256 (rotary_dim <= 0 selects D); pointers 16-byte aligned.
+ * Asynchronous on `cuda_stream`. */
+#define HK_QKN_INTERLEAVED 1
+#define HK_QKN_TABLE_F32 2
+#define HK_QKN_WEIGHT_F32 4
+int hk_qk_norm_rotary(const void* q, const void* k, const void* q_weight, const void* k_weight, const void* cos,
+                      const void* sin, void* q_out, void* k_out, int B, int N, int H, int H_KV, int D, int rotary_dim,
+                      int table_rows, const long long* q_strides, const long long* k_strides, const int32_t* positions,
+                      int pos_offset, float eps, int flags, int device, void* cuda_stream);
+
+/* Its gradients: dq and dk [B, N, H or H_KV, D] contiguous from dq_out and dk_out (contiguous), and dq_weight, dk_weight [D] of
+ * the weights' type (NULL: not wanted). q and k are the forward's inputs. dq may be dq_out and dk may be dk_out. Nothing
+ * is added up with atomics: results are bit-identical from run to run.
+ *   workspace : device scratch of at least hk_qk_norm_rotary_bwd_workspace_bytes(D) bytes, 16-byte aligned; not looked at
+ *               when no weight's gradient is wanted. 0 for a D that is not supported. */
+size_t hk_qk_norm_rotary_bwd_workspace_bytes(int D);
+int hk_qk_norm_rotary_bwd(const void* q, const void* k, const void* q_weight, const void* k_weight, const void* cos,
+                          const void* sin, const void* dq_out, const void* dk_out, void* dq, void* dk, void* dq_weight,
+                          void* dk_weight, int B, int N, int H, int H_KV, int D, int rotary_dim, int table_rows,
+                          const long long* q_strides, const long long* k_strides, const int32_t* positions, int pos_offset,
+                          float eps, int flags, void* workspace, size_t workspace_bytes, int device, void* cuda_stream);
 
 /* Appends T new tokens per sequence to the paged KV cache read by hk_attn_paged_decode.
  * Paged counterpart of the reference's contiguous cache update, kv_cache[b, offset : offset + T] = kv
