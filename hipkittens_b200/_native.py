@@ -41,6 +41,8 @@ EXPORTED_SYMBOLS = (
     "hk_qk_norm_rotary_bwd_workspace_bytes",
     "hk_attn_paged_decode_workspace_bytes",
     "hk_attn_paged_decode",
+    "hk_attn_paged_decode_window_workspace_bytes",
+    "hk_attn_paged_decode_window",
     "hk_attn_paged_decode_static",
     "hk_paged_kv_append",
     "hk_last_device_status",
@@ -128,6 +130,10 @@ def capi() -> ctypes.CDLL:
     lib.hk_attn_paged_decode.argtypes = [vp, vp, vp, vp, vp, vp, vp, ci, ci, ci, ci, ci, ci, ci, cf, vp,
                                          ctypes.c_size_t, ci, vp]
     lib.hk_attn_paged_decode.restype = ci
+    lib.hk_attn_paged_decode_window_workspace_bytes.argtypes = [ci] * 7
+    lib.hk_attn_paged_decode_window_workspace_bytes.restype = ctypes.c_size_t
+    lib.hk_attn_paged_decode_window.argtypes = [vp] * 7 + [ci] * 9 + [cf, vp, ctypes.c_size_t, ci, vp]
+    lib.hk_attn_paged_decode_window.restype = ci
     lib.hk_attn_paged_decode_static.argtypes = [vp, vp, vp, vp, vp, vp, vp, ci, ci, ci, ci, ci, ci, ci, cf, ci, vp,
                                                 ctypes.POINTER(ci)]
     lib.hk_attn_paged_decode_static.restype = ci
@@ -664,7 +670,24 @@ def qk_norm_rotary_bwd(
     return dq, dk, dws[0], dws[1]
 
 
-def paged_decode_workspace_bytes(s: int, h: int, d: int, max_pages: int, page_size: int = 16) -> int:
+def _check_window(window: Optional[int], sinks: int, causal: bool = True) -> None:
+    if window is None:
+        if sinks != 0:
+            raise RuntimeError("sinks need a window")
+        return
+    if not causal:
+        raise RuntimeError("a window needs causal attention")
+    if isinstance(window, bool) or not isinstance(window, int) or not 1 <= window < 2 ** 31:
+        raise RuntimeError("window must be a positive int: the keys that a query sees, its own among them")
+    if isinstance(sinks, bool) or not isinstance(sinks, int) or not 0 <= sinks < 2 ** 31:
+        raise RuntimeError("sinks must be an int, the first keys that every query sees, or 0")
+
+
+def paged_decode_workspace_bytes(s: int, h: int, d: int, max_pages: int, page_size: int = 16, window: Optional[int] = None,
+                                 sinks: int = 0) -> int:
+    _check_window(window, sinks)
+    if window is not None:
+        return int(capi().hk_attn_paged_decode_window_workspace_bytes(s, h, d, max_pages, page_size, window, sinks))
     return int(capi().hk_attn_paged_decode_workspace_bytes(s, h, d, max_pages, page_size))
 
 
@@ -679,12 +702,20 @@ def paged_decode(
     lse: Optional[torch.Tensor] = None,
     workspace: Optional[torch.Tensor] = None,
     stream: Optional[torch.cuda.Stream] = None,
+    window: Optional[int] = None,
+    sinks: int = 0,
 ) -> Tuple[torch.Tensor, torch.Tensor]:
     """Paged-KV decode: q [S,1,H,D] bf16, pages [P,16,H_KV,D] bf16, block_table [S,max_pages] int32,
     ctx_lens [S] int32 -> O [S,1,H,D] bf16, L [S,H,1,1] fp32. `workspace` is a uint8 CUDA tensor of at
-    least ``paged_decode_workspace_bytes(...)`` bytes (allocated here when omitted)."""
+    least ``paged_decode_workspace_bytes(...)`` bytes (allocated here when omitted).
+
+    With a `window` the query, the last token of its context, sees the last `window` keys and the first `sinks` only; the
+    pages in between are not looked up, and D may be 64 as well."""
+    _check_window(window, sinks)
     if stream is None:
-        r = _front().paged_decode(q, k_pages, v_pages, block_table, ctx_lens, softmax_scale, out, lse, workspace)
+        r = (_front().paged_decode(q, k_pages, v_pages, block_table, ctx_lens, softmax_scale, out, lse, workspace)
+             if window is None else
+             _front().paged_decode(q, k_pages, v_pages, block_table, ctx_lens, softmax_scale, out, lse, workspace, window, sinks))
         if r is not None:
             return _done(r, "hk_attn_paged_decode")
     for name, t in (("q", q), ("k_pages", k_pages), ("v_pages", v_pages)):
@@ -706,16 +737,29 @@ def paged_decode(
         out = torch.empty_like(q)
     if lse is None:
         lse = torch.empty((s_n, h, 1, 1), dtype=torch.float32, device=q.device)
-    need = paged_decode_workspace_bytes(s_n, h, d, max_pages, page)
+    need = paged_decode_workspace_bytes(s_n, h, d, max_pages, page, window, sinks)
     if need == 0:
         raise HkError(HK_EUNSUPPORTED, "hk_attn_paged_decode",
-                      "shape outside the decode kernels' limits (D = 128, 16-token pages, S <= 65535, "
-                      "max_pages <= 8192)")
+                      "shape outside the decode kernels' limits (D = 128, with a window 64 or 128, 16-token pages, S <= 65535, "
+                      "max_pages, or pages of a window and its sinks, <= 8192)")
     if workspace is None:
         workspace = torch.empty(max(need, 256), dtype=torch.uint8, device=q.device)
     _require_same_device(q, k_pages=k_pages, v_pages=v_pages, block_table=block_table, ctx_lens=ctx_lens, out=out,
                          lse=lse, workspace=workspace)
     st = stream if stream is not None else torch.cuda.current_stream(q.device)
+    if window is not None:
+        if out.shape != q.shape or out.dtype != torch.bfloat16 or not out.is_contiguous():
+            raise RuntimeError("out must be a contiguous bf16 tensor of q's shape")
+        if lse.shape != (s_n, h, 1, 1) or lse.dtype != torch.float32 or not lse.is_contiguous():
+            raise RuntimeError("lse must be a contiguous fp32 tensor [S, H, 1, 1]")
+        if not workspace.is_contiguous():
+            raise RuntimeError("Tensor must be contiguous")
+        _check(capi().hk_attn_paged_decode_window(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(),
+                                                  ctx_lens.data_ptr(), out.data_ptr(), lse.data_ptr(), s_n, h, hkv, d, page,
+                                                  max_pages, p_n, window, sinks, float(softmax_scale or 0.0),
+                                                  workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+                                                  q.device.index, st.cuda_stream), "hk_attn_paged_decode_window")
+        return out, lse
     rc = capi().hk_attn_paged_decode(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
                                      block_table.data_ptr(), ctx_lens.data_ptr(), out.data_ptr(), lse.data_ptr(),
                                      s_n, h, hkv, d, page, max_pages, p_n, float(softmax_scale or 0.0),

@@ -134,6 +134,7 @@ int init_device(int device) {
   if ((rc = prepare_fwd_kernels<64, false>()) != HK_OK) return rc;
   if ((rc = prepare_fwd_kernels<64, true>()) != HK_OK) return rc;
   if ((rc = hk::prepare_decode_kernels(g_cuda_err, sizeof(g_cuda_err), st.sm_count, &st.decode)) != HK_OK) return rc;
+  if ((rc = hk::prepare_window_decode_kernels(g_cuda_err, sizeof(g_cuda_err))) != HK_OK) return rc;
   if ((rc = prepare_bwd_kernels<128, false>()) != HK_OK) return rc;
   if ((rc = prepare_bwd_kernels<128, true>()) != HK_OK) return rc;
   if ((rc = prepare_bwd_kernels<64, false>()) != HK_OK) return rc;
@@ -1120,6 +1121,68 @@ int hk_attn_paged_decode(const void* q, const void* k_pages, const void* v_pages
   cudaError_t e = hk::launch_paged_decode(p, st->decode, static_cast<cudaStream_t>(cuda_stream), &launched);
   g_launches.fetch_add(launched, std::memory_order_relaxed);
   if (e != cudaSuccess) return cuda_fail(e, "paged decode launch");
+  return HK_OK;
+}
+
+// The pages that a call's contexts can have in their windows; 0 for a window or a table that is refused.
+static int window_span(int max_pages_per_seq, int window, int sinks) {
+  if (window <= 0 || sinks < 0 || max_pages_per_seq <= 0 || max_pages_per_seq > 0x7fffffff / hk::kPageTokens) return 0;
+  return hk::decode_span_pages(max_pages_per_seq, window, sinks);
+}
+
+size_t hk_attn_paged_decode_window_workspace_bytes(int S, int H, int D, int max_pages_per_seq, int page_size, int window,
+                                                   int sinks) {
+  return hk::decode_workspace_bytes(S, H, D, window_span(max_pages_per_seq, window, sinks), page_size, true);
+}
+
+int hk_attn_paged_decode_window(const void* q, const void* k_pages, const void* v_pages, const int32_t* block_table,
+                                const int32_t* ctx_lens, void* o, float* lse, int S, int H, int H_KV, int D, int page_size,
+                                int max_pages_per_seq, int num_pages, int window, int sinks, float softmax_scale,
+                                void* workspace, size_t workspace_bytes, int device, void* cuda_stream) {
+  if (!q || !k_pages || !v_pages || !block_table || !ctx_lens || !o || !lse) return HK_EINVAL;
+  if (S <= 0 || H <= 0 || H_KV <= 0 || max_pages_per_seq <= 0 || num_pages <= 0 || window <= 0 || sinks < 0) return HK_EINVAL;
+  if ((D != 64 && D != 128) || page_size != 16) return HK_EUNSUPPORTED;
+  if (H % H_KV != 0) return HK_EINVAL;
+  const int G = H / H_KV;
+  if (G < 1 || G > 8) return HK_EUNSUPPORTED;  // the heads of a group sit in the 8 usable rows of one MMA tile
+  for (const void* ptr : {q, k_pages, v_pages, static_cast<const void*>(o)})
+    if (!aligned16(ptr)) return HK_EINVAL;
+  for (const void* ptr : {static_cast<const void*>(block_table), static_cast<const void*>(ctx_lens), static_cast<const void*>(lse)})
+    if (reinterpret_cast<uintptr_t>(ptr) & 3) return HK_EINVAL;
+  const int span = window_span(max_pages_per_seq, window, sinks);
+  if (span == 0) return HK_EINVAL;
+  if (!hk::decode_shape_supported(S, H_KV, span)) return unsupported_decode_shape(S, H_KV, span);
+  const size_t need = hk::decode_workspace_bytes(S, H, D, span, page_size, true);
+  if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255)) return HK_EWORKSPACE;
+  DeviceState* st = nullptr;
+  DeviceScope scope;
+  int rc = scope.enter(device, &st);
+  if (rc != HK_OK) return rc;
+  hk::DecodeParams p;
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.k_pages = static_cast<const __nv_bfloat16*>(k_pages);
+  p.v_pages = static_cast<const __nv_bfloat16*>(v_pages);
+  p.block_table = block_table;
+  p.ctx_lens = ctx_lens;
+  p.o = static_cast<__nv_bfloat16*>(o);
+  p.lse = lse;
+  p.S = S;
+  p.H = H;
+  p.H_KV = H_KV;
+  p.max_pages = max_pages_per_seq;
+  p.num_pages = num_pages;
+  p.scale = softmax_scale > 0.f ? softmax_scale : 1.0f / std::sqrt(float(D));
+  p.scale_log2 = p.scale * 1.4426950408889634f;
+  p.workspace = workspace;
+  p.status = st->status;
+  const int capacity = max_pages_per_seq * hk::kPageTokens;  // no context is longer
+  p.window = std::min(window, capacity);
+  p.sinks = std::min(sinks, capacity);
+  p.span_pages = span;
+  int launched = 0;
+  cudaError_t e = hk::launch_window_decode(p, D, st->decode, static_cast<cudaStream_t>(cuda_stream), &launched);
+  g_launches.fetch_add(launched, std::memory_order_relaxed);
+  if (e != cudaSuccess) return cuda_fail(e, "window decode launch");
   return HK_OK;
 }
 

@@ -24,13 +24,16 @@
 namespace hk {
 
 constexpr int kPageTokens = 16;
-constexpr int kDecodeD = 128;
+constexpr int kDecodeD = 128;                         // of the calls without a window
 constexpr int kChunkPagesMin = 32;                    // pages per CTA: 32 (512 tokens) or 64 (1024 tokens),
 constexpr int kChunkPagesMax = 64;                    // chosen per launch by decode_pick_chunk_pages
-constexpr int kDecodeStages = 3;                      // pages in flight per warp
-constexpr int kSlabBytes = kPageTokens * kDecodeD * 2;   // one page of one kv head: 4 KB
-constexpr int kStageBytes = 2 * kSlabBytes;           // K slab + V slab
-constexpr int decode_smem_bytes(int warps) { return warps * kDecodeStages * kStageBytes; }  // 96 or 192 KB
+template <int D>
+struct DecodeRing {
+  static constexpr int kStages = 3 * (128 / D);          // pages in flight per warp: as many bytes for either head dimension
+  static constexpr int kSlabBytes = kPageTokens * D * 2;    // one page of one kv head: 4 KB at D = 128
+  static constexpr int kStageBytes = 2 * kSlabBytes;     // K slab + V slab
+};
+constexpr int decode_smem_bytes(int warps) { return warps * DecodeRing<128>::kStages * DecodeRing<128>::kStageBytes; }  // 96 or 192 KB
 constexpr int kMaxCombineSplits = 256;
 
 enum : int { kStatusBadPage = 2, kStatusBadLen = 4 };  // 3 is the backward kernels' kStatusSmemAlign
@@ -48,7 +51,31 @@ struct DecodeParams {
   float scale, scale_log2;
   void* workspace;
   int* status;
+  // With a window: the query, at position ctx - 1, sees the last `window` keys and the first `sinks`
+  int window, sinks;
+  int span_pages;                // the most pages that hold such keys
 };
+
+// The pages of a context that hold keys the query sees, counted without those between the sinks and the window.
+struct LivePages {
+  int sink_pages, skip;  // the first sink_pages are pages 0, 1, ...; those behind them are `skip` further on
+  int total;
+  int first_key;         // of the window
+  __host__ __device__ LivePages(int ctx, int window, int sinks) {
+    first_key = ctx > window ? ctx - window : 0;
+    const int first_page = first_key / kPageTokens;
+    sink_pages = (sinks + kPageTokens - 1) / kPageTokens;
+    if (sink_pages > first_page) sink_pages = first_page;
+    skip = first_page - sink_pages;
+    total = (ctx + kPageTokens - 1) / kPageTokens - skip;
+  }
+  __host__ __device__ int page(int i) const { return i < sink_pages ? i : i + skip; }
+};
+// The most of them that any context in a table of max_pages has.
+inline int decode_span_pages(int max_pages, int window, int sinks) {
+  const long long most = (1ll * sinks + kPageTokens - 1) / kPageTokens + (1ll * window + kPageTokens - 2) / kPageTokens + 1;
+  return most < max_pages ? int(most) : max_pages;
+}
 
 // The workspace is laid out for the smaller chunk size (the larger split count), whichever size a launch uses.
 __host__ __device__ inline int decode_max_splits(int max_pages) {
@@ -130,11 +157,12 @@ inline bool decode_shape_supported(int S, int H_KV, int max_pages) {
   return S > 0 && S <= 65535 && H_KV > 0 && H_KV <= 65535 && max_pages > 0 &&
          decode_max_splits(max_pages) <= kMaxCombineSplits;
 }
-inline size_t decode_workspace_bytes(int S, int H, int D, int max_pages, int page_size) {
-  if (S <= 0 || S > 65535 || H <= 0 || D != kDecodeD || page_size != kPageTokens || max_pages <= 0) return 0;
+inline size_t decode_workspace_bytes(int S, int H, int D, int max_pages, int page_size, bool any_d = false) {
+  if (S <= 0 || S > 65535 || H <= 0 || page_size != kPageTokens || max_pages <= 0) return 0;
+  if (D != kDecodeD && !(any_d && D == 64)) return 0;
   if (decode_max_splits(max_pages) > kMaxCombineSplits) return 0;
   const size_t splits = decode_max_splits(max_pages);
-  const size_t o_bytes = size_t(S) * H * splits * kDecodeD * sizeof(float);
+  const size_t o_bytes = size_t(S) * H * splits * D * sizeof(float);
   const size_t ml_bytes = size_t(S) * H * splits * 2 * sizeof(float);
   return ((o_bytes + 255) & ~size_t(255)) + ((ml_bytes + 255) & ~size_t(255));
 }
@@ -143,6 +171,10 @@ namespace dec {
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// The same, or 16 zero bytes and nothing read.
+__device__ __forceinline__ void cp_async16_if(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -173,9 +205,12 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
 
 // grid = (max_splits, H_KV, S), or (cluster size, H_KV, S) in clusters along x; block = 32 W threads, dynamic smem =
 // decode_smem_bytes(W).
-template <int G, bool CLUSTER, int W>
+template <int G, bool CLUSTER, int W, int D = kDecodeD, bool WINDOW = false>
 __global__ void __launch_bounds__(W * 32, W == 8 ? 1 : 2) paged_decode_split_kernel(const DecodeParams p) {
   using namespace dec;
+  using Ring = DecodeRing<D>;
+  constexpr int kDecodeStages = Ring::kStages, kSlabBytes = Ring::kSlabBytes, kStageBytes = Ring::kStageBytes;
+  constexpr int kRowBytes = D * 2, kChunks = D / 8;  // of a token: its bytes, and 16-byte chunks
   extern __shared__ __align__(128) uint8_t dsmem[];
   ptx::grid_dep_wait();
   ptx::grid_dep_launch();
@@ -189,15 +224,16 @@ __global__ void __launch_bounds__(W * 32, W == 8 ? 1 : 2) paged_decode_split_ker
   }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
-  const int total_pages = (ctx + kPageTokens - 1) / kPageTokens;
+  const LivePages live(ctx, WINDOW ? p.window : 1, WINDOW ? p.sinks : 0);
+  const int total_pages = WINDOW ? live.total : (ctx + kPageTokens - 1) / kPageTokens;
   // This warp's pages: page_first, page_first + page_step, ... below page_end. A CTA of a cluster takes every n_used-th
   // group of W pages, so that whatever the length the live CTAs of a cluster differ by a page per warp at most.
   int n_used, page_first, page_step, page_end;
   if constexpr (CLUSTER) {
     if (ctx <= 0) {  // defined output for an empty context
       if (split == 0) {
-        for (int i = threadIdx.x; i < G * kDecodeD; i += W * 32)
-          p.o[(size_t(seq) * p.H + kvh * G) * kDecodeD + i] = __float2bfloat16(0.f);
+        for (int i = threadIdx.x; i < G * D; i += W * 32)
+          p.o[(size_t(seq) * p.H + kvh * G) * D + i] = __float2bfloat16(0.f);
         if (threadIdx.x < G) p.lse[size_t(seq) * p.H + kvh * G + threadIdx.x] = -INFINITY;
       }
       return;
@@ -208,7 +244,7 @@ __global__ void __launch_bounds__(W * 32, W == 8 ? 1 : 2) paged_decode_split_ker
     page_step = n_used * W;
     page_end = total_pages;
   } else {
-    if (split * p.chunk_pages * kPageTokens >= ctx) return;
+    if (WINDOW ? ctx <= 0 || split * p.chunk_pages >= total_pages : split * p.chunk_pages * kPageTokens >= ctx) return;
     n_used = 1;
     page_first = split * p.chunk_pages + warp;
     page_step = W;
@@ -216,22 +252,26 @@ __global__ void __launch_bounds__(W * 32, W == 8 ? 1 : 2) paged_decode_split_ker
   }
   const float c = p.scale_log2;
 
-  // page ids of this warp, one per lane: no warp has more than 32 pages (decode_pick_shape and the chunk sizes see to it)
+  // page ids of this warp, one per lane: no warp has more than 32 pages (decode_pick_shape and the chunk sizes see to it).
+  // With a window, 32 at a time; pages without a key that the query sees are not looked up.
   int my_id = 0;
-  if (const int page = page_first + lane * page_step; page < page_end) {
-    my_id = p.block_table[size_t(seq) * p.max_pages + page];
-    if (my_id < 0 || my_id >= p.num_pages) {
-      atomicCAS(p.status, 0, kStatusBadPage);  // never dereference an id outside the pool
-      my_id = 0;
+  auto look_up = [&](int i0) {
+    if (const int page = page_first + (i0 + lane) * page_step; page < page_end) {
+      my_id = p.block_table[size_t(seq) * p.max_pages + (WINDOW ? live.page(page) : page)];
+      if (my_id < 0 || my_id >= p.num_pages) {
+        atomicCAS(p.status, 0, kStatusBadPage);  // never dereference an id outside the pool
+        my_id = 0;
+      }
     }
-  }
+  };
+  look_up(0);
 
-  // Q fragments: row g = head kvh*G+g (rows >= G are zero), 8 k-steps of 16 columns
-  uint32_t qa[8][2];
+  // Q fragments: row g = head kvh*G+g (rows >= G are zero), k-steps of 16 columns
+  uint32_t qa[D / 16][2];
   {
-    const __nv_bfloat16* qrow = p.q + (size_t(seq) * p.H + kvh * G + (g < G ? g : 0)) * kDecodeD;
+    const __nv_bfloat16* qrow = p.q + (size_t(seq) * p.H + kvh * G + (g < G ? g : 0)) * D;
 #pragma unroll
-    for (int ks = 0; ks < 8; ++ks) {
+    for (int ks = 0; ks < D / 16; ++ks) {
       uint32_t lo = *reinterpret_cast<const uint32_t*>(qrow + ks * 16 + 2 * t);
       uint32_t hi = *reinterpret_cast<const uint32_t*>(qrow + ks * 16 + 8 + 2 * t);
       qa[ks][0] = (g < G) ? lo : 0u;
@@ -240,32 +280,41 @@ __global__ void __launch_bounds__(W * 32, W == 8 ? 1 : 2) paged_decode_split_ker
   }
 
   const uint32_t ring = ptx::smem_u32(dsmem) + warp * (kDecodeStages * kStageBytes);
-  const size_t row_elems = size_t(p.H_KV) * kDecodeD;  // elements between consecutive tokens of a page
+  const size_t row_elems = size_t(p.H_KV) * D;  // elements between consecutive tokens of a page
 
-  // 16-byte gather of one page of this kv head: lane copies chunks lane, lane+32, ... of the 256
-  // chunks (16 tokens x 16 chunks) of K and of V; chunk index is XOR-swizzled with the token so that
+  auto sees = [&](int key) { return key < ctx && (key >= live.first_key || key < p.sinks); };
+  // 16-byte gather of one page of this kv head: lane copies chunks lane, lane+32, ... of the
+  // chunks (16 tokens x D / 8 chunks) of K and of V; chunk index is XOR-swizzled with the token so that
   // ldmatrix reads are bank-conflict free.
   auto fetch = [&](int i) {
     if (page_first + i * page_step < page_end) {
-      const int id = __shfl_sync(0xffffffffu, my_id, i);
-      const size_t base = (size_t(id) * kPageTokens) * row_elems + size_t(kvh) * kDecodeD;
+      if (WINDOW && i > 0 && (i & 31) == 0) look_up(i);
+      const int id = __shfl_sync(0xffffffffu, my_id, WINDOW ? i & 31 : i);
+      const size_t base = (size_t(id) * kPageTokens) * row_elems + size_t(kvh) * D;
       const uint32_t st = ring + (i % kDecodeStages) * kStageBytes;
 #pragma unroll
-      for (int r = 0; r < 8; ++r) {
+      for (int r = 0; r < kChunks / 2; ++r) {
         const int ch_lin = r * 32 + lane;
-        const int tok = ch_lin >> 4, ch = ch_lin & 15;
+        const int tok = ch_lin / kChunks, ch = ch_lin % kChunks;
         const size_t src = base + size_t(tok) * row_elems + ch * 8;
-        const uint32_t dst = tok * 256 + ((ch ^ (tok & 7)) << 4);
-        cp_async16(st + dst, p.k_pages + src);
-        cp_async16(st + kSlabBytes + dst, p.v_pages + src);
+        const uint32_t dst = tok * kRowBytes + ((ch ^ (tok & 7)) << 4);
+        if constexpr (WINDOW) {
+          // keys that the query does not see are not read, and are zeros: whatever the cache holds there meets p = 0
+          const bool seen = sees(live.page(page_first + i * page_step) * kPageTokens + tok);
+          cp_async16_if(st + dst, p.k_pages + src, seen);
+          cp_async16_if(st + kSlabBytes + dst, p.v_pages + src, seen);
+        } else {
+          cp_async16(st + dst, p.k_pages + src);
+          cp_async16(st + kSlabBytes + dst, p.v_pages + src);
+        }
       }
     }
     cp_async_commit();
   };
 
-  float oacc[16][4];
+  float oacc[D / 8][4];
 #pragma unroll
-  for (int j = 0; j < 16; ++j) oacc[j][0] = oacc[j][1] = oacc[j][2] = oacc[j][3] = 0.f;
+  for (int j = 0; j < D / 8; ++j) oacc[j][0] = oacc[j][1] = oacc[j][2] = oacc[j][3] = 0.f;
   float m = -INFINITY, l = 0.f;
 
 #pragma unroll
@@ -286,10 +335,10 @@ __global__ void __launch_bounds__(W * 32, W == 8 ? 1 : 2) paged_decode_split_ker
       const int mi = lane >> 3, r = lane & 7;
       const int tok = r + 8 * (mi >> 1);
 #pragma unroll
-      for (int ks = 0; ks < 8; ++ks) {
+      for (int ks = 0; ks < D / 16; ++ks) {
         const int ch = ks * 2 + (mi & 1);
         uint32_t b0, b1, b2, b3;
-        ldmatrix_x4(sK + tok * 256 + ((ch ^ (tok & 7)) << 4), b0, b1, b2, b3);
+        ldmatrix_x4(sK + tok * kRowBytes + ((ch ^ (tok & 7)) << 4), b0, b1, b2, b3);
         mma_16816(ks & 1 ? sd[0] : sc[0], qa[ks][0], 0u, qa[ks][1], 0u, b0, b1);
         mma_16816(ks & 1 ? sd[1] : sc[1], qa[ks][0], 0u, qa[ks][1], 0u, b2, b3);
       }
@@ -300,12 +349,12 @@ __global__ void __launch_bounds__(W * 32, W == 8 ? 1 : 2) paged_decode_split_ker
       }
     }
     // ---- online softmax over this page (row g, tokens nt*8 + 2t + {0,1})
-    const int tok_base = page * kPageTokens;
+    const int tok_base = (WINDOW ? live.page(page) : page) * kPageTokens;
     float sv[4] = {sc[0][0], sc[0][1], sc[1][0], sc[1][1]};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int tok = tok_base + (e >> 1) * 8 + 2 * t + (e & 1);
-      if (tok >= ctx) sv[e] = -INFINITY;
+      if (WINDOW ? !sees(tok) : tok >= ctx) sv[e] = -INFINITY;
     }
     float pm = fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3]));
     pm = fmaxf(pm, __shfl_xor_sync(0xffffffffu, pm, 1));
@@ -315,7 +364,7 @@ __global__ void __launch_bounds__(W * 32, W == 8 ? 1 : 2) paged_decode_split_ker
       const float alpha = ptx::ex2_approx((m - m_new) * c);  // m = -inf on the first page gives 0
       l *= alpha;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
+      for (int j = 0; j < D / 8; ++j) {
         oacc[j][0] *= alpha;
         oacc[j][1] *= alpha;
       }
@@ -335,10 +384,10 @@ __global__ void __launch_bounds__(W * 32, W == 8 ? 1 : 2) paged_decode_split_ker
       const int mi = lane >> 3, r = lane & 7;
       const int tok = r + 8 * (mi & 1);
 #pragma unroll
-      for (int jp = 0; jp < 8; ++jp) {
+      for (int jp = 0; jp < D / 16; ++jp) {
         const int ch = jp * 2 + (mi >> 1);
         uint32_t b0, b1, b2, b3;
-        ldmatrix_x4_trans(sV + tok * 256 + ((ch ^ (tok & 7)) << 4), b0, b1, b2, b3);
+        ldmatrix_x4_trans(sV + tok * kRowBytes + ((ch ^ (tok & 7)) << 4), b0, b1, b2, b3);
         mma_16816(oacc[2 * jp], pa0, 0u, pa2, 0u, b0, b1);
         mma_16816(oacc[2 * jp + 1], pa0, 0u, pa2, 0u, b2, b3);
       }
@@ -352,21 +401,21 @@ __global__ void __launch_bounds__(W * 32, W == 8 ? 1 : 2) paged_decode_split_ker
   // ---- merge the W warps through shared memory (the ring is idle now)
   __syncthreads();
   float* sm_o = reinterpret_cast<float*>(dsmem);  // [W][8][128]
-  float* sm_m = sm_o + W * 8 * kDecodeD;          // [W][8]
+  float* sm_m = sm_o + W * 8 * D;          // [W][8]
   float* sm_l = sm_m + W * 8;                     // [W][8]
 #pragma unroll
-  for (int j = 0; j < 16; ++j) {
+  for (int j = 0; j < D / 8; ++j) {
     float2 v2 = make_float2(oacc[j][0], oacc[j][1]);
-    *reinterpret_cast<float2*>(sm_o + (warp * 8 + g) * kDecodeD + j * 8 + 2 * t) = v2;
+    *reinterpret_cast<float2*>(sm_o + (warp * 8 + g) * D + j * 8 + 2 * t) = v2;
   }
   if (t == 0) {
     sm_m[warp * 8 + g] = m;
     sm_l[warp * 8 + g] = l;
   }
   __syncthreads();
-  // 128 threads <-> 128 output columns; with 8 warps each half of them takes every other head of the group
-  constexpr int kHalves = W / 4, kHeads = (G + kHalves - 1) / kHalves;
-  const int d = threadIdx.x & (kDecodeD - 1), h0 = threadIdx.x / kDecodeD;
+  // D threads <-> D output columns; where there are more threads, each D of them take every kHalves-th head of the group
+  constexpr int kHalves = W * 32 / D, kHeads = (G + kHalves - 1) / kHalves;
+  const int d = threadIdx.x & (D - 1), h0 = threadIdx.x / D;
   // per head of this thread: reference maximum, row sum and this thread's column of the CTA's share
   float M[kHeads], L[kHeads], acc[kHeads];
 #pragma unroll
@@ -379,7 +428,7 @@ __global__ void __launch_bounds__(W * 32, W == 8 ? 1 : 2) paged_decode_split_ker
 #pragma unroll
     for (int w = 0; w < W; ++w) {
       const float wgt = ptx::ex2_approx((sm_m[w * 8 + h] - M[i]) * c);
-      acc[i] += wgt * sm_o[(w * 8 + h) * kDecodeD + d];
+      acc[i] += wgt * sm_o[(w * 8 + h) * D + d];
       L[i] += wgt * sm_l[w * 8 + h];
     }
   }
@@ -388,12 +437,12 @@ __global__ void __launch_bounds__(W * 32, W == 8 ? 1 : 2) paged_decode_split_ker
       // ---- merge the CTAs of the cluster: each leaves its share in its own shared memory, and CTA r reads all of
       // head r, r + n_used, ... in the order of the ranks
       float* cl_o = sm_l + W * 8;          // [G][128]
-      float* cl_ml = cl_o + 8 * kDecodeD;  // [G][2]
+      float* cl_ml = cl_o + 8 * D;  // [G][2]
 #pragma unroll
       for (int i = 0; i < kHeads; ++i) {
         const int h = i * kHalves + h0;
         if (h >= G) break;
-        cl_o[h * kDecodeD + d] = acc[i];
+        cl_o[h * D + d] = acc[i];
         if (d == 0) {
           cl_ml[2 * h] = M[i];
           cl_ml[2 * h + 1] = L[i];
@@ -403,7 +452,7 @@ __global__ void __launch_bounds__(W * 32, W == 8 ? 1 : 2) paged_decode_split_ker
       ptx::cluster_wait();
       for (int h = split * kHalves + h0; h < G; h += n_used * kHalves) {
         float m_r[kMaxCluster], l_r[kMaxCluster], o_r[kMaxCluster];
-        const uint32_t a_ml = ptx::smem_u32(cl_ml + 2 * h), a_o = ptx::smem_u32(cl_o + h * kDecodeD + d);
+        const uint32_t a_ml = ptx::smem_u32(cl_ml + 2 * h), a_o = ptx::smem_u32(cl_o + h * D + d);
 #pragma unroll
         for (int r = 0; r < kMaxCluster; ++r) {
           m_r[r] = -INFINITY;
@@ -426,7 +475,7 @@ __global__ void __launch_bounds__(W * 32, W == 8 ? 1 : 2) paged_decode_split_ker
           out += wgt * o_r[r];
         }
         const size_t row = size_t(seq) * p.H + kvh * G + h;
-        p.o[row * kDecodeD + d] = __float2bfloat16(out / sum);
+        p.o[row * D + d] = __float2bfloat16(out / sum);
         if (d == 0) p.lse[row] = Mc * p.scale + __logf(sum);
       }
       ptx::cluster_arrive();  // nobody leaves while its shared memory is being read
@@ -435,9 +484,9 @@ __global__ void __launch_bounds__(W * 32, W == 8 ? 1 : 2) paged_decode_split_ker
     }
   }
   const int n_splits = CLUSTER ? 1 : (total_pages + p.chunk_pages - 1) / p.chunk_pages;
-  const int max_splits = decode_max_splits(p.max_pages);
+  const int max_splits = decode_max_splits(WINDOW ? p.span_pages : p.max_pages);
   float* ws_o = reinterpret_cast<float*>(p.workspace);
-  const size_t o_bytes = (size_t(p.S) * p.H * max_splits * kDecodeD * sizeof(float) + 255) & ~size_t(255);
+  const size_t o_bytes = (size_t(p.S) * p.H * max_splits * D * sizeof(float) + 255) & ~size_t(255);
   float* ws_ml = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(p.workspace) + o_bytes);
 #pragma unroll
   for (int i = 0; i < kHeads; ++i) {
@@ -445,11 +494,11 @@ __global__ void __launch_bounds__(W * 32, W == 8 ? 1 : 2) paged_decode_split_ker
     if (h >= G) break;
     const size_t row = size_t(seq) * p.H + kvh * G + h;
     if (n_splits == 1) {
-      p.o[row * kDecodeD + d] = __float2bfloat16(acc[i] / L[i]);
+      p.o[row * D + d] = __float2bfloat16(acc[i] / L[i]);
       if (d == 0) p.lse[row] = M[i] * p.scale + __logf(L[i]);
     } else {
       const size_t slot = row * max_splits + split;
-      ws_o[slot * kDecodeD + d] = acc[i];
+      ws_o[slot * D + d] = acc[i];
       if (d == 0) {
         ws_ml[slot * 2] = M[i];
         ws_ml[slot * 2 + 1] = L[i];
@@ -458,25 +507,27 @@ __global__ void __launch_bounds__(W * 32, W == 8 ? 1 : 2) paged_decode_split_ker
   }
 }
 
-// grid = (H, S), block = 128 threads (one per output column). Merges the per-chunk partials of
+// grid = (H, S), block = D threads (one per output column). Merges the per-chunk partials of
 // sequences that span more than one chunk.
-__global__ void __launch_bounds__(kDecodeD) paged_decode_combine_kernel(const DecodeParams p) {
+template <int D, bool WINDOW>
+__global__ void __launch_bounds__(D) paged_decode_combine_kernel(const DecodeParams p) {
   ptx::grid_dep_wait();  // from here on the split grid has completed and its partials are visible
   ptx::grid_dep_launch();
   const int head = blockIdx.x, seq = blockIdx.y;
   const int ctx = min(p.ctx_lens[seq], p.max_pages * kPageTokens);  // clamped as in the split kernel, which reports it
   const int d = threadIdx.x;
   if (ctx <= 0) {  // defined output for an empty context
-    p.o[(size_t(seq) * p.H + head) * kDecodeD + d] = __float2bfloat16(0.f);
+    p.o[(size_t(seq) * p.H + head) * D + d] = __float2bfloat16(0.f);
     if (d == 0) p.lse[size_t(seq) * p.H + head] = -INFINITY;
     return;
   }
   const int chunk_tokens = p.chunk_pages * kPageTokens;
-  const int n_splits = (ctx + chunk_tokens - 1) / chunk_tokens;
+  const int n_splits = WINDOW ? (LivePages(ctx, p.window, p.sinks).total + p.chunk_pages - 1) / p.chunk_pages
+                              : (ctx + chunk_tokens - 1) / chunk_tokens;
   if (n_splits == 1) return;  // finished by the split kernel
-  const int max_splits = decode_max_splits(p.max_pages);
+  const int max_splits = decode_max_splits(WINDOW ? p.span_pages : p.max_pages);
   const float* ws_o = reinterpret_cast<const float*>(p.workspace);
-  const size_t o_bytes = (size_t(p.S) * p.H * max_splits * kDecodeD * sizeof(float) + 255) & ~size_t(255);
+  const size_t o_bytes = (size_t(p.S) * p.H * max_splits * D * sizeof(float) + 255) & ~size_t(255);
   const float* ws_ml = reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(p.workspace) + o_bytes);
   const size_t slot0 = (size_t(seq) * p.H + head) * max_splits;
   __shared__ float s_w[kMaxCombineSplits];
@@ -502,24 +553,47 @@ __global__ void __launch_bounds__(kDecodeD) paged_decode_combine_kernel(const De
   __syncthreads();
   float acc = 0.f;
 #pragma unroll 4
-  for (int i = 0; i < n_splits; ++i) acc += s_w[i] * ws_o[(slot0 + i) * kDecodeD + d];
-  p.o[(size_t(seq) * p.H + head) * kDecodeD + d] = __float2bfloat16(acc / s_L);
+  for (int i = 0; i < n_splits; ++i) acc += s_w[i] * ws_o[(slot0 + i) * D + d];
+  p.o[(size_t(seq) * p.H + head) * D + d] = __float2bfloat16(acc / s_L);
   if (d == 0) p.lse[size_t(seq) * p.H + head] = s_M * p.scale + __logf(s_L);
 }
 
-template <int G, bool CLUSTER, int W>
+template <int G, bool CLUSTER, int W, int D, bool WINDOW>
 cudaError_t prepare_decode_kernel() {
-  auto* fn = paged_decode_split_kernel<G, CLUSTER, W>;
+  auto* fn = paged_decode_split_kernel<G, CLUSTER, W, D, WINDOW>;
   const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, decode_smem_bytes(W));
   if (e != cudaSuccess || !CLUSTER) return e;
   return cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
 }
 template <int G>
 cudaError_t prepare_decode_kernels_of() {
-  cudaError_t e = prepare_decode_kernel<G, false, 4>();
-  if (e == cudaSuccess) e = prepare_decode_kernel<G, true, 4>();
-  if (e == cudaSuccess) e = prepare_decode_kernel<G, true, 8>();
+  cudaError_t e = prepare_decode_kernel<G, false, 4, kDecodeD, false>();
+  if (e == cudaSuccess) e = prepare_decode_kernel<G, true, 4, kDecodeD, false>();
+  if (e == cudaSuccess) e = prepare_decode_kernel<G, true, 8, kDecodeD, false>();
   return e;
+}
+template <int G>
+cudaError_t prepare_window_kernels_of() {
+  cudaError_t e = prepare_decode_kernel<G, false, 4, 128, true>();
+  if (e == cudaSuccess) e = prepare_decode_kernel<G, true, 4, 128, true>();
+  if (e == cudaSuccess) e = prepare_decode_kernel<G, true, 8, 128, true>();
+  if (e == cudaSuccess) e = prepare_decode_kernel<G, false, 4, 64, true>();
+  if (e == cudaSuccess) e = prepare_decode_kernel<G, true, 4, 64, true>();
+  if (e == cudaSuccess) e = prepare_decode_kernel<G, true, 8, 64, true>();
+  return e;
+}
+// Those of calls with a window; the sizes of their clusters that fit are the others'.
+inline int prepare_window_decode_kernels(char* err, size_t err_len) {
+  for (auto* prepare : {prepare_window_kernels_of<1>, prepare_window_kernels_of<2>, prepare_window_kernels_of<3>,
+                        prepare_window_kernels_of<4>, prepare_window_kernels_of<5>, prepare_window_kernels_of<6>,
+                        prepare_window_kernels_of<7>, prepare_window_kernels_of<8>}) {
+    const cudaError_t e = prepare();
+    if (e != cudaSuccess) {
+      snprintf(err, err_len, "window decode kernel attribute: %s", cudaGetErrorString(e));
+      return -3;
+    }
+  }
+  return 0;
 }
 inline int prepare_decode_kernels(char* err, size_t err_len, int sm_count, DecodeLimits* lim) {
   for (auto* prepare : {prepare_decode_kernels_of<1>, prepare_decode_kernels_of<2>, prepare_decode_kernels_of<3>,
@@ -537,34 +611,46 @@ inline int prepare_decode_kernels(char* err, size_t err_len, int sm_count, Decod
   return 0;
 }
 
-template <int G>
+template <int G, int D, bool WINDOW>
 cudaError_t launch_decode_split(const DecodeParams& p, int splits, int cluster, int warps, cudaStream_t stream) {
   const dim3 grid(cluster ? cluster : splits, p.H_KV, p.S);
   if (cluster == 0)
-    return launch_dependent(true, paged_decode_split_kernel<G, false, 4>, grid, 128, decode_smem_bytes(4), stream, p);
-  auto* fn = warps == 8 ? paged_decode_split_kernel<G, true, 8> : paged_decode_split_kernel<G, true, 4>;
+    return launch_dependent(true, paged_decode_split_kernel<G, false, 4, D, WINDOW>, grid, 128, decode_smem_bytes(4), stream, p);
+  auto* fn = warps == 8 ? paged_decode_split_kernel<G, true, 8, D, WINDOW> : paged_decode_split_kernel<G, true, 4, D, WINDOW>;
   return launch_dependent(true, fn, grid, warps * 32, decode_smem_bytes(warps), stream, ClusterX{unsigned(cluster)}, p);
 }
 
-inline cudaError_t launch_paged_decode(DecodeParams p, const DecodeLimits& lim, cudaStream_t stream, int* launched) {
-  const DecodeShape shape = decode_pick_shape(p.S, p.H_KV, p.max_pages, lim);
+template <int D, bool WINDOW>
+cudaError_t launch_decode_shape(DecodeParams p, DecodeShape shape, int pages, int sm_count, cudaStream_t stream, int* launched) {
   const int cluster = shape.cluster, warps = shape.warps;
-  p.chunk_pages = decode_pick_chunk_pages(p.S, p.H_KV, p.max_pages, lim.sm_count);
-  const int splits = (p.max_pages + p.chunk_pages - 1) / p.chunk_pages;
+  p.chunk_pages = decode_pick_chunk_pages(p.S, p.H_KV, pages, sm_count);
+  const int splits = (pages + p.chunk_pages - 1) / p.chunk_pages;
   if (splits > kMaxCombineSplits) return cudaErrorInvalidValue;
   cudaError_t e;
   switch (p.H / p.H_KV) {
 #define HK_CASE(g) \
-  case g: e = launch_decode_split<g>(p, splits, cluster, warps, stream); break;
+  case g: e = launch_decode_split<g, D, WINDOW>(p, splits, cluster, warps, stream); break;
     HK_CASE(1) HK_CASE(2) HK_CASE(3) HK_CASE(4) HK_CASE(5) HK_CASE(6) HK_CASE(7) HK_CASE(8)
 #undef HK_CASE
     default: return cudaErrorInvalidValue;
   }
   *launched += 1;
   if (e != cudaSuccess || cluster) return e;
-  e = launch_dependent(true, paged_decode_combine_kernel, dim3(p.H, p.S), kDecodeD, 0, stream, p);
+  e = launch_dependent(true, paged_decode_combine_kernel<D, WINDOW>, dim3(p.H, p.S), D, 0, stream, p);
   *launched += 1;
   return e;
+}
+
+inline cudaError_t launch_paged_decode(const DecodeParams& p, const DecodeLimits& lim, cudaStream_t stream, int* launched) {
+  const DecodeShape shape = decode_pick_shape(p.S, p.H_KV, p.max_pages, lim);
+  return launch_decode_shape<kDecodeD, false>(p, shape, p.max_pages, lim.sm_count, stream, launched);
+}
+// With p.window, p.sinks and p.span_pages set.
+inline cudaError_t launch_window_decode(const DecodeParams& p, int D, const DecodeLimits& lim, cudaStream_t stream,
+                                        int* launched) {
+  const DecodeShape shape = decode_pick_shape(p.S, p.H_KV, p.span_pages, lim);
+  auto* launch = D == 64 ? launch_decode_shape<64, true> : launch_decode_shape<128, true>;
+  return launch(p, shape, p.span_pages, lim.sm_count, stream, launched);
 }
 
 }  // namespace hk

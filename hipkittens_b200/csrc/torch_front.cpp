@@ -347,13 +347,28 @@ struct Paged {
   }
 };
 
-// paged_decode(q, k_pages, v_pages, block_table, ctx_lens, softmax_scale, out, lse, workspace)
+// A window and its sinks, as the last two arguments; without them, none.
+bool window_args(PyObject* const* a, Py_ssize_t n_args, Py_ssize_t without, int& window, int& sinks) {
+  window = sinks = 0;
+  if (n_args == without) return true;
+  if (n_args != without + 2 || !PyLong_CheckExact(a[without]) || !PyLong_CheckExact(a[without + 1])) return false;
+  int over_w = 0, over_s = 0;
+  const long w = PyLong_AsLongAndOverflow(a[without], &over_w), s = PyLong_AsLongAndOverflow(a[without + 1], &over_s);
+  if (over_w || over_s || w < 1 || s < 0 || !fits({w, s})) return false;
+  window = i32(w), sinks = i32(s);
+  return true;
+}
+
+// paged_decode(q, k_pages, v_pages, block_table, ctx_lens, softmax_scale, out, lse, workspace[, window, sinks])
 PyObject* paged_decode(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   HANDLE_TH_ERRORS
   float scale;
   Paged p;
-  if (n_args != 9 || !number(a[5], scale) || !p.take(a) || p.t != 1) Py_RETURN_NONE;
-  const size_t need = hk_attn_paged_decode_workspace_bytes(i32(p.s), i32(p.h), i32(p.d), i32(p.max_pages), i32(p.page));
+  int window, sinks;
+  if (!window_args(a, n_args, 9, window, sinks) || !number(a[5], scale) || !p.take(a) || p.t != 1) Py_RETURN_NONE;
+  const size_t need =
+      window ? hk_attn_paged_decode_window_workspace_bytes(i32(p.s), i32(p.h), i32(p.d), i32(p.max_pages), i32(p.page), window, sinks)
+             : hk_attn_paged_decode_workspace_bytes(i32(p.s), i32(p.h), i32(p.d), i32(p.max_pages), i32(p.page));
   Tensor out, lse, ws;
   if (need == 0 || !output(a[6], *p.q, p.q->sizes(), at::kBFloat16, out) ||
       !output(a[7], *p.q, {p.s, p.h, 1, 1}, at::kFloat, lse))
@@ -372,6 +387,10 @@ PyObject* paged_decode(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   float* lsep = ptr<float>(lse);
   const size_t ws_bytes = size_t(ws.numel());
   const int rc = unlocked([&] {
+    if (window)
+      return hk_attn_paged_decode_window(p.q_ptr, p.k_pages, p.v_pages, p.table_ptr, p.lens_ptr, outp, lsep, i32(p.s), i32(p.h),
+                                         i32(p.hkv), i32(p.d), i32(p.page), i32(p.max_pages), i32(p.pool), window, sinks, scale,
+                                         wsp, ws_bytes, p.device, st);
     return hk_attn_paged_decode(p.q_ptr, p.k_pages, p.v_pages, p.table_ptr, p.lens_ptr, outp, lsep, i32(p.s), i32(p.h),
                                 i32(p.hkv), i32(p.d), i32(p.page), i32(p.max_pages), i32(p.pool), scale, wsp, ws_bytes,
                                 p.device, st);

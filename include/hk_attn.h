@@ -115,6 +115,21 @@ int hk_attn_paged_decode(const void* q, const void* k_pages, const void* v_pages
                          float softmax_scale, void* workspace, size_t workspace_bytes,
                          int device, void* cuda_stream);
 
+/* hk_attn_paged_decode for layers whose queries see a window of the context and its first tokens: the query, at position
+ * p = ctx_lens[s] - 1, sees the keys c with p - c < window or c < sinks. Only pages that hold such a key are looked up in the block
+ * table, so those between the sinks and the window may have been given away; keys that are not seen are not read, whatever the
+ * cache holds there.
+ *   window >= 1, sinks >= 0; D = 64 or 128; the rest as in hk_attn_paged_decode, where max_pages_per_seq may be as large as
+ *   16 max_pages_per_seq < 2^31 if the pages that a window and its sinks can touch are at most 8192.
+ *   workspace : device scratch of at least hk_attn_paged_decode_window_workspace_bytes(...) bytes, 256-byte aligned. */
+size_t hk_attn_paged_decode_window_workspace_bytes(int S, int H, int D, int max_pages_per_seq, int page_size, int window,
+                                                   int sinks);
+int hk_attn_paged_decode_window(const void* q, const void* k_pages, const void* v_pages,
+                                const int32_t* block_table, const int32_t* ctx_lens, void* o, float* lse,
+                                int S, int H, int H_KV, int D, int page_size, int max_pages_per_seq, int num_pages,
+                                int window, int sinks, float softmax_scale, void* workspace, size_t workspace_bytes,
+                                int device, void* cuda_stream);
+
 /* ---- attention backward ------------------------------------------------------------------------------
  * The reference runs three kernels per backward pass (training/llama/llama/models/attentions/hipkittens.py:
  * 110-112): tk_kernel_bkwd_prep.dispatch_prep(O, dO, delta), tk_kernel_bkwd.dispatch_bwd_combined(q, k, v,
