@@ -25,7 +25,9 @@ EXPORTED_SYMBOLS = (
     "hk_attn_fwd_strided",
     "hk_attn_fwd_varlen",
     "hk_attn_fwd_cross",
+    "hk_attn_fwd_window",
     "hk_attn_fwd_paged",
+    "hk_attn_fwd_paged_window",
     "hk_attn_bwd_prep",
     "hk_attn_bwd",
     "hk_attn_bwd_varlen",
@@ -98,6 +100,10 @@ def capi() -> ctypes.CDLL:
     lib.hk_attn_fwd_cross.restype = ci
     lib.hk_attn_fwd_paged.argtypes = [vp, vp, vp, vp, vp, vp, vp, ci, ci, ci, ci, ci, ci, ci, ci, ci, cf, ci, vp]
     lib.hk_attn_fwd_paged.restype = ci
+    lib.hk_attn_fwd_window.argtypes = [vp] * 5 + [ci] * 6 + [ll3] * 3 + [vp, ci, ci, cf, ci, vp]
+    lib.hk_attn_fwd_window.restype = ci
+    lib.hk_attn_fwd_paged_window.argtypes = [vp] * 7 + [ci] * 10 + [cf, ci, vp]
+    lib.hk_attn_fwd_paged_window.restype = ci
     lib.hk_attn_bwd_prep.argtypes = [vp, vp, vp, ci, ci, ci, ci, ci, vp]
     lib.hk_attn_bwd_prep.restype = ci
     lib.hk_attn_bwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, ci, ci, ci, ci, ci, ci, cf, ci, ci, vp]
@@ -224,6 +230,11 @@ def _require_same_device(ref: torch.Tensor, **tensors) -> None:
                                f"{t.device if isinstance(t, torch.Tensor) else type(t).__name__})")
 
 
+def _strides3(t):
+    # a dimension of size 1 has no stride that matters: give it one the library takes
+    return (ctypes.c_longlong * 3)(*(st if n > 1 else t.shape[3] for st, n in zip(t.stride()[:3], t.shape[:3])))
+
+
 def _dense_lens(kv_lens: Optional[torch.Tensor], b: int, device: torch.device, stream) -> Optional[torch.Tensor]:
     """Key lengths as the kernels index them, one int32 after the other: a view with other strides (every second length, one
     length expanded to all) is copied on the stream that reads it."""
@@ -247,6 +258,8 @@ def attn_fwd(
     lse: Optional[torch.Tensor] = None,
     stream: Optional[torch.cuda.Stream] = None,
     kv_lens: Optional[torch.Tensor] = None,
+    window: Optional[int] = None,
+    sinks: int = 0,
 ) -> Tuple[torch.Tensor, torch.Tensor]:
     """O = softmax(scale q k^T) v and L = logsumexp(scale q k^T) on the GPU.
 
@@ -256,10 +269,13 @@ def attn_fwd(
     (default: torch's current stream). `kv_lens` (int32 [B]) restricts batch element b to its first kv_lens[b]
     keys, the reference's key_padding_mask (base.py:97-103). With `causal`, query row r sees keys up to
     r + (kv_len_b - N): the mask is aligned to the last query and the last kept key as in base.py:104-116; a row
-    that sees no key gets O = 0 and L = -inf.
+    that sees no key gets O = 0 and L = -inf. With `causal`, `window` leaves a row the last `window` of those keys (its own
+    among them) and the first `sinks` of all.
     """
+    _check_window(window, sinks, causal)
     if stream is None:
-        r = _front().attn_fwd(q, k, v, bool(causal), softmax_scale, out, lse, kv_lens)
+        r = (_front().attn_fwd(q, k, v, bool(causal), softmax_scale, out, lse, kv_lens) if window is None else
+             _front().attn_fwd(q, k, v, bool(causal), softmax_scale, out, lse, kv_lens, window, sinks))
         if r is not None:
             return _done(r, "hk_attn_fwd")
     strided = not (q.is_contiguous() and k.is_contiguous() and v.is_contiguous())
@@ -289,7 +305,14 @@ def attn_fwd(
         raise RuntimeError("lse must be a contiguous fp32 tensor [B, H, 1, N]")
     _require_same_device(q, k=k, v=v, out=out, lse=lse)
     s = stream if stream is not None else torch.cuda.current_stream(q.device)
-    if kv_lens is not None or nk != n:
+    if window is not None:
+        kv_lens = _dense_lens(kv_lens, b, q.device, s)
+        arr = _strides3
+        rc = capi().hk_attn_fwd_window(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
+                                       b, n, nk, h, hkv, d, arr(q), arr(k), arr(v),
+                                       kv_lens.data_ptr() if kv_lens is not None else None, window, sinks,
+                                       float(softmax_scale or 0.0), q.device.index, s.cuda_stream)
+    elif kv_lens is not None or nk != n:
         kv_lens = _dense_lens(kv_lens, b, q.device, s)
         arr = lambda t: (ctypes.c_longlong * 3)(*t.stride()[:3])  # noqa: E731
         rc = capi().hk_attn_fwd_cross(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
@@ -569,11 +592,6 @@ def _qkn_check(q, k, q_weight, k_weight, cos, sin, positions, pos_offset, eps):
     return flags
 
 
-def _qkn_strides(t):
-    # a dimension of size 1 has no stride that matters: give it one the library takes
-    return (ctypes.c_longlong * 3)(*(st if n > 1 else t.shape[3] for st, n in zip(t.stride()[:3], t.shape[:3])))
-
-
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -620,7 +638,7 @@ def qk_norm_rotary(
     s = stream if stream is not None else torch.cuda.current_stream(q.device)
     _check(capi().hk_qk_norm_rotary(q.data_ptr(), k.data_ptr(), _ptr(q_weight), _ptr(k_weight), cos.data_ptr(), sin.data_ptr(),
                                     outs[0].data_ptr(), outs[1].data_ptr(), b, n, h, k.shape[2], d, 2 * cos.shape[1],
-                                    cos.shape[0], _qkn_strides(q), _qkn_strides(k), _ptr(positions), int(pos_offset), float(eps),
+                                    cos.shape[0], _strides3(q), _strides3(k), _ptr(positions), int(pos_offset), float(eps),
                                     flags | (HK_QKN_INTERLEAVED if interleaved else 0), q.device.index, s.cuda_stream),
            "hk_qk_norm_rotary")
     return outs[0], outs[1]
@@ -663,8 +681,8 @@ def qk_norm_rotary_bwd(
         ws = torch.empty(need, dtype=torch.uint8, device=q.device) if any(w is not None for w in dws) else None
     _check(capi().hk_qk_norm_rotary_bwd(q.data_ptr(), k.data_ptr(), _ptr(q_weight), _ptr(k_weight), cos.data_ptr(), sin.data_ptr(),
                                         dq_out.data_ptr(), dk_out.data_ptr(), dq.data_ptr(), dk.data_ptr(), _ptr(dws[0]),
-                                        _ptr(dws[1]), b, n, h, k.shape[2], d, 2 * cos.shape[1], cos.shape[0], _qkn_strides(q),
-                                        _qkn_strides(k), _ptr(positions), int(pos_offset), float(eps),
+                                        _ptr(dws[1]), b, n, h, k.shape[2], d, 2 * cos.shape[1], cos.shape[0], _strides3(q),
+                                        _strides3(k), _ptr(positions), int(pos_offset), float(eps),
                                         flags | (HK_QKN_INTERLEAVED if interleaved else 0), _ptr(ws), need, q.device.index,
                                         s.cuda_stream), "hk_qk_norm_rotary_bwd")
     return dq, dk, dws[0], dws[1]
@@ -779,12 +797,19 @@ def attn_fwd_paged(
     out: Optional[torch.Tensor] = None,
     lse: Optional[torch.Tensor] = None,
     stream: Optional[torch.cuda.Stream] = None,
+    window: Optional[int] = None,
+    sinks: int = 0,
 ) -> Tuple[torch.Tensor, torch.Tensor]:
     """Chunked prefill against the paged KV cache: q [S,T,H,D] bf16 (the last T tokens of each context when `causal`),
     pages [P,16,H_KV,D] bf16, block_table [S,max_pages] int32, ctx_lens [S] int32 -> O [S,T,H,D] bf16,
-    L [S,H,1,T] fp32. The chunk's keys must already be in the cache (`paged_kv_append` first)."""
+    L [S,H,1,T] fp32. The chunk's keys must already be in the cache (`paged_kv_append` first). `window` and `sinks` as in `attn_fwd`; pages that no row of the chunk
+    sees a key of are not looked up."""
+    _check_window(window, sinks, causal)
     if stream is None:
-        r = _front().attn_fwd_paged(q, k_pages, v_pages, block_table, ctx_lens, bool(causal), softmax_scale, out, lse)
+        r = (_front().attn_fwd_paged(q, k_pages, v_pages, block_table, ctx_lens, bool(causal), softmax_scale, out, lse)
+             if window is None else
+             _front().attn_fwd_paged(q, k_pages, v_pages, block_table, ctx_lens, bool(causal), softmax_scale, out, lse, window,
+                                     sinks))
         if r is not None:
             return _done(r, "hk_attn_fwd_paged")
     for name, t in (("q", q), ("k_pages", k_pages), ("v_pages", v_pages)):
@@ -812,6 +837,12 @@ def attn_fwd_paged(
     _require_same_device(q, k_pages=k_pages, v_pages=v_pages, block_table=block_table, ctx_lens=ctx_lens, out=out,
                          lse=lse)
     st = stream if stream is not None else torch.cuda.current_stream(q.device)
+    if window is not None:
+        _check(capi().hk_attn_fwd_paged_window(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(),
+                                               ctx_lens.data_ptr(), out.data_ptr(), lse.data_ptr(), s_n, t_n, h, hkv, d, page,
+                                               block_table.shape[1], p_n, window, sinks, float(softmax_scale or 0.0),
+                                               q.device.index, st.cuda_stream), "hk_attn_fwd_paged_window")
+        return out, lse
     rc = capi().hk_attn_fwd_paged(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(),
                                   ctx_lens.data_ptr(), out.data_ptr(), lse.data_ptr(), s_n, t_n, h, hkv, d, page,
                                   block_table.shape[1], p_n, int(bool(causal)), float(softmax_scale or 0.0),

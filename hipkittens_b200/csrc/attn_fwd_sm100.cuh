@@ -80,6 +80,9 @@ constexpr uint64_t kWaitLimitCycles = 8000ull * 1000 * 1000;  // SM cycles, > 4 
 // Device status codes written to FwdParams::status (0 = OK).
 enum : int { kStatusOk = 0, kStatusTimeout = 1, kStatusFwdBadPage = 2 };  // 2 = the decode kernels' kStatusBadPage
 
+// What a query row sees: every key, those up to its own position, or of those the last `window` and the first `sinks`.
+enum Mask : int { kMaskNone = 0, kMaskCausal = 1, kMaskWindow = 2 };
+
 // Division of a non-negative int below 2^31 by a divisor fixed at launch: a multiply-high and a shift instead of the
 // ~40 dependent instructions of a 32-bit division. The work-item decode below divides ten times per item, on the
 // critical path of the MMA issuer and of the softmax warps between two items (1 600 clocks per item before).
@@ -135,6 +138,7 @@ struct FwdParams {
   // the pools as [num_pages * 16 rows, H_KV, D] with a 16-row box, and NK = max_pages * 16.
   const int* block_table;
   int max_pages, num_pages;
+  int window, sinks;    // kMaskWindow: the query at position p sees the keys c <= p with p - c < window or c < sinks
   int* status;          // device word: first non-zero status wins
 #ifdef HK_TRACE
   long long* trace;     // [3 roles][4096] clock stamps of CTA 0 (debug builds only)
@@ -163,22 +167,37 @@ struct WorkItem {
   int qb[2];
   int n[2];  // KV tiles each slot consumes (0 = slot unused)
 };
+// With a window the tiles are those of the sinks and then, `skip` tiles further on, those from the first that a row of the
+// item has in its window. The slots share the list: with two query tiles the second one's first may be masked throughout.
+struct WindowItem : WorkItem {
+  int sink_tiles, skip;
+  int first_key;  // of the item's windows
+};
+template <int MASK>
+using ItemOf = std::conditional_t<MASK == kMaskWindow, WindowItem, WorkItem>;
+// The tile of keys at place j of a slot's list.
+__device__ __forceinline__ int kv_tile(const WorkItem&, int j) { return j; }
+__device__ __forceinline__ int kv_tile(const WindowItem& w, int j) { return j >= w.sink_tiles ? j + w.skip : j; }
+__device__ __forceinline__ int first_key(const WorkItem&) { return 0; }
+__device__ __forceinline__ int first_key(const WindowItem& w) { return w.first_key; }
 
 // Work-item order. Non-causal: (batch, kv head) outermost so one unit's K/V stay in L2 while all of
 // its query tiles stream through. Causal: units are swept in groups whose K/V fit in L2 together; inside
 // a group the longest rows come first (q block descending), with the slot pairs that share a K/V prefix
 // adjacent. (One sweep over all units at once keeps every unit's K/V live at the same time - 128 MB at
-// N = 8192 - and was measured to re-read K/V from HBM 2.6 times over.)
-template <bool CAUSAL>
-__device__ __forceinline__ WorkItem decode_item(const FwdParams& p, int idx) {
-  WorkItem w;
+// N = 8192 - and was measured to re-read K/V from HBM 2.6 times over.) With a window all but the first rows have as many
+// keys, and neighbouring query tiles share most of them: the order is that without a mask.
+template <int MASK>
+__device__ __forceinline__ ItemOf<MASK> decode_item(const FwdParams& p, int idx) {
+  constexpr bool CAUSAL = MASK != kMaskNone;
+  ItemOf<MASK> w;
   const int G = p.G;
   const int NQB = p.nqb;  // the last block may be partial
   // an item is (unit, q position, pair inside the group); a q position is a q tile (two heads per item) or a pair
   // of q tiles (one head per item), of which there are nq per unit
   const int nq = p.pair_heads ? NQB : (NQB + 1) / 2;
   int unit, qx, hx;
-  if (CAUSAL) {
+  if (MASK == kMaskCausal) {
     const int grp = min(p.fd_group_items.div(idx), p.last_group);
     const int within = idx - grp * p.group_items;
     int qd, rem;
@@ -217,6 +236,15 @@ __device__ __forceinline__ WorkItem decode_item(const FwdParams& p, int idx) {
   auto causal_tiles = [&](int qb) { return min(max((qb * kBlockM + kBlockM + w.off + kBlockN - 1) / kBlockN, 0), n_kv); };
   w.n[0] = CAUSAL ? causal_tiles(qb0) : n_kv;
   w.n[1] = (qb1 < NQB) ? (CAUSAL ? causal_tiles(qb1) : n_kv) : 0;
+  if constexpr (MASK == kMaskWindow) {
+    // keys below a row's window are below its position too: whole tiles of them are behind the causal limit of every row
+    w.first_key = max(qb0 * kBlockM + w.off - p.window + 1, 0);
+    const int lo = w.first_key / kBlockN;
+    w.sink_tiles = min((p.sinks + kBlockN - 1) / kBlockN, lo);
+    w.skip = lo - w.sink_tiles;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) w.n[s] = max(w.n[s] - w.skip, 0);
+  }
   return w;
 }
 
@@ -278,16 +306,17 @@ inline void set_item_decode(FwdParams& p) {
 // -> without): B16 N4096 H16 D64 1317.0 -> 1309.4, B4 N8192 H64/8 D128 causal 3414 -> 3407, B8 N4096 H32/8 D64 causal
 // 0.3 % less; but B16 N2048 H64/8 D128 1718.6 -> 1722.4, which therefore keeps them. A run-time branch around them is
 // no way out: it costs D128 0.5 %.
-template <int D, bool CAUSAL>
-constexpr bool kLongFwdDependent = D == 128 && !CAUSAL;
+template <int D, int MASK>
+constexpr bool kLongFwdDependent = D == 128 && MASK == kMaskNone;
 
 // DEP: may be launched as a dependent (launch_dependent with `early`); false: only the ordinary way.
-template <int D, bool CAUSAL, bool DEP>
+template <int D, int MASK, bool DEP>
 __global__ void __launch_bounds__(kFwdThreads, 1)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                 const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_o,
                 const FwdParams p) {
   using namespace ptx;
+  constexpr bool CAUSAL = MASK != kMaskNone, WINDOW = MASK == kMaskWindow;
   using SM = FwdSmem<D, CAUSAL>;
   constexpr int kStages = SM::kStages;
   constexpr int kTile = SM::kTileBytes;
@@ -305,7 +334,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
   constexpr int kOtherRegs = (D == 64 && !CAUSAL) ? 72 : 88;
   static_assert(8 * kSoftmaxRegs + 4 * kOtherRegs == 12 * kFwdRegsAtLaunch, "registers taken = registers released");
   constexpr int kEmuMod = (D == 64 && !CAUSAL) ? HK_EMU_MOD_D64_NONCAUSAL : HK_EMU_MOD;
-  constexpr int kEmuCnt = (D == 64) ? (CAUSAL ? HK_EMU_CNT_D64 : HK_EMU_CNT_D64_NONCAUSAL) : HK_EMU_CNT_D128;
+  constexpr int kEmuCnt = WINDOW ? 0 : (D == 64) ? (CAUSAL ? HK_EMU_CNT_D64 : HK_EMU_CNT_D64_NONCAUSAL) : HK_EMU_CNT_D128;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -393,7 +422,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
       if (round >= p.total_rounds) break;
       const int idx = item_for_round(p, round, blockIdx.x, gridDim.x);
       if (idx < 0) continue;  // a partial round leaves some CTAs without an item
-      const WorkItem w = decode_item<CAUSAL>(p, idx);
+      const ItemOf<MASK> w = decode_item<MASK>(p, idx);
       const int nkv = w.n[slot];
       // causal: the last key this thread's row sees, and the first tile the diagonal (or the end of the keys) runs
       // through - the last one, and the one before it when off is not a multiple of the tile. Key j*128 + i is
@@ -402,6 +431,16 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
       // fixed for the item, so the per-tile test is one comparison.
       const int row_last_key = min(w.qb[slot] * kBlockM + row + w.off, w.kv_len - 1);
       const int j_mask = (min(w.qb[slot] * kBlockM + w.off, w.kv_len - 1) + 1) >> 7;
+      // window: the row's first key, and masks for the tiles that some row of the block does not see whole
+      [[maybe_unused]] const int row_first_key = w.qb[slot] * kBlockM + row + w.off - p.window + 1;
+      [[maybe_unused]] auto window_mask = [&](uint32_t* su, int j) {
+        const int t = kv_tile(w, j);
+        if (t < j_mask && (t * kBlockN > w.qb[slot] * kBlockM + kBlockM - 1 + w.off - p.window ||
+                           (t + 1) * kBlockN <= p.sinks)) return;  // CTA-uniform
+        const int hi = row_last_key - t * kBlockN, lo = row_first_key - t * kBlockN, sinks = p.sinks - t * kBlockN;
+#pragma unroll
+        for (int i = 0; i < kBlockN; ++i) su[i] = (i > hi || (i < lo && i >= sinks)) ? 0xff800000u : su[i];
+      };
       if (nkv == 0) {
         if (CAUSAL && w.qb[slot] * kBlockM < p.N) {
           // a query block that sees no key at all (more queries than keys): defined output, no products
@@ -437,7 +476,9 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
             __syncwarp();
             if (lane == 0) mbar_arrive(&s_free[slot]);
           }
-          if (CAUSAL && j >= j_mask) {
+          if (WINDOW) {
+            window_mask(su, j);
+          } else if (CAUSAL && j >= j_mask) {
             const int lim = row_last_key - j * kBlockN;
 #pragma unroll
             for (int i = 0; i < kBlockN; ++i) su[i] = (i > lim) ? 0xff800000u : su[i];
@@ -518,7 +559,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
             unpack2(lacc1, b0, b1);
             return (a0 + a1) + (b0 + b1);
           };
-          bool exact = j == 0 || (CAUSAL && w.off < 0 && __any_sync(0xffffffffu, m == -INFINITY));
+          bool exact = j == 0 || (CAUSAL && (WINDOW || w.off < 0) && __any_sync(0xffffffffu, m == -INFINITY));
           float bm_first = 0.f;
           if (exact) bm_first = row_max();
           if (kSepP && pv_cnt > 0) {
@@ -556,7 +597,9 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
 #pragma unroll
             for (int cc = 0; cc < 4; ++cc) tmem_ld32(tS + cc * 32, su + cc * 32);
             tmem_wait_ld();
-            if (CAUSAL && j >= j_mask) {
+            if (WINDOW) {
+              window_mask(su, j);
+            } else if (CAUSAL && j >= j_mask) {
               const int lim = row_last_key - j * kBlockN;
 #pragma unroll
               for (int i = 0; i < kBlockN; ++i) su[i] = (i > lim) ? 0xff800000u : su[i];
@@ -572,7 +615,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
           HK_STAMP2(slot, 2);
           // the first tile fixes m; so does any tile of a row that has not seen a key yet (only possible with more
           // queries than kept keys, off < 0)
-          bool exact = j == 0 || (CAUSAL && w.off < 0 && __any_sync(0xffffffffu, m == -INFINITY));
+          bool exact = j == 0 || (CAUSAL && (WINDOW || w.off < 0) && __any_sync(0xffffffffu, m == -INFINITY));
           uint32_t pk[kBlockN / 2];
           float l_tile;
           for (;;) {
@@ -788,7 +831,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
         int ring_st = 0;        // next ring stage to fill
         uint32_t ring_par = 0;  // its phase parity
         bool ok = true;
-        auto push_kv = [&](const CUtensorMap* tm, int b, int kvh, int tile, int kv_len) -> bool {
+        auto push_kv = [&](const CUtensorMap* tm, int b, int kvh, int tile, int kv_len, [[maybe_unused]] int first_key) -> bool {
           const int st = ring_st;
           bool good = true;
           if (lane == 0) {
@@ -807,8 +850,13 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
             // repeat its last page, so that every row of the tile holds cache contents (those keys are masked; their
             // V rows meet p = 0). An id outside the pool is reported and replaced, never dereferenced.
             const int total_pages = (kv_len + 15) >> 4;
-            int id = p.block_table[static_cast<size_t>(b) * p.max_pages +
-                                   min(tile * (kBlockN / 16) + lane, total_pages - 1)];
+            int page = min(tile * (kBlockN / 16) + lane, total_pages - 1);
+            if (WINDOW) {
+              // nor are pages between the sinks and the windows looked up, which may have been given away
+              const int last_sink = (p.sinks + 15) / 16 - 1, first = first_key / 16;
+              if (page > last_sink) page = tile * kBlockN + kBlockN > first_key ? max(page, first) : max(last_sink, 0);
+            }
+            int id = p.block_table[static_cast<size_t>(b) * p.max_pages + page];
             if (id < 0 || id >= p.num_pages) {
               atomicCAS(p.status, kStatusOk, kStatusFwdBadPage);
               id = 0;
@@ -827,11 +875,11 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
           if (round >= p.total_rounds) break;
           const int idx = item_for_round(p, round, blockIdx.x, gridDim.x);
           if (idx < 0) continue;
-          const WorkItem w = decode_item<CAUSAL>(p, idx);
+          const ItemOf<MASK> w = decode_item<MASK>(p, idx);
           const int nmax = max(w.n[0], w.n[1]);
           // the first K tile is requested before the Q tiles: the stage it goes to is free two K/V tiles before the
           // previous item ends, the Q tiles only when that item's last Q K^T has been issued
-          if (nmax > 0) ok = push_kv(&tmap_k, w.b, w.kvh, 0, w.kv_len);
+          if (nmax > 0) ok = push_kv(&tmap_k, w.b, w.kvh, kv_tile(w, 0), w.kv_len, first_key(w));
           if (!kQThread && lane == 0 && ok) {
             for (int s = 0; s < 2 && ok; ++s) {
               if (w.n[s] == 0) continue;
@@ -847,8 +895,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
           }
           if (kPaged) ok = __shfl_sync(0xffffffffu, ok, 0);
           for (int j = 0; j < nmax && ok; ++j) {
-            ok = push_kv(&tmap_v, w.b, w.kvh, j, w.kv_len);
-            if (ok && j + 1 < nmax) ok = push_kv(&tmap_k, w.b, w.kvh, j + 1, w.kv_len);
+            ok = push_kv(&tmap_v, w.b, w.kvh, kv_tile(w, j), w.kv_len, first_key(w));
+            if (ok && j + 1 < nmax) ok = push_kv(&tmap_k, w.b, w.kvh, kv_tile(w, j + 1), w.kv_len, first_key(w));
           }
         }
       };
@@ -874,7 +922,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
         if (round >= p.total_rounds) break;
         const int idx = item_for_round(p, round, blockIdx.x, gridDim.x);
         if (idx < 0) continue;
-        const WorkItem w = decode_item<CAUSAL>(p, idx);
+        const ItemOf<MASK> w = decode_item<MASK>(p, idx);
         const int nmax = max(w.n[0], w.n[1]);
         for (int j = 0; j < nmax && ok; ++j) {
           const int st = static_cast<int>(pos % kStages);
@@ -999,13 +1047,13 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
       };
       int idx = -1, nidx = -1;
       int round = next_round(0, idx), nround = 0;
-      WorkItem w, wn;
-      if (idx >= 0) w = decode_item<CAUSAL>(p, idx);
+      ItemOf<MASK> w, wn;
+      if (idx >= 0) w = decode_item<MASK>(p, idx);
       for (; ok && round < p.total_rounds; round = nround, w = wn) {
         // the item after this one, for the early issue of its first products
         nround = next_round(round + 1, nidx);
         wn.n[0] = wn.n[1] = 0;
-        if (nidx >= 0) wn = decode_item<CAUSAL>(p, nidx);
+        if (nidx >= 0) wn = decode_item<MASK>(p, nidx);
         const int n0 = w.n[0], n1 = w.n[1];
         const int nmax = max(n0, n1);
         if (nmax == 0) continue;  // causal with more queries than keys: neither block sees a key
@@ -1117,7 +1165,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
         if (round >= p.total_rounds) break;
         const int idx = item_for_round(p, round, blockIdx.x, gridDim.x);
         if (idx < 0) continue;
-        const WorkItem w = decode_item<CAUSAL>(p, idx);
+        const ItemOf<MASK> w = decode_item<MASK>(p, idx);
         if (w.n[0] > 0) {
           ok = mbar_wait(&q_empty[0], (q_cnt0 & 1) ^ 1, abortp, kWaitLimitCycles);
           if (!ok) break;
@@ -1148,7 +1196,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
         if (round >= p.total_rounds) break;
         const int idx = item_for_round(p, round, blockIdx.x, gridDim.x);
         if (idx < 0) continue;
-        const WorkItem w = decode_item<CAUSAL>(p, idx);
+        const ItemOf<MASK> w = decode_item<MASK>(p, idx);
         const int first = (w.n[1] < w.n[0]) ? 1 : 0;
         for (int t = 0; t < 2 && ok; ++t) {
           const int s = t == 0 ? first : 1 - first;

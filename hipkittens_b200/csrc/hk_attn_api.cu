@@ -66,10 +66,10 @@ struct DeviceState {
 };
 DeviceState g_dev[kMaxDevices];
 
-template <int D, bool CAUSAL, bool DEP>
+template <int D, int MASK, bool DEP>
 int prepare_fwd_kernel() {
-  auto* fn = hk::attn_fwd_kernel<D, CAUSAL, DEP>;
-  HK_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, hk::FwdSmem<D, CAUSAL>::kDynBytes));
+  auto* fn = hk::attn_fwd_kernel<D, MASK, DEP>;
+  HK_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, hk::FwdSmem<D, MASK != hk::kMaskNone>::kDynBytes));
   cudaFuncAttributes attr;
   HK_CUDA(cudaFuncGetAttributes(&attr, fn));
   // The kernel re-balances registers between warpgroups (208 per softmax thread, 88 per producer thread);
@@ -77,17 +77,17 @@ int prepare_fwd_kernel() {
   // Refuse to launch otherwise: a register pool that is too small would block the re-allocation forever.
   if (attr.numRegs != hk::kFwdRegsAtLaunch) {
     snprintf(g_cuda_err, sizeof(g_cuda_err), "attn_fwd_kernel<%d,%d,%d> compiled to %d registers, expected %d", D,
-             int(CAUSAL), int(DEP), attr.numRegs, hk::kFwdRegsAtLaunch);
+             MASK, int(DEP), attr.numRegs, hk::kFwdRegsAtLaunch);
     return HK_EUNSUPPORTED;
   }
   return HK_OK;
 }
 
-template <int D, bool CAUSAL>
+template <int D, int MASK>
 int prepare_fwd_kernels() {
-  const int rc = prepare_fwd_kernel<D, CAUSAL, true>();
+  const int rc = prepare_fwd_kernel<D, MASK, true>();
   if (rc != HK_OK) return rc;
-  return prepare_fwd_kernel<D, CAUSAL, hk::kLongFwdDependent<D, CAUSAL>>();
+  return prepare_fwd_kernel<D, MASK, hk::kLongFwdDependent<D, MASK>>();
 }
 
 template <typename Kernel>
@@ -129,10 +129,12 @@ int init_device(int device) {
     return HK_EUNSUPPORTED;
   }
   int rc;
-  if ((rc = prepare_fwd_kernels<128, false>()) != HK_OK) return rc;
-  if ((rc = prepare_fwd_kernels<128, true>()) != HK_OK) return rc;
-  if ((rc = prepare_fwd_kernels<64, false>()) != HK_OK) return rc;
-  if ((rc = prepare_fwd_kernels<64, true>()) != HK_OK) return rc;
+  if ((rc = prepare_fwd_kernels<128, hk::kMaskNone>()) != HK_OK) return rc;
+  if ((rc = prepare_fwd_kernels<128, hk::kMaskCausal>()) != HK_OK) return rc;
+  if ((rc = prepare_fwd_kernels<128, hk::kMaskWindow>()) != HK_OK) return rc;
+  if ((rc = prepare_fwd_kernels<64, hk::kMaskNone>()) != HK_OK) return rc;
+  if ((rc = prepare_fwd_kernels<64, hk::kMaskCausal>()) != HK_OK) return rc;
+  if ((rc = prepare_fwd_kernels<64, hk::kMaskWindow>()) != HK_OK) return rc;
   if ((rc = hk::prepare_decode_kernels(g_cuda_err, sizeof(g_cuda_err), st.sm_count, &st.decode)) != HK_OK) return rc;
   if ((rc = hk::prepare_window_decode_kernels(g_cuda_err, sizeof(g_cuda_err))) != HK_OK) return rc;
   if ((rc = prepare_bwd_kernels<128, false>()) != HK_OK) return rc;
@@ -304,13 +306,20 @@ int group_for_fewest_rounds(long long u, long long units, long long per_unit, lo
   return int(u);
 }
 
-template <int D, bool CAUSAL>
+// The most tiles of keys that a query tile meets, two of them together with a window.
+int kv_tiles(int NK, int mask, int window, int sinks) {
+  const long long all = (NK + hk::kBlockN - 1ll) / hk::kBlockN;
+  if (mask != hk::kMaskWindow) return int(all);
+  const long long live = (2ll * hk::kBlockM + window + hk::kBlockN - 1) / hk::kBlockN + (1ll * sinks + hk::kBlockN - 1) / hk::kBlockN;
+  return int(std::min(all, live));
+}
+
+template <int D, int MASK>
 int launch_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& to,
                const hk::FwdParams& p, int grid, cudaStream_t stream) {
-  const int nk_tiles = (p.NK + hk::kBlockN - 1) / hk::kBlockN;
-  const bool early = short_kernel(1ll * p.n_items * nk_tiles, grid);
-  auto* fn = early ? hk::attn_fwd_kernel<D, CAUSAL, true> : hk::attn_fwd_kernel<D, CAUSAL, hk::kLongFwdDependent<D, CAUSAL>>;
-  HK_CUDA(hk::launch_dependent(early, fn, grid, hk::kFwdThreads, hk::FwdSmem<D, CAUSAL>::kDynBytes, stream, tq, tk, tv, to, p));
+  const bool early = short_kernel(1ll * p.n_items * kv_tiles(p.NK, MASK, p.window, p.sinks), grid);
+  auto* fn = early ? hk::attn_fwd_kernel<D, MASK, true> : hk::attn_fwd_kernel<D, MASK, hk::kLongFwdDependent<D, MASK>>;
+  HK_CUDA(hk::launch_dependent(early, fn, grid, hk::kFwdThreads, hk::FwdSmem<D, MASK != hk::kMaskNone>::kDynBytes, stream, tq, tk, tv, to, p));
   g_launches.fetch_add(1, std::memory_order_relaxed);
   return HK_OK;
 }
@@ -607,7 +616,10 @@ int hk_attn_fwd_varlen(const void* q, const void* k, const void* v, void* o, flo
 static int fwd_launch(const void* q, const void* k, const void* v, void* o, float* lse, int B, int N, int NK, int H,
                       int H_KV, int D, const long long* q_strides, const long long* k_strides,
                       const long long* v_strides, const int32_t* kv_lens, const int32_t* block_table, int max_pages,
-                      int num_pages, int causal, float softmax_scale, int device, void* cuda_stream) {
+                      int num_pages, int mask, int window, int sinks, float softmax_scale, int device, void* cuda_stream) {
+  // a window that no key lies behind masks nothing that the causal mask does not
+  if (mask == hk::kMaskWindow && (window >= NK || sinks >= NK)) mask = hk::kMaskCausal;
+  const bool causal = mask == hk::kMaskCausal;
   DeviceState* st = nullptr;
   DeviceScope scope;
   int rc = scope.enter(device, &st);
@@ -665,6 +677,8 @@ static int fwd_launch(const void* q, const void* k, const void* v, void* o, floa
   p.block_table = block_table;
   p.max_pages = max_pages;
   p.num_pages = num_pages;
+  p.window = mask == hk::kMaskWindow ? window : 0;
+  p.sinks = mask == hk::kMaskWindow ? sinks : 0;
   p.status = st->status;
 #ifdef HK_TRACE
   p.trace = g_trace_buf;
@@ -680,16 +694,17 @@ static int fwd_launch(const void* q, const void* k, const void* v, void* o, floa
   }
   hk::set_item_decode(p);
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
-  if (D == 128) return causal ? launch_fwd<128, true>(tq, tk, tv, to, p, grid, stream)
-                              : launch_fwd<128, false>(tq, tk, tv, to, p, grid, stream);
-  return causal ? launch_fwd<64, true>(tq, tk, tv, to, p, grid, stream)
-                : launch_fwd<64, false>(tq, tk, tv, to, p, grid, stream);
+  const bool d128 = D == 128;
+  auto* launch = mask == hk::kMaskWindow   ? (d128 ? launch_fwd<128, hk::kMaskWindow> : launch_fwd<64, hk::kMaskWindow>)
+                 : mask == hk::kMaskCausal ? (d128 ? launch_fwd<128, hk::kMaskCausal> : launch_fwd<64, hk::kMaskCausal>)
+                                           : (d128 ? launch_fwd<128, hk::kMaskNone> : launch_fwd<64, hk::kMaskNone>);
+  return launch(tq, tk, tv, to, p, grid, stream);
 }
 
-int hk_attn_fwd_cross(const void* q, const void* k, const void* v, void* o, float* lse, int B, int N, int NK, int H,
-                      int H_KV, int D, const long long* q_strides, const long long* k_strides,
-                      const long long* v_strides, const int32_t* kv_lens, int causal, float softmax_scale,
-                      int device, void* cuda_stream) {
+static int fwd_contiguous(const void* q, const void* k, const void* v, void* o, float* lse, int B, int N, int NK, int H,
+                          int H_KV, int D, const long long* q_strides, const long long* k_strides,
+                          const long long* v_strides, const int32_t* kv_lens, int mask, int window, int sinks,
+                          float softmax_scale, int device, void* cuda_stream) {
   if (!q || !k || !v || !o || !lse || !q_strides || !k_strides || !v_strides) return HK_EINVAL;
   if (B <= 0 || N <= 0 || NK <= 0 || H <= 0 || H_KV <= 0) return HK_EINVAL;
   if (D != 64 && D != 128) return HK_EUNSUPPORTED;
@@ -702,13 +717,30 @@ int hk_attn_fwd_cross(const void* q, const void* k, const void* v, void* o, floa
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || (reinterpret_cast<uintptr_t>(lse) & 3))
     return HK_EINVAL;
   return fwd_launch(q, k, v, o, lse, B, N, NK, H, H_KV, D, q_strides, k_strides, v_strides, kv_lens, nullptr, 0, 0,
-                    causal, softmax_scale, device, cuda_stream);
+                    mask, window, sinks, softmax_scale, device, cuda_stream);
 }
 
-int hk_attn_fwd_paged(const void* q, const void* k_pages, const void* v_pages, const int32_t* block_table,
-                      const int32_t* ctx_lens, void* o, float* lse, int S, int T, int H, int H_KV, int D,
-                      int page_size, int max_pages_per_seq, int num_pages, int causal, float softmax_scale,
+int hk_attn_fwd_cross(const void* q, const void* k, const void* v, void* o, float* lse, int B, int N, int NK, int H,
+                      int H_KV, int D, const long long* q_strides, const long long* k_strides,
+                      const long long* v_strides, const int32_t* kv_lens, int causal, float softmax_scale,
                       int device, void* cuda_stream) {
+  return fwd_contiguous(q, k, v, o, lse, B, N, NK, H, H_KV, D, q_strides, k_strides, v_strides, kv_lens,
+                        causal ? hk::kMaskCausal : hk::kMaskNone, 0, 0, softmax_scale, device, cuda_stream);
+}
+
+int hk_attn_fwd_window(const void* q, const void* k, const void* v, void* o, float* lse, int B, int N, int NK, int H,
+                       int H_KV, int D, const long long* q_strides, const long long* k_strides,
+                       const long long* v_strides, const int32_t* kv_lens, int window, int sinks, float softmax_scale,
+                       int device, void* cuda_stream) {
+  if (window <= 0 || sinks < 0) return HK_EINVAL;
+  return fwd_contiguous(q, k, v, o, lse, B, N, NK, H, H_KV, D, q_strides, k_strides, v_strides, kv_lens, hk::kMaskWindow,
+                        window, sinks, softmax_scale, device, cuda_stream);
+}
+
+static int fwd_paged(const void* q, const void* k_pages, const void* v_pages, const int32_t* block_table,
+                     const int32_t* ctx_lens, void* o, float* lse, int S, int T, int H, int H_KV, int D,
+                     int page_size, int max_pages_per_seq, int num_pages, int mask, int window, int sinks,
+                     float softmax_scale, int device, void* cuda_stream) {
   if (!q || !k_pages || !v_pages || !block_table || !ctx_lens || !o || !lse) return HK_EINVAL;
   if (S <= 0 || T <= 0 || H <= 0 || H_KV <= 0 || max_pages_per_seq <= 0 || num_pages <= 0) return HK_EINVAL;
   if ((D != 64 && D != 128) || page_size != 16) return HK_EUNSUPPORTED;
@@ -720,7 +752,24 @@ int hk_attn_fwd_paged(const void* q, const void* k_pages, const void* v_pages, c
     return HK_EINVAL;
   const long long qs[3] = {(long long)T * H * D, (long long)H * D, D};
   return fwd_launch(q, k_pages, v_pages, o, lse, S, T, max_pages_per_seq * 16, H, H_KV, D, qs, qs, qs, ctx_lens,
-                    block_table, max_pages_per_seq, num_pages, causal, softmax_scale, device, cuda_stream);
+                    block_table, max_pages_per_seq, num_pages, mask, window, sinks, softmax_scale, device, cuda_stream);
+}
+
+int hk_attn_fwd_paged(const void* q, const void* k_pages, const void* v_pages, const int32_t* block_table,
+                      const int32_t* ctx_lens, void* o, float* lse, int S, int T, int H, int H_KV, int D,
+                      int page_size, int max_pages_per_seq, int num_pages, int causal, float softmax_scale,
+                      int device, void* cuda_stream) {
+  return fwd_paged(q, k_pages, v_pages, block_table, ctx_lens, o, lse, S, T, H, H_KV, D, page_size, max_pages_per_seq,
+                   num_pages, causal ? hk::kMaskCausal : hk::kMaskNone, 0, 0, softmax_scale, device, cuda_stream);
+}
+
+int hk_attn_fwd_paged_window(const void* q, const void* k_pages, const void* v_pages, const int32_t* block_table,
+                             const int32_t* ctx_lens, void* o, float* lse, int S, int T, int H, int H_KV, int D,
+                             int page_size, int max_pages_per_seq, int num_pages, int window, int sinks,
+                             float softmax_scale, int device, void* cuda_stream) {
+  if (window <= 0 || sinks < 0) return HK_EINVAL;
+  return fwd_paged(q, k_pages, v_pages, block_table, ctx_lens, o, lse, S, T, H, H_KV, D, page_size, max_pages_per_seq,
+                   num_pages, hk::kMaskWindow, window, sinks, softmax_scale, device, cuda_stream);
 }
 
 static int prep_launch(const void* o, const void* d_o, float* delta, int B, int N, int H, int D, cudaStream_t stream) {

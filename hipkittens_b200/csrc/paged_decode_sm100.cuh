@@ -149,6 +149,35 @@ inline DecodeShape decode_pick_shape(int S, int H_KV, int max_pages, const Decod
   const int useful = (max_pages + warps - 1) / warps;  // a page per warp
   return {cluster < useful ? cluster : useful, warps};
 }
+// With a window, `span` pages are the most that any context holds, and most contexts of a serving batch hold all of them: a CTA may
+// meet up to 320 (5120 tokens), and what one long context beside short ones loses is bounded by the window (75 us there, in chunks
+// 15). Otherwise as above; a unit of its own has 8 warps while all of them are one wave and 4 from there on.
+// us, chunks of 64 pages / clusters or CTAs of 4 warps (size) / of 8, H64/8 D128 unless said, contexts longer than the window:
+// 64 contexts, window 512 36.0 / 31.2 (1) / 39.2 (1); 2048 100.9 / 88.1 (1) / 96.5 (1); 4096 182 / 164 (1) / 172 (1); 32, 2048 55.0 / 46.7
+// (1) / 48.2 (1); 16, 2048 33.0 / 29.1 (2) / 25.9 (1); 8, 4096 33.2 / 27.3 (4) / 27.7 (2); 8, 1024 21.0 / 12.3 (4) / 12.5 (2); 4, 1024 20.7 / 9.1
+// (8) / 9.1 (4); H32/8, 1 context, 4096 20.4 / 10.2 (16) / 10.4 (8); D = 64, 33 contexts of H48/8, 500 12.7 / 10.3 (1) / 13.5 (1); H64/8,
+// 64 contexts, 2048 61.4 / 51.2 (1) / 56.4 (1). Few units with long windows stay in chunks: H1, 1 context, 32768 17.1 (of 32 pages) /
+// 33.2 (16) / 22.1 (16); H32/8 D = 64, 2 contexts, 16384 18.8 / 19.3 (12) / 19.7 (6).
+inline DecodeShape decode_pick_window_shape(int S, int H_KV, int span, const DecodeLimits& lim) {
+  const long long units = 1ll * S * H_KV;
+  constexpr DecodeShape kChunks{0, 4};
+  constexpr int kMost = 320;
+  int cluster = kMaxCluster, warps = 4;
+  while (cluster > 1 && lim.clusters4[cluster] < units) --cluster;
+  if (cluster < 3) {
+    cluster = 1;
+    warps = units <= lim.sm_count ? 8 : 4;
+    if (span > kMost) return kChunks;
+  } else if (span > 256 && units <= lim.clusters8) {
+    cluster = kMaxCluster;
+    warps = 8;
+    if (span > 64 * cluster) return kChunks;
+  } else if (span > (cluster == kMaxCluster ? 44 : kMost) * cluster) {
+    return kChunks;
+  }
+  const int useful = (span + warps - 1) / warps;  // a page per warp
+  return {cluster < useful ? cluster : useful, warps};
+}
 // Workspace: partial O as fp32 [S][H][splits][128], then (m, l) pairs as fp32 [S][H][splits][2].
 // Shapes the two kernels can be launched for: the combine kernel holds one weight per split in shared memory
 // (kMaxCombineSplits of them, counted for the smaller chunk size so that either chunk choice fits), and sequences
@@ -648,7 +677,7 @@ inline cudaError_t launch_paged_decode(const DecodeParams& p, const DecodeLimits
 // With p.window, p.sinks and p.span_pages set.
 inline cudaError_t launch_window_decode(const DecodeParams& p, int D, const DecodeLimits& lim, cudaStream_t stream,
                                         int* launched) {
-  const DecodeShape shape = decode_pick_shape(p.S, p.H_KV, p.span_pages, lim);
+  const DecodeShape shape = decode_pick_window_shape(p.S, p.H_KV, p.span_pages, lim);
   auto* launch = D == 64 ? launch_decode_shape<64, true> : launch_decode_shape<128, true>;
   return launch(p, shape, p.span_pages, lim.sm_count, stream, launched);
 }

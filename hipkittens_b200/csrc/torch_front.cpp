@@ -89,11 +89,25 @@ bool tma_strides(const Tensor& t, long long* st) {
   return good;
 }
 
-// attn_fwd(q, k, v, causal, softmax_scale, out, lse, kv_lens)
+// A window and its sinks, as the last two arguments; without them, none.
+bool window_args(PyObject* const* a, Py_ssize_t n_args, Py_ssize_t without, int& window, int& sinks) {
+  window = sinks = 0;
+  if (n_args == without) return true;
+  if (n_args != without + 2 || !PyLong_CheckExact(a[without]) || !PyLong_CheckExact(a[without + 1])) return false;
+  int over_w = 0, over_s = 0;
+  const long w = PyLong_AsLongAndOverflow(a[without], &over_w), s = PyLong_AsLongAndOverflow(a[without + 1], &over_s);
+  if (over_w || over_s || w < 1 || s < 0 || !fits({w, s})) return false;
+  window = i32(w), sinks = i32(s);
+  return true;
+}
+
+// attn_fwd(q, k, v, causal, softmax_scale, out, lse, kv_lens[, window, sinks])
 PyObject* attn_fwd(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   HANDLE_TH_ERRORS
   float scale;
-  if (n_args != 8 || !PyBool_Check(a[3]) || !number(a[4], scale)) Py_RETURN_NONE;
+  int window, sinks;
+  if (!window_args(a, n_args, 8, window, sinks) || !PyBool_Check(a[3]) || !number(a[4], scale)) Py_RETURN_NONE;
+  if (window && a[3] != Py_True) Py_RETURN_NONE;
   const Tensor *q = plain(a[0]), *k = plain(a[1]), *v = plain(a[2]);
   for (const Tensor* t : {q, k, v})
     if (!is(t, at::kBFloat16, 4)) Py_RETURN_NONE;
@@ -104,7 +118,7 @@ PyObject* attn_fwd(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   const bool strided = !(q->is_contiguous() && k->is_contiguous() && v->is_contiguous());
   long long qs[3], ks[3], vs[3];
   const bool q_ok = tma_strides(*q, qs), k_ok = tma_strides(*k, ks), v_ok = tma_strides(*v, vs);
-  if (strided && !(q_ok && k_ok && v_ok)) Py_RETURN_NONE;
+  if ((strided || window) && !(q_ok && k_ok && v_ok)) Py_RETURN_NONE;
   const Tensor* lens = nullptr;
   if (a[7] != Py_None) {
     lens = plain(a[7]);
@@ -120,6 +134,9 @@ PyObject* attn_fwd(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   float* lsep = ptr<float>(lse);
   const int32_t* lensp = lens ? ptr<int32_t>(*lens) : nullptr;
   const int rc = unlocked([&] {
+    if (window)
+      return hk_attn_fwd_window(qp, kp, vp, outp, lsep, i32(b), i32(n), i32(nk), i32(h), i32(hkv), i32(d), qs, ks, vs, lensp,
+                                window, sinks, scale, dev, st);
     if (lens || nk != n || strided)
       return hk_attn_fwd_cross(qp, kp, vp, outp, lsep, i32(b), i32(n), i32(nk), i32(h), i32(hkv), i32(d), qs, ks, vs, lensp,
                                causal, scale, dev, st);
@@ -347,18 +364,6 @@ struct Paged {
   }
 };
 
-// A window and its sinks, as the last two arguments; without them, none.
-bool window_args(PyObject* const* a, Py_ssize_t n_args, Py_ssize_t without, int& window, int& sinks) {
-  window = sinks = 0;
-  if (n_args == without) return true;
-  if (n_args != without + 2 || !PyLong_CheckExact(a[without]) || !PyLong_CheckExact(a[without + 1])) return false;
-  int over_w = 0, over_s = 0;
-  const long w = PyLong_AsLongAndOverflow(a[without], &over_w), s = PyLong_AsLongAndOverflow(a[without + 1], &over_s);
-  if (over_w || over_s || w < 1 || s < 0 || !fits({w, s})) return false;
-  window = i32(w), sinks = i32(s);
-  return true;
-}
-
 // paged_decode(q, k_pages, v_pages, block_table, ctx_lens, softmax_scale, out, lse, workspace[, window, sinks])
 PyObject* paged_decode(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   HANDLE_TH_ERRORS
@@ -399,12 +404,14 @@ PyObject* paged_decode(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
-// attn_fwd_paged(q, k_pages, v_pages, block_table, ctx_lens, causal, softmax_scale, out, lse)
+// attn_fwd_paged(q, k_pages, v_pages, block_table, ctx_lens, causal, softmax_scale, out, lse[, window, sinks])
 PyObject* attn_fwd_paged(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   HANDLE_TH_ERRORS
   float scale;
   Paged p;
-  if (n_args != 9 || !PyBool_Check(a[5]) || !number(a[6], scale) || !p.take(a)) Py_RETURN_NONE;
+  int window, sinks;
+  if (!window_args(a, n_args, 9, window, sinks) || !PyBool_Check(a[5]) || !number(a[6], scale) || !p.take(a)) Py_RETURN_NONE;
+  if (window && a[5] != Py_True) Py_RETURN_NONE;
   Tensor out, lse;
   if (!output(a[7], *p.q, p.q->sizes(), at::kBFloat16, out) ||
       !output(a[8], *p.q, {p.s, p.h, 1, p.t}, at::kFloat, lse))
@@ -415,6 +422,10 @@ PyObject* attn_fwd_paged(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   void* outp = ptr(out);
   float* lsep = ptr<float>(lse);
   const int rc = unlocked([&] {
+    if (window)
+      return hk_attn_fwd_paged_window(p.q_ptr, p.k_pages, p.v_pages, p.table_ptr, p.lens_ptr, outp, lsep, i32(p.s), i32(p.t),
+                                      i32(p.h), i32(p.hkv), i32(p.d), i32(p.page), i32(p.max_pages), i32(p.pool), window, sinks,
+                                      scale, p.device, st);
     return hk_attn_fwd_paged(p.q_ptr, p.k_pages, p.v_pages, p.table_ptr, p.lens_ptr, outp, lsep, i32(p.s), i32(p.t),
                              i32(p.h), i32(p.hkv), i32(p.d), i32(p.page), i32(p.max_pages), i32(p.pool), causal, scale,
                              p.device, st);
