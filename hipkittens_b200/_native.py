@@ -33,6 +33,8 @@ EXPORTED_SYMBOLS = (
     "hk_attn_bwd_varlen",
     "hk_attn_bwd_cross",
     "hk_attn_bwd_strided",
+    "hk_attn_bwd_window",
+    "hk_attn_bwd_window_workspace_bytes",
     "hk_key_padding_lens",
     "hk_attn_dq_shuffle",
     "hk_rotary",
@@ -114,6 +116,10 @@ def capi() -> ctypes.CDLL:
     lib.hk_attn_bwd_cross.restype = ci
     lib.hk_attn_bwd_strided.argtypes = [vp] * 10 + [ci] * 6 + [ll3] * 6 + [vp, ci, cf, ci, vp]
     lib.hk_attn_bwd_strided.restype = ci
+    lib.hk_attn_bwd_window.argtypes = [vp] * 10 + [ci] * 6 + [ll3] * 6 + [vp, ci, ci, cf, vp, ctypes.c_size_t, ci, vp]
+    lib.hk_attn_bwd_window.restype = ci
+    lib.hk_attn_bwd_window_workspace_bytes.argtypes = [ci] * 8
+    lib.hk_attn_bwd_window_workspace_bytes.restype = ctypes.c_size_t
     lib.hk_key_padding_lens.argtypes = [vp, vp, vp, ci, ci, ci, vp]
     lib.hk_key_padding_lens.restype = ci
     lib.hk_attn_dq_shuffle.argtypes = [vp, vp, ci, ci, ci, ci, ci, vp]
@@ -425,11 +431,16 @@ def attn_bwd_strided(
     causal: bool = False,
     softmax_scale: Optional[float] = None,
     kv_lens: Optional[torch.Tensor] = None,
+    window: Optional[int] = None,
+    sinks: int = 0,
 ) -> None:
     """The backward in one call: delta = rowsum(O * dO), then dQ, dK, dV written into the given tensors. q, k, v, dq,
     dk and dv may be strided views with a contiguous last dimension (slices of a packed projection and of its
-    gradient); o and d_o [B,N,H,D] are contiguous. Asynchronous on torch's current stream."""
-    r = _front().attn_bwd_strided(q, k, v, o, d_o, lse, dq, dk, dv, bool(causal), softmax_scale, kv_lens)
+    gradient); o and d_o [B,N,H,D] are contiguous. `window` and `sinks` as in `attn_fwd`. Asynchronous on torch's current
+    stream."""
+    _check_window(window, sinks, causal)
+    r = (_front().attn_bwd_strided(q, k, v, o, d_o, lse, dq, dk, dv, bool(causal), softmax_scale, kv_lens) if window is None else
+         _front().attn_bwd_strided(q, k, v, o, d_o, lse, dq, dk, dv, bool(causal), softmax_scale, kv_lens, window, sinks))
     if r is not None:
         return _done(r, "hk_attn_bwd_strided")
     b, n, h, d = q.shape
@@ -449,9 +460,16 @@ def attn_bwd_strided(
     kv_lens = _dense_lens(kv_lens, b, q.device, s)
     delta = torch.empty_like(lse)
 
-    def arr(t):  # a dimension of size 1 has no stride that matters: give it one the library takes
-        return (ctypes.c_longlong * 3)(*(st if n_i > 1 else d for st, n_i in zip(t.stride()[:3], t.shape[:3])))
-
+    arr = _strides3
+    if window is not None:
+        need = int(capi().hk_attn_bwd_window_workspace_bytes(b, n, nk, h, hkv, d, window, sinks))
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        _check(capi().hk_attn_bwd_window(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), d_o.data_ptr(), lse.data_ptr(),
+                                         delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), b, n, nk, h, hkv, d, arr(q),
+                                         arr(k), arr(v), arr(dq), arr(dk), arr(dv), _ptr(kv_lens), window, sinks,
+                                         float(softmax_scale or 0.0), _ptr(ws), need, q.device.index, s.cuda_stream),
+               "hk_attn_bwd_window")
+        return
     rc = capi().hk_attn_bwd_strided(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), d_o.data_ptr(),
                                     lse.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                                     b, n, nk, h, hkv, d, arr(q), arr(k), arr(v), arr(dq), arr(dk), arr(dv),

@@ -25,7 +25,7 @@ import torch.nn as nn
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
-from ._native import attn_bwd_strided, attn_fwd, device_status, key_padding_lens, qk_norm_rotary, qk_norm_rotary_bwd
+from ._native import _check_window, attn_bwd_strided, attn_fwd, device_status, key_padding_lens, qk_norm_rotary, qk_norm_rotary_bwd
 
 
 def _tma_viewable(t: torch.Tensor) -> bool:
@@ -56,8 +56,8 @@ def _blocking_status(dev, what):
         raise RuntimeError(f"attention {what} failed on the device (status {status})")
 
 
-def _forward(q, k, v, causal, softmax_scale, kv_lens):
-    O, L = attn_fwd(q, k, v, causal=causal, softmax_scale=softmax_scale, kv_lens=kv_lens)
+def _forward(q, k, v, causal, softmax_scale, kv_lens, window, sinks):
+    O, L = attn_fwd(q, k, v, causal=causal, softmax_scale=softmax_scale, kv_lens=kv_lens, window=window, sinks=sinks)
     _blocking_status(q.device, "forward")
     return O, L
 
@@ -66,7 +66,7 @@ def _backward(ctx, q, k, v, O, L, dO_bnhd, dQ, dK, dV):
     assert dO_bnhd.shape == O.shape, f"dO shape mismatch: expected {tuple(O.shape)}, got {dO_bnhd.shape}"
     assert dO_bnhd.is_cuda and dO_bnhd.device == O.device, "dO must be on correct CUDA device"
     dO = dO_bnhd.to(torch.bfloat16).contiguous()
-    rest = dict(causal=ctx.causal, softmax_scale=ctx.softmax_scale, kv_lens=ctx.kv_lens)
+    rest = dict(causal=ctx.causal, softmax_scale=ctx.softmax_scale, kv_lens=ctx.kv_lens, window=ctx.window, sinks=ctx.sinks)
     try:
         attn_bwd_strided(q, k, v, O, dO, L, dQ, dK, dV, **rest)
     except RuntimeError:
@@ -82,17 +82,18 @@ def _backward(ctx, q, k, v, O, L, dO_bnhd, dQ, dK, dV):
 class HipAttnFunction(Function):
     @staticmethod
     def forward(ctx, q_bnhd: torch.Tensor, k_bnhd: torch.Tensor, v_bnhd: torch.Tensor, causal: bool = True,
-                softmax_scale=None, kv_lens=None):
+                softmax_scale=None, kv_lens=None, window=None, sinks=0):
         _check_qkv(q_bnhd, k_bnhd, v_bnhd)
         if all(_tma_viewable(t) for t in (q_bnhd, k_bnhd, v_bnhd)):
             q, k, v = q_bnhd, k_bnhd, v_bnhd
         else:
             q, k, v = (t.to(torch.bfloat16).contiguous() for t in (q_bnhd, k_bnhd, v_bnhd))
-        O, L = _forward(q, k, v, bool(causal), softmax_scale, kv_lens)
+        O, L = _forward(q, k, v, bool(causal), softmax_scale, kv_lens, window, sinks)
         ctx.save_for_backward(q, k, v, O, L)
         ctx.causal = bool(causal)
         ctx.softmax_scale = softmax_scale
         ctx.kv_lens = kv_lens
+        ctx.window, ctx.sinks = window, sinks
         return O.to(q_bnhd.dtype)
 
     @staticmethod
@@ -100,7 +101,7 @@ class HipAttnFunction(Function):
         q, k, v, O, L = ctx.saved_tensors
         dQ, dK, dV = (torch.empty(t.shape, dtype=torch.bfloat16, device=t.device) for t in (q, k, v))
         _backward(ctx, q, k, v, O, L, dO_bnhd, dQ, dK, dV)
-        return dQ.to(dO_bnhd.dtype), dK.to(dO_bnhd.dtype), dV.to(dO_bnhd.dtype), None, None, None
+        return dQ.to(dO_bnhd.dtype), dK.to(dO_bnhd.dtype), dV.to(dO_bnhd.dtype), None, None, None, None, None
 
 
 class _PackedAttnFunction(Function):
@@ -109,14 +110,15 @@ class _PackedAttnFunction(Function):
     ``unbind`` outputs the three gradients would be stacked by a copy of them all)."""
 
     @staticmethod
-    def forward(ctx, q, packed, causal, softmax_scale, kv_lens):
+    def forward(ctx, q, packed, causal, softmax_scale, kv_lens, window=None, sinks=0):
         qkv = packed.unbind(dim=2) if q is None else (q, *packed.unbind(dim=2))
         _check_qkv(*qkv)
-        O, L = _forward(*qkv, causal, softmax_scale, kv_lens)
+        O, L = _forward(*qkv, causal, softmax_scale, kv_lens, window, sinks)
         ctx.save_for_backward(*([packed] if q is None else [q, packed]), O, L)
         ctx.causal = causal
         ctx.softmax_scale = softmax_scale
         ctx.kv_lens = kv_lens
+        ctx.window, ctx.sinks = window, sinks
         return O
 
     @staticmethod
@@ -125,17 +127,17 @@ class _PackedAttnFunction(Function):
         d_packed = torch.empty(packed.shape, dtype=torch.bfloat16, device=packed.device)
         d_q = [torch.empty(t.shape, dtype=torch.bfloat16, device=t.device) for t in q]
         _backward(ctx, *q, *packed.unbind(dim=2), O, L, dO_bnhd, *d_q, *d_packed.unbind(dim=2))
-        return d_q[0] if q else None, d_packed, None, None, None
+        return d_q[0] if q else None, d_packed, None, None, None, None, None
 
 
-def _attend(q, packed, causal, softmax_scale, key_padding_mask):
+def _attend(q, packed, causal, softmax_scale, key_padding_mask, window=None, sinks=0):
     """Attention of q (None: the first of the packed tensors) over a packed projection [B, S, 2 or 3, H, D]."""
     if key_padding_mask is None:
-        out = _apply(q, packed, causal, softmax_scale, None)
+        out = _apply(q, packed, causal, softmax_scale, None, window, sinks)
     else:
         kv_lens, bad = _lens_from_key_padding_mask(key_padding_mask, packed)
         try:
-            out = _apply(q, packed, causal, softmax_scale, kv_lens)
+            out = _apply(q, packed, causal, softmax_scale, kv_lens, window, sinks)
         except BaseException:
             torch.cuda.synchronize(packed.device)  # the flag may still be written: it is given back only then
             raise
@@ -145,11 +147,11 @@ def _attend(q, packed, causal, softmax_scale, key_padding_mask):
     return out.to((packed if q is None else q).dtype).contiguous()
 
 
-def _apply(q, packed, causal, softmax_scale, kv_lens):
+def _apply(q, packed, causal, softmax_scale, kv_lens, window, sinks):
     if _packed_viewable(packed) and (q is None or _tma_viewable(q)):
-        return _PackedAttnFunction.apply(q, packed, bool(causal), softmax_scale, kv_lens)
+        return _PackedAttnFunction.apply(q, packed, bool(causal), softmax_scale, kv_lens, window, sinks)
     views = packed.unbind(dim=2) if q is None else (q, *packed.unbind(dim=2))
-    return HipAttnFunction.apply(*views, causal, softmax_scale, kv_lens)
+    return HipAttnFunction.apply(*views, causal, softmax_scale, kv_lens, window, sinks)
 
 
 _BAD_MASK = "only right-padded key_padding_mask (a kept prefix of at least one key per row) is supported"
@@ -172,10 +174,14 @@ def _lens_from_key_padding_mask(mask: torch.Tensor, packed: torch.Tensor):
 class HipSelfAttention(nn.Module):
     """qkv [B, S, 3, H, D] -> [B, S, H, D] (hipkittens.py:122-162). Same constructor as the reference;
     `causal` and `softmax_scale` take effect here, dropout is not applied (the reference builds an
-    nn.Dropout but never calls it, hipkittens.py:141,158-161)."""
+    nn.Dropout but never calls it, hipkittens.py:141,158-161). With `causal`, `window` and `sinks` leave a query the last `window`
+    keys and the first `sinks` (``attn_fwd``)."""
 
-    def __init__(self, causal=False, softmax_scale=None, attention_dropout=0.0, deterministic=False):
+    def __init__(self, causal=False, softmax_scale=None, attention_dropout=0.0, deterministic=False,
+                 window=None, sinks=0):
         super().__init__()
+        _check_window(window, sinks)
+        self.window, self.sinks = window, sinks
         self.causal = causal
         self.softmax_scale = softmax_scale
         self.drop = nn.Dropout(attention_dropout)
@@ -185,16 +191,19 @@ class HipSelfAttention(nn.Module):
         assert qkv.dtype in [torch.float16, torch.bfloat16]
         assert qkv.is_cuda
         causal = self.causal if causal is None else causal
-        return _attend(None, qkv, causal, self.softmax_scale, key_padding_mask)
+        return _attend(None, qkv, causal, self.softmax_scale, key_padding_mask, self.window, self.sinks)
 
 
 class HipCrossAttention(nn.Module):
     """q [B, Sq, H, D], kv [B, Sk, 2, H_KV, D] -> [B, Sq, H, D] (hipkittens.py:165-202). Sq may differ from Sk and
     `causal` may be combined with a right-padded `key_padding_mask`, with the reference math path's alignment of the
-    causal mask to the last query and the last kept key (base.py:104-116)."""
+    causal mask to the last query and the last kept key (base.py:104-116). `window` and `sinks` as in HipSelfAttention."""
 
-    def __init__(self, causal=False, softmax_scale=None, attention_dropout=0.0, deterministic=False):
+    def __init__(self, causal=False, softmax_scale=None, attention_dropout=0.0, deterministic=False,
+                 window=None, sinks=0):
         super().__init__()
+        _check_window(window, sinks)
+        self.window, self.sinks = window, sinks
         self.causal = causal
         self.softmax_scale = softmax_scale
         self.drop = nn.Dropout(attention_dropout)
@@ -204,7 +213,7 @@ class HipCrossAttention(nn.Module):
         batch_size = q.shape[0]
         causal = self.causal if causal is None else causal
         assert kv.shape[0] == batch_size and kv.shape[4] == q.shape[3]
-        return _attend(q, kv, causal, self.softmax_scale, key_padding_mask)
+        return _attend(q, kv, causal, self.softmax_scale, key_padding_mask, self.window, self.sinks)
 
 
 class QkNormRotaryFunction(Function):

@@ -84,6 +84,12 @@ struct BwdParams {
   float scale;
   float scale_log2;
   const int* kv_lens;   // optional device [B]: batch b attends to keys [0, kv_lens[b]) only; null = NK
+  // kMaskWindow: as in FwdParams. The first `shared_blocks` key blocks of a unit are shared by `shares` work items each, which leave
+  // their partial sums in `partial`, [unit][block][share][dK, dV][128][D]; attn_bwd_shares_kernel adds them up.
+  int window, sinks;
+  int shared_blocks, shares;
+  FastDiv fd_shares;
+  float* partial;
   int* status;
 #ifdef HK_TRACE
   long long* trace;     // [4 roles][4096] clock stamps of CTA 0 (debug builds only)
@@ -302,6 +308,21 @@ __device__ __forceinline__ void bwd_store_part_row(uint32_t taddr, __nv_bfloat16
   }
 }
 
+// The same columns, scaled, as fp32.
+template <int D>
+__device__ __forceinline__ void bwd_store_part_row_f32(uint32_t taddr, float* dst, float mul) {
+#pragma unroll
+  for (int cc = 0; cc < D / kBwdParts / 32; ++cc) {
+    uint32_t o[32];
+    ptx::tmem_ld32(taddr + cc * 32, o);
+    ptx::tmem_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * mul);
+#pragma unroll
+    for (int v8 = 0; v8 < 4; ++v8) ptx::st_global_v8(dst + cc * 32 + v8 * 8, o + v8 * 8);
+  }
+}
+
 // The same columns, scaled, into a [128][D] fp32 tile in shared memory whose 16-byte units are exchanged inside a row by the
 // row's low bits, so that neither the rows of a warp here nor the units of a row there meet in a bank.
 template <int D>
@@ -349,8 +370,11 @@ __device__ __forceinline__ int dkdv_share(int r, int ranks, int n) { return r * 
 // (j, NBK - 1 - j) of the same unit, which all cost the same - a CTA's round 2r is the first block of its r-th pair and
 // round 2r + 1 the second (none for the middle block of an odd count) -, or singly (n_pairs = 0), the longest of all
 // units first, in snake order.
-template <bool CAUSAL, bool SPLIT>
+// With a window every key block meets about as many query tiles, but those of the sinks, which all queries see: these are shared
+// (BwdParams::shares), so that no item is much longer than the others, and the items go in the order without a mask.
+template <int MASK, bool SPLIT>
 __device__ __forceinline__ int dkdv_item_for_round(const BwdParams& p, int round) {
+  constexpr bool CAUSAL = MASK == kMaskCausal;
   const int cta = SPLIT ? p.fd_split.div(blockIdx.x) : static_cast<int>(blockIdx.x);
   const int n_cta = SPLIT ? p.n_items : static_cast<int>(gridDim.x);
   if (!CAUSAL) return item_for_round(p, round, cta, n_cta);
@@ -371,8 +395,9 @@ __device__ __forceinline__ int dkdv_item_for_round(const BwdParams& p, int round
   return unit * nbk + j;
 }
 
-template <bool CAUSAL, bool SPLIT>
+template <int MASK, bool SPLIT>
 __device__ __forceinline__ DkdvItem decode_dkdv_item(const BwdParams& p, int idx) {
+  constexpr bool CAUSAL = MASK != kMaskNone;
   DkdvItem w;
   const int NBQ = (p.N + kBlockM - 1) / kBlockM;   // query tiles
   int unit;
@@ -382,14 +407,36 @@ __device__ __forceinline__ DkdvItem decode_dkdv_item(const BwdParams& p, int idx
   w.off = w.kv_len - p.N;
   // causal: key c is seen by query rows r >= c - off; the first key of the block, j*128, is the one seen by most
   w.i_min = CAUSAL ? max(w.j * kBlockN - w.off, 0) / kBlockM : 0;
+  [[maybe_unused]] int share = 0, of = 1;
+  if constexpr (MASK == kMaskWindow) {
+    if (w.j < p.shared_blocks * p.shares) {
+      p.fd_shares.divmod(w.j, w.j, share);
+      of = p.shares;
+    } else {
+      w.j -= p.shared_blocks * (p.shares - 1);
+    }
+    w.i_min = max(w.j * kBlockN - w.off, 0) / kBlockM;
+  }
   w.cnt_i = max(NBQ - w.i_min, 0);
+  if constexpr (MASK == kMaskWindow) {
+    if (w.j * kBlockN >= p.sinks) {
+      // the block's last key is seen up to window - 1 rows behind its own
+      const long long last = static_cast<long long>(min(w.j * kBlockN + kBlockN, w.kv_len) - 1 - w.off) + p.window - 1;
+      if (last < static_cast<long long>(NBQ) * kBlockM) w.cnt_i = max(static_cast<int>(max(last, -1ll) + kBlockM) / kBlockM - w.i_min, 0);
+    }
+  }
   w.n_iter = (w.j * kBlockN >= w.kv_len) ? 0 : p.G * w.cnt_i;
   w.n_first = w.g_first = w.i_first = w.rank = 0;
   w.n_end = w.n_iter;
-  if constexpr (SPLIT) {
-    w.rank = static_cast<int>(blockIdx.x) - p.fd_split.div(blockIdx.x) * p.split;
-    w.n_first = dkdv_share(w.rank, p.split, w.n_iter);
-    w.n_end = dkdv_share(w.rank + 1, p.split, w.n_iter);
+  if constexpr (SPLIT || MASK == kMaskWindow) {
+    if constexpr (SPLIT) {
+      w.rank = static_cast<int>(blockIdx.x) - p.fd_split.div(blockIdx.x) * p.split;
+      of = p.split;
+    } else {
+      w.rank = share;
+    }
+    w.n_first = dkdv_share(w.rank, of, w.n_iter);
+    w.n_end = dkdv_share(w.rank + 1, of, w.n_iter);
     if (w.n_end > w.n_first) {
       w.g_first = w.n_first / w.cnt_i;
       w.i_first = w.n_first - w.g_first * w.cnt_i;
@@ -401,12 +448,13 @@ __device__ __forceinline__ DkdvItem decode_dkdv_item(const BwdParams& p, int idx
 // SPLIT: an item is shared by the CTAs of a cluster (p.split of them), each with its part of the (head, query tile) pairs; the
 // partial dK and dV are added up through distributed shared memory, row by row in the order of the ranks, so that the
 // gradients stay the same from run to run. One item per cluster and launch.
-template <int D, bool CAUSAL, bool SPLIT>
+template <int D, int MASK, bool SPLIT>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                      const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_do,
                      const BwdParams p) {
   using namespace ptx;
+  constexpr bool CAUSAL = MASK != kMaskNone, WINDOW = MASK == kMaskWindow;
   using SM = BwdSmem<D>;
   constexpr int kTile = SM::kTileBytes;
   constexpr int kSub = SM::kSubTileBytes;
@@ -511,13 +559,14 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
 #endif
     for (int round = 0; ok; ++round) {
       if (round >= p.total_rounds) break;
-      const int idx = dkdv_item_for_round<CAUSAL, SPLIT>(p, round);
+      const int idx = dkdv_item_for_round<MASK, SPLIT>(p, round);
       if (idx < 0) continue;  // a partial round leaves some CTAs without an item
-      const DkdvItem w = decode_dkdv_item<CAUSAL, SPLIT>(p, idx);
+      const DkdvItem w = decode_dkdv_item<MASK, SPLIT>(p, idx);
       const bool pad_row = w.j * kBlockN + row >= w.kv_len;  // this key is padding (or lies beyond NK)
       const bool pad_block = (w.j + 1) * kBlockN > w.kv_len;  // uniform over the CTA: only such a block has padded keys
       if (w.n_iter == 0) {
         if (SPLIT && w.rank != 0) continue;
+        if (WINDOW && w.j < p.shared_blocks) continue;  // whoever adds the shares up writes them
         // nobody sees this key block (padding, or causal with every query before it): its gradients are zero and no
         // product was issued for it
         if (w.j * kBlockN + row < p.NK) {
@@ -532,7 +581,7 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         continue;
       }
       // i_rel: position of the pair's query tile among the cnt_i tiles of its head (n % cnt_i, without the division)
-      if (SPLIT && w.n_first == w.n_end) continue;
+      if ((SPLIT || WINDOW) && w.n_first == w.n_end) continue;
       for (int n = w.n_first, i_rel = w.i_first; n < w.n_end && ok; ++n, ++it, i_rel = (i_rel + 1 == w.cnt_i) ? 0 : i_rel + 1) {
         HK_STAMP(trole, 0);
         // a query tile the diagonal runs through: its first row does not see the block's last key (with an offset
@@ -590,6 +639,12 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
             const int lim = row + (w.j - i_t) * kBlockN - w.off;
 #pragma unroll
             for (int col = 0; col < kBwdPC; ++col) su[col] = (part * kBwdPC + col) < lim ? 0u : su[col];
+          }
+          if (WINDOW && (w.j + 1) * kBlockN > p.sinks && (i_t - w.j) * kBlockM + kBlockM - 1 + w.off >= p.window) {
+            // a query tile some rows of which are a window or more behind some of the keys
+            const int lim = w.j * kBlockN + row < p.sinks ? 0x7fffffff : row + (w.j - i_t) * kBlockN - w.off + p.window;
+#pragma unroll
+            for (int col = 0; col < kBwdPC; ++col) su[col] = (part * kBwdPC + col) >= lim ? 0u : su[col];
           }
           if (pad_block) {
             // a padded key is seen by nobody: P^T and dS^T rows are zero, so are its dK and dV rows
@@ -666,6 +721,14 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         bwd_stage_part_row<D>(tmem + lane_addr + cDV + part * (D / kBwdParts), bwd_smem + kPartBytes, row, part, 1.0f);
         continue;
       }
+      if (WINDOW && w.j < p.shared_blocks) {
+        const long long slot = (static_cast<long long>(w.b * p.H_KV + w.kvh) * p.shared_blocks + w.j) * p.shares + w.rank;
+        float* const dst = p.partial + (slot * 2 * kBlockN + row) * D + part * (D / kBwdParts);
+        bwd_store_part_row_f32<D>(tmem + lane_addr + cDK + part * (D / kBwdParts), dst, p.scale);
+        bwd_store_part_row_f32<D>(tmem + lane_addr + cDV + part * (D / kBwdParts), dst + kBlockN * D, 1.0f);
+        tc_fence_before();
+        continue;
+      }
       const bool row_exists = w.j * kBlockN + row < p.NK;  // keys of a partial last block beyond NK are computed, not stored
       const int key = w.j * kBlockN + row;
       bwd_store_part_row<D>(tmem + lane_addr + cDK + part * (D / kBwdParts),
@@ -680,7 +743,7 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       cluster_wait();
       if (ok) {
         // every n-th row of the key block is added up here
-        const DkdvItem w = decode_dkdv_item<CAUSAL, SPLIT>(p, dkdv_item_for_round<CAUSAL, SPLIT>(p, 0));
+        const DkdvItem w = decode_dkdv_item<MASK, SPLIT>(p, dkdv_item_for_round<MASK, SPLIT>(p, 0));
         constexpr int kUnits = 2 * (D / 8);         // 8 columns each: dK, then dV
         for (int u = tid; w.n_iter > 0; u += 32 * kBwdCW) {
           const int r_row = w.rank + (u / kUnits) * p.split, unit = u % kUnits;
@@ -726,9 +789,9 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       bool ok = true;
       for (int round = 0; ok; ++round) {
         if (round >= p.total_rounds) break;
-        const int idx = dkdv_item_for_round<CAUSAL, SPLIT>(p, round);
+        const int idx = dkdv_item_for_round<MASK, SPLIT>(p, round);
         if (idx < 0) continue;  // a partial round leaves some CTAs without an item
-        const DkdvItem w = decode_dkdv_item<CAUSAL, SPLIT>(p, idx);
+        const DkdvItem w = decode_dkdv_item<MASK, SPLIT>(p, idx);
         if (w.n_first == w.n_end) continue;  // key block wholly beyond this batch element's length: nothing to do
         ok = mbar_wait(bars + KV_EMPTY, (item_cnt & 1) ^ 1, abortp, kWaitLimitCycles);
         if (!ok) break;
@@ -788,9 +851,9 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
 #endif
       for (int round = 0; ok; ++round) {
         if (round >= p.total_rounds) break;
-        const int idx = dkdv_item_for_round<CAUSAL, SPLIT>(p, round);
+        const int idx = dkdv_item_for_round<MASK, SPLIT>(p, round);
         if (idx < 0) continue;  // a partial round leaves some CTAs without an item
-        const DkdvItem w = decode_dkdv_item<CAUSAL, SPLIT>(p, idx);
+        const DkdvItem w = decode_dkdv_item<MASK, SPLIT>(p, idx);
         if (w.n_first == w.n_end) continue;  // key block wholly beyond this batch element's length: nothing to do
         ok = iss_wait(bars + KV_FULL, item_cnt & 1, abortp, kWaitLimitCycles);
         if (!ok) break;
@@ -849,9 +912,9 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
 #endif
       for (int round = 0; ok; ++round) {
         if (round >= p.total_rounds) break;
-        const int idx = dkdv_item_for_round<CAUSAL, SPLIT>(p, round);
+        const int idx = dkdv_item_for_round<MASK, SPLIT>(p, round);
         if (idx < 0) continue;  // a partial round leaves some CTAs without an item
-        const DkdvItem w = decode_dkdv_item<CAUSAL, SPLIT>(p, idx);
+        const DkdvItem w = decode_dkdv_item<MASK, SPLIT>(p, idx);
         if (w.n_first == w.n_end) continue;  // key block wholly beyond this batch element's length: nothing to do
         for (int n = w.n_first; n < w.n_end && ok; ++n, ++it) {
           ok = iss_wait(bars + P_FULL, it & 1, abortp, kWaitLimitCycles) &&
@@ -919,9 +982,9 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       };
       for (int round = 0; ok; ++round) {
         if (round >= p.total_rounds) break;
-        const int idx = dkdv_item_for_round<CAUSAL, SPLIT>(p, round);
+        const int idx = dkdv_item_for_round<MASK, SPLIT>(p, round);
         if (idx < 0) continue;  // a partial round leaves some CTAs without an item
-        const DkdvItem w = decode_dkdv_item<CAUSAL, SPLIT>(p, idx);
+        const DkdvItem w = decode_dkdv_item<MASK, SPLIT>(p, idx);
         if (w.n_first == w.n_end) continue;  // key block wholly beyond this batch element's length: nothing to do
         fetch(w, w.n_first);
         for (int n = w.n_first; n < w.n_end && ok; ++n, ++it) {
@@ -966,6 +1029,33 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   }
 }
 
+// dK and dV of the shared key blocks: the shares that had pairs to work on, in their order. A thread has 8 columns of a row.
+// grid = (ceil(2 * 128 * D / 8 / 256), units * shared blocks), block = 256.
+template <int D>
+__global__ void __launch_bounds__(256) attn_bwd_shares_kernel(const __grid_constant__ BwdParams p) {
+  ptx::grid_dep_wait();
+  ptx::grid_dep_launch();
+  constexpr int kUnits = D / 8;
+  const int t = blockIdx.x * 256 + threadIdx.x, c8 = t % kUnits, row = t / kUnits % kBlockN;
+  const bool is_dv = t / kUnits >= kBlockN;
+  const int block = blockIdx.y, unit = block / p.shared_blocks;
+  const DkdvItem w = decode_dkdv_item<kMaskWindow, false>(p, unit * static_cast<int>(p.fd_unit.d) + (block - unit * p.shared_blocks) * p.shares);
+  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  const float4* src = reinterpret_cast<const float4*>(p.partial + (static_cast<long long>(block) * p.shares * 2 * kBlockN + (is_dv ? kBlockN : 0) + row) * D + c8 * 8);
+  for (int r = 0; r < p.shares; ++r, src += 2 * kBlockN * D / 4) {
+    if (dkdv_share(r, p.shares, w.n_iter) == dkdv_share(r + 1, p.shares, w.n_iter)) continue;  // it had nothing to do
+    const float4 x = src[0], y = src[1];
+    acc[0] += x.x, acc[1] += x.y, acc[2] += x.z, acc[3] += x.w;
+    acc[4] += y.x, acc[5] += y.y, acc[6] += y.z, acc[7] += y.w;
+  }
+  const int key = w.j * kBlockN + row;
+  if (key < p.NK) {
+    __nv_bfloat16* const dst = (is_dv ? dv_row(p, w.b, key, w.kvh) : dk_row(p, w.b, key, w.kvh)) + c8 * 8;
+    *reinterpret_cast<uint4*>(dst) = make_uint4(ptx::pack_bf16x2(acc[0], acc[1]), ptx::pack_bf16x2(acc[2], acc[3]),
+                                                ptx::pack_bf16x2(acc[4], acc[5]), ptx::pack_bf16x2(acc[6], acc[7]));
+  }
+}
+
 // ------------------------------------------------------------------------------------ dQ
 struct DqItem {
   int b, h, kvh, i;  // batch, query head, its kv head, query tile
@@ -973,16 +1063,25 @@ struct DqItem {
   int off;           // causal: query row r sees keys [0, r + off], off = kv_len - N
   int n_iter;        // key tiles this query tile meets (0: none of its rows sees a key; dQ = 0)
 };
+// With a window: those of the sinks and then, `skip` tiles further on, those from the first of the tile's windows.
+struct DqWindowItem : DqItem {
+  int sink_tiles, skip;
+};
+template <int MASK>
+using DqItemOf = std::conditional_t<MASK == kMaskWindow, DqWindowItem, DqItem>;
+__device__ __forceinline__ int dq_tile(const DqItem&, int n) { return n; }
+__device__ __forceinline__ int dq_tile(const DqWindowItem& w, int n) { return n >= w.sink_tiles ? n + w.skip : n; }
 
 // Work order: the query tiles of one (batch, kv head) unit are adjacent so that concurrently running CTAs
 // stream the same K / V tiles from L2. Causal: L2-sized groups of units, last query tile (the longest) first.
-template <bool CAUSAL>
-__device__ __forceinline__ DqItem decode_dq_item(const BwdParams& p, int idx) {
-  DqItem w;
+template <int MASK>
+__device__ __forceinline__ DqItemOf<MASK> decode_dq_item(const BwdParams& p, int idx) {
+  constexpr bool CAUSAL = MASK != kMaskNone;
+  DqItemOf<MASK> w;
   const int NB = (p.N + kBlockM - 1) / kBlockM;  // the last tile may be partial
   const int G = p.G;
   int unit, g;
-  if (CAUSAL) {
+  if (MASK == kMaskCausal) {
     const int grp = min(p.fd_group.div(idx), p.last_group);
     const int within = idx - grp * p.group_items;
     int qd, rem;
@@ -1004,15 +1103,22 @@ __device__ __forceinline__ DqItem decode_dq_item(const BwdParams& p, int idx) {
   const int n_kv = (w.kv_len + kBlockN - 1) / kBlockN;
   // causal: the last row of the tile sees keys up to i*128 + 127 + off
   w.n_iter = CAUSAL ? min(max((w.i * kBlockM + kBlockM + w.off + kBlockN - 1) / kBlockN, 0), n_kv) : n_kv;
+  if constexpr (MASK == kMaskWindow) {
+    const int lo = max(w.i * kBlockM + w.off - p.window + 1, 0) / kBlockN;
+    w.sink_tiles = min((p.sinks + kBlockN - 1) / kBlockN, lo);
+    w.skip = lo - w.sink_tiles;
+    w.n_iter = max(w.n_iter - w.skip, 0);
+  }
   return w;
 }
 
-template <int D, bool CAUSAL>
+template <int D, int MASK>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                    const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_do,
                    const BwdParams p) {
   using namespace ptx;
+  constexpr bool CAUSAL = MASK != kMaskNone, WINDOW = MASK == kMaskWindow;
   using SM = BwdSmem<D>;
   constexpr int kTile = SM::kTileBytes;
   constexpr int kSub = SM::kSubTileBytes;
@@ -1100,7 +1206,7 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       if (round >= p.total_rounds) break;
       const int idx = item_for_round(p, round, blockIdx.x, gridDim.x);
       if (idx < 0) continue;  // a partial round leaves some CTAs without an item
-      const DqItem w = decode_dq_item<CAUSAL>(p, idx);
+      const DqItemOf<MASK> w = decode_dq_item<MASK>(p, idx);
       const size_t srow = (static_cast<size_t>(w.b) * p.H + w.h) * p.N + static_cast<size_t>(w.i) * kBlockM + row;
       const bool row_exists = w.i * kBlockM + row < p.N;  // rows of a partial last tile beyond N: zero statistics
       if (w.n_iter == 0) {
@@ -1118,7 +1224,8 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       for (int n = 0; n < w.n_iter && ok; ++n, ++it) {
         // a key tile the diagonal (or the end of the kept keys) runs through: the tile's first row does not see
         // its last key
-        const bool diag = CAUSAL && ((n + 1) * kBlockN - 1 > min(w.i * kBlockM + w.off, w.kv_len - 1));
+        const int kv = dq_tile(w, n);
+        const bool diag = CAUSAL && ((kv + 1) * kBlockN - 1 > min(w.i * kBlockM + w.off, w.kv_len - 1));
         HK_STAMP(0, 0);
         ok = mbar_wait(bars + S_FULL, it & 1, abortp, kWaitLimitCycles);
         ok = __all_sync(0xffffffffu, ok);
@@ -1150,9 +1257,16 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           if (diag) {
             // key n*128 + col is seen by query i*128 + row iff it is <= query + off and < kv_len (this also zeroes
             // the infinities of a row without any key, whose L is -inf)
-            const int lim = min(w.i * kBlockM + row + w.off, w.kv_len - 1) - n * kBlockN;
+            const int lim = min(w.i * kBlockM + row + w.off, w.kv_len - 1) - kv * kBlockN;
 #pragma unroll
             for (int col = 0; col < kBwdPC; ++col) su[col] = (part * kBwdPC + col) > lim ? 0u : su[col];
+          }
+          if (WINDOW && kv * kBlockN <= w.i * kBlockM + kBlockM - 1 + w.off - p.window && (kv + 1) * kBlockN > p.sinks) {
+            // a tile whose first key some rows have behind their window
+            const int lo = w.i * kBlockM + row + w.off - p.window + 1 - kv * kBlockN, sinks = p.sinks - kv * kBlockN;
+#pragma unroll
+            for (int col = 0; col < kBwdPC; ++col)
+              su[col] = (part * kBwdPC + col) < lo && (part * kBwdPC + col) >= sinks ? 0u : su[col];
           }
           if (!CAUSAL && n == w.n_iter - 1 && (w.kv_len & (kBlockN - 1)) != 0) {
             // partial last tile: keys at or beyond the length are padding
@@ -1225,7 +1339,7 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         if (round >= p.total_rounds) break;
         const int idx = item_for_round(p, round, blockIdx.x, gridDim.x);
         if (idx < 0) continue;  // a partial round leaves some CTAs without an item
-        const DqItem w = decode_dq_item<CAUSAL>(p, idx);
+        const DqItemOf<MASK> w = decode_dq_item<MASK>(p, idx);
         if (w.n_iter == 0) continue;  // no row of this tile sees a key: nothing is loaded or issued
         ok = mbar_wait(bars + QDO_EMPTY, (item_cnt & 1) ^ 1, abortp, kWaitLimitCycles);
         if (!ok) break;
@@ -1242,7 +1356,7 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           mbar_expect_tx(bars + KA_FULL + ka, kTile);
 #pragma unroll
           for (int ch = 0; ch < kChunks; ++ch)
-            tma_load_4d(sK + ka * kTile + ch * kSub, &tmap_k, bars + KA_FULL + ka, ch * 64, w.kvh, n * kBlockN, w.b);
+            tma_load_4d(sK + ka * kTile + ch * kSub, &tmap_k, bars + KA_FULL + ka, ch * 64, w.kvh, dq_tile(w, n) * kBlockN, w.b);
           if (++ka == RA) {
             ka = 0;
             ka_par ^= 1;
@@ -1252,7 +1366,7 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           mbar_expect_tx(bars + VB_FULL + vb, kTile);
 #pragma unroll
           for (int ch = 0; ch < kChunks; ++ch)
-            tma_load_4d(sV + vb * kTile + ch * kSub, &tmap_v, bars + VB_FULL + vb, ch * 64, w.kvh, n * kBlockN, w.b);
+            tma_load_4d(sV + vb * kTile + ch * kSub, &tmap_v, bars + VB_FULL + vb, ch * 64, w.kvh, dq_tile(w, n) * kBlockN, w.b);
           if (++vb == RB) {
             vb = 0;
             vb_par ^= 1;
@@ -1278,7 +1392,7 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         if (round >= p.total_rounds) break;
         const int idx = item_for_round(p, round, blockIdx.x, gridDim.x);
         if (idx < 0) continue;  // a partial round leaves some CTAs without an item
-        const DqItem w = decode_dq_item<CAUSAL>(p, idx);
+        const DqItemOf<MASK> w = decode_dq_item<MASK>(p, idx);
         if (w.n_iter == 0) continue;  // no row of this tile sees a key: nothing is loaded or issued
         ok = iss_wait(bars + QDO_FULL, item_cnt & 1, abortp, kWaitLimitCycles);
         if (!ok) break;
@@ -1337,7 +1451,7 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         if (round >= p.total_rounds) break;
         const int idx = item_for_round(p, round, blockIdx.x, gridDim.x);
         if (idx < 0) continue;  // a partial round leaves some CTAs without an item
-        const DqItem w = decode_dq_item<CAUSAL>(p, idx);
+        const DqItemOf<MASK> w = decode_dq_item<MASK>(p, idx);
         if (w.n_iter == 0) continue;  // no row of this tile sees a key: nothing is loaded or issued
         ok = iss_wait(bars + QDO_FULL, item_cnt & 1, abortp, kWaitLimitCycles);
         if (!ok) break;

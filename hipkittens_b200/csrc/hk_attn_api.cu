@@ -109,12 +109,15 @@ int prepare_bwd_kernel(Kernel* fn, int dyn_bytes, const char* name) {
   return HK_OK;
 }
 
-template <int D, bool CAUSAL>
+template <int D, int MASK>
 int prepare_bwd_kernels() {
-  int rc = HK_OK;
-  for (auto* fn : {hk::attn_bwd_dkdv_kernel<D, CAUSAL, false>, hk::attn_bwd_dkdv_kernel<D, CAUSAL, true>})
-    if ((rc = prepare_bwd_kernel(fn, hk::BwdSmem<D>::kDynBytes, "attn_bwd_dkdv_kernel")) != HK_OK) return rc;
-  return prepare_bwd_kernel(hk::attn_bwd_dq_kernel<D, CAUSAL>, hk::BwdSmem<D>::kDynBytes, "attn_bwd_dq_kernel");
+  int rc = prepare_bwd_kernel(hk::attn_bwd_dkdv_kernel<D, MASK, false>, hk::BwdSmem<D>::kDynBytes, "attn_bwd_dkdv_kernel");
+  if (rc != HK_OK) return rc;
+  if constexpr (MASK != hk::kMaskWindow) {
+    rc = prepare_bwd_kernel(hk::attn_bwd_dkdv_kernel<D, MASK, true>, hk::BwdSmem<D>::kDynBytes, "attn_bwd_dkdv_kernel");
+    if (rc != HK_OK) return rc;
+  }
+  return prepare_bwd_kernel(hk::attn_bwd_dq_kernel<D, MASK>, hk::BwdSmem<D>::kDynBytes, "attn_bwd_dq_kernel");
 }
 
 int init_device(int device) {
@@ -137,10 +140,12 @@ int init_device(int device) {
   if ((rc = prepare_fwd_kernels<64, hk::kMaskWindow>()) != HK_OK) return rc;
   if ((rc = hk::prepare_decode_kernels(g_cuda_err, sizeof(g_cuda_err), st.sm_count, &st.decode)) != HK_OK) return rc;
   if ((rc = hk::prepare_window_decode_kernels(g_cuda_err, sizeof(g_cuda_err))) != HK_OK) return rc;
-  if ((rc = prepare_bwd_kernels<128, false>()) != HK_OK) return rc;
-  if ((rc = prepare_bwd_kernels<128, true>()) != HK_OK) return rc;
-  if ((rc = prepare_bwd_kernels<64, false>()) != HK_OK) return rc;
-  if ((rc = prepare_bwd_kernels<64, true>()) != HK_OK) return rc;
+  if ((rc = prepare_bwd_kernels<128, hk::kMaskNone>()) != HK_OK) return rc;
+  if ((rc = prepare_bwd_kernels<128, hk::kMaskCausal>()) != HK_OK) return rc;
+  if ((rc = prepare_bwd_kernels<128, hk::kMaskWindow>()) != HK_OK) return rc;
+  if ((rc = prepare_bwd_kernels<64, hk::kMaskNone>()) != HK_OK) return rc;
+  if ((rc = prepare_bwd_kernels<64, hk::kMaskCausal>()) != HK_OK) return rc;
+  if ((rc = prepare_bwd_kernels<64, hk::kMaskWindow>()) != HK_OK) return rc;
   for (int n = 2; n <= hk::kMaxDkdvSplit; ++n)
     st.bwd_clusters[n] = hk::clusters_held(hk::attn_bwd_dkdv_kernel<128, true, true>, hk::kBwdThreads, hk::BwdSmem<128>::kDynBytes, n);
   // the one allocation this library makes: the status word (last, so that a failure above leaves nothing behind). It
@@ -579,6 +584,76 @@ int qkn_pick(int D, int flags, const Fn& fn) {
   return layout(std::integral_constant<int, 16>{});
 }
 
+// How many key blocks of a unit are shared by several work items of the dK/dV kernel with a window, and by how many; a share's
+// partial sums take 256 D fp32 values of the caller's workspace. The blocks of the sinks meet every query tile and would be the
+// longest items by far, so they are cut to about the length of the others; or, where all blocks together are at most half as many
+// as the SMs, all are cut. Estimated in (query tile, key block) pairs, of which an item costs two more than it has. The number
+// of SMs is that of a B200, whatever the device: the workspace does not depend on it.
+struct WindowShares {
+  int blocks, shares;
+};
+WindowShares window_shares(int units, int G, int N, int NK, int window, int sinks) {
+  constexpr long long kSms = 148;
+  const long long nbq = (N + hk::kBlockM - 1) / hk::kBlockM, nbk = (NK + hk::kBlockN - 1) / hk::kBlockN;
+  const long long own = G * std::min(nbq, (1ll * window + hk::kBlockN - 2) / hk::kBlockM + 2);  // a block's pairs by its window
+  const long long sink_blocks = (1ll * std::min(sinks, NK) + hk::kBlockN - 1) / hk::kBlockN, all = G * nbq;
+  const long long items = units * nbk;
+  // the CTA with the longest item has one of the others in each further round
+  auto span = [&](long long longest, long long other, long long n) {
+    const long long rounds = (n - 1) / kSms + 1;
+    return double(longest + (rounds - 1) * other + 2 * rounds);
+  };
+  WindowShares best = {0, 1};
+  double least = span(sink_blocks ? all : own, own, items);
+  auto consider = [&](long long blocks, long long n, double time) {
+    if (n < 2 || time >= 0.95 * least) return;
+    best = {int(blocks), int(n)};
+    least = time;
+  };
+  if (sink_blocks) {
+    const long long n = std::min<long long>({(all - 1) / std::max(own, 16ll) + 1, 4 * kSms / (units * sink_blocks) + 1, 32});
+    consider(sink_blocks, n, span(std::max(nbk > sink_blocks ? own : 0, (all - 1) / n + 1), own, items + units * sink_blocks * (n - 1)));
+  }
+  if (2 * items <= kSms) {
+    const long long longest = sink_blocks ? all : own, n = std::min<long long>({kSms / items, (longest + 1) / 2, 16});
+    if (n > 1) consider(nbk, n, span((longest - 1) / n + 1, (own - 1) / n + 1, items * n));
+  }
+  return best;
+}
+
+template <int D>
+int launch_bwd_window(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tdo, hk::BwdParams p,
+                      bool dq_beside, int sm_count, cudaStream_t stream) {
+  const int nbq = (p.N + hk::kBlockM - 1) / hk::kBlockM, nbk = (p.NK + hk::kBlockN - 1) / hk::kBlockN;
+  const int units = p.B * p.H_KV, per_unit = nbk + p.shared_blocks * (p.shares - 1);
+  if (1ll * p.B * p.H * nbq > 0x3fffffffll || 1ll * units * per_unit > 0x3fffffffll || 1ll * units * p.shared_blocks > 65535)
+    return HK_EINVAL;  // work items are indexed with int
+  p.split = 1;
+  p.n_pairs = 0;
+  p.fd_shares = hk::FastDiv(p.shares);
+  p.n_items = units * per_unit;
+  int grid = p.n_items < sm_count ? p.n_items : sm_count;
+  set_bwd_decode(p, per_unit, 1, 1, grid, false);
+  const hk::BwdParams dkdv = p;
+  const long long tiles = 1ll * p.B * p.H * nbq * kv_tiles(p.NK, hk::kMaskWindow, p.window, p.sinks);
+  HK_CUDA(hk::launch_dependent(short_kernel(tiles, grid), hk::attn_bwd_dkdv_kernel<D, hk::kMaskWindow, false>, grid, hk::kBwdThreads,
+                               hk::BwdSmem<D>::kDynBytes, stream, tq, tk, tv, tdo, p));
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  p.n_items = p.B * p.H * nbq;
+  grid = p.n_items < sm_count ? p.n_items : sm_count;
+  p.dq_waits = !dq_beside || tiles > 40ll * grid;
+  set_bwd_decode(p, (p.H / p.H_KV) * nbq, p.H / p.H_KV, nbq, grid, false);
+  HK_CUDA(hk::launch_dependent(!p.dq_waits || short_kernel(tiles, grid), hk::attn_bwd_dq_kernel<D, hk::kMaskWindow>, grid,
+                               hk::kBwdThreads, hk::BwdSmem<D>::kDynBytes, stream, tq, tk, tv, tdo, p));
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  if (p.shared_blocks > 0) {
+    HK_CUDA(hk::launch_dependent(true, hk::attn_bwd_shares_kernel<D>, dim3(2 * hk::kBlockN * (D / 8) / 256, units * p.shared_blocks), 256,
+                                 0, stream, dkdv));
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+  }
+  return HK_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -831,8 +906,8 @@ struct Span {
 // Shared tail of the backward entries. o != null: delta is computed here first.
 static int bwd_launch(const void* q, const void* k, const void* v, const void* o, const void* d_o, const float* lse,
                       float* delta, void* dq, void* dk, void* dv, int B, int N, int NK, int H, int H_KV, int D,
-                      const BwdStrides& s, const int32_t* kv_lens, int causal, float softmax_scale, int device,
-                      void* cuda_stream) {
+                      const BwdStrides& s, const int32_t* kv_lens, int mask, int window, int sinks, void* workspace,
+                      size_t workspace_bytes, float softmax_scale, int device, void* cuda_stream) {
   if (!q || !k || !v || !d_o || !lse || !delta || !dq || !dk || !dv) return HK_EINVAL;
   if (B <= 0 || N <= 0 || NK <= 0 || H <= 0 || H_KV <= 0) return HK_EINVAL;
   if (D != 64 && D != 128) return HK_EUNSUPPORTED;
@@ -843,6 +918,16 @@ static int bwd_launch(const void* q, const void* k, const void* v, const void* o
   if ((o && !aligned16(o)) || !aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(d_o) || !aligned16(dq) || !aligned16(dk) ||
       !aligned16(dv) || (reinterpret_cast<uintptr_t>(lse) & 3) || (reinterpret_cast<uintptr_t>(delta) & 3))
     return HK_EINVAL;
+  // a window that no key lies behind masks nothing that the causal mask does not
+  if (mask == hk::kMaskWindow && (window >= NK || sinks >= NK)) mask = hk::kMaskCausal;
+  const bool causal = mask == hk::kMaskCausal;
+  WindowShares shared = {0, 1};
+  if (mask == hk::kMaskWindow) {
+    if (1ll * B * H_KV > 0x3fffffffll) return HK_EINVAL;
+    shared = window_shares(B * H_KV, H / H_KV, N, NK, window, sinks);
+    const size_t need = hk_attn_bwd_window_workspace_bytes(B, N, NK, H, H_KV, D, window, sinks);
+    if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255))) return HK_EWORKSPACE;
+  }
   DeviceState* st = nullptr;
   DeviceScope scope;
   int rc = scope.enter(device, &st);
@@ -884,6 +969,11 @@ static int bwd_launch(const void* q, const void* k, const void* v, const void* o
   p.scale = softmax_scale > 0.f ? softmax_scale : 1.0f / std::sqrt(float(D));
   p.scale_log2 = p.scale * 1.4426950408889634f;
   p.kv_lens = kv_lens;
+  p.window = window;
+  p.sinks = sinks;
+  p.shared_blocks = shared.blocks;
+  p.shares = shared.shares;
+  p.partial = static_cast<float*>(workspace);
   p.status = st->status;
 #ifdef HK_TRACE
   p.trace = g_trace_buf;
@@ -897,6 +987,8 @@ static int bwd_launch(const void* q, const void* k, const void* v, const void* o
                          !out.meets({k, s.k, B, NK, H_KV, D}) && !out.meets({v, s.v, B, NK, H_KV, D}) &&
                          !out.meets({lse, stats}) && !out.meets({delta, stats}) &&
                          !(kv_lens && out.meets({kv_lens, 4ll * B}));
+  if (mask == hk::kMaskWindow)
+    return (D == 128 ? launch_bwd_window<128> : launch_bwd_window<64>)(tq, tk, tv, tdo, p, dq_beside, st->sm_count, stream);
   if (D == 128) return causal ? launch_bwd<128, true>(tq, tk, tv, tdo, p, B, N, NK, H, H_KV, dq_beside, st->sm_count, st->bwd_clusters, stream)
                               : launch_bwd<128, false>(tq, tk, tv, tdo, p, B, N, NK, H, H_KV, dq_beside, st->sm_count, st->bwd_clusters, stream);
   return causal ? launch_bwd<64, true>(tq, tk, tv, tdo, p, B, N, NK, H, H_KV, dq_beside, st->sm_count, st->bwd_clusters, stream)
@@ -917,7 +1009,7 @@ int hk_attn_bwd_cross(const void* q, const void* k, const void* v, const void* d
   const long long dqs[3] = {(long long)N * H * D, D, (long long)N * D};  // [B, H, N, D]
   const BwdStrides s{qs, ks, ks, dq_layout == HK_DQ_BNHD ? qs : dqs, ks, ks};
   return bwd_launch(q, k, v, nullptr, d_o, lse, const_cast<float*>(delta), dq, dk, dv, B, N, NK, H, H_KV, D, s, kv_lens,
-                    causal, softmax_scale, device, cuda_stream);
+                    causal ? hk::kMaskCausal : hk::kMaskNone, 0, 0, nullptr, 0, softmax_scale, device, cuda_stream);
 }
 
 int hk_attn_bwd_strided(const void* q, const void* k, const void* v, const void* o, const void* d_o, const float* lse,
@@ -927,8 +1019,29 @@ int hk_attn_bwd_strided(const void* q, const void* k, const void* v, const void*
                         const int32_t* kv_lens, int causal, float softmax_scale, int device, void* cuda_stream) {
   if (!q_strides || !k_strides || !v_strides || !dq_strides || !dk_strides || !dv_strides) return HK_EINVAL;
   const BwdStrides s{q_strides, k_strides, v_strides, dq_strides, dk_strides, dv_strides};
-  return bwd_launch(q, k, v, o, d_o, lse, delta, dq, dk, dv, B, N, NK, H, H_KV, D, s, kv_lens, causal, softmax_scale,
-                    device, cuda_stream);
+  return bwd_launch(q, k, v, o, d_o, lse, delta, dq, dk, dv, B, N, NK, H, H_KV, D, s, kv_lens,
+                    causal ? hk::kMaskCausal : hk::kMaskNone, 0, 0, nullptr, 0, softmax_scale, device, cuda_stream);
+}
+
+size_t hk_attn_bwd_window_workspace_bytes(int B, int N, int NK, int H, int H_KV, int D, int window, int sinks) {
+  if (B <= 0 || N <= 0 || NK <= 0 || H <= 0 || H_KV <= 0 || H % H_KV != 0 || (D != 64 && D != 128) || window <= 0 || sinks < 0)
+    return 0;
+  if (window >= NK || sinks >= NK || 1ll * B * H_KV > 0x3fffffffll) return 0;
+  const WindowShares n = window_shares(B * H_KV, H / H_KV, N, NK, window, sinks);
+  return size_t(B) * H_KV * n.blocks * (n.blocks ? n.shares : 0) * 2 * hk::kBlockN * D * sizeof(float);
+}
+
+int hk_attn_bwd_window(const void* q, const void* k, const void* v, const void* o, const void* d_o, const float* lse,
+                       float* delta, void* dq, void* dk, void* dv, int B, int N, int NK, int H, int H_KV, int D,
+                       const long long* q_strides, const long long* k_strides, const long long* v_strides,
+                       const long long* dq_strides, const long long* dk_strides, const long long* dv_strides,
+                       const int32_t* kv_lens, int window, int sinks, float softmax_scale, void* workspace,
+                       size_t workspace_bytes, int device, void* cuda_stream) {
+  if (!q_strides || !k_strides || !v_strides || !dq_strides || !dk_strides || !dv_strides) return HK_EINVAL;
+  if (window <= 0 || sinks < 0) return HK_EINVAL;
+  const BwdStrides s{q_strides, k_strides, v_strides, dq_strides, dk_strides, dv_strides};
+  return bwd_launch(q, k, v, o, d_o, lse, delta, dq, dk, dv, B, N, NK, H, H_KV, D, s, kv_lens, hk::kMaskWindow, window, sinks,
+                    workspace, workspace_bytes, softmax_scale, device, cuda_stream);
 }
 
 int hk_key_padding_lens(const unsigned char* mask, int32_t* lens, int32_t* bad, int B, int N, int device,

@@ -146,11 +146,13 @@ PyObject* attn_fwd(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
-// attn_bwd_strided(q, k, v, o, d_o, lse, dq, dk, dv, causal, softmax_scale, kv_lens): 0 when launched
+// attn_bwd_strided(q, k, v, o, d_o, lse, dq, dk, dv, causal, softmax_scale, kv_lens[, window, sinks]): 0 when launched
 PyObject* attn_bwd_strided(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   HANDLE_TH_ERRORS
   float scale;
-  if (n_args != 12 || !PyBool_Check(a[9]) || !number(a[10], scale)) Py_RETURN_NONE;
+  int window, sinks;
+  if (!window_args(a, n_args, 12, window, sinks) || !PyBool_Check(a[9]) || !number(a[10], scale)) Py_RETURN_NONE;
+  if (window && a[9] != Py_True) Py_RETURN_NONE;
   const Tensor *q = plain(a[0]), *k = plain(a[1]), *v = plain(a[2]), *o = plain(a[3]), *d_o = plain(a[4]),
                *lse = plain(a[5]), *dq = plain(a[6]), *dk = plain(a[7]), *dv = plain(a[8]);
   for (const Tensor* t : {q, k, v, dq, dk, dv})
@@ -175,6 +177,10 @@ PyObject* attn_bwd_strided(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   }
   const Tensor delta = at::empty({b, h, 1, n}, lse->options().requires_grad(false));
   if (!delta.has_storage()) Py_RETURN_NONE;
+  Tensor ws;
+  const size_t need =
+      window ? hk_attn_bwd_window_workspace_bytes(i32(b), i32(n), i32(nk), i32(h), i32(hkv), i32(d), window, sinks) : 0;
+  if (need && !output(Py_None, *q, {int64_t(need)}, at::kByte, ws)) Py_RETURN_NONE;
   void* stream = stream_of(*q);
   const int causal = a[9] == Py_True, dev = q->device().index();
   const void *qp = ptr(*q), *kp = ptr(*k), *vp = ptr(*v), *op = ptr(*o), *dop = ptr(*d_o);
@@ -182,7 +188,12 @@ PyObject* attn_bwd_strided(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   float* deltap = ptr<float>(delta);
   void *dqp = ptr(*dq), *dkp = ptr(*dk), *dvp = ptr(*dv);
   const int32_t* lensp = lens ? ptr<int32_t>(*lens) : nullptr;
+  void* wsp = need ? ptr(ws) : nullptr;
   const int rc = unlocked([&] {
+    if (window)
+      return hk_attn_bwd_window(qp, kp, vp, op, dop, lsep, deltap, dqp, dkp, dvp, i32(b), i32(n), i32(nk), i32(h), i32(hkv),
+                                i32(d), st[0], st[1], st[2], st[3], st[4], st[5], lensp, window, sinks, scale, wsp, need, dev,
+                                stream);
     return hk_attn_bwd_strided(qp, kp, vp, op, dop, lsep, deltap, dqp, dkp, dvp, i32(b), i32(n), i32(nk), i32(h),
                                i32(hkv), i32(d), st[0], st[1], st[2], st[3], st[4], st[5], lensp, causal, scale, dev,
                                stream);

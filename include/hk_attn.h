@@ -209,6 +209,19 @@ int hk_attn_bwd_strided(const void* q, const void* k, const void* v, const void*
                         const long long* dq_strides, const long long* dk_strides, const long long* dv_strides,
                         const int32_t* kv_lens, int causal, float softmax_scale, int device, void* cuda_stream);
 
+/* The backward of hk_attn_fwd_window: hk_attn_bwd_strided(causal = 1) with its window and sinks. Results are bit-identical from run to
+ * run; dK and dV of the sinks' key blocks, and where there are few blocks of all, are sums of shares in a fixed order, in places
+ * that depend on the whole call's shape.
+ *   workspace : device scratch of at least hk_attn_bwd_window_workspace_bytes(...) bytes, 256-byte aligned, for those shares; the
+ *               size may be 0, and then NULL is taken. */
+size_t hk_attn_bwd_window_workspace_bytes(int B, int Nq, int Nk, int H, int H_KV, int D, int window, int sinks);
+int hk_attn_bwd_window(const void* q, const void* k, const void* v, const void* o, const void* d_o, const float* lse,
+                       float* delta, void* dq, void* dk, void* dv, int B, int Nq, int Nk, int H, int H_KV, int D,
+                       const long long* q_strides, const long long* k_strides, const long long* v_strides,
+                       const long long* dq_strides, const long long* dk_strides, const long long* dv_strides,
+                       const int32_t* kv_lens, int window, int sinks, float softmax_scale, void* workspace,
+                       size_t workspace_bytes, int device, void* cuda_stream);
+
 /* Key lengths of a right-padded batch: mask is DEVICE bool (one byte) [B, N] contiguous, True = keep (base.py:88-103);
  * lens[b] = kept keys of row b. *bad, zero on entry, becomes 1 if a row does not keep a prefix of at least one key. */
 int hk_key_padding_lens(const unsigned char* mask, int32_t* lens, int32_t* bad, int B, int N, int device,
