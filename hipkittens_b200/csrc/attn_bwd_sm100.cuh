@@ -448,12 +448,13 @@ __device__ __forceinline__ DkdvItem decode_dkdv_item(const BwdParams& p, int idx
 // SPLIT: an item is shared by the CTAs of a cluster (p.split of them), each with its part of the (head, query tile) pairs; the
 // partial dK and dV are added up through distributed shared memory, row by row in the order of the ranks, so that the
 // gradients stay the same from run to run. One item per cluster and launch.
-template <int D, int MASK, bool SPLIT>
+template <int D, auto KIND, bool SPLIT>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                      const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_do,
                      const BwdParams p) {
   using namespace ptx;
+  constexpr int MASK = static_cast<int>(KIND);
   constexpr bool CAUSAL = MASK != kMaskNone, WINDOW = MASK == kMaskWindow;
   using SM = BwdSmem<D>;
   constexpr int kTile = SM::kTileBytes;
@@ -1112,12 +1113,13 @@ __device__ __forceinline__ DqItemOf<MASK> decode_dq_item(const BwdParams& p, int
   return w;
 }
 
-template <int D, int MASK>
+template <int D, auto KIND>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                    const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_do,
                    const BwdParams p) {
   using namespace ptx;
+  constexpr int MASK = static_cast<int>(KIND);
   constexpr bool CAUSAL = MASK != kMaskNone, WINDOW = MASK == kMaskWindow;
   using SM = BwdSmem<D>;
   constexpr int kTile = SM::kTileBytes;

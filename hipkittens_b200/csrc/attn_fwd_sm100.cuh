@@ -81,6 +81,7 @@ constexpr uint64_t kWaitLimitCycles = 8000ull * 1000 * 1000;  // SM cycles, > 4 
 enum : int { kStatusOk = 0, kStatusTimeout = 1, kStatusFwdBadPage = 2 };  // 2 = the decode kernels' kStatusBadPage
 
 // What a query row sees: every key, those up to its own position, or of those the last `window` and the first `sinks`.
+// Where a template takes `auto KIND` it is false, true or kMaskWindow: whether a call is causal, which a call with a window is too.
 enum Mask : int { kMaskNone = 0, kMaskCausal = 1, kMaskWindow = 2 };
 
 // Division of a non-negative int below 2^31 by a divisor fixed at launch: a multiply-high and a shift instead of the
@@ -306,16 +307,17 @@ inline void set_item_decode(FwdParams& p) {
 // -> without): B16 N4096 H16 D64 1317.0 -> 1309.4, B4 N8192 H64/8 D128 causal 3414 -> 3407, B8 N4096 H32/8 D64 causal
 // 0.3 % less; but B16 N2048 H64/8 D128 1718.6 -> 1722.4, which therefore keeps them. A run-time branch around them is
 // no way out: it costs D128 0.5 %.
-template <int D, int MASK>
-constexpr bool kLongFwdDependent = D == 128 && MASK == kMaskNone;
+template <int D, auto KIND>
+constexpr bool kLongFwdDependent = D == 128 && KIND == kMaskNone;
 
 // DEP: may be launched as a dependent (launch_dependent with `early`); false: only the ordinary way.
-template <int D, int MASK, bool DEP>
+template <int D, auto KIND, bool DEP>
 __global__ void __launch_bounds__(kFwdThreads, 1)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                 const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ CUtensorMap tmap_o,
                 const FwdParams p) {
   using namespace ptx;
+  constexpr int MASK = static_cast<int>(KIND);
   constexpr bool CAUSAL = MASK != kMaskNone, WINDOW = MASK == kMaskWindow;
   using SM = FwdSmem<D, CAUSAL>;
   constexpr int kStages = SM::kStages;

@@ -66,10 +66,10 @@ struct DeviceState {
 };
 DeviceState g_dev[kMaxDevices];
 
-template <int D, int MASK, bool DEP>
+template <int D, auto KIND, bool DEP>
 int prepare_fwd_kernel() {
-  auto* fn = hk::attn_fwd_kernel<D, MASK, DEP>;
-  HK_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, hk::FwdSmem<D, MASK != hk::kMaskNone>::kDynBytes));
+  auto* fn = hk::attn_fwd_kernel<D, KIND, DEP>;
+  HK_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, hk::FwdSmem<D, int(KIND) != hk::kMaskNone>::kDynBytes));
   cudaFuncAttributes attr;
   HK_CUDA(cudaFuncGetAttributes(&attr, fn));
   // The kernel re-balances registers between warpgroups (208 per softmax thread, 88 per producer thread);
@@ -77,17 +77,17 @@ int prepare_fwd_kernel() {
   // Refuse to launch otherwise: a register pool that is too small would block the re-allocation forever.
   if (attr.numRegs != hk::kFwdRegsAtLaunch) {
     snprintf(g_cuda_err, sizeof(g_cuda_err), "attn_fwd_kernel<%d,%d,%d> compiled to %d registers, expected %d", D,
-             MASK, int(DEP), attr.numRegs, hk::kFwdRegsAtLaunch);
+             int(KIND), int(DEP), attr.numRegs, hk::kFwdRegsAtLaunch);
     return HK_EUNSUPPORTED;
   }
   return HK_OK;
 }
 
-template <int D, int MASK>
+template <int D, auto KIND>
 int prepare_fwd_kernels() {
-  const int rc = prepare_fwd_kernel<D, MASK, true>();
+  const int rc = prepare_fwd_kernel<D, KIND, true>();
   if (rc != HK_OK) return rc;
-  return prepare_fwd_kernel<D, MASK, hk::kLongFwdDependent<D, MASK>>();
+  return prepare_fwd_kernel<D, KIND, hk::kLongFwdDependent<D, KIND>>();
 }
 
 template <typename Kernel>
@@ -109,15 +109,15 @@ int prepare_bwd_kernel(Kernel* fn, int dyn_bytes, const char* name) {
   return HK_OK;
 }
 
-template <int D, int MASK>
+template <int D, auto KIND>
 int prepare_bwd_kernels() {
-  int rc = prepare_bwd_kernel(hk::attn_bwd_dkdv_kernel<D, MASK, false>, hk::BwdSmem<D>::kDynBytes, "attn_bwd_dkdv_kernel");
+  int rc = prepare_bwd_kernel(hk::attn_bwd_dkdv_kernel<D, KIND, false>, hk::BwdSmem<D>::kDynBytes, "attn_bwd_dkdv_kernel");
   if (rc != HK_OK) return rc;
-  if constexpr (MASK != hk::kMaskWindow) {
-    rc = prepare_bwd_kernel(hk::attn_bwd_dkdv_kernel<D, MASK, true>, hk::BwdSmem<D>::kDynBytes, "attn_bwd_dkdv_kernel");
+  if constexpr (int(KIND) != hk::kMaskWindow) {
+    rc = prepare_bwd_kernel(hk::attn_bwd_dkdv_kernel<D, KIND, true>, hk::BwdSmem<D>::kDynBytes, "attn_bwd_dkdv_kernel");
     if (rc != HK_OK) return rc;
   }
-  return prepare_bwd_kernel(hk::attn_bwd_dq_kernel<D, MASK>, hk::BwdSmem<D>::kDynBytes, "attn_bwd_dq_kernel");
+  return prepare_bwd_kernel(hk::attn_bwd_dq_kernel<D, KIND>, hk::BwdSmem<D>::kDynBytes, "attn_bwd_dq_kernel");
 }
 
 int init_device(int device) {
@@ -132,19 +132,19 @@ int init_device(int device) {
     return HK_EUNSUPPORTED;
   }
   int rc;
-  if ((rc = prepare_fwd_kernels<128, hk::kMaskNone>()) != HK_OK) return rc;
-  if ((rc = prepare_fwd_kernels<128, hk::kMaskCausal>()) != HK_OK) return rc;
+  if ((rc = prepare_fwd_kernels<128, false>()) != HK_OK) return rc;
+  if ((rc = prepare_fwd_kernels<128, true>()) != HK_OK) return rc;
   if ((rc = prepare_fwd_kernels<128, hk::kMaskWindow>()) != HK_OK) return rc;
-  if ((rc = prepare_fwd_kernels<64, hk::kMaskNone>()) != HK_OK) return rc;
-  if ((rc = prepare_fwd_kernels<64, hk::kMaskCausal>()) != HK_OK) return rc;
+  if ((rc = prepare_fwd_kernels<64, false>()) != HK_OK) return rc;
+  if ((rc = prepare_fwd_kernels<64, true>()) != HK_OK) return rc;
   if ((rc = prepare_fwd_kernels<64, hk::kMaskWindow>()) != HK_OK) return rc;
   if ((rc = hk::prepare_decode_kernels(g_cuda_err, sizeof(g_cuda_err), st.sm_count, &st.decode)) != HK_OK) return rc;
   if ((rc = hk::prepare_window_decode_kernels(g_cuda_err, sizeof(g_cuda_err))) != HK_OK) return rc;
-  if ((rc = prepare_bwd_kernels<128, hk::kMaskNone>()) != HK_OK) return rc;
-  if ((rc = prepare_bwd_kernels<128, hk::kMaskCausal>()) != HK_OK) return rc;
+  if ((rc = prepare_bwd_kernels<128, false>()) != HK_OK) return rc;
+  if ((rc = prepare_bwd_kernels<128, true>()) != HK_OK) return rc;
   if ((rc = prepare_bwd_kernels<128, hk::kMaskWindow>()) != HK_OK) return rc;
-  if ((rc = prepare_bwd_kernels<64, hk::kMaskNone>()) != HK_OK) return rc;
-  if ((rc = prepare_bwd_kernels<64, hk::kMaskCausal>()) != HK_OK) return rc;
+  if ((rc = prepare_bwd_kernels<64, false>()) != HK_OK) return rc;
+  if ((rc = prepare_bwd_kernels<64, true>()) != HK_OK) return rc;
   if ((rc = prepare_bwd_kernels<64, hk::kMaskWindow>()) != HK_OK) return rc;
   for (int n = 2; n <= hk::kMaxDkdvSplit; ++n)
     st.bwd_clusters[n] = hk::clusters_held(hk::attn_bwd_dkdv_kernel<128, true, true>, hk::kBwdThreads, hk::BwdSmem<128>::kDynBytes, n);
@@ -319,12 +319,12 @@ int kv_tiles(int NK, int mask, int window, int sinks) {
   return int(std::min(all, live));
 }
 
-template <int D, int MASK>
+template <int D, auto KIND>
 int launch_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& to,
                const hk::FwdParams& p, int grid, cudaStream_t stream) {
-  const bool early = short_kernel(1ll * p.n_items * kv_tiles(p.NK, MASK, p.window, p.sinks), grid);
-  auto* fn = early ? hk::attn_fwd_kernel<D, MASK, true> : hk::attn_fwd_kernel<D, MASK, hk::kLongFwdDependent<D, MASK>>;
-  HK_CUDA(hk::launch_dependent(early, fn, grid, hk::kFwdThreads, hk::FwdSmem<D, MASK != hk::kMaskNone>::kDynBytes, stream, tq, tk, tv, to, p));
+  const bool early = short_kernel(1ll * p.n_items * kv_tiles(p.NK, int(KIND), p.window, p.sinks), grid);
+  auto* fn = early ? hk::attn_fwd_kernel<D, KIND, true> : hk::attn_fwd_kernel<D, KIND, hk::kLongFwdDependent<D, KIND>>;
+  HK_CUDA(hk::launch_dependent(early, fn, grid, hk::kFwdThreads, hk::FwdSmem<D, int(KIND) != hk::kMaskNone>::kDynBytes, stream, tq, tk, tv, to, p));
   g_launches.fetch_add(1, std::memory_order_relaxed);
   return HK_OK;
 }
@@ -771,8 +771,8 @@ static int fwd_launch(const void* q, const void* k, const void* v, void* o, floa
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
   const bool d128 = D == 128;
   auto* launch = mask == hk::kMaskWindow   ? (d128 ? launch_fwd<128, hk::kMaskWindow> : launch_fwd<64, hk::kMaskWindow>)
-                 : mask == hk::kMaskCausal ? (d128 ? launch_fwd<128, hk::kMaskCausal> : launch_fwd<64, hk::kMaskCausal>)
-                                           : (d128 ? launch_fwd<128, hk::kMaskNone> : launch_fwd<64, hk::kMaskNone>);
+                 : mask == hk::kMaskCausal ? (d128 ? launch_fwd<128, true> : launch_fwd<64, true>)
+                                           : (d128 ? launch_fwd<128, false> : launch_fwd<64, false>);
   return launch(tq, tk, tv, to, p, grid, stream);
 }
 
