@@ -634,18 +634,25 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
             su[q4 * 4 + 2] = __float_as_uint(x2);
             su[q4 * 4 + 3] = __float_as_uint(x3);
           }
-          if (diag) {
+          if constexpr (WINDOW) {
+            // ... iff query + off - key lies in [0, window), or key < sinks and it is not negative
+            const bool far = (w.j + 1) * kBlockN > p.sinks && (i_t - w.j) * kBlockM + kBlockM - 1 + w.off >= p.window;
+            if (diag || far) {
+              const int own = row + (w.j - i_t) * kBlockN - w.off - part * kBwdPC;  // the column of the query at the key's position
+              const int end = w.j * kBlockN + row < p.sinks ? kBwdPC : own + p.window;
+#pragma unroll
+              for (int cc = 0; cc < kBwdPC / 32; ++cc) {
+                const uint32_t seen = seen_bits(cc * 32, own, end - 1, 0);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) su[cc * 32 + i] = (seen >> i) & 1u ? su[cc * 32 + i] : 0u;
+              }
+            }
+          } else if (diag) {
             // key j*128 + row is seen by query i_t*128 + col iff key <= query + off: earlier queries see nothing
             // (this also zeroes the infinities that rows without any key, whose L is -inf, produce above)
             const int lim = row + (w.j - i_t) * kBlockN - w.off;
 #pragma unroll
             for (int col = 0; col < kBwdPC; ++col) su[col] = (part * kBwdPC + col) < lim ? 0u : su[col];
-          }
-          if (WINDOW && (w.j + 1) * kBlockN > p.sinks && (i_t - w.j) * kBlockM + kBlockM - 1 + w.off >= p.window) {
-            // a query tile some rows of which are a window or more behind some of the keys
-            const int lim = w.j * kBlockN + row < p.sinks ? 0x7fffffff : row + (w.j - i_t) * kBlockN - w.off + p.window;
-#pragma unroll
-            for (int col = 0; col < kBwdPC; ++col) su[col] = (part * kBwdPC + col) >= lim ? 0u : su[col];
           }
           if (pad_block) {
             // a padded key is seen by nobody: P^T and dS^T rows are zero, so are its dK and dV rows
@@ -1256,19 +1263,25 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             su[2 * i] = __float_as_uint(x0);
             su[2 * i + 1] = __float_as_uint(x1);
           }
-          if (diag) {
+          if constexpr (WINDOW) {
+            // ... or behind the window of some rows: a first key that the tile's last row does not see
+            const bool far = kv * kBlockN <= w.i * kBlockM + kBlockM - 1 + w.off - p.window && (kv + 1) * kBlockN > p.sinks;
+            if (diag || far) {
+              const int base = kv * kBlockN + part * kBwdPC, own = w.i * kBlockM + row + w.off;
+              const int hi = min(own, w.kv_len - 1) - base, lo = own - p.window + 1 - base;
+#pragma unroll
+              for (int cc = 0; cc < kBwdPC / 32; ++cc) {
+                const uint32_t seen = seen_bits(cc * 32, lo, hi, p.sinks - base);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) su[cc * 32 + i] = (seen >> i) & 1u ? su[cc * 32 + i] : 0u;
+              }
+            }
+          } else if (diag) {
             // key n*128 + col is seen by query i*128 + row iff it is <= query + off and < kv_len (this also zeroes
             // the infinities of a row without any key, whose L is -inf)
             const int lim = min(w.i * kBlockM + row + w.off, w.kv_len - 1) - kv * kBlockN;
 #pragma unroll
             for (int col = 0; col < kBwdPC; ++col) su[col] = (part * kBwdPC + col) > lim ? 0u : su[col];
-          }
-          if (WINDOW && kv * kBlockN <= w.i * kBlockM + kBlockM - 1 + w.off - p.window && (kv + 1) * kBlockN > p.sinks) {
-            // a tile whose first key some rows have behind their window
-            const int lo = w.i * kBlockM + row + w.off - p.window + 1 - kv * kBlockN, sinks = p.sinks - kv * kBlockN;
-#pragma unroll
-            for (int col = 0; col < kBwdPC; ++col)
-              su[col] = (part * kBwdPC + col) < lo && (part * kBwdPC + col) >= sinks ? 0u : su[col];
           }
           if (!CAUSAL && n == w.n_iter - 1 && (w.kv_len & (kBlockN - 1)) != 0) {
             // partial last tile: keys at or beyond the length are padding
