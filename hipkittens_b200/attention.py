@@ -25,7 +25,7 @@ import torch.nn as nn
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
-from ._native import _check_window, attn_bwd_strided, attn_fwd, device_status, key_padding_lens, qk_norm_rotary, qk_norm_rotary_bwd
+from ._native import _check_window, _front, attn_bwd_strided, attn_fwd, device_status, key_padding_lens, qk_norm_rotary, qk_norm_rotary_bwd
 
 
 def _tma_viewable(t: torch.Tensor) -> bool:
@@ -148,6 +148,9 @@ def _attend(q, packed, causal, softmax_scale, key_padding_mask, window=None, sin
 
 
 def _apply(q, packed, causal, softmax_scale, kv_lens, window, sinks):
+    out = _front().packed_attention(q, packed, bool(causal), softmax_scale, kv_lens, window, sinks)
+    if out is not None:
+        return out
     if _packed_viewable(packed) and (q is None or _tma_viewable(q)):
         return _PackedAttnFunction.apply(q, packed, bool(causal), softmax_scale, kv_lens, window, sinks)
     views = packed.unbind(dim=2) if q is None else (q, *packed.unbind(dim=2))
@@ -220,8 +223,15 @@ class QkNormRotaryFunction(Function):
     """``qk_norm_rotary`` with gradients of q, k and the weights. The tables are constants. Asynchronous in both directions, as
     the call itself is."""
 
+    @classmethod
+    def apply(cls, q, k, q_weight, k_weight, cos, sin, positions=None, pos_offset=0, eps=1e-6, interleaved=False):
+        out = _front().norm_rotary(q, k, q_weight, k_weight, cos, sin, positions, pos_offset, eps, interleaved)
+        if out is not None:
+            return out
+        return super().apply(q, k, q_weight, k_weight, cos, sin, positions, pos_offset, eps, interleaved)
+
     @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions=None, pos_offset=0, eps=1e-6, interleaved=False):
+    def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, pos_offset, eps, interleaved):
         if ctx.needs_input_grad[4] or ctx.needs_input_grad[5]:
             raise RuntimeError("cos and sin have no gradients: pass tensors that do not require them")
         ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)

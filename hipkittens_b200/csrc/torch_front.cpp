@@ -12,7 +12,11 @@
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+
+#include <optional>
 
 #include "../../include/hk_attn.h"
 
@@ -478,10 +482,273 @@ PyObject* paged_kv_append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- autograd. A step through the Python functions behind these spends about 55 us on them, in the caller's thread and in the
+// engine's, which has to have the interpreter for its part; small steps are made of little else.
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// Thrown by a forward that the Python code behind is to look at: it makes the call again, and raises what there is to raise.
+struct Refused {};
+
+void fail(const char* what, int rc) {
+  TORCH_CHECK(false, what, ": error ", rc, " (", hk_strerror(rc), ")");
+}
+// Waits for the device, as the Python functions do behind each direction.
+void check_device(int device, const char* direction) {
+  const int status = hk_last_device_status(device);
+  TORCH_CHECK(status == HK_OK, "attention ", direction, " failed on the device (status ", status, ")");
+}
+
+// The parts of a packed projection [B, S, 2 or 3, H, D], or of its gradient.
+struct Parts {
+  char* base;
+  int64_t part;       // bytes between two of them
+  long long st[3];    // element strides of batch, sequence and head
+  bool good;          // as the kernels read and write them
+  explicit Parts(const Tensor& t) : base(static_cast<char*>(t.data_ptr())), part(2 * t.stride(2)) {
+    good = t.stride(4) == 1 && t.stride(2) % 8 == 0 && (reinterpret_cast<uintptr_t>(base) & 15) == 0;
+    int i = 0;
+    for (int dim : {0, 1, 3}) {
+      st[i] = t.stride(dim);
+      good = good && st[i] > 0 && st[i] % 8 == 0;
+      ++i;
+    }
+  }
+  void* at(int i) const { return base + i * part; }
+};
+
+// One call of the attention modules: q [B, Sq, H, D] with packed [B, Sk, 2, H_KV, D], or an undefined q and packed [B, S, 3, H, D].
+struct Attention {
+  bool causal;
+  float scale;
+  int window, sinks;
+  Tensor lens;
+  int b, n, nk, h, hkv, d, device;
+  void shape(const Tensor& q, const Tensor& packed) {
+    b = i32(packed.size(0)), nk = i32(packed.size(1)), hkv = i32(packed.size(3)), d = i32(packed.size(4));
+    n = q.defined() ? i32(q.size(1)) : nk, h = q.defined() ? i32(q.size(2)) : hkv;
+    device = packed.device().index();
+  }
+  const int32_t* lens_ptr() const { return lens.defined() ? ptr<int32_t>(lens) : nullptr; }
+};
+
+class PackedAttention : public torch::autograd::Function<PackedAttention> {
+ public:
+  static Tensor forward(AutogradContext* ctx, const std::optional<Tensor>& q_or_none, const Tensor& packed, const Attention& a) {
+    const Tensor q = q_or_none.value_or(Tensor());
+    const Tensor o = at::empty({a.b, a.n, a.h, a.d}, packed.options().requires_grad(false));
+    const Tensor lse = at::empty({a.b, a.h, 1, a.n}, packed.options().dtype(at::kFloat).requires_grad(false));
+    const Parts p(packed);
+    long long qs[3] = {p.st[0], p.st[1], p.st[2]};
+    const bool own_q = q.defined();
+    if (!p.good || (own_q && !tma_strides(q, qs))) throw Refused();
+    const void *qp = own_q ? ptr(q) : p.at(0), *kp = p.at(own_q ? 0 : 1), *vp = p.at(own_q ? 1 : 2);
+    void *op = ptr(o), *stream = stream_of(packed);
+    float* lp = ptr<float>(lse);
+    const int32_t* lens = a.lens_ptr();
+    int rc = HK_OK, status = HK_OK;
+    unlocked([&] {
+      rc = a.window ? hk_attn_fwd_window(qp, kp, vp, op, lp, a.b, a.n, a.nk, a.h, a.hkv, a.d, qs, p.st, p.st, lens, a.window, a.sinks,
+                                         a.scale, a.device, stream)
+                    : hk_attn_fwd_cross(qp, kp, vp, op, lp, a.b, a.n, a.nk, a.h, a.hkv, a.d, qs, p.st, p.st, lens, a.causal, a.scale,
+                                        a.device, stream);
+      if (rc == HK_OK) status = hk_last_device_status(a.device);
+      return rc;
+    });
+    if (rc != HK_OK) throw Refused();
+    TORCH_CHECK(status == HK_OK, "attention forward failed on the device (status ", status, ")");
+    ctx->save_for_backward({q, packed, o, lse});
+    ctx->saved_data["causal"] = a.causal;
+    ctx->saved_data["scale"] = static_cast<double>(a.scale);
+    ctx->saved_data["window"] = int64_t(a.window);
+    ctx->saved_data["sinks"] = int64_t(a.sinks);
+    if (a.lens.defined()) ctx->saved_data["lens"] = a.lens;
+    return o;
+  }
+
+  // In a thread of the engine, without the interpreter.
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    // saved-tensor hooks may have given them back in a layout that the kernels do not read
+    Tensor q = saved[0], packed = saved[1];
+    const Tensor o = saved[2].contiguous(), lse = saved[3].contiguous();
+    TORCH_CHECK(grads[0].defined() && grads[0].sizes() == o.sizes(), "dO shape mismatch: expected ", o.sizes());
+    TORCH_CHECK(grads[0].device() == o.device(), "dO must be on correct CUDA device");
+    const Tensor d_o = grads[0].to(at::kBFloat16).contiguous();
+    if (!Parts(packed).good) packed = packed.contiguous();
+    const Parts p(packed);
+    long long qs[3] = {p.st[0], p.st[1], p.st[2]};
+    if (q.defined() && !tma_strides(q, qs)) {
+      q = q.contiguous();
+      tma_strides(q, qs);
+    }
+    Attention a;
+    a.shape(q, packed);
+    a.causal = ctx->saved_data["causal"].toBool();
+    a.scale = static_cast<float>(ctx->saved_data["scale"].toDouble());
+    a.window = i32(ctx->saved_data["window"].toInt()), a.sinks = i32(ctx->saved_data["sinks"].toInt());
+    if (const auto it = ctx->saved_data.find("lens"); it != ctx->saved_data.end()) a.lens = it->second.toTensor();
+    const Tensor d_packed = at::empty(packed.sizes(), packed.options().requires_grad(false));
+    const Tensor dq = q.defined() ? at::empty(q.sizes(), q.options().requires_grad(false)) : Tensor();
+    const Tensor delta = at::empty(lse.sizes(), lse.options().requires_grad(false));
+    const Parts dp(d_packed);
+    const size_t need = a.window ? hk_attn_bwd_window_workspace_bytes(a.b, a.n, a.nk, a.h, a.hkv, a.d, a.window, a.sinks) : 0;
+    const Tensor ws = need ? at::empty({int64_t(need)}, packed.options().dtype(at::kByte).requires_grad(false)) : Tensor();
+    const bool own_q = q.defined();
+    long long dqs[3] = {dp.st[0], dp.st[1], dp.st[2]};
+    if (own_q) tma_strides(dq, dqs);
+    const void *qp = own_q ? ptr(q) : p.at(0), *kp = p.at(own_q ? 0 : 1), *vp = p.at(own_q ? 1 : 2);
+    void *dqp = own_q ? ptr(dq) : dp.at(0), *dkp = dp.at(own_q ? 0 : 1), *dvp = dp.at(own_q ? 1 : 2);
+    void *stream = stream_of(packed), *wsp = need ? ptr(ws) : nullptr;
+    const int rc =
+        a.window ? hk_attn_bwd_window(qp, kp, vp, ptr(o), ptr(d_o), ptr<float>(lse), ptr<float>(delta), dqp, dkp, dvp, a.b, a.n, a.nk,
+                                      a.h, a.hkv, a.d, qs, p.st, p.st, dqs, dp.st, dp.st, a.lens_ptr(), a.window, a.sinks, a.scale,
+                                      wsp, need, a.device, stream)
+                 : hk_attn_bwd_strided(qp, kp, vp, ptr(o), ptr(d_o), ptr<float>(lse), ptr<float>(delta), dqp, dkp, dvp, a.b, a.n, a.nk,
+                                       a.h, a.hkv, a.d, qs, p.st, p.st, dqs, dp.st, dp.st, a.lens_ptr(), a.causal, a.scale, a.device,
+                                       stream);
+    if (rc != HK_OK) fail("hk_attn_bwd_strided", rc);
+    check_device(a.device, "backward");
+    return {dq, d_packed, Tensor()};
+  }
+};
+
+// packed_attention(q or None, packed, causal, softmax_scale, kv_lens, window or None, sinks): O, or None
+PyObject* packed_attention(PyObject*, PyObject* const* arg, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  Attention a;
+  if (n_args != 7 || !PyBool_Check(arg[2]) || !number(arg[3], a.scale)) Py_RETURN_NONE;
+  a.window = a.sinks = 0;
+  if (arg[5] != Py_None && !window_args(arg, n_args, 5, a.window, a.sinks)) Py_RETURN_NONE;
+  a.causal = arg[2] == Py_True;
+  if (a.window && !a.causal) Py_RETURN_NONE;
+  const Tensor *q = nullptr, *packed = plain(arg[1]);
+  if (!is(packed, at::kBFloat16, 5) || packed->size(2) != (arg[0] == Py_None ? 3 : 2)) Py_RETURN_NONE;
+  for (int64_t v : packed->sizes())
+    if (v == 0 || !fits({v})) Py_RETURN_NONE;
+  if (arg[0] != Py_None) {
+    q = plain(arg[0]);
+    if (!is(q, at::kBFloat16, 4) || q->size(0) != packed->size(0) || q->size(3) != packed->size(4) ||
+        q->size(2) % packed->size(3) != 0 || q->device() != packed->device() || q->numel() == 0 || !fits({q->size(1), q->size(2)}))
+      Py_RETURN_NONE;
+  }
+  if (arg[4] != Py_None) {
+    const Tensor* lens = plain(arg[4]);
+    if (!dense(lens, at::kInt, 1) || lens->size(0) != packed->size(0) || lens->device() != packed->device()) Py_RETURN_NONE;
+    a.lens = *lens;
+  }
+  const Tensor none;
+  a.shape(q ? *q : none, *packed);
+  try {
+    return THPVariable_Wrap(PackedAttention::apply(q ? std::optional<Tensor>(*q) : std::nullopt, *packed, a));
+  } catch (const Refused&) {
+    Py_RETURN_NONE;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
+// One call of the norm and rotation, as its gradients need it.
+struct QknCall {
+  long long qs[3], ks[3];
+  int flags, pos_offset, b, n, h, hkv, d, r, rows, device;
+  float eps;
+};
+
+class NormRotary : public torch::autograd::Function<NormRotary> {
+ public:
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const std::optional<Tensor>& q_weight,
+                               const std::optional<Tensor>& k_weight, const Tensor& cos, const Tensor& sin,
+                               const std::optional<Tensor>& positions_or_none, const QknCall& c) {
+    const Tensor none, wq = q_weight.value_or(none), wk = k_weight.value_or(none), positions = positions_or_none.value_or(none);
+    const Tensor qo = at::empty(q.sizes(), q.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
+    const Tensor ko = at::empty(k.sizes(), k.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
+    const void *qp = ptr(q), *kp = ptr(k), *wqp = wq.defined() ? ptr(wq) : nullptr, *wkp = wk.defined() ? ptr(wk) : nullptr,
+               *cp = ptr(cos), *sp = ptr(sin);
+    const int32_t* pp = positions.defined() ? ptr<int32_t>(positions) : nullptr;
+    void *qop = ptr(qo), *kop = ptr(ko), *stream = stream_of(q);
+    const int rc = unlocked([&] {
+      return hk_qk_norm_rotary(qp, kp, wqp, wkp, cp, sp, qop, kop, c.b, c.n, c.h, c.hkv, c.d, c.r, c.rows, c.qs, c.ks, pp,
+                               c.pos_offset, c.eps, c.flags, c.device, stream);
+    });
+    if (rc != HK_OK) throw Refused();
+    ctx->save_for_backward({q, k, wq, wk, cos, sin, positions});
+    ctx->saved_data["flags"] = int64_t(c.flags);
+    ctx->saved_data["offset"] = int64_t(c.pos_offset);
+    ctx->saved_data["eps"] = static_cast<double>(c.eps);
+    return {qo, ko};
+  }
+
+  // In a thread of the engine, without the interpreter.
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list s = ctx->get_saved_variables();
+    QknCall c;
+    long long* const st[2] = {c.qs, c.ks};
+    Tensor dy[2], dx[2], dw[2];
+    bool weights = false;  // the tensors of the call are numbered without those that it does not have
+    for (size_t i = 2, end = 2 + s[2].defined() + s[3].defined(); i < end; ++i) weights |= ctx->needs_input_grad(i);
+    for (int i = 0; i < 2; ++i) {
+      if (!tma_strides(s[i], st[i])) {  // saved-tensor hooks may have given it back in another layout
+        s[i] = s[i].contiguous();
+        tma_strides(s[i], st[i]);
+      }
+      dy[i] = grads[i].defined() ? grads[i].to(at::kBFloat16).contiguous()
+                                 : at::zeros(s[i].sizes(), s[i].options().requires_grad(false));
+      dx[i] = at::empty(s[i].sizes(), s[i].options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
+      if (weights && s[2 + i].defined()) {
+        s[2 + i] = s[2 + i].contiguous();
+        dw[i] = at::empty(s[2 + i].sizes(), s[2 + i].options().requires_grad(false));
+      }
+    }
+    for (int i = 2; i < 7; ++i)
+      if (s[i].defined()) s[i] = s[i].contiguous();
+    const size_t need = dw[0].defined() || dw[1].defined() ? hk_qk_norm_rotary_bwd_workspace_bytes(i32(s[0].size(3))) : 0;
+    const Tensor ws = need ? at::empty({int64_t(need)}, s[0].options().dtype(at::kByte).requires_grad(false)) : Tensor();
+    auto opt = [](const Tensor& t) { return t.defined() ? ptr(t) : nullptr; };
+    const int rc = hk_qk_norm_rotary_bwd(
+        ptr(s[0]), ptr(s[1]), opt(s[2]), opt(s[3]), ptr(s[4]), ptr(s[5]), ptr(dy[0]), ptr(dy[1]), ptr(dx[0]), ptr(dx[1]), opt(dw[0]),
+        opt(dw[1]), i32(s[0].size(0)), i32(s[0].size(1)), i32(s[0].size(2)), i32(s[1].size(2)), i32(s[0].size(3)),
+        i32(2 * s[4].size(1)), i32(s[4].size(0)), c.qs, c.ks, static_cast<const int32_t*>(opt(s[6])),
+        i32(ctx->saved_data["offset"].toInt()), static_cast<float>(ctx->saved_data["eps"].toDouble()),
+        i32(ctx->saved_data["flags"].toInt()), opt(ws), need, s[0].device().index(), stream_of(s[0]));
+    if (rc != HK_OK) fail("hk_qk_norm_rotary_bwd", rc);
+    variable_list out = {dx[0], dx[1], dw[0], dw[1]};
+    if (at::GradMode::is_enabled()) {  // a graph of the gradients: they have none of their own
+      for (Tensor& t : out)
+        if (t.defined()) t.requires_grad_();
+      out = (*std::make_shared<torch::autograd::DelayedError>(
+          "trying to differentiate twice a function that was marked with @once_differentiable", 4))(std::move(out));
+    }
+    out.resize(8);
+    return out;
+  }
+};
+
+// norm_rotary(q, k, q_weight, k_weight, cos, sin, positions, pos_offset, eps, interleaved): q and k with their gradients, or None
+PyObject* norm_rotary(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  Qkn p;
+  if (n_args != 10 || !p.take(a, a[6], a[7], a[8], a[9]) || p.cos->requires_grad() || p.sin->requires_grad()) Py_RETURN_NONE;
+  QknCall c;
+  for (int i = 0; i < 3; ++i) c.qs[i] = p.qs[i], c.ks[i] = p.ks[i];
+  c.flags = p.flags, c.pos_offset = p.pos_offset, c.eps = p.eps;
+  c.b = p.b, c.n = p.n, c.h = p.h, c.hkv = p.hkv, c.d = p.d, c.r = p.r, c.rows = p.rows, c.device = p.device;
+  auto given = [](const Tensor* t) { return t ? std::optional<Tensor>(*t) : std::nullopt; };
+  try {
+    const variable_list y =
+        NormRotary::apply(*p.q, *p.k, given(p.w[0]), given(p.w[1]), *p.cos, *p.sin, given(p.positions), c);
+    return Py_BuildValue("(NN)", THPVariable_Wrap(y[0]), THPVariable_Wrap(y[1]));
+  } catch (const Refused&) {
+    Py_RETURN_NONE;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
 #define HK_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {HK_METHOD(attn_fwd),       HK_METHOD(attn_bwd_strided), HK_METHOD(rotary_bnhd),
                          HK_METHOD(paged_decode),   HK_METHOD(attn_fwd_paged),   HK_METHOD(paged_kv_append),
                          HK_METHOD(qk_norm_rotary), HK_METHOD(qk_norm_rotary_bwd),
+                         HK_METHOD(packed_attention), HK_METHOD(norm_rotary),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_front", "Native tensor front ends of hipkittens_b200", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};
