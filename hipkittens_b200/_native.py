@@ -645,15 +645,16 @@ def qk_norm_rotary(
             return _done(r, "hk_qk_norm_rotary")
     flags = _qkn_check(q, k, q_weight, k_weight, cos, sin, positions, pos_offset, eps)
     b, n, h, d = q.shape
+    s = stream if stream is not None else torch.cuda.current_stream(q.device)
     outs = []
     for name, t, o in (("q_out", q, q_out), ("k_out", k, k_out)):
         if o is None:
-            o = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+            with torch.cuda.stream(s):  # memory of the stream that writes it
+                o = torch.empty(t.shape, dtype=t.dtype, device=t.device)
         if not isinstance(o, torch.Tensor) or o.shape != t.shape or o.dtype != t.dtype or not o.is_contiguous():
             raise RuntimeError(f"{name} must be a contiguous bf16 tensor of its input's shape")
         _require_same_device(q, **{name: o})
         outs.append(o)
-    s = stream if stream is not None else torch.cuda.current_stream(q.device)
     _check(capi().hk_qk_norm_rotary(q.data_ptr(), k.data_ptr(), _ptr(q_weight), _ptr(k_weight), cos.data_ptr(), sin.data_ptr(),
                                     outs[0].data_ptr(), outs[1].data_ptr(), b, n, h, k.shape[2], d, 2 * cos.shape[1],
                                     cos.shape[0], _strides3(q), _strides3(k), _ptr(positions), int(pos_offset), float(eps),
@@ -691,11 +692,11 @@ def qk_norm_rotary_bwd(
         if not isinstance(g, torch.Tensor) or g.shape != t.shape or g.dtype != t.dtype or not g.is_contiguous():
             raise RuntimeError(f"{name} must be a contiguous bf16 tensor of its output's shape")
     _require_same_device(q, dq_out=dq_out, dk_out=dk_out)
-    dq, dk = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
-    dws = [torch.empty_like(w) if weight_grads and w is not None else None for w in (q_weight, k_weight)]
     s = stream if stream is not None else torch.cuda.current_stream(q.device)
     need = int(capi().hk_qk_norm_rotary_bwd_workspace_bytes(d))
-    with torch.cuda.stream(s):  # the workspace goes back to the pool of the stream that uses it
+    with torch.cuda.stream(s):  # memory of the stream that writes it
+        dq, dk = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
+        dws = [torch.empty_like(w) if weight_grads and w is not None else None for w in (q_weight, k_weight)]
         ws = torch.empty(need, dtype=torch.uint8, device=q.device) if any(w is not None for w in dws) else None
     _check(capi().hk_qk_norm_rotary_bwd(q.data_ptr(), k.data_ptr(), _ptr(q_weight), _ptr(k_weight), cos.data_ptr(), sin.data_ptr(),
                                         dq_out.data_ptr(), dk_out.data_ptr(), dq.data_ptr(), dk.data_ptr(), _ptr(dws[0]),
@@ -778,11 +779,12 @@ def paged_decode(
         raise HkError(HK_EUNSUPPORTED, "hk_attn_paged_decode",
                       "shape outside the decode kernels' limits (D = 128, with a window 64 or 128, 16-token pages, S <= 65535, "
                       "max_pages, or pages of a window and its sinks, <= 8192)")
+    st = stream if stream is not None else torch.cuda.current_stream(q.device)
     if workspace is None:
-        workspace = torch.empty(max(need, 256), dtype=torch.uint8, device=q.device)
+        with torch.cuda.stream(st):  # it goes back to the stream that uses it
+            workspace = torch.empty(max(need, 256), dtype=torch.uint8, device=q.device)
     _require_same_device(q, k_pages=k_pages, v_pages=v_pages, block_table=block_table, ctx_lens=ctx_lens, out=out,
                          lse=lse, workspace=workspace)
-    st = stream if stream is not None else torch.cuda.current_stream(q.device)
     if window is not None:
         if out.shape != q.shape or out.dtype != torch.bfloat16 or not out.is_contiguous():
             raise RuntimeError("out must be a contiguous bf16 tensor of q's shape")

@@ -57,6 +57,7 @@ EncodeTiledFn get_encode() {
 struct DeviceState {
   std::mutex mu;
   bool ready = false;     // set once init_device succeeded; a failed attempt is retried by the next call
+  bool window_ready = false;  // the kernels of calls with a window, which have attributes of their own to set
   int sm_count = 0;
   int cc_major = 0;
   hk::DecodeLimits decode;
@@ -134,18 +135,13 @@ int init_device(int device) {
   int rc;
   if ((rc = prepare_fwd_kernels<128, false>()) != HK_OK) return rc;
   if ((rc = prepare_fwd_kernels<128, true>()) != HK_OK) return rc;
-  if ((rc = prepare_fwd_kernels<128, hk::kMaskWindow>()) != HK_OK) return rc;
   if ((rc = prepare_fwd_kernels<64, false>()) != HK_OK) return rc;
   if ((rc = prepare_fwd_kernels<64, true>()) != HK_OK) return rc;
-  if ((rc = prepare_fwd_kernels<64, hk::kMaskWindow>()) != HK_OK) return rc;
   if ((rc = hk::prepare_decode_kernels(g_cuda_err, sizeof(g_cuda_err), st.sm_count, &st.decode)) != HK_OK) return rc;
-  if ((rc = hk::prepare_window_decode_kernels(g_cuda_err, sizeof(g_cuda_err))) != HK_OK) return rc;
   if ((rc = prepare_bwd_kernels<128, false>()) != HK_OK) return rc;
   if ((rc = prepare_bwd_kernels<128, true>()) != HK_OK) return rc;
-  if ((rc = prepare_bwd_kernels<128, hk::kMaskWindow>()) != HK_OK) return rc;
   if ((rc = prepare_bwd_kernels<64, false>()) != HK_OK) return rc;
   if ((rc = prepare_bwd_kernels<64, true>()) != HK_OK) return rc;
-  if ((rc = prepare_bwd_kernels<64, hk::kMaskWindow>()) != HK_OK) return rc;
   for (int n = 2; n <= hk::kMaxDkdvSplit; ++n)
     st.bwd_clusters[n] = hk::clusters_held(hk::attn_bwd_dkdv_kernel<128, true, true>, hk::kBwdThreads, hk::BwdSmem<128>::kDynBytes, n);
   // the one allocation this library makes: the status word (last, so that a failure above leaves nothing behind). It
@@ -163,6 +159,16 @@ int init_device(int device) {
   st.status_host = static_cast<int*>(word);
   st.status = static_cast<int*>(dev_word);
   return HK_OK;
+}
+
+// What the first call with a window on a device adds to that: kernels that a program without windows does not load.
+int init_windows() {
+  int rc;
+  if ((rc = prepare_fwd_kernels<128, hk::kMaskWindow>()) != HK_OK) return rc;
+  if ((rc = prepare_fwd_kernels<64, hk::kMaskWindow>()) != HK_OK) return rc;
+  if ((rc = prepare_bwd_kernels<128, hk::kMaskWindow>()) != HK_OK) return rc;
+  if ((rc = prepare_bwd_kernels<64, hk::kMaskWindow>()) != HK_OK) return rc;
+  return hk::prepare_window_decode_kernels(g_cuda_err, sizeof(g_cuda_err));
 }
 
 // Makes a device current for the duration of one entry point and puts the caller's current device back when the
@@ -186,9 +192,9 @@ class DeviceScope {
     *resolved = device;
     return HK_OK;
   }
-  // enter_raw plus the device's state, initialised on first use. A failed initialisation is not remembered: the
-  // next call tries again (the failing thread finds the reason in hk_last_cuda_error()).
-  int enter(int device, DeviceState** out) {
+  // enter_raw plus the device's state, initialised on first use (with `window`, for calls with one as well). A failed initialisation is
+  // not remembered: the next call tries again (the failing thread finds the reason in hk_last_cuda_error()).
+  int enter(int device, DeviceState** out, bool window = false) {
     int rc = enter_raw(device, &device);
     if (rc != HK_OK) return rc;
     DeviceState& st = g_dev[device];
@@ -198,6 +204,11 @@ class DeviceScope {
         rc = init_device(device);
         if (rc != HK_OK) return rc;
         st.ready = true;
+      }
+      if (window && !st.window_ready) {
+        rc = init_windows();
+        if (rc != HK_OK) return rc;
+        st.window_ready = true;
       }
     }
     *out = &st;
@@ -700,7 +711,7 @@ static int fwd_launch(const void* q, const void* k, const void* v, void* o, floa
   const bool causal = mask == hk::kMaskCausal;
   DeviceState* st = nullptr;
   DeviceScope scope;
-  int rc = scope.enter(device, &st);
+  int rc = scope.enter(device, &st, mask == hk::kMaskWindow);
   if (rc != HK_OK) return rc;
 
   CUtensorMap tq, tk, tv, to;
@@ -933,7 +944,7 @@ static int bwd_launch(const void* q, const void* k, const void* v, const void* o
   }
   DeviceState* st = nullptr;
   DeviceScope scope;
-  int rc = scope.enter(device, &st);
+  int rc = scope.enter(device, &st, mask == hk::kMaskWindow);
   if (rc != HK_OK) return rc;
 
   const long long dos[3] = {(long long)N * H * D, (long long)H * D, D};
@@ -1321,7 +1332,7 @@ int hk_attn_paged_decode_window(const void* q, const void* k_pages, const void* 
   if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255)) return HK_EWORKSPACE;
   DeviceState* st = nullptr;
   DeviceScope scope;
-  int rc = scope.enter(device, &st);
+  int rc = scope.enter(device, &st, true);
   if (rc != HK_OK) return rc;
   hk::DecodeParams p;
   p.q = static_cast<const __nv_bfloat16*>(q);

@@ -81,7 +81,8 @@ int hk_attn_fwd_cross(const void* q, const void* k, const void* v, void* o, floa
 
 /* hk_attn_fwd_cross(causal = 1) for layers whose queries see a window of the keys before them and the first keys: with the query of
  * row r at position p = r + (kv_len_b - Nq), key c is seen iff c <= p and (p - c < window or c < sinks), so that a row
- * sees its own key and the window - 1 before it. window >= 1, sinks >= 0. A row that sees no key gets O = 0, L = -inf.
+ * sees its own key and the window - 1 before it. window >= 1, sinks >= 0. A row that sees no key gets O = 0, L = -inf. Keys that
+ * a row does not see may hold anything; V has to be finite throughout, as without a window (0 times infinity).
  * Keys that no row of a block sees are neither loaded nor multiplied; with window >= Nk this is hk_attn_fwd_cross. */
 int hk_attn_fwd_window(const void* q, const void* k, const void* v, void* o, float* lse,
                        int B, int Nq, int Nk, int H, int H_KV, int D,
@@ -105,7 +106,8 @@ int hk_attn_fwd_paged(const void* q, const void* k_pages, const void* v_pages, c
                       int device, void* cuda_stream);
 
 /* hk_attn_fwd_paged(causal = 1) with the window and sinks of hk_attn_fwd_window. Pages without a key that a row of the chunk sees
- * are not looked up in the block table, so those between the sinks and the chunk's first window may have been given away. */
+ * are not looked up in the block table, so those between the sinks and the chunk's first window may have been given away. All rows of
+ * a page that is looked up must hold finite values. */
 int hk_attn_fwd_paged_window(const void* q, const void* k_pages, const void* v_pages, const int32_t* block_table,
                              const int32_t* ctx_lens, void* o, float* lse, int S, int T, int H, int H_KV, int D,
                              int page_size, int max_pages_per_seq, int num_pages, int window, int sinks,
