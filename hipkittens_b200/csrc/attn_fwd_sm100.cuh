@@ -441,19 +441,20 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
       // fixed for the item, so the per-tile test is one comparison.
       const int row_last_key = min(w.qb[slot] * kBlockM + row + w.off, w.kv_len - 1);
       const int j_mask = (min(w.qb[slot] * kBlockM + w.off, w.kv_len - 1) + 1) >> 7;
-      // window: the row's first key, and masks for the tiles that some row of the block does not see whole
-      [[maybe_unused]] const int row_first_key = w.qb[slot] * kBlockM + row + w.off - p.window + 1;
-      [[maybe_unused]] auto window_mask = [&](uint32_t* su, int j) {
-        const int t = kv_tile(w, j);
-        if (t < j_mask && (t * kBlockN > w.qb[slot] * kBlockM + kBlockM - 1 + w.off - p.window ||
-                           (t + 1) * kBlockN <= p.sinks)) return;  // CTA-uniform
-        const int hi = row_last_key - t * kBlockN, lo = row_first_key - t * kBlockN, sinks = p.sinks - t * kBlockN;
-#pragma unroll
-        for (int cc = 0; cc < kBlockN / 32; ++cc) {
-          const uint32_t seen = seen_bits(cc * 32, lo, hi, sinks);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) su[cc * 32 + i] = (seen >> i) & 1u ? su[cc * 32 + i] : 0xff800000u;
-        }
+      // With a window: masks for the tiles that some row of the block does not see whole. D = 128 masks the scores where they lie, 32
+      // columns at a time, ahead of the code for all tiles, which a mask in the middle of it slows down for every tile. What a mask needs
+      // is derived from `pos0`, the position of the block's first row, only there: limits that live through an item's loop do the same. us, mask in registers / there / there without such limits / no masks at all (wrong): B1 N16384 H32/8 window 2048 504 / 485
+      // / 481 / 461, B2 N8192 H32/8 window 1024 298 / 288 / 285 / 262, B1 N16384 window 128 123 / 115 / 111 / 97. At D = 64 the scores
+      // are better masked in registers (B1 N16384 H32/8 window 128 97 / 107 / - / 85, B8 N1024 H16 window 256 44.5 / 47.4 / - / 38.9).
+      [[maybe_unused]] const int pos0 = w.qb[slot] * kBlockM + w.off;
+      [[maybe_unused]] auto masked = [&](int j, auto&& select) {
+        int pos = pos0;
+        asm volatile("" : "+r"(pos));
+        const int t = kv_tile(w, j), first = t * kBlockN;
+        if (first + kBlockN - 1 <= min(pos, w.kv_len - 1) && (first > pos + kBlockM - 1 - p.window || first + kBlockN <= p.sinks))
+          return;  // CTA-uniform
+        const int hi = min(pos + row, w.kv_len - 1) - first, lo = pos + row - p.window + 1 - first;
+        select([&](int base) { return seen_bits(base, lo, hi, p.sinks - first); });
       };
       if (nkv == 0) {
         if (CAUSAL && w.qb[slot] * kBlockM < p.N) {
@@ -477,6 +478,22 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
         ++s_cnt;
         tc_fence_after();
         HK_STAMP(slot, 1);
+        if constexpr (WINDOW && !kSepP) {
+          masked(j, [&](auto&& seen_from) {
+#pragma unroll 1
+            for (int cc = 0; cc < kBlockN / 32; ++cc) {
+              const uint32_t seen = seen_from(cc * 32);
+              if (__all_sync(0xffffffffu, seen == ~0u)) continue;
+              uint32_t x[32];
+              tmem_ld32(tS + cc * 32, x);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) x[i] = (seen >> i) & 1u ? x[i] : 0xff800000u;
+              tmem_st32(tS + cc * 32, x);
+            }
+            tmem_wait_st();
+          });
+        }
         if constexpr (kSepP) {
           uint32_t su[kBlockN];  // one row of S, fp32 bit patterns
 #define HK_S(i) __uint_as_float(su[(i)])
@@ -490,9 +507,17 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
             __syncwarp();
             if (lane == 0) mbar_arrive(&s_free[slot]);
           }
-          if (WINDOW) {
-            window_mask(su, j);
-          } else if (CAUSAL && j >= j_mask) {
+          if constexpr (WINDOW) {
+            masked(j, [&](auto&& seen_from) {
+#pragma unroll
+              for (int cc = 0; cc < kBlockN / 32; ++cc) {
+                const uint32_t seen = seen_from(cc * 32);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) su[cc * 32 + i] = (seen >> i) & 1u ? su[cc * 32 + i] : 0xff800000u;
+              }
+            });
+          }
+          if (!WINDOW && CAUSAL && j >= j_mask) {
             const int lim = row_last_key - j * kBlockN;
 #pragma unroll
             for (int i = 0; i < kBlockN; ++i) su[i] = (i > lim) ? 0xff800000u : su[i];
@@ -611,9 +636,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
 #pragma unroll
             for (int cc = 0; cc < 4; ++cc) tmem_ld32(tS + cc * 32, su + cc * 32);
             tmem_wait_ld();
-            if (WINDOW) {
-              window_mask(su, j);
-            } else if (CAUSAL && j >= j_mask) {
+            if (!WINDOW && CAUSAL && j >= j_mask) {
               const int lim = row_last_key - j * kBlockN;
 #pragma unroll
               for (int i = 0; i < kBlockN; ++i) su[i] = (i > lim) ? 0xff800000u : su[i];
