@@ -87,6 +87,7 @@ struct BwdParams {
   // kMaskWindow: as in FwdParams. The first `shared_blocks` key blocks of a unit are shared by `shares` work items each, which leave
   // their partial sums in `partial`, [unit][block][share][dK, dV][128][D]; attn_bwd_shares_kernel adds them up.
   int window, sinks;
+  int longest_first;
   int shared_blocks, shares;
   FastDiv fd_shares;
   float* partial;
@@ -691,6 +692,13 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         if (lane == 0) mbar_arrive(bars + P_FULL);
         HK_STAMP(trole, 4);
         // ---- dS^T = P^T * (dP^T - delta)
+        if (WINDOW && ((diag && w.j == 0) || (p.window == 1 && p.sinks == 0))) {
+          // the query at the key's position, where that is all it sees, has dS = 0 (as in the dQ kernel)
+          const bool one_key = w.j * kBlockN + row == 0 || (p.window == 1 && p.sinks == 0);
+          const int own = row + (w.j - i_t) * kBlockN - w.off - part * kBwdPC;
+#pragma unroll
+          for (int col = 0; col < kBwdPC; ++col) su[col] = one_key && col == own ? 0u : su[col];
+        }
         {
           uint32_t pk[kBwdPC / 2];
 #pragma unroll
@@ -1089,7 +1097,7 @@ __device__ __forceinline__ DqItemOf<MASK> decode_dq_item(const BwdParams& p, int
   const int NB = (p.N + kBlockM - 1) / kBlockM;  // the last tile may be partial
   const int G = p.G;
   int unit, g;
-  if (MASK == kMaskCausal) {
+  if (MASK == kMaskCausal || (MASK == kMaskWindow && p.longest_first)) {
     const int grp = min(p.fd_group.div(idx), p.last_group);
     const int within = idx - grp * p.group_items;
     int qd, rem;
@@ -1268,7 +1276,9 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
             const bool far = kv * kBlockN <= w.i * kBlockM + kBlockM - 1 + w.off - p.window && (kv + 1) * kBlockN > p.sinks;
             if (diag || far) {
               const int base = kv * kBlockN + part * kBwdPC, own = w.i * kBlockM + row + w.off;
-              const int hi = min(own, w.kv_len - 1) - base, lo = own - p.window + 1 - base;
+              // a row that sees one key has P = 1 and dP = delta there: dS = 0, which delta, of the rounded O, is not exact enough for
+              const bool one_key = own == 0 || (p.window == 1 && p.sinks == 0);
+              const int hi = (one_key ? -1 : min(own, w.kv_len - 1)) - base, lo = own - p.window + 1 - base;
 #pragma unroll
               for (int cc = 0; cc < kBwdPC / 32; ++cc) {
                 const uint32_t seen = seen_bits(cc * 32, lo, hi, p.sinks - base);

@@ -140,6 +140,7 @@ struct FwdParams {
   const int* block_table;
   int max_pages, num_pages;
   int window, sinks;    // kMaskWindow: the query at position p sees the keys c <= p with p - c < window or c < sinks
+  int longest_first;    // kMaskWindow: in the causal order, for windows that most rows do not fill
   int* status;          // device word: first non-zero status wins
 #ifdef HK_TRACE
   long long* trace;     // [3 roles][4096] clock stamps of CTA 0 (debug builds only)
@@ -187,7 +188,7 @@ __device__ __forceinline__ int first_key(const WindowItem& w) { return w.first_k
 // a group the longest rows come first (q block descending), with the slot pairs that share a K/V prefix
 // adjacent. (One sweep over all units at once keeps every unit's K/V live at the same time - 128 MB at
 // N = 8192 - and was measured to re-read K/V from HBM 2.6 times over.) With a window all but the first rows have as many
-// keys, and neighbouring query tiles share most of them: the order is that without a mask.
+// keys, and neighbouring query tiles share most of them: the order is that without a mask, unless the window is long for the sequence.
 template <int MASK>
 __device__ __forceinline__ ItemOf<MASK> decode_item(const FwdParams& p, int idx) {
   constexpr bool CAUSAL = MASK != kMaskNone;
@@ -198,7 +199,7 @@ __device__ __forceinline__ ItemOf<MASK> decode_item(const FwdParams& p, int idx)
   // of q tiles (one head per item), of which there are nq per unit
   const int nq = p.pair_heads ? NQB : (NQB + 1) / 2;
   int unit, qx, hx;
-  if (MASK == kMaskCausal) {
+  if (MASK == kMaskCausal || (MASK == kMaskWindow && p.longest_first)) {
     const int grp = min(p.fd_group_items.div(idx), p.last_group);
     const int within = idx - grp * p.group_items;
     int qd, rem;

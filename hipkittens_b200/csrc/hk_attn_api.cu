@@ -608,8 +608,12 @@ int qkn_pick(int D, int flags, const Fn& fn) {
 struct WindowShares {
   int blocks, shares;
 };
+// A window that no key lies behind masks nothing that the causal mask does not: the backward is the causal one, but for a single tile
+// of keys, where rows that see one key weigh most (their dS is exactly zero with a window).
+bool covers_all(int NK, int window, int sinks) { return NK > hk::kBlockN && (window >= NK || sinks >= NK); }
 WindowShares window_shares(int units, int G, int N, int NK, int D, int window, int sinks) {
   constexpr long long kSms = 148, kMost = 32;
+  window = std::min(window, NK), sinks = std::min(sinks, NK);
   const long long nbq = (N + hk::kBlockM - 1) / hk::kBlockM, nbk = (NK + hk::kBlockN - 1) / hk::kBlockN;
   const long long own = G * std::min(nbq, (1ll * window + hk::kBlockN - 2) / hk::kBlockM + 2);  // a block's pairs by its window
   const long long sink_blocks = (1ll * std::min(sinks, NK) + hk::kBlockN - 1) / hk::kBlockN, all = G * nbq;
@@ -656,7 +660,7 @@ int launch_bwd_window(const CUtensorMap& tq, const CUtensorMap& tk, const CUtens
   p.n_items = p.B * p.H * nbq;
   grid = p.n_items < sm_count ? p.n_items : sm_count;
   p.dq_waits = !dq_beside || (tiles > 40ll * grid && dkdv.n_items > 4 * sm_count);
-  set_bwd_decode(p, (p.H / p.H_KV) * nbq, p.H / p.H_KV, nbq, grid, false);
+  set_bwd_decode(p, (p.H / p.H_KV) * nbq, p.H / p.H_KV, p.longest_first ? p.H / p.H_KV : nbq, grid, p.longest_first);
   HK_CUDA(hk::launch_dependent(!p.dq_waits || short_kernel(tiles, grid), hk::attn_bwd_dq_kernel<D, hk::kMaskWindow>, grid,
                                hk::kBwdThreads, hk::BwdSmem<D>::kDynBytes, stream, tq, tk, tv, tdo, p));
   g_launches.fetch_add(1, std::memory_order_relaxed);
@@ -706,9 +710,11 @@ static int fwd_launch(const void* q, const void* k, const void* v, void* o, floa
                       int H_KV, int D, const long long* q_strides, const long long* k_strides,
                       const long long* v_strides, const int32_t* kv_lens, const int32_t* block_table, int max_pages,
                       int num_pages, int mask, int window, int sinks, float softmax_scale, int device, void* cuda_stream) {
-  // a window that no key lies behind masks nothing that the causal mask does not
-  if (mask == hk::kMaskWindow && (window >= NK || sinks >= NK)) mask = hk::kMaskCausal;
-  const bool causal = mask == hk::kMaskCausal;
+  // a window that no key lies behind masks nothing that the causal mask does not (at D = 64 that kernel's L is the less exact one: a
+  // share of its exponentials is a polynomial's)
+  if (mask == hk::kMaskWindow && D == 128 && (window >= NK || sinks >= NK)) mask = hk::kMaskCausal;
+  if (mask == hk::kMaskWindow) window = std::min(window, NK), sinks = std::min(sinks, NK);
+  const bool longest_first = mask == hk::kMaskWindow && (window > NK / 2 || sinks > NK / 2), causal = mask == hk::kMaskCausal || longest_first;
   DeviceState* st = nullptr;
   DeviceScope scope;
   int rc = scope.enter(device, &st, mask == hk::kMaskWindow);
@@ -768,6 +774,7 @@ static int fwd_launch(const void* q, const void* k, const void* v, void* o, floa
   p.num_pages = num_pages;
   p.window = mask == hk::kMaskWindow ? window : 0;
   p.sinks = mask == hk::kMaskWindow ? sinks : 0;
+  p.longest_first = longest_first;
   p.status = st->status;
 #ifdef HK_TRACE
   p.trace = g_trace_buf;
@@ -932,8 +939,8 @@ static int bwd_launch(const void* q, const void* k, const void* v, const void* o
   if ((o && !aligned16(o)) || !aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(d_o) || !aligned16(dq) || !aligned16(dk) ||
       !aligned16(dv) || (reinterpret_cast<uintptr_t>(lse) & 3) || (reinterpret_cast<uintptr_t>(delta) & 3))
     return HK_EINVAL;
-  // a window that no key lies behind masks nothing that the causal mask does not
-  if (mask == hk::kMaskWindow && (window >= NK || sinks >= NK)) mask = hk::kMaskCausal;
+  if (mask == hk::kMaskWindow && covers_all(NK, window, sinks)) mask = hk::kMaskCausal;
+  if (mask == hk::kMaskWindow) window = std::min(window, NK), sinks = std::min(sinks, NK);
   const bool causal = mask == hk::kMaskCausal;
   WindowShares shared = {0, 1};
   if (mask == hk::kMaskWindow) {
@@ -985,6 +992,7 @@ static int bwd_launch(const void* q, const void* k, const void* v, const void* o
   p.kv_lens = kv_lens;
   p.window = window;
   p.sinks = sinks;
+  p.longest_first = window > NK / 2 || sinks > NK / 2;
   p.shared_blocks = shared.blocks;
   p.shares = shared.shares;
   p.partial = static_cast<float*>(workspace);
@@ -1040,7 +1048,7 @@ int hk_attn_bwd_strided(const void* q, const void* k, const void* v, const void*
 size_t hk_attn_bwd_window_workspace_bytes(int B, int N, int NK, int H, int H_KV, int D, int window, int sinks) {
   if (B <= 0 || N <= 0 || NK <= 0 || H <= 0 || H_KV <= 0 || H % H_KV != 0 || (D != 64 && D != 128) || window <= 0 || sinks < 0)
     return 0;
-  if (window >= NK || sinks >= NK || 1ll * B * H_KV > 0x3fffffffll) return 0;
+  if (covers_all(NK, window, sinks) || 1ll * B * H_KV > 0x3fffffffll) return 0;
   const WindowShares n = window_shares(B * H_KV, H / H_KV, N, NK, D, window, sinks);
   return size_t(B) * H_KV * n.blocks * (n.blocks ? n.shares : 0) * 2 * hk::kBlockN * D * sizeof(float);
 }

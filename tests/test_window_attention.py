@@ -56,12 +56,13 @@ def test_backward_refuses(native_built, change, code):
 def test_workspace_of_the_backward(native_built):
     of = _native.capi().hk_attn_bwd_window_workspace_bytes
     share = 2 * 128 * 128 * 4
-    assert of(1, 128, 128, 8, 2, 128, 128, 0) == 0                    # nothing hidden
+    assert of(1, 129, 129, 8, 2, 128, 129, 0) == 0                    # nothing hidden
     assert of(16, 8192, 8192, 32, 8, 128, 1024, 0) == 0               # no sinks, blocks for every SM
     n = of(2, 8192, 8192, 32, 8, 128, 1024, 4)
     assert n > 0 and n % (16 * share) == 0 and n // (16 * share) <= 32  # one block of each unit shared
     assert of(2, 8192, 8192, 32, 8, 64, 1024, 4) % (16 * share // 2) == 0
     assert of(1, 384, 384, 8, 2, 128, 128, 2) % (6 * share) == 0 < of(1, 384, 384, 8, 2, 128, 128, 2)  # all six blocks
+    assert of(1, 1000, 100, 8, 2, 128, 500, 0) == of(1, 1000, 100, 8, 2, 128, 100, 0)  # a longer window is no longer one
     assert of(1, 2 ** 30, 2 ** 30, 1, 1, 128, 1, 2 ** 30 - 1) >= 0
     for bad in ((0, 8, 8, 2, 2, 64, 4, 0), (1, 8, 8, 3, 2, 64, 4, 0), (1, 8, 8, 2, 2, 96, 4, 0), (1, 8, 8, 2, 2, 64, 0, 0), (1, 8, 8, 2, 2, 64, 4, -1)):
         assert of(*bad) == 0

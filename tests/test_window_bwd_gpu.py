@@ -136,6 +136,34 @@ def test_a_window_over_all_keys_is_the_causal_backward(dev):
     assert all(torch.equal(x, y) for x, y in zip(plain, grads(q, k, v, d_o, 500, 3)))
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n,nk,lens", [(1, 1, None), (300, 300, None), (200, 333, None), (200, 455, None), (300, 300, [300, 128])])
+def test_rows_that_see_one_key_have_no_gradient_of_their_scores(dev, n, nk, lens, d):
+    """P is 1 whatever the score: dQ and dK are zero, not what rounding O leaves of dP - delta. (A chunk of 200 rows behind 255 keys
+    starts on the last key of a block.)"""
+    b = 1 if lens is None else len(lens)
+    q, k, v, d_o = make(dev, b, n, nk, 4, 2, d, seed=n)
+    dq, dk, dv = grads(q, k, v, d_o, 1, 0, None if lens is None else torch.tensor(lens, dtype=torch.int32, device=dev))
+    assert not dq.any() and not dk.any()
+    (_, _), (_, _), (rv, bv) = ref.backward(q, k, v, d_o, 1, 0, lens)
+    ref.close(dv, rv, bv, "dV")
+    dq, dk, _ = grads(q, k, v, d_o, 50, 3, None if lens is None else torch.tensor(lens, dtype=torch.int32, device=dev))
+    if n == nk:
+        assert not dq[0, 0].any()  # the first row of a sequence sees its own key alone
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n,nk,window", [(700, 700, 500), (700, 700, 699), (700, 700, 700), (300, 1000, 900), (9, 9, 40), (100, 3, 5)])
+def test_windows_long_for_the_sequence(dev, n, nk, window, d):
+    q, k, v, d_o = make(dev, 2, n, nk, 6, 2, d, seed=window)
+    o, lse = hk.attn_fwd(q, k, v, causal=True, window=window, sinks=1)
+    want = ref.forward(q, k, v, window, 1)
+    ref.close(o, want[0], want[1], "O")
+    ref.close(lse, want[2], want[3], "L")
+    for name, g, (r, bound) in zip(("dQ", "dK", "dV"), grads(q, k, v, d_o, window, 1), ref.backward(q, k, v, d_o, window, 1)):
+        ref.close(g, r, bound, name)
+
+
 @pytest.mark.parametrize("sinks", [0, 4])
 def test_dq_in_the_place_of_q_and_the_others_in_theirs(dev, sinks):
     q, k, v, d_o = make(dev, 1, 700, 700, 4, 2, 128, seed=9)
