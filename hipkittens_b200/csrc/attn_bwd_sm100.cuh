@@ -181,6 +181,124 @@ __global__ void __launch_bounds__(256) attn_bwd_prep_kernel(const __nv_bfloat16*
   }
 }
 
+// The same with a window, where rows of few keys are common. delta is the sum of P dP over a row's keys, and where these are few, what
+// the rounding of O and of P left in O does not average out of dP - delta: with O alone dQ is off by 3.8e-3 (relative, 2048 rows) at two
+// keys a row, 3.0e-3 at 4, 2.7e-3 at 8 and 2.4e-3 at 256, of which 2.35e-3 are the roundings of dS and of dQ itself. So rows of up to
+// kFewKeys keys take the sum over their keys, in fp32 and from the scores, in place of rowsum(dO * O): the first ones of a sequence,
+// or, with a window and sinks of so few, all. They are blocks of their own behind the others, a row to D / 8 lanes, with the keys of a
+// row asked for at once. (Per backward, without them and with: B3 N1777 H12/4 D64 window 300 77.8 -> 80.9 us, B2 N8192 H32/8 D128 window 1024 1014 ->
+// 1015, N16384 window 9 335.5 -> 335.9, window 2 336 -> 433. Up to 8 keys, one by one, in the threads of the other rows: 87.4, 1020,
+// 342, 469.)
+constexpr int kFewKeys = 4;
+struct FewKeysParams {
+  const __nv_bfloat16 *q, *k, *v;
+  const float* lse;                // [B,H,1,N]
+  const int* kv_lens;              // or null
+  long long q_stride[3], k_stride[3], v_stride[3];  // batch, sequence, head; elements
+  int NK, window, sinks;
+  int all;                         // no row sees more
+  int few_rows;                    // rows of the blocks behind: all, or kFewKeys positions of each sequence and head
+  float scale_log2;
+  FastDiv fd_g;                    // heads to a K/V head
+};
+// The keys of a row: the first `first` of all, and those from `lo` to its own.
+struct RowKeys {
+  int lo, first, count;
+  __device__ __forceinline__ RowKeys(int pos, int window, int sinks) {
+    lo = max(pos - window + 1, 0);
+    first = min(lo, sinks);
+    count = pos < 0 ? 0 : first + pos - lo + 1;
+  }
+};
+
+template <int D>
+__global__ void __launch_bounds__(256) attn_bwd_prep_window_kernel(const __nv_bfloat16* o, const __nv_bfloat16* d_o, float* delta,
+                                                                   int rows, int N, int H, FastDiv fd_h, FastDiv fd_n, int blocks,
+                                                                   const __grid_constant__ FewKeysParams p) {
+  constexpr int kLanesPerRow = D / 8;               // 16 or 8
+  constexpr int kRowsPerWarp = 32 / kLanesPerRow;   // 2 or 4
+  const int lane = threadIdx.x & 31;
+  const int sub = lane % kLanesPerRow;
+  ptx::grid_dep_wait();
+  ptx::grid_dep_launch();
+  auto dot8 = [](const uint4& x, const uint4& y) {
+    const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+    float acc = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      acc = fmaf(__uint_as_float(xw[i] << 16), __uint_as_float(yw[i] << 16), acc);
+      acc = fmaf(__uint_as_float(xw[i] & 0xffff0000u), __uint_as_float(yw[i] & 0xffff0000u), acc);
+    }
+    return acc;
+  };
+  auto row_sum = [](float acc) {
+#pragma unroll
+    for (int off = kLanesPerRow / 2; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
+    return acc;
+  };
+  auto length = [&](int b) { return p.kv_lens ? min(max(p.kv_lens[b], 1), p.NK) : p.NK; };
+  if (static_cast<int>(blockIdx.x) < blocks) {
+    const int row0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * (kRowsPerWarp * kRowPassUnroll) + lane / kLanesPerRow;
+    uint4 a[kRowPassUnroll], b[kRowPassUnroll];
+#pragma unroll
+    for (int u = 0; u < kRowPassUnroll; ++u) {
+      const int row = min(row0 + u * kRowsPerWarp, rows - 1);  // a row beyond the last: that one again, and not stored
+      a[u] = __ldcs(reinterpret_cast<const uint4*>(o + static_cast<size_t>(row) * D) + sub);
+      b[u] = __ldcs(reinterpret_cast<const uint4*>(d_o + static_cast<size_t>(row) * D) + sub);
+    }
+    float sum[kRowPassUnroll];
+#pragma unroll
+    for (int u = 0; u < kRowPassUnroll; ++u) sum[u] = row_sum(dot8(a[u], b[u]));
+#pragma unroll
+    for (int u = 0; u < kRowPassUnroll; ++u) {
+      const int row = row0 + u * kRowsPerWarp;
+      if (row < rows && sub == 0) {
+        int bn, h, bi, n;
+        fd_h.divmod(row, bn, h);
+        fd_n.divmod(bn, bi, n);
+        const int pos = n + length(bi) - N;  // not the rows of the blocks behind: those of the first kFewKeys positions
+        if (pos < 0 || pos >= kFewKeys) delta[(static_cast<size_t>(bi) * H + h) * N + n] = sum[u];
+      }
+    }
+    return;
+  }
+  const int few = ((blockIdx.x - blocks) * 8 + (threadIdx.x >> 5)) * kRowsPerWarp + lane / kLanesPerRow;
+  int bn, h, bi, n;
+  fd_h.divmod(min(few, p.few_rows - 1), bn, h);
+  if (p.all) fd_n.divmod(bn, bi, n);
+  else bi = bn / kFewKeys, n = bn % kFewKeys;
+  const int behind = length(bi) - N;  // a row's position less its number
+  if (!p.all) n -= behind;            // the row at that position, which this sequence may not have
+  const int pos = n + behind;
+  const bool mine = few < p.few_rows && n >= 0 && n < N;
+  const RowKeys r(pos, p.window, p.sinks);
+  const int count = mine ? r.count : 0;
+  uint4 qv = make_uint4(0, 0, 0, 0), g = qv, kv[kFewKeys], vv[kFewKeys];
+  float nl = 0.f;
+  if (count > 0) {
+    nl = p.lse[(static_cast<size_t>(bi) * H + h) * N + n] * -1.4426950408889634f;
+    qv = *reinterpret_cast<const uint4*>(p.q + bi * p.q_stride[0] + n * p.q_stride[1] + h * p.q_stride[2] + sub * 8);
+    g = *(reinterpret_cast<const uint4*>(d_o + (static_cast<size_t>(bi) * N + n) * H * D + static_cast<size_t>(h) * D) + sub);
+  }
+  const int kvh = p.fd_g.div(h);
+#pragma unroll
+  for (int i = 0; i < kFewKeys; ++i) {
+    kv[i] = vv[i] = make_uint4(0, 0, 0, 0);
+    if (i < count) {
+      const long long key = i < r.first ? i : r.lo + i - r.first;
+      kv[i] = *reinterpret_cast<const uint4*>(p.k + bi * p.k_stride[0] + key * p.k_stride[1] + kvh * p.k_stride[2] + sub * 8);
+      vv[i] = *reinterpret_cast<const uint4*>(p.v + bi * p.v_stride[0] + key * p.v_stride[1] + kvh * p.v_stride[2] + sub * 8);
+    }
+  }
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kFewKeys; ++i) {  // the lanes of a warp stay together: sums over a row are shuffles
+    const float s = row_sum(dot8(qv, kv[i])), dp = row_sum(dot8(g, vv[i]));
+    if (i < count) sum = fmaf(ptx::ex2_approx(fmaf(s, p.scale_log2, nl)), dp, sum);
+  }
+  if (mine && sub == 0) delta[(static_cast<size_t>(bi) * H + h) * N + n] = sum;
+}
+
 // ------------------------------------------------------------------------------------ dQ [B,H,N,D] -> [B,N,H,D]
 // Pure byte movement, bound by HBM: 16-byte units, kRowPassUnroll of them per thread, all requested before the first is
 // written (B16 N2048 H64 D128: 201 us in a loop and 208 alone with one unit per thread and three 64-bit divisions for it,

@@ -924,6 +924,33 @@ struct Span {
   bool meets(const Span& o) const { return begin < o.end && o.begin < end; }
 };
 
+// delta of a call with a window; p as the kernels behind will have it.
+static int prep_window_launch(const void* q, const void* k, const void* v, const void* o, const void* d_o, float* delta,
+                              const BwdStrides& s, const hk::BwdParams& p, int D, cudaStream_t stream) {
+  const long long rows = 1ll * p.B * p.N * p.H;
+  if (rows > 0x7fffffffll || 1ll * p.B * p.H > 0x7fffffffll / (2 * hk::kFewKeys)) return HK_EINVAL;  // rows are indexed with int
+  hk::FewKeysParams f;
+  f.q = static_cast<const __nv_bfloat16*>(q);
+  f.k = static_cast<const __nv_bfloat16*>(k);
+  f.v = static_cast<const __nv_bfloat16*>(v);
+  f.lse = p.lse;
+  f.kv_lens = p.kv_lens;
+  for (int i = 0; i < 3; ++i) f.q_stride[i] = s.q[i], f.k_stride[i] = s.k[i], f.v_stride[i] = s.v[i];
+  f.NK = p.NK, f.window = p.window, f.sinks = p.sinks;
+  f.all = 1ll * p.window + p.sinks <= hk::kFewKeys || p.NK <= hk::kFewKeys;
+  f.few_rows = f.all ? int(rows) : p.B * hk::kFewKeys * p.H;
+  f.scale_log2 = p.scale_log2;
+  f.fd_g = hk::FastDiv(p.H / p.H_KV);
+  const int rows_per_block = hk::row_pass_rows(D / 8), few_per_block = rows_per_block / hk::kRowPassUnroll;
+  const int blocks = f.all ? 0 : int((rows + rows_per_block - 1) / rows_per_block);
+  auto* fn = D == 128 ? hk::attn_bwd_prep_window_kernel<128> : hk::attn_bwd_prep_window_kernel<64>;
+  HK_CUDA(hk::launch_dependent(true, fn, unsigned(blocks + (f.few_rows - 1) / few_per_block + 1), 256, 0, stream,
+                               static_cast<const __nv_bfloat16*>(o), static_cast<const __nv_bfloat16*>(d_o), delta, int(rows), p.N, p.H,
+                               hk::FastDiv(p.H), hk::FastDiv(p.N), blocks, f));
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  return HK_OK;
+}
+
 // Shared tail of the backward entries. o != null: delta is computed here first.
 static int bwd_launch(const void* q, const void* k, const void* v, const void* o, const void* d_o, const float* lse,
                       float* delta, void* dq, void* dk, void* dv, int B, int N, int NK, int H, int H_KV, int D,
@@ -939,8 +966,9 @@ static int bwd_launch(const void* q, const void* k, const void* v, const void* o
   if ((o && !aligned16(o)) || !aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(d_o) || !aligned16(dq) || !aligned16(dk) ||
       !aligned16(dv) || (reinterpret_cast<uintptr_t>(lse) & 3) || (reinterpret_cast<uintptr_t>(delta) & 3))
     return HK_EINVAL;
+  const bool windowed = mask == hk::kMaskWindow;
   if (mask == hk::kMaskWindow && covers_all(NK, window, sinks)) mask = hk::kMaskCausal;
-  if (mask == hk::kMaskWindow) window = std::min(window, NK), sinks = std::min(sinks, NK);
+  if (windowed) window = std::min(window, NK), sinks = std::min(sinks, NK);
   const bool causal = mask == hk::kMaskCausal;
   WindowShares shared = {0, 1};
   if (mask == hk::kMaskWindow) {
@@ -961,8 +989,6 @@ static int bwd_launch(const void* q, const void* k, const void* v, const void* o
   if ((rc = make_bnhd_map(&tv, v, B, NK, H_KV, D, s.v)) != HK_OK) return rc;
   if ((rc = make_bnhd_map(&tdo, d_o, B, N, H, D, dos)) != HK_OK) return rc;
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
-  if (o && (rc = prep_launch(o, d_o, delta, B, N, H, D, stream)) != HK_OK) return rc;
-
   hk::BwdParams p;
   p.lse = lse;
   p.delta = delta;
@@ -1000,6 +1026,9 @@ static int bwd_launch(const void* q, const void* k, const void* v, const void* o
 #ifdef HK_TRACE
   p.trace = g_trace_buf;
 #endif
+  if (o && windowed) rc = prep_window_launch(q, k, v, o, d_o, delta, s, p, D, stream);
+  else if (o) rc = prep_launch(o, d_o, delta, B, N, H, D, stream);
+  if (rc != HK_OK) return rc;
   // The dQ kernel starts while the dK/dV kernel is still reading, unless it would write over what that reads: dQ in the place
   // of an input whose rows are read by the CTA that writes there, and before it does (Q and dO; K and V with one tile of
   // each and as many K/V heads as heads), is as good as anywhere else when one kernel follows the other.

@@ -129,11 +129,15 @@ def test_cross_module_with_a_padded_batch(dev):
 
 
 def test_a_window_over_all_keys_is_the_causal_backward(dev):
+    """... but for the rows of few keys, whose delta is summed over their keys (dK is a sum over all rows)."""
     q, k, v, d_o = make(dev, 2, 500, 500, 8, 2, 128)
     o, lse = hk.attn_fwd(q, k, v, causal=True)
     plain = [torch.empty_like(t) for t in (q, k, v)]
     _native.attn_bwd_strided(q, k, v, o, d_o, lse, *plain, causal=True)
-    assert all(torch.equal(x, y) for x, y in zip(plain, grads(q, k, v, d_o, 500, 3)))
+    got = grads(q, k, v, d_o, 500, 3)
+    assert torch.equal(plain[0][:, 4:], got[0][:, 4:]) and torch.equal(plain[2], got[2])
+    for name, g, (r, bound) in zip(("dQ", "dK", "dV"), got, ref.backward(q, k, v, d_o, 500, 3)):
+        ref.close(g, r, bound, name)
 
 
 @pytest.mark.parametrize("d", [64, 128])
@@ -150,6 +154,18 @@ def test_rows_that_see_one_key_have_no_gradient_of_their_scores(dev, n, nk, lens
     dq, dk, _ = grads(q, k, v, d_o, 50, 3, None if lens is None else torch.tensor(lens, dtype=torch.int32, device=dev))
     if n == nk:
         assert not dq[0, 0].any()  # the first row of a sequence sees its own key alone
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("b,n,nk,window,sinks,h", [(1, 2000, 2000, 2, 0, 4), (1, 2000, 2000, 1, 1, 3), (1, 2000, 2000, 4, 0, 4), (1, 2000, 2000, 1, 3, 4),
+                                                   (300, 2, 2, 9, 0, 4), (200, 4, 4, 9, 1, 4), (300, 3, 4, 2, 0, 3)])
+def test_rows_of_few_keys_are_as_exact_as_others(dev, b, n, nk, window, sinks, h, d):
+    """dQ and dK are off by two roundings to bf16, theirs and that of dS: each is uniform over a step, 2^-8 / sqrt(3) of the lower end of a
+    binade and 0.74 of that over a binade, 1.67e-3, so 2.36e-3 for the two, and a tenth more for sums that are not random. With delta from
+    the rounded O it was 3 to 4e-3."""
+    q, k, v, d_o = make(dev, b, n, nk, h, 1, d, seed=b + window)
+    for g, (r, _) in list(zip(grads(q, k, v, d_o, window, sinks), ref.backward(q, k, v, d_o, window, sinks)))[:2]:
+        assert float((g.double() - r).norm() / r.norm()) <= 2.6e-3
 
 
 @pytest.mark.parametrize("d", [64, 128])
