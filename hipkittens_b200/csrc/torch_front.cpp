@@ -11,6 +11,7 @@
 
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAStream.h>
+#include <cuda_runtime_api.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -648,6 +649,27 @@ PyObject* packed_attention(PyObject*, PyObject* const* arg, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
+bool captured(cudaStream_t stream) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(stream, &status) == cudaSuccess) return status != cudaStreamCaptureStatusNone;
+  (void)cudaGetLastError();  // the legacy stream, while another one is captured that waits for it
+  return false;
+}
+// A gradient goes to the stream on which its tensor's node was made. Where that is not captured and this backward is, as with a leaf that
+// a graph from before the capture holds as well, the engine would make that stream wait for a captured one: this ends the capture, and
+// may end the process.
+void check_next_streams(AutogradContext* ctx, cudaStream_t stream) {
+  if (!captured(stream)) return;
+  const auto node = torch::autograd::get_current_node();
+  if (!node) return;
+  for (size_t i = 0; i < node->num_outputs(); ++i) {
+    const auto& next = node->next_edge(i).function;
+    const auto to = next && ctx->needs_input_grad(i) ? next->stream() : std::nullopt;
+    TORCH_CHECK(!to || captured(c10::cuda::CUDAStream(*to).stream()), "a captured backward needs tensors that no graph from before the capture"
+                " holds: delete that graph first, or capture with tensors of their own");
+  }
+}
+
 // One call of the norm and rotation, as its gradients need it.
 struct QknCall {
   long long qs[3], ks[3];
@@ -682,6 +704,7 @@ class NormRotary : public torch::autograd::Function<NormRotary> {
   // In a thread of the engine, without the interpreter.
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     variable_list s = ctx->get_saved_variables();
+    check_next_streams(ctx, static_cast<cudaStream_t>(stream_of(s[0])));
     QknCall c;
     long long* const st[2] = {c.qs, c.ks};
     Tensor dy[2], dx[2], dw[2];

@@ -190,6 +190,28 @@ def test_norm_and_rotation_in_a_graph(dev):
     assert all(torch.equal(a, b) for a, b in zip(inside, want))
 
 
+def test_a_captured_backward_of_leaves_that_an_eager_graph_holds_is_refused(dev):
+    """... before torch joins the two graphs' streams."""
+    gen = torch.Generator().manual_seed(6)
+    x = [rand(gen, 2, 70, 4, 64).requires_grad_(), rand(gen, 2, 70, 2, 64).requires_grad_()]
+    cos = torch.ones(70, 32, device=dev)
+    dy = rand(gen, 2, 70, 4, 64), rand(gen, 2, 70, 2, 64)
+    m = QkNormRotary(64, device=dev, dtype=torch.bfloat16)
+    eager = m(*x, cos, cos)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="no graph from before the capture"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            torch.autograd.grad(m(*x, cos, cos), (*x, m.q_weight), dy)
+    want = torch.autograd.grad(eager, (*x, m.q_weight), dy)
+    del eager
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        inside = torch.autograd.grad(m(*x, cos, cos), (*x, m.q_weight), dy)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(inside, want))
+
+
 def test_a_failure_of_the_backward_is_an_error(dev, monkeypatch):
     """A status that the device reports ends the call in either direction."""
     gen = torch.Generator().manual_seed(7)
