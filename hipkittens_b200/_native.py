@@ -822,8 +822,8 @@ def attn_fwd_paged(
 ) -> Tuple[torch.Tensor, torch.Tensor]:
     """Chunked prefill against the paged KV cache: q [S,T,H,D] bf16 (the last T tokens of each context when `causal`),
     pages [P,16,H_KV,D] bf16, block_table [S,max_pages] int32, ctx_lens [S] int32 -> O [S,T,H,D] bf16,
-    L [S,H,1,T] fp32. The chunk's keys must already be in the cache (`paged_kv_append` first). `window` and `sinks` as in `attn_fwd`; pages that no row of the chunk
-    sees a key of are not looked up."""
+    L [S,H,1,T] fp32. The chunk's keys must already be in the cache (`paged_kv_append` first). `window` and `sinks` as in
+    `attn_fwd`; pages that no row of the chunk sees a key of are not looked up."""
     _check_window(window, sinks, causal)
     if stream is None:
         r = (_front().attn_fwd_paged(q, k_pages, v_pages, block_table, ctx_lens, bool(causal), softmax_scale, out, lse)

@@ -186,9 +186,9 @@ __global__ void __launch_bounds__(256) attn_bwd_prep_kernel(const __nv_bfloat16*
 // keys a row, 3.0e-3 at 4, 2.7e-3 at 8 and 2.4e-3 at 256, of which 2.35e-3 are the roundings of dS and of dQ itself. So rows of up to
 // kFewKeys keys take the sum over their keys, in fp32 and from the scores, in place of rowsum(dO * O): the first ones of a sequence,
 // or, with a window and sinks of so few, all. They are blocks of their own behind the others, a row to D / 8 lanes, with the keys of a
-// row asked for at once. (Per backward, without them and with: B3 N1777 H12/4 D64 window 300 77.8 -> 80.9 us, B2 N8192 H32/8 D128 window 1024 1014 ->
-// 1015, N16384 window 9 335.5 -> 335.9, window 2 336 -> 433. Up to 8 keys, one by one, in the threads of the other rows: 87.4, 1020,
-// 342, 469.)
+// row asked for at once. us per backward, without them / with / up to 8 keys, one by one, in the threads of the other rows: B3 N1777
+// H12/4 D64 window 300 77.8 / 80.9 / 87.4, B2 N8192 H32/8 D128 window 1024 1014 / 1015 / 1020, B1 N16384 H32/8 D128 window 9 335.5 /
+// 335.9 / 341.7, window 2 336 / 433 / 469.
 constexpr int kFewKeys = 4;
 struct FewKeysParams {
   const __nv_bfloat16 *q, *k, *v;
@@ -1173,9 +1173,11 @@ __global__ void __launch_bounds__(256) attn_bwd_shares_kernel(const __grid_const
   const int t = blockIdx.x * 256 + threadIdx.x, c8 = t % kUnits, row = t / kUnits % kBlockN;
   const bool is_dv = t / kUnits >= kBlockN;
   const int block = blockIdx.y, unit = block / p.shared_blocks;
-  const DkdvItem w = decode_dkdv_item<kMaskWindow, false>(p, unit * static_cast<int>(p.fd_unit.d) + (block - unit * p.shared_blocks) * p.shares);
+  const int item = unit * static_cast<int>(p.fd_unit.d) + (block - unit * p.shared_blocks) * p.shares;
+  const DkdvItem w = decode_dkdv_item<kMaskWindow, false>(p, item);
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  const float4* src = reinterpret_cast<const float4*>(p.partial + (static_cast<long long>(block) * p.shares * 2 * kBlockN + (is_dv ? kBlockN : 0) + row) * D + c8 * 8);
+  const long long src_row = static_cast<long long>(block) * p.shares * 2 * kBlockN + (is_dv ? kBlockN : 0) + row;
+  const float4* src = reinterpret_cast<const float4*>(p.partial + src_row * D + c8 * 8);
   for (int r = 0; r < p.shares; ++r, src += 2 * kBlockN * D / 4) {
     if (dkdv_share(r, p.shares, w.n_iter) == dkdv_share(r + 1, p.shares, w.n_iter)) continue;  // it had nothing to do
     const float4 x = src[0], y = src[1];

@@ -444,9 +444,11 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
       const int j_mask = (min(w.qb[slot] * kBlockM + w.off, w.kv_len - 1) + 1) >> 7;
       // With a window: masks for the tiles that some row of the block does not see whole. D = 128 masks the scores where they lie, 32
       // columns at a time, ahead of the code for all tiles, which a mask in the middle of it slows down for every tile. What a mask needs
-      // is derived from `pos0`, the position of the block's first row, only there: limits that live through an item's loop do the same. us, mask in registers / there / there without such limits / no masks at all (wrong): B1 N16384 H32/8 window 2048 504 / 485
-      // / 481 / 461, B2 N8192 H32/8 window 1024 298 / 288 / 285 / 262, B1 N16384 window 128 123 / 115 / 111 / 97. At D = 64 the scores
-      // are better masked in registers (B1 N16384 H32/8 window 128 97 / 107 / - / 85, B8 N1024 H16 window 256 44.5 / 47.4 / - / 38.9).
+      // is derived from `pos0`, the position of the block's first row, only there: limits that live through an item's loop do the
+      // same. us, mask in registers / there / there without such limits / no masks at all (wrong): B1 N16384 H32/8 window 2048 504 /
+      // 485 / 481 / 461, B2 N8192 H32/8 window 1024 298 / 288 / 285 / 262, B1 N16384 window 128 123 / 115 / 111 / 97. At D = 64 the
+      // scores are better masked in registers (B1 N16384 H32/8 window 128 97 / 107 / - / 85, B8 N1024 H16 window 256 44.5 / 47.4 / - /
+      // 38.9).
       [[maybe_unused]] const int pos0 = w.qb[slot] * kBlockM + w.off;
       [[maybe_unused]] auto masked = [&](int j, auto&& select) {
         int pos = pos0;

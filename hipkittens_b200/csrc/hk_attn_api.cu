@@ -335,7 +335,8 @@ int launch_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& 
                const hk::FwdParams& p, int grid, cudaStream_t stream) {
   const bool early = short_kernel(1ll * p.n_items * kv_tiles(p.NK, int(KIND), p.window, p.sinks), grid);
   auto* fn = early ? hk::attn_fwd_kernel<D, KIND, true> : hk::attn_fwd_kernel<D, KIND, hk::kLongFwdDependent<D, KIND>>;
-  HK_CUDA(hk::launch_dependent(early, fn, grid, hk::kFwdThreads, hk::FwdSmem<D, int(KIND) != hk::kMaskNone>::kDynBytes, stream, tq, tk, tv, to, p));
+  constexpr int kSmem = hk::FwdSmem<D, int(KIND) != hk::kMaskNone>::kDynBytes;
+  HK_CUDA(hk::launch_dependent(early, fn, grid, hk::kFwdThreads, kSmem, stream, tq, tk, tv, to, p));
   g_launches.fetch_add(1, std::memory_order_relaxed);
   return HK_OK;
 }
@@ -714,7 +715,8 @@ static int fwd_launch(const void* q, const void* k, const void* v, void* o, floa
   // share of its exponentials is a polynomial's)
   if (mask == hk::kMaskWindow && D == 128 && (window >= NK || sinks >= NK)) mask = hk::kMaskCausal;
   if (mask == hk::kMaskWindow) window = std::min(window, NK), sinks = std::min(sinks, NK);
-  const bool longest_first = mask == hk::kMaskWindow && (window > NK / 2 || sinks > NK / 2), causal = mask == hk::kMaskCausal || longest_first;
+  const bool longest_first = mask == hk::kMaskWindow && (window > NK / 2 || sinks > NK / 2);
+  const bool causal = mask == hk::kMaskCausal || longest_first;
   DeviceState* st = nullptr;
   DeviceScope scope;
   int rc = scope.enter(device, &st, mask == hk::kMaskWindow);

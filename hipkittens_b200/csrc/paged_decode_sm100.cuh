@@ -430,7 +430,7 @@ __global__ void __launch_bounds__(W * 32, W == 8 ? 1 : 2) paged_decode_split_ker
   // ---- merge the W warps through shared memory (the ring is idle now)
   __syncthreads();
   float* sm_o = reinterpret_cast<float*>(dsmem);  // [W][8][128]
-  float* sm_m = sm_o + W * 8 * D;          // [W][8]
+  float* sm_m = sm_o + W * 8 * D;                // [W][8]
   float* sm_l = sm_m + W * 8;                     // [W][8]
 #pragma unroll
   for (int j = 0; j < D / 8; ++j) {
@@ -466,7 +466,7 @@ __global__ void __launch_bounds__(W * 32, W == 8 ? 1 : 2) paged_decode_split_ker
       // ---- merge the CTAs of the cluster: each leaves its share in its own shared memory, and CTA r reads all of
       // head r, r + n_used, ... in the order of the ranks
       float* cl_o = sm_l + W * 8;          // [G][128]
-      float* cl_ml = cl_o + 8 * D;  // [G][2]
+      float* cl_ml = cl_o + 8 * D;         // [G][2]
 #pragma unroll
       for (int i = 0; i < kHeads; ++i) {
         const int h = i * kHalves + h0;

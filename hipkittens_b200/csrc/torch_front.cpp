@@ -665,8 +665,8 @@ void check_next_streams(AutogradContext* ctx, cudaStream_t stream) {
   for (size_t i = 0; i < node->num_outputs(); ++i) {
     const auto& next = node->next_edge(i).function;
     const auto to = next && ctx->needs_input_grad(i) ? next->stream() : std::nullopt;
-    TORCH_CHECK(!to || captured(c10::cuda::CUDAStream(*to).stream()), "a captured backward needs tensors that no graph from before the capture"
-                " holds: delete that graph first, or capture with tensors of their own");
+    TORCH_CHECK(!to || captured(c10::cuda::CUDAStream(*to).stream()), "a captured backward needs tensors that no graph from before",
+                " the capture holds: delete that graph first, or capture with tensors of their own");
   }
 }
 

@@ -213,7 +213,8 @@ int hk_attn_bwd_strided(const void* q, const void* k, const void* v, const void*
 
 /* The backward of hk_attn_fwd_window: hk_attn_bwd_strided(causal = 1) with its window and sinks. Results are bit-identical from run to
  * run; dK and dV of the sinks' key blocks, and where there are few blocks of all, are sums of shares in a fixed order, in places
- * that depend on the whole call's shape.
+ * that depend on the whole call's shape. q, k, v, o and d_o have to be finite throughout, as without a window. Rows that see one key have
+ * no gradient of its score: zeros in dQ, and nothing of them in dK.
  *   workspace : device scratch of at least hk_attn_bwd_window_workspace_bytes(...) bytes, 256-byte aligned, for those shares; the
  *               size may be 0, and then NULL is taken. */
 size_t hk_attn_bwd_window_workspace_bytes(int B, int Nq, int Nk, int H, int H_KV, int D, int window, int sinks);
