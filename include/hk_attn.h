@@ -7,8 +7,8 @@
  * `device` is the CUDA device index the pointers live on (< 0 = the calling thread's current device). An entry
  * point makes that device current while it runs and puts the caller's current device back before it returns.
  * The first call on a device sets the kernels' attributes and allocates one 4-byte status word there (the only
- * allocation the library makes; hk_attn_paged_decode_static does not need it); if that set-up fails the call
- * returns the error and the next call tries again.
+ * allocation the library makes; hk_attn_paged_decode_static does not need it), and the first call with a window those of
+ * the kernels with one; if that set-up fails the call returns the error and the next call tries again.
  */
 #ifndef HK_ATTN_H_
 #define HK_ATTN_H_
