@@ -180,6 +180,8 @@ class HipSelfAttention(nn.Module):
     nn.Dropout but never calls it, hipkittens.py:141,158-161). With `causal`, `window` and `sinks` leave a query the last `window`
     keys and the first `sinks` (``attn_fwd``)."""
 
+    window, sinks = None, 0  # also of modules that were saved before there were windows
+
     def __init__(self, causal=False, softmax_scale=None, attention_dropout=0.0, deterministic=False,
                  window=None, sinks=0):
         super().__init__()
@@ -201,6 +203,8 @@ class HipCrossAttention(nn.Module):
     """q [B, Sq, H, D], kv [B, Sk, 2, H_KV, D] -> [B, Sq, H, D] (hipkittens.py:165-202). Sq may differ from Sk and
     `causal` may be combined with a right-padded `key_padding_mask`, with the reference math path's alignment of the
     causal mask to the last query and the last kept key (base.py:104-116). `window` and `sinks` as in HipSelfAttention."""
+
+    window, sinks = None, 0  # also of modules that were saved before there were windows
 
     def __init__(self, causal=False, softmax_scale=None, attention_dropout=0.0, deterministic=False,
                  window=None, sinks=0):
