@@ -183,62 +183,41 @@ __global__ void __launch_bounds__(256) attn_bwd_prep_kernel(const __nv_bfloat16*
 
 // The same with a window, where rows of few keys are common. delta is the sum of P dP over a row's keys, and where these are few, what
 // the rounding of O and of P left in O does not average out of dP - delta: with O alone dQ is off by 3.8e-3 (relative, 2048 rows) at two
-// keys a row, 3.0e-3 at 4, 2.7e-3 at 8 and 2.4e-3 at 256, of which 2.35e-3 are the roundings of dS and of dQ itself. So rows of up to
-// kFewKeys keys take the sum over their keys, in fp32 and from the scores, in place of rowsum(dO * O): the first ones of a sequence,
-// or, with a window and sinks of so few, all. They are blocks of their own behind the others, a row to D / 8 lanes, with the keys of a
-// row asked for at once. us per backward, without them / with / up to 8 keys, one by one, in the threads of the other rows: B3 N1777
-// H12/4 D64 window 300 77.8 / 80.9 / 87.4, B2 N8192 H32/8 D128 window 1024 1014 / 1015 / 1020, B1 N16384 H32/8 D128 window 9 335.5 /
-// 335.9 / 341.7, window 2 336 / 433 / 469.
-constexpr int kFewKeys = 4;
+// keys a row, 3.0e-3 at 4, 2.7e-3 at 8 and 2.4e-3 at 256, of which 2.35e-3 are the roundings of dS and of dQ itself. So rows of few
+// keys take that sum, in fp32 and from the scores, in place of rowsum(dO * O): those at the first kFewRows positions of a sequence, and
+// with a window and sinks of up to kFewKeys all. They are warps of their own in the first blocks, 16 rows of a head each, and
+// take their keys in groups of 8 through `mma.sync`: these products are 2 D flops a pair of what is a pass over memory otherwise.
+// They come first, so that their chains of loads run beside the others' pass. us per backward, without them / with: B3 N1777 H12/4 D64
+// window 300 79.9 / 82.6, B2 N8192 H32/8 D128 window 1024 1017 / 1020, B8 N1024 H16 D64 window 256 146.8 / 146.8, B1 N16384 H32/8 D128
+// window 2 335 / 383, 9 335 / 384, 24 335 / 401, D64 window 24 263 / 299. (A row to D / 8 lanes, its keys one after the other: window 2
+// 432, 4 454, 8 660.) With 25 to 40 keys a row and delta from O, dQ is off by 2.5e-3.
+constexpr int kFewRows = 32, kFewKeys = 24;
 struct FewKeysParams {
   const __nv_bfloat16 *q, *k, *v;
   const float* lse;                // [B,H,1,N]
   const int* kv_lens;              // or null
   long long q_stride[3], k_stride[3], v_stride[3];  // batch, sequence, head; elements
   int NK, window, sinks;
-  int all;                         // no row sees more
-  int few_rows;                    // rows of the blocks behind: all, or kFewKeys positions of each sequence and head
+  int tiles;                       // of 16 rows, of all sequences and heads
   float scale_log2;
-  FastDiv fd_g;                    // heads to a K/V head
-};
-// The keys of a row: the first `first` of all, and those from `lo` to its own.
-struct RowKeys {
-  int lo, first, count;
-  __device__ __forceinline__ RowKeys(int pos, int window, int sinks) {
-    lo = max(pos - window + 1, 0);
-    first = min(lo, sinks);
-    count = pos < 0 ? 0 : first + pos - lo + 1;
-  }
+  FastDiv fd_g, fd_tiles;          // heads to a K/V head, tiles of a sequence and head
 };
 
-template <int D>
-__global__ void __launch_bounds__(256) attn_bwd_prep_window_kernel(const __nv_bfloat16* o, const __nv_bfloat16* d_o, float* delta,
-                                                                   int rows, int N, int H, FastDiv fd_h, FastDiv fd_n, int blocks,
-                                                                   const __grid_constant__ FewKeysParams p) {
-  constexpr int kLanesPerRow = D / 8;               // 16 or 8
-  constexpr int kRowsPerWarp = 32 / kLanesPerRow;   // 2 or 4
-  const int lane = threadIdx.x & 31;
-  const int sub = lane % kLanesPerRow;
+// ALL: all rows are such rows, and a warp keeps its own in registers.
+template <int D, bool ALL>
+__global__ void __launch_bounds__(256, ALL && D == 128 ? 2 : 3)
+attn_bwd_prep_window_kernel(const __nv_bfloat16* o, const __nv_bfloat16* d_o, float* delta, int rows, int N, int H, FastDiv fd_h,
+                            FastDiv fd_n, int few_blocks, const __grid_constant__ FewKeysParams p) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   ptx::grid_dep_wait();
   ptx::grid_dep_launch();
-  auto dot8 = [](const uint4& x, const uint4& y) {
-    const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
-    float acc = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      acc = fmaf(__uint_as_float(xw[i] << 16), __uint_as_float(yw[i] << 16), acc);
-      acc = fmaf(__uint_as_float(xw[i] & 0xffff0000u), __uint_as_float(yw[i] & 0xffff0000u), acc);
-    }
-    return acc;
-  };
-  auto row_sum = [](float acc) {
-#pragma unroll
-    for (int off = kLanesPerRow / 2; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
-    return acc;
-  };
   auto length = [&](int b) { return p.kv_lens ? min(max(p.kv_lens[b], 1), p.NK) : p.NK; };
-  if (static_cast<int>(blockIdx.x) < blocks) {
-    const int row0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * (kRowsPerWarp * kRowPassUnroll) + lane / kLanesPerRow;
+  const int block = static_cast<int>(blockIdx.x) - few_blocks;
+  if (!ALL && block >= 0) {
+    constexpr int kLanesPerRow = D / 8;               // 16 or 8
+    constexpr int kRowsPerWarp = 32 / kLanesPerRow;   // 2 or 4
+    const int sub = lane % kLanesPerRow;
+    const int row0 = (block * 8 + warp) * (kRowsPerWarp * kRowPassUnroll) + lane / kLanesPerRow;
     uint4 a[kRowPassUnroll], b[kRowPassUnroll];
 #pragma unroll
     for (int u = 0; u < kRowPassUnroll; ++u) {
@@ -246,57 +225,91 @@ __global__ void __launch_bounds__(256) attn_bwd_prep_window_kernel(const __nv_bf
       a[u] = __ldcs(reinterpret_cast<const uint4*>(o + static_cast<size_t>(row) * D) + sub);
       b[u] = __ldcs(reinterpret_cast<const uint4*>(d_o + static_cast<size_t>(row) * D) + sub);
     }
-    float sum[kRowPassUnroll];
-#pragma unroll
-    for (int u = 0; u < kRowPassUnroll; ++u) sum[u] = row_sum(dot8(a[u], b[u]));
 #pragma unroll
     for (int u = 0; u < kRowPassUnroll; ++u) {
+      const uint32_t aw[4] = {a[u].x, a[u].y, a[u].z, a[u].w}, bw[4] = {b[u].x, b[u].y, b[u].z, b[u].w};
+      float acc = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        acc = fmaf(__uint_as_float(aw[i] << 16), __uint_as_float(bw[i] << 16), acc);
+        acc = fmaf(__uint_as_float(aw[i] & 0xffff0000u), __uint_as_float(bw[i] & 0xffff0000u), acc);
+      }
+#pragma unroll
+      for (int off = kLanesPerRow / 2; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
       const int row = row0 + u * kRowsPerWarp;
       if (row < rows && sub == 0) {
         int bn, h, bi, n;
         fd_h.divmod(row, bn, h);
         fd_n.divmod(bn, bi, n);
-        const int pos = n + length(bi) - N;  // not the rows of the blocks behind: those of the first kFewKeys positions
-        if (pos < 0 || pos >= kFewKeys) delta[(static_cast<size_t>(bi) * H + h) * N + n] = sum[u];
+        const int pos = n + length(bi) - N;
+        if (pos < 0 || pos >= kFewRows) delta[(static_cast<size_t>(bi) * H + h) * N + n] = acc;
       }
     }
     return;
   }
-  const int few = ((blockIdx.x - blocks) * 8 + (threadIdx.x >> 5)) * kRowsPerWarp + lane / kLanesPerRow;
-  int bn, h, bi, n;
-  fd_h.divmod(min(few, p.few_rows - 1), bn, h);
-  if (p.all) fd_n.divmod(bn, bi, n);
-  else bi = bn / kFewKeys, n = bn % kFewKeys;
-  const int behind = length(bi) - N;  // a row's position less its number
-  if (!p.all) n -= behind;            // the row at that position, which this sequence may not have
-  const int pos = n + behind;
-  const bool mine = few < p.few_rows && n >= 0 && n < N;
-  const RowKeys r(pos, p.window, p.sinks);
-  const int count = mine ? r.count : 0;
-  uint4 qv = make_uint4(0, 0, 0, 0), g = qv, kv[kFewKeys], vv[kFewKeys];
-  float nl = 0.f;
-  if (count > 0) {
-    nl = p.lse[(static_cast<size_t>(bi) * H + h) * N + n] * -1.4426950408889634f;
-    qv = *reinterpret_cast<const uint4*>(p.q + bi * p.q_stride[0] + n * p.q_stride[1] + h * p.q_stride[2] + sub * 8);
-    g = *(reinterpret_cast<const uint4*>(d_o + (static_cast<size_t>(bi) * N + n) * H * D + static_cast<size_t>(h) * D) + sub);
+  const int tile = blockIdx.x * 8 + warp;
+  if (tile >= p.tiles) return;
+  int bt, h, bi, first;
+  fd_h.divmod(tile, bt, h);
+  p.fd_tiles.divmod(bt, bi, first);
+  const int kv_len = length(bi), behind = kv_len - N;  // a row's position less its number
+  first = first * 16 + (ALL ? behind : 0);             // position of the first row
+  if (first - behind >= N || first + 15 - behind < 0) return;
+  const int g = lane >> 2, t = lane & 3;
+  const __nv_bfloat16 *q[2], *grad[2];  // rows g and g + 8
+  float nl[2], sum[2] = {0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int n = min(max(first + g + 8 * i - behind, 0), N - 1);  // a row that is not there: another one, and not stored
+    q[i] = p.q + bi * p.q_stride[0] + n * p.q_stride[1] + h * p.q_stride[2] + t * 8;
+    grad[i] = d_o + ((static_cast<size_t>(bi) * N + n) * H + h) * D + t * 8;
+    nl[i] = p.lse[(static_cast<size_t>(bi) * H + h) * N + n] * -1.4426950408889634f;
   }
   const int kvh = p.fd_g.div(h);
+  const __nv_bfloat16 *const k = p.k + bi * p.k_stride[0] + kvh * p.k_stride[2] + t * 8,
+                      *const v = p.v + bi * p.v_stride[0] + kvh * p.v_stride[2] + t * 8;
+  auto load = [](const __nv_bfloat16* x) { return *reinterpret_cast<const uint4*>(x); };
+  [[maybe_unused]] uint4 own[ALL ? D / 32 : 1][4];
+  if constexpr (ALL) {
 #pragma unroll
-  for (int i = 0; i < kFewKeys; ++i) {
-    kv[i] = vv[i] = make_uint4(0, 0, 0, 0);
-    if (i < count) {
-      const long long key = i < r.first ? i : r.lo + i - r.first;
-      kv[i] = *reinterpret_cast<const uint4*>(p.k + bi * p.k_stride[0] + key * p.k_stride[1] + kvh * p.k_stride[2] + sub * 8);
-      vv[i] = *reinterpret_cast<const uint4*>(p.v + bi * p.v_stride[0] + key * p.v_stride[1] + kvh * p.v_stride[2] + sub * 8);
+    for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) own[c][i] = load(q[i] + c * 32), own[c][2 + i] = load(grad[i] + c * 32);
+  }
+  // keys [0, sinks) in front of the first window, then those from its first to the last row's own
+  const int lo = max(first - p.window + 1, 0), sinks = min(p.sinks, lo), end = min(first + 16, kv_len);
+#pragma unroll 1
+  for (int key0 = sinks > 0 ? 0 : lo; key0 < end; key0 = key0 < sinks && key0 + 8 >= sinks ? lo : key0 + 8) {
+    const int limit = key0 < sinks ? sinks : end;  // of the range that this group lies in
+    const long long key = min(key0 + g, kv_len - 1);
+    float s[4] = {0.f, 0.f, 0.f, 0.f}, dp[4] = {0.f, 0.f, 0.f, 0.f};
+    // A lane has 8 neighbouring columns of its rows and of its key at a time, in place of those that the products name: the sum over
+    // columns is the same
+#pragma unroll(ALL ? D / 32 : 1)
+    for (int c = 0; c < D / 32; ++c) {
+      const uint4 kc = load(k + key * p.k_stride[1] + c * 32), vc = load(v + key * p.v_stride[1] + c * 32);
+      uint4 q0, q1, g0, g1;
+      if constexpr (ALL) q0 = own[c][0], q1 = own[c][1], g0 = own[c][2], g1 = own[c][3];
+      else q0 = load(q[0] + c * 32), q1 = load(q[1] + c * 32), g0 = load(grad[0] + c * 32), g1 = load(grad[1] + c * 32);
+      ptx::mma_16816(s, q0.x, q1.x, q0.y, q1.y, kc.x, kc.y);
+      ptx::mma_16816(dp, g0.x, g1.x, g0.y, g1.y, vc.x, vc.y);
+      ptx::mma_16816(s, q0.z, q1.z, q0.w, q1.w, kc.z, kc.w);
+      ptx::mma_16816(dp, g0.z, g1.z, g0.w, g1.w, vc.z, vc.w);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {  // rows g and g + 8, keys 2 t and 2 t + 1
+      const int at = key0 + 2 * t + (e & 1), pos = first + g + 8 * (e >> 1);
+      const bool seen = at < limit && at <= pos && (pos - at < p.window || at < p.sinks);
+      if (seen) sum[e >> 1] = fmaf(ptx::ex2_approx(fmaf(s[e], p.scale_log2, nl[e >> 1])), dp[e], sum[e >> 1]);
     }
   }
-  float sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < kFewKeys; ++i) {  // the lanes of a warp stay together: sums over a row are shuffles
-    const float s = row_sum(dot8(qv, kv[i])), dp = row_sum(dot8(g, vv[i]));
-    if (i < count) sum = fmaf(ptx::ex2_approx(fmaf(s, p.scale_log2, nl)), dp, sum);
+  for (int i = 0; i < 2; ++i) {
+    sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
+    sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
+    const int n = first + g + 8 * i - behind;
+    if (t == 0 && n >= 0 && n < N) delta[(static_cast<size_t>(bi) * H + h) * N + n] = sum[i];
   }
-  if (mine && sub == 0) delta[(static_cast<size_t>(bi) * H + h) * N + n] = sum;
 }
 
 // ------------------------------------------------------------------------------------ dQ [B,H,N,D] -> [B,N,H,D]

@@ -930,7 +930,6 @@ struct Span {
 static int prep_window_launch(const void* q, const void* k, const void* v, const void* o, const void* d_o, float* delta,
                               const BwdStrides& s, const hk::BwdParams& p, int D, cudaStream_t stream) {
   const long long rows = 1ll * p.B * p.N * p.H;
-  if (rows > 0x7fffffffll || 1ll * p.B * p.H > 0x7fffffffll / (2 * hk::kFewKeys)) return HK_EINVAL;  // rows are indexed with int
   hk::FewKeysParams f;
   f.q = static_cast<const __nv_bfloat16*>(q);
   f.k = static_cast<const __nv_bfloat16*>(k);
@@ -939,16 +938,20 @@ static int prep_window_launch(const void* q, const void* k, const void* v, const
   f.kv_lens = p.kv_lens;
   for (int i = 0; i < 3; ++i) f.q_stride[i] = s.q[i], f.k_stride[i] = s.k[i], f.v_stride[i] = s.v[i];
   f.NK = p.NK, f.window = p.window, f.sinks = p.sinks;
-  f.all = 1ll * p.window + p.sinks <= hk::kFewKeys || p.NK <= hk::kFewKeys;
-  f.few_rows = f.all ? int(rows) : p.B * hk::kFewKeys * p.H;
+  const bool all = 1ll * p.window + p.sinks <= hk::kFewKeys;
+  const int per_head = (all ? p.N - 1 : hk::kFewRows - 1) / 16 + 1;
+  if (rows > 0x7fffffffll || 1ll * p.B * p.H * per_head > 0x3fffffffll) return HK_EINVAL;  // rows and tiles are indexed with int
+  f.tiles = p.B * p.H * per_head;
   f.scale_log2 = p.scale_log2;
   f.fd_g = hk::FastDiv(p.H / p.H_KV);
-  const int rows_per_block = hk::row_pass_rows(D / 8), few_per_block = rows_per_block / hk::kRowPassUnroll;
-  const int blocks = f.all ? 0 : int((rows + rows_per_block - 1) / rows_per_block);
-  auto* fn = D == 128 ? hk::attn_bwd_prep_window_kernel<128> : hk::attn_bwd_prep_window_kernel<64>;
-  HK_CUDA(hk::launch_dependent(true, fn, unsigned(blocks + (f.few_rows - 1) / few_per_block + 1), 256, 0, stream,
-                               static_cast<const __nv_bfloat16*>(o), static_cast<const __nv_bfloat16*>(d_o), delta, int(rows), p.N, p.H,
-                               hk::FastDiv(p.H), hk::FastDiv(p.N), blocks, f));
+  f.fd_tiles = hk::FastDiv(per_head);
+  const int rows_per_block = hk::row_pass_rows(D / 8), few_blocks = (f.tiles - 1) / 8 + 1;
+  const int blocks = all ? 0 : int((rows + rows_per_block - 1) / rows_per_block);
+  auto* fn = D == 128 ? (all ? hk::attn_bwd_prep_window_kernel<128, true> : hk::attn_bwd_prep_window_kernel<128, false>)
+                      : (all ? hk::attn_bwd_prep_window_kernel<64, true> : hk::attn_bwd_prep_window_kernel<64, false>);
+  HK_CUDA(hk::launch_dependent(true, fn, unsigned(few_blocks + blocks), 256, 0, stream, static_cast<const __nv_bfloat16*>(o),
+                               static_cast<const __nv_bfloat16*>(d_o), delta, int(rows), p.N, p.H, hk::FastDiv(p.H), hk::FastDiv(p.N),
+                               few_blocks, f));
   g_launches.fetch_add(1, std::memory_order_relaxed);
   return HK_OK;
 }
