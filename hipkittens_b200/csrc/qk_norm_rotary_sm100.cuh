@@ -206,6 +206,8 @@ struct Walk {
     b += seqs;
     return true;
   }
+  // What `step` more heads of the same token are away. In 64 bits: a head's stride alone may be 2^30 units.
+  static __device__ __forceinline__ long long heads_on(const QknSide& s, int step) { return static_cast<long long>(step) * s.stride_h; }
   __device__ __forceinline__ const uint4* place(const QknSide& s) const {
     return reinterpret_cast<const uint4*>(s.x) + (b * s.stride_b + static_cast<long long>(n) * s.stride_n + static_cast<long long>(h) * s.stride_h);
   }
@@ -284,7 +286,7 @@ __global__ void __launch_bounds__(kQknThreads, 6) qk_norm_rotary_kernel(const __
     }
     cp_async_commit();
     ahead_row += kStep;
-    x += kStep * s.stride_h;
+    x += Walk::heads_on(s, kStep);
     if (ahead.next(p, s, kStep)) x = ahead.place(s);
   };
 #pragma unroll
@@ -364,7 +366,7 @@ __global__ void __launch_bounds__(kQknThreads, 4) qk_norm_rotary_bwd_kernel(cons
     cp_async_commit();
     ahead_row += kStep;
     dy += kStep * (p.D / 8);
-    x_ahead += kStep * s.stride_h;
+    x_ahead += Walk::heads_on(s, kStep);
     if (ahead.next(p, s, kStep)) x_ahead = ahead.place(s);
   };
 #pragma unroll
