@@ -236,6 +236,15 @@ def _require_same_device(ref: torch.Tensor, **tensors) -> None:
                                f"{t.device if isinstance(t, torch.Tensor) else type(t).__name__})")
 
 
+def _new(shape, dtype: torch.dtype, device: torch.device, stream) -> torch.Tensor:
+    """An output, from the memory of the stream that writes it (None: torch's current one): what another stream gave back may
+    still be read by work that waits there."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
 def _strides3(t):
     # a dimension of size 1 has no stride that matters: give it one the library takes
     return (ctypes.c_longlong * 3)(*(st if n > 1 else t.shape[3] for st, n in zip(t.stride()[:3], t.shape[:3])))
@@ -302,9 +311,9 @@ def attn_fwd(
     if k.shape != v.shape or k.shape[0] != b or k.shape[3] != d:
         raise RuntimeError("k/v must be [B, Nk, H_KV, D] matching q's batch and head dimension")
     if out is None:
-        out = torch.empty((b, n, h, d), dtype=torch.bfloat16, device=q.device)
+        out = _new((b, n, h, d), torch.bfloat16, q.device, stream)
     if lse is None:
-        lse = torch.empty((b, h, 1, n), dtype=torch.float32, device=q.device)
+        lse = _new((b, h, 1, n), torch.float32, q.device, stream)
     if out.shape != q.shape or out.dtype != torch.bfloat16 or not out.is_contiguous():
         raise RuntimeError("out must be a contiguous bf16 tensor of q's shape")
     if lse.shape != (b, h, 1, n) or lse.dtype != torch.float32 or not lse.is_contiguous():
@@ -353,7 +362,7 @@ def attn_bwd_prep(o: torch.Tensor, d_o: torch.Tensor, delta: Optional[torch.Tens
         raise RuntimeError("o and d_o must have the same shape")
     b, n, h, d = o.shape
     if delta is None:
-        delta = torch.empty((b, h, 1, n), dtype=torch.float32, device=o.device)
+        delta = _new((b, h, 1, n), torch.float32, o.device, stream)
     if delta.shape != (b, h, 1, n) or delta.dtype != torch.float32 or not delta.is_contiguous():
         raise RuntimeError("delta must be a contiguous fp32 tensor [B, H, 1, N]")
     _require_same_device(o, d_o=d_o, delta=delta)
@@ -398,11 +407,11 @@ def attn_bwd(
             raise RuntimeError(f"{name} must be a contiguous fp32 tensor [B, H, 1, N] on q's device")
     dq_shape = (b, n, h, d) if dq_layout == HK_DQ_BNHD else (b, h, n, d)
     if dq is None:
-        dq = torch.empty(dq_shape, dtype=torch.bfloat16, device=q.device)
+        dq = _new(dq_shape, torch.bfloat16, q.device, stream)
     if dk is None:
-        dk = torch.empty_like(k)
+        dk = _new(k.shape, k.dtype, k.device, stream)
     if dv is None:
-        dv = torch.empty_like(v)
+        dv = _new(v.shape, v.dtype, v.device, stream)
     for name, t, shp in (("dq", dq, dq_shape), ("dk", dk, tuple(k.shape)), ("dv", dv, tuple(v.shape))):
         if tuple(t.shape) != tuple(shp) or t.dtype != torch.bfloat16 or not t.is_contiguous():
             raise RuntimeError(f"{name} must be a contiguous bf16 tensor of shape {tuple(shp)}")
@@ -501,7 +510,7 @@ def dq_shuffle(dq_bhnd: torch.Tensor, dq_bnhd: Optional[torch.Tensor] = None,
     _require_cuda_bf16("dq_bhnd", dq_bhnd, 4)
     b, h, n, d = dq_bhnd.shape
     if dq_bnhd is None:
-        dq_bnhd = torch.empty((b, n, h, d), dtype=dq_bhnd.dtype, device=dq_bhnd.device)
+        dq_bnhd = _new((b, n, h, d), dq_bhnd.dtype, dq_bhnd.device, stream)
     if dq_bnhd.shape != (b, n, h, d) or dq_bnhd.dtype != dq_bhnd.dtype or not dq_bnhd.is_contiguous():
         raise RuntimeError("dq_bnhd must be a contiguous tensor [B, N, H, D] of the source's dtype")
     if dq_bhnd.dtype != torch.bfloat16:
@@ -530,7 +539,7 @@ def rotary(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, out: Optional[
         raise RuntimeError("x must be [B,H,N,D] and cos/sin [N, R/2]")
     b, h, n, d = x.shape
     if out is None:
-        out = torch.empty_like(x)
+        out = _new(x.shape, x.dtype, x.device, stream)
     if out.shape != x.shape or out.dtype != x.dtype or not out.is_contiguous():
         raise RuntimeError("out must be a contiguous bf16 tensor of x's shape")
     _require_same_device(x, cos=cos, sin=sin, out=out)
@@ -555,7 +564,7 @@ def rotary_bnhd(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, out: Opti
         raise RuntimeError("x must be [B,N,H,D] and cos/sin [>= N + pos_offset, R/2]")
     b, n, h, d = x.shape
     if out is None:
-        out = torch.empty_like(x)
+        out = _new(x.shape, x.dtype, x.device, stream)
     if out.shape != x.shape or out.dtype != x.dtype or not out.is_contiguous():
         raise RuntimeError("out must be a contiguous bf16 tensor of x's shape")
     _require_same_device(x, cos=cos, sin=sin, out=out)
@@ -649,8 +658,7 @@ def qk_norm_rotary(
     outs = []
     for name, t, o in (("q_out", q, q_out), ("k_out", k, k_out)):
         if o is None:
-            with torch.cuda.stream(s):  # memory of the stream that writes it
-                o = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+            o = _new(t.shape, t.dtype, t.device, stream)
         if not isinstance(o, torch.Tensor) or o.shape != t.shape or o.dtype != t.dtype or not o.is_contiguous():
             raise RuntimeError(f"{name} must be a contiguous bf16 tensor of its input's shape")
         _require_same_device(q, **{name: o})
@@ -694,10 +702,9 @@ def qk_norm_rotary_bwd(
     _require_same_device(q, dq_out=dq_out, dk_out=dk_out)
     s = stream if stream is not None else torch.cuda.current_stream(q.device)
     need = int(capi().hk_qk_norm_rotary_bwd_workspace_bytes(d))
-    with torch.cuda.stream(s):  # memory of the stream that writes it
-        dq, dk = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
-        dws = [torch.empty_like(w) if weight_grads and w is not None else None for w in (q_weight, k_weight)]
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if any(w is not None for w in dws) else None
+    dq, dk = (_new(t.shape, t.dtype, t.device, stream) for t in (q, k))
+    dws = [_new(w.shape, w.dtype, w.device, stream) if weight_grads and w is not None else None for w in (q_weight, k_weight)]
+    ws = _new(need, torch.uint8, q.device, stream) if any(w is not None for w in dws) else None
     _check(capi().hk_qk_norm_rotary_bwd(q.data_ptr(), k.data_ptr(), _ptr(q_weight), _ptr(k_weight), cos.data_ptr(), sin.data_ptr(),
                                         dq_out.data_ptr(), dk_out.data_ptr(), dq.data_ptr(), dk.data_ptr(), _ptr(dws[0]),
                                         _ptr(dws[1]), b, n, h, k.shape[2], d, 2 * cos.shape[1], cos.shape[0], _strides3(q),
@@ -771,9 +778,9 @@ def paged_decode(
         raise RuntimeError("block_table must be [S, max_pages] and ctx_lens [S]")
     max_pages = block_table.shape[1]
     if out is None:
-        out = torch.empty_like(q)
+        out = _new(q.shape, q.dtype, q.device, stream)
     if lse is None:
-        lse = torch.empty((s_n, h, 1, 1), dtype=torch.float32, device=q.device)
+        lse = _new((s_n, h, 1, 1), torch.float32, q.device, stream)
     need = paged_decode_workspace_bytes(s_n, h, d, max_pages, page, window, sinks)
     if need == 0:
         raise HkError(HK_EUNSUPPORTED, "hk_attn_paged_decode",
@@ -781,8 +788,7 @@ def paged_decode(
                       "max_pages, or pages of a window and its sinks, <= 8192)")
     st = stream if stream is not None else torch.cuda.current_stream(q.device)
     if workspace is None:
-        with torch.cuda.stream(st):  # it goes back to the stream that uses it
-            workspace = torch.empty(max(need, 256), dtype=torch.uint8, device=q.device)
+        workspace = _new(max(need, 256), torch.uint8, q.device, stream)  # it goes back to the stream that uses it
     _require_same_device(q, k_pages=k_pages, v_pages=v_pages, block_table=block_table, ctx_lens=ctx_lens, out=out,
                          lse=lse, workspace=workspace)
     if window is not None:
@@ -847,9 +853,9 @@ def attn_fwd_paged(
     if block_table.dim() != 2 or block_table.shape[0] != s_n or ctx_lens.shape != (s_n,):
         raise RuntimeError("block_table must be [S, max_pages] and ctx_lens [S]")
     if out is None:
-        out = torch.empty_like(q)
+        out = _new(q.shape, q.dtype, q.device, stream)
     if lse is None:
-        lse = torch.empty((s_n, h, 1, t_n), dtype=torch.float32, device=q.device)
+        lse = _new((s_n, h, 1, t_n), torch.float32, q.device, stream)
     if out.shape != q.shape or out.dtype != torch.bfloat16 or not out.is_contiguous():
         raise RuntimeError("out must be a contiguous bf16 tensor of q's shape")
     if lse.shape != (s_n, h, 1, t_n) or lse.dtype != torch.float32 or not lse.is_contiguous():
