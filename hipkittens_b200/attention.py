@@ -97,6 +97,7 @@ class HipAttnFunction(Function):
         return O.to(q_bnhd.dtype)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dO_bnhd: torch.Tensor):
         q, k, v, O, L = ctx.saved_tensors
         dQ, dK, dV = (torch.empty(t.shape, dtype=torch.bfloat16, device=t.device) for t in (q, k, v))
@@ -122,6 +123,7 @@ class _PackedAttnFunction(Function):
         return O
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dO_bnhd):
         *q, packed, O, L = ctx.saved_tensors
         d_packed = torch.empty(packed.shape, dtype=torch.bfloat16, device=packed.device)

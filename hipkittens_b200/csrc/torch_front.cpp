@@ -501,6 +501,20 @@ void check_device(int device, const char* direction) {
   TORCH_CHECK(status == HK_OK, "attention ", direction, " failed on the device (status ", status, ")");
 }
 
+// What a backward returns, of `arguments` of its call. Where a graph of the gradients is wanted they have none of their own, and whoever
+// differentiates them again is told so.
+variable_list without_a_second(variable_list grads, size_t arguments) {
+  if (at::GradMode::is_enabled()) {
+    for (Tensor& t : grads)
+      if (t.defined()) t.requires_grad_();
+    const int n = static_cast<int>(grads.size());
+    grads = (*std::make_shared<torch::autograd::DelayedError>(
+        "trying to differentiate twice a function that was marked with @once_differentiable", n))(std::move(grads));
+  }
+  grads.resize(arguments);
+  return grads;
+}
+
 // The parts of a packed projection [B, S, 2 or 3, H, D], or of its gradient.
 struct Parts {
   char* base;
@@ -611,7 +625,7 @@ class PackedAttention : public torch::autograd::Function<PackedAttention> {
                                        stream);
     if (rc != HK_OK) fail("hk_attn_bwd_strided", rc);
     check_device(a.device, "backward");
-    return {dq, d_packed, Tensor()};
+    return without_a_second({dq, d_packed}, 3);
   }
 };
 
@@ -735,15 +749,7 @@ class NormRotary : public torch::autograd::Function<NormRotary> {
         i32(ctx->saved_data["offset"].toInt()), static_cast<float>(ctx->saved_data["eps"].toDouble()),
         i32(ctx->saved_data["flags"].toInt()), opt(ws), need, s[0].device().index(), stream_of(s[0]));
     if (rc != HK_OK) fail("hk_qk_norm_rotary_bwd", rc);
-    variable_list out = {dx[0], dx[1], dw[0], dw[1]};
-    if (at::GradMode::is_enabled()) {  // a graph of the gradients: they have none of their own
-      for (Tensor& t : out)
-        if (t.defined()) t.requires_grad_();
-      out = (*std::make_shared<torch::autograd::DelayedError>(
-          "trying to differentiate twice a function that was marked with @once_differentiable", 4))(std::move(out));
-    }
-    out.resize(8);
-    return out;
+    return without_a_second({dx[0], dx[1], dw[0], dw[1]}, 8);
   }
 };
 
