@@ -663,24 +663,31 @@ PyObject* packed_attention(PyObject*, PyObject* const* arg, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
-bool captured(cudaStream_t stream) {
+// The capture that a stream is part of, 0 for none.
+unsigned long long capture_of(cudaStream_t stream) {
   cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
-  if (cudaStreamIsCapturing(stream, &status) == cudaSuccess) return status != cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo(stream, &status, &id) == cudaSuccess) return status == cudaStreamCaptureStatusNone ? 0 : id;
   (void)cudaGetLastError();  // the legacy stream, while another one is captured that waits for it
-  return false;
+  return 0;
 }
-// A gradient goes to the stream on which its tensor's node was made. Where that is not captured and this backward is, as with a leaf that
-// a graph from before the capture holds as well, the engine would make that stream wait for a captured one: this ends the capture, and
-// may end the process.
-void check_next_streams(AutogradContext* ctx, cudaStream_t stream) {
-  if (!captured(stream)) return;
+// A gradient goes to the stream on which its tensor's node was made, and the engine makes that stream wait for the one of this backward.
+// Where this backward is captured and that stream is not, as with a leaf that a graph from before the capture holds as well, the wait
+// takes it into the capture. The legacy stream cannot be, nor one of another capture: the wait ends the capture and may end the process.
+void check_next_streams(cudaStream_t stream) {
+  const unsigned long long capture = capture_of(stream);
+  if (!capture) return;
   const auto node = torch::autograd::get_current_node();
   if (!node) return;
   for (size_t i = 0; i < node->num_outputs(); ++i) {
     const auto& next = node->next_edge(i).function;
-    const auto to = next && ctx->needs_input_grad(i) ? next->stream() : std::nullopt;
-    TORCH_CHECK(!to || captured(c10::cuda::CUDAStream(*to).stream()), "a captured backward needs tensors that no graph from before",
-                " the capture holds: delete that graph first, or capture with tensors of their own");
+    const auto to = next && node->task_should_compute_output(i) ? next->stream() : std::nullopt;
+    if (!to) continue;
+    const cudaStream_t other = c10::cuda::CUDAStream(*to).stream();
+    const bool legacy = other == nullptr || other == cudaStreamLegacy;
+    const unsigned long long others = legacy ? 0 : capture_of(other);
+    TORCH_CHECK(!legacy && (others == 0 || others == capture), "a captured backward needs tensors that no graph from before",
+                " the capture holds on the default stream: delete that graph first, or capture with tensors of their own");
   }
 }
 
@@ -718,7 +725,7 @@ class NormRotary : public torch::autograd::Function<NormRotary> {
   // In a thread of the engine, without the interpreter.
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     variable_list s = ctx->get_saved_variables();
-    check_next_streams(ctx, static_cast<cudaStream_t>(stream_of(s[0])));
+    check_next_streams(static_cast<cudaStream_t>(stream_of(s[0])));
     QknCall c;
     long long* const st[2] = {c.qs, c.ks};
     Tensor dy[2], dx[2], dw[2];
