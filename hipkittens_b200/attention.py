@@ -248,6 +248,7 @@ class QkNormRotaryFunction(Function):
     @once_differentiable
     def backward(ctx, dq_out, dk_out):
         *saved, positions = ctx.saved_tensors
+        _front().captured_backward(dq_out)
         dy = (t.to(torch.bfloat16).contiguous() for t in (dq_out, dk_out))
         wanted = ctx.needs_input_grad[2] or ctx.needs_input_grad[3]
         grads = qk_norm_rotary_bwd(*saved, *dy, positions, *ctx.rest, weight_grads=wanted)

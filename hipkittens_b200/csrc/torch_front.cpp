@@ -780,11 +780,21 @@ PyObject* norm_rotary(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
+// captured_backward(tensor): raises what the backward of `norm_rotary` does, for a Python function whose backward is running on the
+// tensor's device
+PyObject* captured_backward(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  const Tensor* t = n_args == 1 ? plain(a[0]) : nullptr;
+  if (t) check_next_streams(static_cast<cudaStream_t>(stream_of(*t)));
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
 #define HK_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {HK_METHOD(attn_fwd),       HK_METHOD(attn_bwd_strided), HK_METHOD(rotary_bnhd),
                          HK_METHOD(paged_decode),   HK_METHOD(attn_fwd_paged),   HK_METHOD(paged_kv_append),
                          HK_METHOD(qk_norm_rotary), HK_METHOD(qk_norm_rotary_bwd),
-                         HK_METHOD(packed_attention), HK_METHOD(norm_rotary),
+                         HK_METHOD(packed_attention), HK_METHOD(norm_rotary), HK_METHOD(captured_backward),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_front", "Native tensor front ends of hipkittens_b200", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};

@@ -59,7 +59,7 @@ def test_leaves_of_a_graph_on_a_side_stream_are_captured(native, into_grad):
     assert all(torch.equal(t.grad, b) for t, b in zip(leaves, want))
 
 
-@pytest.mark.parametrize("native", [True])
+@pytest.mark.parametrize("native", [True, False])
 def test_leaves_of_a_graph_on_the_default_stream_are_refused(native):
     """... before the engine makes that stream wait, which ends the capture and may end the process."""
     x, dy, m, cos, sin = setup(native, 2)
