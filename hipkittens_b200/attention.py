@@ -134,18 +134,25 @@ class _PackedAttnFunction(Function):
 
 def _attend(q, packed, causal, softmax_scale, key_padding_mask, window=None, sinks=0):
     """Attention of q (None: the first of the packed tensors) over a packed projection [B, S, 2 or 3, H, D]."""
+    # queries that are padded with their keys stand at their rows' positions: no kept one sees the padding behind it, whose rows
+    # come back as zeros, with no gradient
+    in_place = q is None and window is not None
     if key_padding_mask is None:
         out = _apply(q, packed, causal, softmax_scale, None, window, sinks)
     else:
+        if in_place and key_padding_mask.shape[0] != packed.shape[0]:
+            raise ValueError(_MASK_SHAPE)
         kv_lens, bad = _lens_from_key_padding_mask(key_padding_mask, packed)
         try:
-            out = _apply(q, packed, causal, softmax_scale, kv_lens, window, sinks)
+            out = _apply(q, packed, causal, softmax_scale, None if in_place else kv_lens, window, sinks)
         except BaseException:
             torch.cuda.synchronize(packed.device)  # the flag may still be written: it is given back only then
             raise
         # whatever the mask, the kernels clamp the lengths
         if bad.item() != 0:
             raise ValueError(_BAD_MASK)
+        if in_place:
+            out = out.masked_fill(~key_padding_mask[:, :, None, None], 0)
     return out.to((packed if q is None else q).dtype).contiguous()
 
 
@@ -159,6 +166,7 @@ def _apply(q, packed, causal, softmax_scale, kv_lens, window, sinks):
     return HipAttnFunction.apply(*views, causal, softmax_scale, kv_lens, window, sinks)
 
 
+_MASK_SHAPE = "key_padding_mask must be a bool tensor (batch, seqlen), True = keep"
 _BAD_MASK = "only right-padded key_padding_mask (a kept prefix of at least one key per row) is supported"
 
 
@@ -167,7 +175,7 @@ def _lens_from_key_padding_mask(mask: torch.Tensor, packed: torch.Tensor):
     (right padding, what padded batches have), and a flag that becomes non-zero if a row is anything else, which
     cannot be expressed as lengths and is refused."""
     if mask.dim() != 2 or mask.shape[1] != packed.shape[1] or mask.dtype != torch.bool:
-        raise ValueError("key_padding_mask must be a bool tensor (batch, seqlen), True = keep")
+        raise ValueError(_MASK_SHAPE)
     assert packed.is_cuda, "All tensors must be on CUDA device"
     if mask.device != packed.device:
         raise RuntimeError("key_padding_mask must be on the device of q, k and v")
@@ -180,7 +188,12 @@ class HipSelfAttention(nn.Module):
     """qkv [B, S, 3, H, D] -> [B, S, H, D] (hipkittens.py:122-162). Same constructor as the reference;
     `causal` and `softmax_scale` take effect here, dropout is not applied (the reference builds an
     nn.Dropout but never calls it, hipkittens.py:141,158-161). With `causal`, `window` and `sinks` leave a query the last `window`
-    keys and the first `sinks` (``attn_fwd``)."""
+    keys and the first `sinks` (``attn_fwd``).
+
+    With a window and a right-padded `key_padding_mask`, row r of a sequence is at position r, as without a mask, and rows of padding
+    come back as zeros, whose gradients go nowhere. `causal` without a window aligns the mask as HipCrossAttention does, the last row
+    to the last kept key, which is not the position of a row that has padding behind it: such a batch needs no mask there, since no
+    kept row sees what follows it."""
 
     window, sinks = None, 0  # also of modules that were saved before there were windows
 
@@ -204,7 +217,8 @@ class HipSelfAttention(nn.Module):
 class HipCrossAttention(nn.Module):
     """q [B, Sq, H, D], kv [B, Sk, 2, H_KV, D] -> [B, Sq, H, D] (hipkittens.py:165-202). Sq may differ from Sk and
     `causal` may be combined with a right-padded `key_padding_mask`, with the reference math path's alignment of the
-    causal mask to the last query and the last kept key (base.py:104-116). `window` and `sinks` as in HipSelfAttention."""
+    causal mask to the last query and the last kept key (base.py:104-116): of a chunk of queries behind a cache, the last one is at the
+    last kept key's position. `window` and `sinks` count from there, as in ``attn_fwd``."""
 
     window, sinks = None, 0  # also of modules that were saved before there were windows
 
