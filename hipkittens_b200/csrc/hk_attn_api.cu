@@ -610,7 +610,8 @@ struct WindowShares {
   int blocks, shares;
 };
 // A window that no key lies behind masks nothing that the causal mask does not: the backward is the causal one, but for a single tile
-// of keys, where rows that see one key weigh most (their dS is exactly zero with a window).
+// of keys, where the row that sees one key weighs most. (Its dS is exactly zero with a window; the causal kernels, whose dP comes from
+// other instructions than its delta, leave it the difference of two fp32 sums.)
 bool covers_all(int NK, int window, int sinks) { return NK > hk::kBlockN && (window >= NK || sinks >= NK); }
 WindowShares window_shares(int units, int G, int N, int NK, int D, int window, int sinks) {
   constexpr long long kSms = 148, kMost = 32;

@@ -83,7 +83,8 @@ int hk_attn_fwd_cross(const void* q, const void* k, const void* v, void* o, floa
  * row r at position p = r + (kv_len_b - Nq), key c is seen iff c <= p and (p - c < window or c < sinks), so that a row
  * sees its own key and the window - 1 before it. window >= 1, sinks >= 0. A row that sees no key gets O = 0, L = -inf. Keys that
  * a row does not see may hold anything; V has to be finite throughout, as without a window (0 times infinity).
- * Keys that no row of a block sees are neither loaded nor multiplied; with window >= Nk this is hk_attn_fwd_cross. */
+ * Keys that no row of a block sees are neither loaded nor multiplied. Where nothing is hidden, window or sinks >= Nk, the results are
+ * those of hk_attn_fwd_cross(causal = 1): bit for bit at D = 128, within roundings at D = 64, where L is the more exact one here. */
 int hk_attn_fwd_window(const void* q, const void* k, const void* v, void* o, float* lse,
                        int B, int Nq, int Nk, int H, int H_KV, int D,
                        const long long* q_strides, const long long* k_strides, const long long* v_strides,
@@ -214,7 +215,9 @@ int hk_attn_bwd_strided(const void* q, const void* k, const void* v, const void*
 /* The backward of hk_attn_fwd_window: hk_attn_bwd_strided(causal = 1) with its window and sinks. Results are bit-identical from run to
  * run; dK and dV of the sinks' key blocks, and where there are few blocks of all, are sums of shares in a fixed order, in places
  * that depend on the whole call's shape. q, k, v, o and d_o have to be finite throughout, as without a window. Rows that see one key have
- * no gradient of its score: zeros in dQ, and nothing of them in dK.
+ * no gradient of its score: zeros in dQ, and nothing of them in dK. (Where nothing is hidden, window or sinks >= Nk > 128, this is
+ * hk_attn_bwd_strided(causal = 1) with a delta that is more exact for rows of few keys: there the row at position 0 keeps what two fp32
+ * sums of the same D products differ by.)
  *   workspace : device scratch of at least hk_attn_bwd_window_workspace_bytes(...) bytes, 256-byte aligned, for those shares; the
  *               size may be 0, and then NULL is taken. */
 size_t hk_attn_bwd_window_workspace_bytes(int B, int Nq, int Nk, int H, int H_KV, int D, int window, int sinks);
