@@ -70,12 +70,12 @@ def _backward(ctx, q, k, v, O, L, dO_bnhd, dQ, dK, dV):
     try:
         attn_bwd_strided(q, k, v, O, dO, L, dQ, dK, dV, **rest)
     except RuntimeError:
-        # saved-tensor hooks may have given q, k or v back in a layout that the kernels cannot read (looked for only here,
+        # saved-tensor hooks may have given q, k, v, O or L back in a layout that the kernels cannot read (looked for only here,
         # where the call was refused: the look takes 4 us)
-        dense = [t if _tma_viewable(t) else t.contiguous() for t in (q, k, v)]
-        if all(a is b for a, b in zip(dense, (q, k, v))):
+        dense = [*(t if _tma_viewable(t) else t.contiguous() for t in (q, k, v)), O.contiguous(), L.contiguous()]
+        if all(a is b for a, b in zip(dense, (q, k, v, O, L))):
             raise
-        attn_bwd_strided(*dense, O, dO, L, dQ, dK, dV, **rest)
+        attn_bwd_strided(*dense[:4], dO, dense[4], dQ, dK, dV, **rest)
     _blocking_status(O.device, "backward")
 
 
