@@ -55,6 +55,9 @@ constexpr float kRescaleThresholdLog2 = 8.0f;
 // at D = 128. Which pairs matters as much as how many, through the instruction schedule the compiler arrives at: the
 // non-causal D = 64 kernel is fastest with the first two of every eight pairs (+1.4 % over one of every four; the
 // same quarter at other offsets or in runs of four is 0.5 to 3 % slower), the causal one with one of every four.
+// With a window none do. Short ones leave room at the MUFU, and long ones gain less than the error of L is worth. us at D = 64, one of
+// every four / none: B1 N16384 H32/8 window 128 99.6 / 96.3, B8 N1024 H16 window 256 47.4 / 45.7, B3 N1777 H12/4 window 300 27.2 / 27.2,
+// B2 N8192 H32/8 window 1024 262.2 / 268.4, B1 N16384 H32/8 window 4096 704 / 714; error of L 1.3e-5 to 3.3e-5 / 7e-7 to 1.3e-6.
 #ifndef HK_EMU_MOD
 #define HK_EMU_MOD 4
 #endif

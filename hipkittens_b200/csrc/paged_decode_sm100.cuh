@@ -39,12 +39,12 @@ constexpr int kMaxCombineSplits = 256;
 enum : int { kStatusBadPage = 2, kStatusBadLen = 4 };  // 3 is the backward kernels' kStatusSmemAlign
 
 struct DecodeParams {
-  const __nv_bfloat16* q;        // [S,1,H,128]
-  const __nv_bfloat16* k_pages;  // [P,16,H_KV,128]
+  const __nv_bfloat16* q;        // [S,1,H,D]
+  const __nv_bfloat16* k_pages;  // [P,16,H_KV,D]
   const __nv_bfloat16* v_pages;
   const int32_t* block_table;    // [S,max_pages]
   const int32_t* ctx_lens;       // [S]
-  __nv_bfloat16* o;              // [S,1,H,128]
+  __nv_bfloat16* o;              // [S,1,H,D]
   float* lse;                    // [S,H,1,1]
   int S, H, H_KV, max_pages, num_pages;
   int chunk_pages;               // pages per CTA (kChunkPagesMin or kChunkPagesMax)
@@ -178,7 +178,6 @@ inline DecodeShape decode_pick_window_shape(int S, int H_KV, int span, const Dec
   const int useful = (span + warps - 1) / warps;  // a page per warp
   return {cluster < useful ? cluster : useful, warps};
 }
-// Workspace: partial O as fp32 [S][H][splits][128], then (m, l) pairs as fp32 [S][H][splits][2].
 // Shapes the two kernels can be launched for: the combine kernel holds one weight per split in shared memory
 // (kMaxCombineSplits of them, counted for the smaller chunk size so that either chunk choice fits), and sequences
 // and kv heads are grid dimensions y and z.
@@ -186,6 +185,7 @@ inline bool decode_shape_supported(int S, int H_KV, int max_pages) {
   return S > 0 && S <= 65535 && H_KV > 0 && H_KV <= 65535 && max_pages > 0 &&
          decode_max_splits(max_pages) <= kMaxCombineSplits;
 }
+// Workspace: partial O as fp32 [S][H][splits][D], then, from the next multiple of 256 bytes, (m, l) pairs as fp32 [S][H][splits][2].
 inline size_t decode_workspace_bytes(int S, int H, int D, int max_pages, int page_size, bool any_d = false) {
   if (S <= 0 || S > 65535 || H <= 0 || page_size != kPageTokens || max_pages <= 0) return 0;
   if (D != kDecodeD && !(any_d && D == 64)) return 0;
@@ -422,7 +422,7 @@ __global__ void __launch_bounds__(W * 32, W == 8 ? 1 : 2) paged_decode_split_ker
 
   // ---- merge the W warps through shared memory (the ring is idle now)
   __syncthreads();
-  float* sm_o = reinterpret_cast<float*>(dsmem);  // [W][8][128]
+  float* sm_o = reinterpret_cast<float*>(dsmem);  // [W][8][D]
   float* sm_m = sm_o + W * 8 * D;                // [W][8]
   float* sm_l = sm_m + W * 8;                     // [W][8]
 #pragma unroll
@@ -458,7 +458,7 @@ __global__ void __launch_bounds__(W * 32, W == 8 ? 1 : 2) paged_decode_split_ker
     if (n_used > 1) {
       // ---- merge the CTAs of the cluster: each leaves its share in its own shared memory, and CTA r reads all of
       // head r, r + n_used, ... in the order of the ranks
-      float* cl_o = sm_l + W * 8;          // [G][128]
+      float* cl_o = sm_l + W * 8;          // [G][D]
       float* cl_ml = cl_o + 8 * D;         // [G][2]
 #pragma unroll
       for (int i = 0; i < kHeads; ++i) {

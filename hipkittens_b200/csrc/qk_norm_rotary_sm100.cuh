@@ -15,11 +15,11 @@
 // lanes of 16 values, which a lane takes as two 16-byte pieces: the two halves of eight pairs, or 16 neighbours. Sums over a
 // row are shuffles. The rows of q and those of k are counted apart, and a block has rows of one of them only: so a thread
 // keeps its 16 weights in registers, and in the backward its 16 sums of dw.
-// The first form took four rows a thread at a time, scalar, each with divisions for its place and angles of its own: 300
-// instructions for 16 values, which bound it (issue slots 63 % busy, 4.5 TB/s). Now a warp has a run of rows, so that the
-// heads of one token share the angles in registers and the next row is an addition away, arithmetic is packed in pairs, and the
-// rows to come wait in a ring of cp.async stages and take no registers. us, B4 N4096 H32/8 D128: forward 73.7 -> 55.4 (336 MB,
-// 6.06 TB/s), backward 106 -> 87 (503 MB, 5.8 TB/s).
+// A warp has a run of rows, so that the heads of one token share the angles in registers and the next row is an addition away;
+// arithmetic is packed in pairs; the rows to come wait in a ring of cp.async stages and take no registers. Instructions are what
+// would bound it otherwise: with four unrelated rows a thread, each with divisions for its place and angles of its own in scalar
+// arithmetic, 16 values take 300 of them. us, B4 N4096 H32/8 D128, so / as it is: forward 73.7 / 55.4 (336 MB, 6.06 TB/s),
+// backward 106 / 87 to 89 (503 MB, 5.7 TB/s).
 #pragma once
 
 #include <cuda_bf16.h>
