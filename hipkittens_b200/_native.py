@@ -238,11 +238,14 @@ def _require_same_device(ref: torch.Tensor, **tensors) -> None:
 
 def _new(shape, dtype: torch.dtype, device: torch.device, stream) -> torch.Tensor:
     """An output, from the memory of the stream that writes it (None: torch's current one): what another stream gave back may
-    still be read by work that waits there."""
+    still be read by work that waits there. The caller's current stream is noted as a reader, so that an output that it is done with
+    is not written over before that stream is."""
     if stream is None:
         return torch.empty(shape, dtype=dtype, device=device)
     with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=device)
+        t = torch.empty(shape, dtype=dtype, device=device)
+    t.record_stream(torch.cuda.current_stream(device))
+    return t
 
 
 def _strides3(t):

@@ -59,3 +59,21 @@ def test_outputs_lie_in_memory_of_the_stream(name):
     assert all(stream_of_memory(t) == side.cuda_stream for t in got)
     assert all(torch.equal(x, y) for x, y in zip(got, want))
     assert _native.device_status(0) == 0
+
+
+@pytest.mark.parametrize("name", ["attn_fwd_window", "paged_decode", "qk_norm_rotary_bwd"])
+def test_what_the_caller_s_stream_still_reads_is_not_given_away(name):
+    call = calls()[name]
+    want = call(None)
+    here, side = torch.cuda.current_stream(), torch.cuda.Stream()
+    side.wait_stream(here)
+    got = call(side)
+    here.wait_stream(side)
+    torch.cuda._sleep(200_000_000)  # a tenth of a second
+    read = [t.clone() for t in got]
+    places, shapes = [t.data_ptr() for t in got], [(t.shape, t.dtype) for t in got]
+    del got
+    with torch.cuda.stream(side):
+        others = [torch.empty(shape, dtype=dtype, device="cuda").zero_() for shape, dtype in shapes]
+    assert not here.query() and not set(places) & {t.data_ptr() for t in others}
+    assert all(torch.equal(x, y) for x, y in zip(read, want))
