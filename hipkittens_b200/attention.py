@@ -140,7 +140,7 @@ def _attend(q, packed, causal, softmax_scale, key_padding_mask, window=None, sin
     if key_padding_mask is None:
         out = _apply(q, packed, causal, softmax_scale, None, window, sinks)
     else:
-        if in_place and key_padding_mask.shape[0] != packed.shape[0]:
+        if in_place and key_padding_mask.shape[:1] != packed.shape[:1]:
             raise ValueError(_MASK_SHAPE)
         kv_lens, bad = _lens_from_key_padding_mask(key_padding_mask, packed)
         try:
