@@ -20,9 +20,11 @@ Run as ``python -m hipkittens_b200._build``. nvcc cross-compiles without a GPU.
 from __future__ import annotations
 
 import os
+import re
 import subprocess
 import sys
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
@@ -33,7 +35,7 @@ INCLUDE = os.path.join(os.path.dirname(PKG), "include")
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-std=c++17", "-lineinfo",
-    "-Xcompiler", "-fPIC", "-shared",
+    "-Xcompiler", "-fPIC",
 ]
 
 # (directory under the package, module name, entry name, default causal, sync after launch)
@@ -73,13 +75,39 @@ def nvcc_path() -> str:
     return cand if os.path.exists(cand) else "nvcc"
 
 
+# the library's translation units, compiled side by side
+LIB_UNITS = ["hk_attn_api.cu"]
+OBJ_DIR = os.path.join(PKG, "build")
+
+
+def _includes(path: str, seen=None):
+    """A source file and what it includes by a quoted name, all the way down."""
+    seen = set() if seen is None else seen
+    path = os.path.normpath(path)
+    if path not in seen and os.path.exists(path):
+        seen.add(path)
+        with open(path) as f:
+            for name in re.findall(r'^#include "([^"]+)"', f.read(), re.M):
+                _includes(os.path.join(os.path.dirname(path), name), seen)
+    return seen
+
+
+def _build_unit(unit: str, force: bool) -> str:
+    src, obj = os.path.join(CSRC, unit), os.path.join(OBJ_DIR, unit.replace(".cu", ".o"))
+    if force or not _newer(obj, _includes(src)):
+        _run([nvcc_path(), *NVCC_FLAGS, "-c", "-o", obj, src])
+    return obj
+
+
 def build_lib(force: bool = False) -> str:
-    srcs = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cu", ".cuh"))]
-    srcs.append(os.path.join(INCLUDE, "hk_attn.h"))
-    if not force and _newer(LIB_PATH, srcs):
+    sources = set().union(*(_includes(os.path.join(CSRC, unit)) for unit in LIB_UNITS))
+    if not force and _newer(LIB_PATH, sources):
         return LIB_PATH
     os.makedirs(LIB_DIR, exist_ok=True)
-    _run([nvcc_path(), *NVCC_FLAGS, "-o", LIB_PATH, os.path.join(CSRC, "hk_attn_api.cu")])
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    with ThreadPoolExecutor(len(LIB_UNITS)) as pool:
+        objects = list(pool.map(lambda unit: _build_unit(unit, force), LIB_UNITS))
+    _run([nvcc_path(), *NVCC_FLAGS, "-shared", "-o", LIB_PATH, *objects])
     return LIB_PATH
 
 

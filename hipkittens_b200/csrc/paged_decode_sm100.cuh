@@ -36,7 +36,8 @@ struct DecodeRing {
 constexpr int decode_smem_bytes(int warps) { return warps * DecodeRing<128>::kStages * DecodeRing<128>::kStageBytes; }  // 96 or 192 KB
 constexpr int kMaxCombineSplits = 256;
 
-enum : int { kStatusBadPage = 2, kStatusBadLen = 4 };  // 3 is the backward kernels' kStatusSmemAlign
+// 3 is the backward kernels' kStatusSmemAlign; kStatusBadPos: a position outside rotary tables
+enum : int { kStatusBadPage = 2, kStatusBadLen = 4, kStatusBadPos = 5 };
 
 struct DecodeParams {
   const __nv_bfloat16* q;        // [S,1,H,D]

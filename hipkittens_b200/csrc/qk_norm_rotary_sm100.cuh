@@ -27,11 +27,11 @@
 #include <stdint.h>
 
 #include "attn_fwd_sm100.cuh"
+#include "paged_decode_sm100.cuh"
 #include "sm100_ptx.cuh"
 
 namespace hk {
 
-enum : int { kStatusBadPos = 5 };  // a position outside the tables
 
 constexpr int kQknThreads = 128;
 constexpr int kQknStages = 3;
