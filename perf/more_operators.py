@@ -217,7 +217,6 @@ def run(state):
 
 def _run_own(s):
     import hipkittens_b200 as hk
-    from hipkittens_b200.attention import HipRaggedAttention
 
     c = s["case"]
     if c["kind"] in ("append", "read", "decode"):
@@ -232,6 +231,8 @@ def _run_own(s):
     if c["kind"] == "prompts":
         return hk.attn_fwd_ragged(s["q"], s["k"], s["v"], s["cu_q"], s["cu_k"], causal=c["causal"])
     if "module" not in s:  # which a program makes once
+        from hipkittens_b200.attention import HipRaggedAttention
+
         s["module"] = HipRaggedAttention(causal=c["causal"])
     o = s["module"](s["q"], s["kv"], s["cu_q"], s["cu_k"])
     return (o.detach(), *torch.autograd.grad(o, (s["q"], s["kv"]), s["d_o"]))
