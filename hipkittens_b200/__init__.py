@@ -9,6 +9,8 @@ Public surface
 * ``attn_fwd(q, k, v, causal=False, ...) -> (O, L)``, ``attn_bwd_prep`` / ``attn_bwd`` / ``dq_shuffle`` (the
   backward pass), ``paged_decode(...) -> (O, L)`` and ``paged_kv_append(...)``: torch-tensor front ends over
   the C ABI (ctypes).
+* ``paged_kv_append_fp8(...)``, ``paged_kv_read_fp8(...)`` and ``paged_decode_fp8(...)``: the paged cache in 8 bits, with a scale for
+  each page and head.
 * ``qk_norm_rotary(...)`` and ``qk_norm_rotary_bwd(...)``: RMS norm of every head of q and k with the rotation of its position.
 * ``load_tk_kernel(causal)`` / ``load_tk_kernel_fwd(causal)`` / ``load_tk_kernel_bkwd(causal)`` /
   ``load_tk_kernel_bkwd_prep(causal)``: the reference's extension modules (``tk_kernel.dispatch_micro``,
@@ -34,10 +36,14 @@ from ._native import (  # noqa: F401
     load_tk_kernel_fwd,
     load_tk_kernel_rotary,
     paged_decode,
+    paged_decode_fp8,
+    paged_decode_fp8_workspace_bytes,
     paged_decode_workspace_bytes,
     attn_fwd_paged,
     paged_kv_append,
+    paged_kv_append_fp8,
     paged_kv_append_rotary,
+    paged_kv_read_fp8,
     qk_norm_rotary,
     qk_norm_rotary_bwd,
     rotary,
@@ -61,9 +67,13 @@ __all__ = [
     "load_tk_kernel_fwd",
     "load_tk_kernel_rotary",
     "paged_decode",
+    "paged_decode_fp8",
+    "paged_decode_fp8_workspace_bytes",
     "attn_fwd_paged",
     "paged_kv_append",
+    "paged_kv_append_fp8",
     "paged_kv_append_rotary",
+    "paged_kv_read_fp8",
     "paged_decode_workspace_bytes",
     "qk_norm_rotary",
     "qk_norm_rotary_bwd",

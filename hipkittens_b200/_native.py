@@ -49,6 +49,10 @@ EXPORTED_SYMBOLS = (
     "hk_attn_paged_decode_window",
     "hk_attn_paged_decode_static",
     "hk_paged_kv_append",
+    "hk_paged_kv_append_fp8",
+    "hk_paged_kv_read_fp8",
+    "hk_attn_paged_decode_fp8_workspace_bytes",
+    "hk_attn_paged_decode_fp8",
     "hk_last_device_status",
     "hk_selftest_bounded_wait",
     "hk_selftest_fastdiv",
@@ -151,6 +155,14 @@ def capi() -> ctypes.CDLL:
     lib.hk_attn_paged_decode_static.restype = ci
     lib.hk_paged_kv_append.argtypes = [vp, vp, vp, vp, vp, vp, ci, ci, ci, ci, ci, ci, ci, ci, vp]
     lib.hk_paged_kv_append.restype = ci
+    lib.hk_paged_kv_append_fp8.argtypes = [vp] * 11 + [ci] * 4 + [ll3] * 2 + [ci] * 7 + [vp]
+    lib.hk_paged_kv_append_fp8.restype = ci
+    lib.hk_paged_kv_read_fp8.argtypes = [vp] * 9 + [ci] * 9 + [vp]
+    lib.hk_paged_kv_read_fp8.restype = ci
+    lib.hk_attn_paged_decode_fp8_workspace_bytes.argtypes = [ci] * 7
+    lib.hk_attn_paged_decode_fp8_workspace_bytes.restype = ctypes.c_size_t
+    lib.hk_attn_paged_decode_fp8.argtypes = [vp] * 9 + [ci] * 9 + [cf, vp, ctypes.c_size_t, ci, vp]
+    lib.hk_attn_paged_decode_fp8.restype = ci
     lib.hk_last_device_status.argtypes = [ci]
     lib.hk_last_device_status.restype = ci
     lib.hk_selftest_bounded_wait.argtypes = [ci, ctypes.c_uint]
@@ -963,6 +975,224 @@ def paged_kv_append_rotary(
                                           s_n, t_n, hkv, d, 2 * cos.shape[1], cos.shape[0], page, block_table.shape[1],
                                           p_n, k_new.device.index, st.cuda_stream)
     _check(rc, "hk_paged_kv_append_rotary")
+
+
+HK_FP8_TABLE_F32 = 1
+
+
+def _check_fp8_cache(k_pages, v_pages, k_scales, v_scales, block_table) -> Tuple[int, int, int, int]:
+    """The tensors of an 8-bit paged cache; returns S, the pages of the pool, H_KV and D."""
+    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+        _require_cuda_bf16(name, t, 4)
+        if t.dtype != torch.float8_e4m3fn:
+            raise RuntimeError(f"{name} must be torch.float8_e4m3fn")
+    if v_pages.shape != k_pages.shape:
+        raise RuntimeError("k_pages and v_pages must be [P,page,H_KV,D]")
+    p_n, _, hkv, d = k_pages.shape
+    for name, t in (("k_scales", k_scales), ("v_scales", v_scales)):
+        _require_cuda_bf16(name, t, 2)
+        if t.dtype != torch.float32 or t.shape != (p_n, hkv):
+            raise RuntimeError(f"{name} must be an fp32 tensor [P, H_KV], a scale for each page and head")
+    _require_cuda_bf16("block_table", block_table, 2)
+    if block_table.dtype != torch.int32:
+        raise RuntimeError("block_table must be torch.int32")
+    _require_same_device(k_pages, v_pages=v_pages, k_scales=k_scales, v_scales=v_scales, block_table=block_table)
+    return block_table.shape[0], p_n, hkv, d
+
+
+def _check_int32(name: str, t, n: int, ref: torch.Tensor) -> None:
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous():
+        raise RuntimeError(f"{name} must be a contiguous int32 tensor [{n}]")
+    _require_same_device(ref, **{name: t})
+
+
+def paged_kv_append_fp8(
+    k_new: torch.Tensor,
+    v_new: torch.Tensor,
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    k_scales: torch.Tensor,
+    v_scales: torch.Tensor,
+    block_table: torch.Tensor,
+    start_pos: torch.Tensor,
+    cos: Optional[torch.Tensor] = None,
+    sin: Optional[torch.Tensor] = None,
+    cu_seqlens: Optional[torch.Tensor] = None,
+    stream: Optional[torch.cuda.Stream] = None,
+) -> None:
+    """`paged_kv_append` into a cache of 8 bits: pages [P,16,H_KV,D] torch.float8_e4m3fn and an fp32 scale for each page and head
+    [P,H_KV], for K and for V; a token's value is code * scale.
+
+    k_new, v_new [S,T,H_KV,D] bf16, token t of sequence s at position start_pos[s] + t; or, with `cu_seqlens` (int32 [S+1]), rows
+    cu_seqlens[s] .. cu_seqlens[s+1]-1 of [T,H_KV,D] (sequences of different lengths without padding). Contiguous, or views with a
+    contiguous last dimension and other strides that are multiples of 8. With cos, sin [rows, R/2] (bf16 or fp32, both) K is rotated
+    on the way, the pairs (i, i + R/2) of a token at position p by row p. fp32 throughout, rounded once.
+
+    A block (a page's tokens of one head) has the smallest power of two as its scale that brings its largest value to 448 at most. A block
+    whose first row is written starts anew; otherwise its scale never shrinks, and where it grows the other rows are rounded anew. A NaN
+    makes its whole block NaN, an infinity becomes the block's largest value. A page that several sequences share takes no new tokens."""
+    if stream is None:
+        r = _front().paged_kv_append_fp8(k_new, v_new, k_pages, v_pages, k_scales, v_scales, block_table, start_pos, cos, sin,
+                                         cu_seqlens)
+        if r is not None:
+            return _done(r, "hk_paged_kv_append_fp8")
+    s_n, p_n, hkv, d = _check_fp8_cache(k_pages, v_pages, k_scales, v_scales, block_table)
+    ndim = 4 if cu_seqlens is None else 3
+    for name, t in (("k_new", k_new), ("v_new", v_new)):
+        if not isinstance(t, torch.Tensor) or t.device.type != "cuda" or t.dim() != ndim:
+            raise RuntimeError(f"{name} must be a {ndim}-D CUDA tensor")
+        if t.dtype != torch.bfloat16:
+            raise RuntimeError(f"{name} must be torch.bfloat16")
+        if t.shape[-2:] != (hkv, d) or (ndim == 4 and t.shape[0] != s_n):
+            raise RuntimeError("k_new/v_new must be [S,T,H_KV,D], or [T,H_KV,D] with cu_seqlens")
+        if t.numel() and (t.stride(-1) != 1 or any(st <= 0 or st % 8 for st, n in zip(t.stride()[:-1], t.shape) if n > 1)):
+            raise RuntimeError(f"{name}: the last dimension must be contiguous and the other strides positive multiples of 8 elements")
+    if k_new.shape != v_new.shape:
+        raise RuntimeError("k_new and v_new must have the same shape")
+    _check_int32("start_pos", start_pos, s_n, k_pages)
+    if cu_seqlens is not None:
+        _check_int32("cu_seqlens", cu_seqlens, s_n + 1, k_pages)
+    if (cos is None) != (sin is None):
+        raise RuntimeError("cos and sin belong together")
+    for name, t in (("cos", cos), ("sin", sin)):
+        if t is not None and (not isinstance(t, torch.Tensor) or t.dim() != 2 or not t.is_contiguous()
+                              or t.dtype not in (torch.bfloat16, torch.float32)):
+            raise RuntimeError(f"{name} must be a contiguous bf16 or fp32 tensor [rows, R/2]")
+    if cos is not None and (cos.shape != sin.shape or cos.dtype != sin.dtype):
+        raise RuntimeError("cos and sin must have the same shape and type")
+    _require_same_device(k_pages, k_new=k_new, v_new=v_new, cos=cos, sin=sin)
+    if k_new.numel() == 0:
+        return
+    st = stream if stream is not None else torch.cuda.current_stream(k_pages.device)
+
+    def strides(t):
+        three = t if t.dim() == 4 else t[None]
+        return (ctypes.c_longlong * 3)(*(v if n > 1 else d for v, n in zip(three.stride()[:3], three.shape[:3])))
+
+    _check(capi().hk_paged_kv_append_fp8(
+        k_new.data_ptr(), v_new.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
+        block_table.data_ptr(), start_pos.data_ptr(), _ptr(cu_seqlens), _ptr(sin), _ptr(cos), s_n, k_new.shape[ndim - 3], hkv, d,
+        strides(k_new), strides(v_new), 0 if cos is None else 2 * cos.shape[1], 0 if cos is None else cos.shape[0],
+        HK_FP8_TABLE_F32 if cos is not None and cos.dtype == torch.float32 else 0, k_pages.shape[1], block_table.shape[1], p_n,
+        k_pages.device.index, st.cuda_stream), "hk_paged_kv_append_fp8")
+
+
+def paged_kv_read_fp8(
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    k_scales: torch.Tensor,
+    v_scales: torch.Tensor,
+    block_table: torch.Tensor,
+    rows: int,
+    ctx_lens: Optional[torch.Tensor] = None,
+    cu_seqlens: Optional[torch.Tensor] = None,
+    k_out: Optional[torch.Tensor] = None,
+    v_out: Optional[torch.Tensor] = None,
+    stream: Optional[torch.cuda.Stream] = None,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Tokens of an 8-bit paged cache (`paged_kv_append_fp8`) as bf16 K and V, for the attention of a chunk of a prompt.
+
+    With `ctx_lens` (int32 [S]): [S,rows,H_KV,D], the first ctx_lens[s] tokens of each sequence and zeros behind them, as ``attn_fwd(...,
+    kv_lens=ctx_lens)`` takes them. With `cu_seqlens` (int32 [S+1]): [rows,H_KV,D], the first cu_seqlens[s+1] - cu_seqlens[s] tokens
+    of sequence s from row cu_seqlens[s] on, as ``attn_fwd_ragged`` takes them; rows behind the last sequence are zeros in new outputs,
+    and left as they are in `k_out` and `v_out`."""
+    if stream is None:
+        r = _front().paged_kv_read_fp8(k_pages, v_pages, k_scales, v_scales, block_table, rows, ctx_lens, cu_seqlens, k_out, v_out)
+        if r is not None:
+            return _done(r, "hk_paged_kv_read_fp8")
+    s_n, p_n, hkv, d = _check_fp8_cache(k_pages, v_pages, k_scales, v_scales, block_table)
+    if isinstance(rows, bool) or not isinstance(rows, int) or not 0 <= rows < 2 ** 31:
+        raise RuntimeError("rows must be an int, the rows of the outputs (per sequence, with ctx_lens)")
+    if (ctx_lens is None) == (cu_seqlens is None):
+        raise RuntimeError("either ctx_lens or cu_seqlens says which tokens are read")
+    if ctx_lens is not None:
+        _check_int32("ctx_lens", ctx_lens, s_n, k_pages)
+    else:
+        _check_int32("cu_seqlens", cu_seqlens, s_n + 1, k_pages)
+    if (k_out is None) != (v_out is None):
+        raise RuntimeError("k_out and v_out belong together")
+    zero_tail = k_out is None
+    shape = (s_n, rows, hkv, d) if cu_seqlens is None else (rows, hkv, d)
+    outs = []
+    for name, t in (("k_out", k_out), ("v_out", v_out)):
+        t = _new(shape, torch.bfloat16, k_pages.device, stream) if t is None else t
+        if not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype != torch.bfloat16 or not t.is_contiguous():
+            raise RuntimeError(f"{name} must be a contiguous bf16 tensor of shape {shape}")
+        _require_same_device(k_pages, **{name: t})
+        outs.append(t)
+    if outs[0].numel():
+        st = stream if stream is not None else torch.cuda.current_stream(k_pages.device)
+        _check(capi().hk_paged_kv_read_fp8(
+            k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), block_table.data_ptr(), _ptr(ctx_lens),
+            _ptr(cu_seqlens), outs[0].data_ptr(), outs[1].data_ptr(), s_n, rows, hkv, d, int(zero_tail), k_pages.shape[1],
+            block_table.shape[1], p_n, k_pages.device.index, st.cuda_stream), "hk_paged_kv_read_fp8")
+    return outs[0], outs[1]
+
+
+def paged_decode_fp8_workspace_bytes(s: int, h: int, d: int, max_pages: int, page_size: int = 16, window: Optional[int] = None,
+                                     sinks: int = 0) -> int:
+    _check_window(window, sinks)
+    return int(capi().hk_attn_paged_decode_fp8_workspace_bytes(s, h, d, max_pages, page_size, window or 0, sinks))
+
+
+def paged_decode_fp8(
+    q: torch.Tensor,
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    k_scales: torch.Tensor,
+    v_scales: torch.Tensor,
+    block_table: torch.Tensor,
+    ctx_lens: torch.Tensor,
+    softmax_scale: Optional[float] = None,
+    out: Optional[torch.Tensor] = None,
+    lse: Optional[torch.Tensor] = None,
+    workspace: Optional[torch.Tensor] = None,
+    stream: Optional[torch.cuda.Stream] = None,
+    window: Optional[int] = None,
+    sinks: int = 0,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """`paged_decode` against an 8-bit cache (`paged_kv_append_fp8`): q [S,1,H,D] bf16, D = 64 or 128 and up to 8 heads to a K/V head,
+    pages [P,16,H_KV,D] torch.float8_e4m3fn, scales [P,H_KV] fp32 -> O [S,1,H,D] bf16, L [S,H,1,1] fp32. `window` and `sinks` as there.
+    `workspace` is a uint8 CUDA tensor of at least ``paged_decode_fp8_workspace_bytes(...)`` bytes (allocated here when omitted)."""
+    _check_window(window, sinks)
+    if stream is None:
+        r = _front().paged_decode_fp8(q, k_pages, v_pages, k_scales, v_scales, block_table, ctx_lens, softmax_scale, out, lse, workspace,
+                                      window or 0, sinks)
+        if r is not None:
+            return _done(r, "hk_attn_paged_decode_fp8")
+    s_n, p_n, hkv, d = _check_fp8_cache(k_pages, v_pages, k_scales, v_scales, block_table)
+    _require_cuda_bf16("q", q, 4)
+    if q.dtype != torch.bfloat16:
+        raise RuntimeError("q must be torch.bfloat16")
+    if q.shape[0] != s_n or q.shape[1] != 1 or q.shape[3] != d:
+        raise RuntimeError("q must be [S,1,H,D] and k_pages/v_pages [P,page,H_KV,D]")
+    h, max_pages = q.shape[2], block_table.shape[1]
+    _check_int32("ctx_lens", ctx_lens, s_n, k_pages)
+    if out is None:
+        out = _new(q.shape, q.dtype, q.device, stream)
+    if lse is None:
+        lse = _new((s_n, h, 1, 1), torch.float32, q.device, stream)
+    if not isinstance(out, torch.Tensor) or out.shape != q.shape or out.dtype != torch.bfloat16 or not out.is_contiguous():
+        raise RuntimeError("out must be a contiguous bf16 tensor of q's shape")
+    if not isinstance(lse, torch.Tensor) or lse.shape != (s_n, h, 1, 1) or lse.dtype != torch.float32 or not lse.is_contiguous():
+        raise RuntimeError("lse must be a contiguous fp32 tensor [S, H, 1, 1]")
+    need = paged_decode_fp8_workspace_bytes(s_n, h, d, max_pages, k_pages.shape[1], window, sinks)
+    if need == 0:
+        raise HkError(HK_EUNSUPPORTED, "hk_attn_paged_decode_fp8",
+                      "shape outside the decode kernels' limits (D = 64 or 128, 16-token pages, 1 <= S <= 65535, max_pages, or pages of "
+                      "a window and its sinks, <= 8192)")
+    if workspace is None:
+        workspace = _new(max(need, 256), torch.uint8, q.device, stream)  # it goes back to the stream that uses it
+    if not isinstance(workspace, torch.Tensor) or not workspace.is_contiguous():
+        raise RuntimeError("workspace must be a contiguous tensor")
+    _require_same_device(k_pages, q=q, out=out, lse=lse, workspace=workspace)
+    st = stream if stream is not None else torch.cuda.current_stream(q.device)
+    _check(capi().hk_attn_paged_decode_fp8(
+        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), block_table.data_ptr(),
+        ctx_lens.data_ptr(), out.data_ptr(), lse.data_ptr(), s_n, h, hkv, d, k_pages.shape[1], max_pages, p_n, window or 0, sinks,
+        float(softmax_scale or 0.0), workspace.data_ptr(), workspace.numel() * workspace.element_size(), q.device.index,
+        st.cuda_stream), "hk_attn_paged_decode_fp8")
+    return out, lse
 
 
 def device_status(device: int = 0) -> int:

@@ -12,7 +12,7 @@
 #include "attn_bwd_sm100.cuh"
 #include "attn_fwd_sm100.cuh"
 #include "dependent_launch.cuh"
-#include "paged_decode_sm100.cuh"
+#include "paged_decode_common.cuh"
 
 #pragma GCC visibility push(hidden)
 namespace hk_host {
@@ -56,6 +56,8 @@ struct DeviceState {
   int sm_count = 0;
   int cc_major = 0;
   hk::DecodeLimits decode;
+  bool decode_fp8_ready = false;  // the decode over 8-bit pages, set up by its first call
+  hk::DecodeLimits decode_fp8;
   int bwd_clusters[hk::kMaxDkdvSplit + 1] = {};  // clusters of so many dK/dV CTAs that the device holds at once
   int* status = nullptr;       // the status word, device address (kernels write it only when something went wrong)
   int* status_host = nullptr;  // ... and host address: mapped memory, so that reading it needs no copy

@@ -1,0 +1,188 @@
+// Host side of libhk_attn's 8-bit paged cache: append, read back and decode. C ABI in include/hk_attn.h.
+#include <algorithm>
+#include <cmath>
+
+#include "hk_host.cuh"
+#include "paged_decode_fp8_sm100.cuh"
+#include "paged_kv_fp8_sm100.cuh"
+
+using namespace hk_host;
+
+namespace {
+
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
+
+// Everything that the three entries have in common. `st` is entered only if all of it is right.
+int fp8_cache(hk::Fp8Cache& c, const void* k_pages, const void* v_pages, const float* k_scales, const float* v_scales,
+              const int32_t* block_table, int S, int H_KV, int D, int page_size, int max_pages, int num_pages) {
+  if (!k_pages || !v_pages || !k_scales || !v_scales || !block_table) return HK_EINVAL;
+  if (S <= 0 || H_KV <= 0 || D <= 0 || max_pages <= 0 || num_pages <= 0) return HK_EINVAL;
+  if (page_size != hk::kPageTokens || (D != 64 && D != 128)) return HK_EUNSUPPORTED;
+  if (S > 65535 || H_KV > 65535 || max_pages > 0x7fffffff / hk::kPageTokens) return HK_EINVAL;
+  if (!aligned16(k_pages) || !aligned16(v_pages) || !aligned4(k_scales) || !aligned4(v_scales) || !aligned4(block_table)) return HK_EINVAL;
+  c.k_pages = static_cast<uint8_t*>(const_cast<void*>(k_pages));
+  c.v_pages = static_cast<uint8_t*>(const_cast<void*>(v_pages));
+  c.k_scales = const_cast<float*>(k_scales);
+  c.v_scales = const_cast<float*>(v_scales);
+  c.block_table = block_table;
+  c.S = S, c.H_KV = H_KV, c.max_pages = max_pages, c.num_pages = num_pages;
+  return HK_OK;
+}
+
+// The units of 16 tokens of a call and with them its warps, `per_unit` each; false if there are too many for an int.
+bool fp8_warps(long long units, int per_unit, int* warps) {
+  const long long n = units * per_unit;
+  *warps = static_cast<int>(n);
+  return n <= 0x7ffffff0ll;
+}
+
+template <typename Params>
+int launch_blocks(void (*fn)(Params), const Params& p, void* cuda_stream) {
+  HK_CUDA(hk::launch_dependent(true, fn, unsigned((p.warps + 7ll) / 8), 256, 0, static_cast<cudaStream_t>(cuda_stream), p));
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  return HK_OK;
+}
+
+int decode_fp8_span(int max_pages, int window, int sinks) {
+  if (window < 0 || sinks < 0 || max_pages <= 0 || max_pages > 0x7fffffff / hk::kPageTokens) return 0;
+  return window == 0 ? max_pages : hk::decode_span_pages(max_pages, window, sinks);
+}
+
+}  // namespace
+
+extern "C" {
+
+int hk_paged_kv_append_fp8(const void* k_new, const void* v_new, void* k_pages, void* v_pages, float* k_scales, float* v_scales,
+                           const int32_t* block_table, const int32_t* start_pos, const int32_t* cu_seqlens, const void* sin,
+                           const void* cos, int S, int T, int H_KV, int D, const long long* k_strides, const long long* v_strides,
+                           int rotary_dim, int table_rows, int flags, int page_size, int max_pages_per_seq, int num_pages,
+                           int device, void* cuda_stream) {
+  hk::AppendFp8Params p = {};
+  int rc = fp8_cache(p.c, k_pages, v_pages, k_scales, v_scales, block_table, S, H_KV, D, page_size, max_pages_per_seq, num_pages);
+  if (rc != HK_OK) return rc;
+  if (!k_new || !v_new || !start_pos || !k_strides || !v_strides || T <= 0 || (!sin) != (!cos)) return HK_EINVAL;
+  if (flags & ~HK_FP8_TABLE_F32) return HK_EINVAL;
+  if (!aligned16(k_new) || !aligned16(v_new) || !aligned4(start_pos) || !aligned4(cu_seqlens) || !aligned16(sin) || !aligned16(cos))
+    return HK_EINVAL;
+  for (int i = cu_seqlens ? 1 : 0; i < 3; ++i)
+    for (const long long* st : {k_strides, v_strides})
+      if (st[i] <= 0 || st[i] % 8 != 0 || st[i] >= (1ll << 39)) return HK_EINVAL;
+  if (sin) {
+    if (rotary_dim <= 0) rotary_dim = D;
+    if (rotary_dim % 16 != 0 || rotary_dim > D) return HK_EUNSUPPORTED;
+    if (table_rows <= 0) return HK_EINVAL;
+  }
+  const long long units = cu_seqlens ? T / hk::kPageTokens + 2ll * S : S * ((T + 30ll) / hk::kPageTokens);
+  if (!fp8_warps(units, 2 * H_KV, &p.warps)) return HK_EINVAL;
+  DeviceState* st = nullptr;
+  DeviceScope scope;
+  if ((rc = scope.enter(device, &st)) != HK_OK) return rc;
+  p.c.status = st->status;
+  p.rows.cu = cu_seqlens;
+  p.rows.T = T;
+  p.rows.fd_units = hk::FastDiv(static_cast<int>((T + 30ll) / hk::kPageTokens));
+  p.k_new = static_cast<const __nv_bfloat16*>(k_new);
+  p.v_new = static_cast<const __nv_bfloat16*>(v_new);
+  for (int i = 0; i < 3; ++i) p.k_stride[i] = k_strides[i], p.v_stride[i] = v_strides[i];
+  if (cu_seqlens) p.k_stride[0] = p.v_stride[0] = 0;
+  p.start_pos = start_pos;
+  p.cos = cos, p.sin = sin;
+  p.R = rotary_dim, p.table_rows = table_rows;
+  p.fd_heads2 = hk::FastDiv(2 * H_KV);
+  p.fd_heads = hk::FastDiv(H_KV);
+  const int rot = !sin ? hk::kFp8Plain : flags & HK_FP8_TABLE_F32 ? hk::kFp8TableF32 : hk::kFp8TableBf16;
+  auto pick = [&](auto d) {
+    constexpr int kD = decltype(d)::value;
+    return rot == hk::kFp8Plain       ? hk::paged_kv_append_fp8_kernel<kD, hk::kFp8Plain>
+           : rot == hk::kFp8TableBf16 ? hk::paged_kv_append_fp8_kernel<kD, hk::kFp8TableBf16>
+                                      : hk::paged_kv_append_fp8_kernel<kD, hk::kFp8TableF32>;
+  };
+  return launch_blocks(D == 128 ? pick(std::integral_constant<int, 128>{}) : pick(std::integral_constant<int, 64>{}), p, cuda_stream);
+}
+
+int hk_paged_kv_read_fp8(const void* k_pages, const void* v_pages, const float* k_scales, const float* v_scales,
+                         const int32_t* block_table, const int32_t* ctx_lens, const int32_t* cu_seqlens, void* k_out, void* v_out,
+                         int S, int rows, int H_KV, int D, int zero_tail, int page_size, int max_pages_per_seq, int num_pages,
+                         int device, void* cuda_stream) {
+  hk::ReadFp8Params p = {};
+  int rc = fp8_cache(p.c, k_pages, v_pages, k_scales, v_scales, block_table, S, H_KV, D, page_size, max_pages_per_seq, num_pages);
+  if (rc != HK_OK) return rc;
+  if (!k_out || !v_out || (!ctx_lens) == (!cu_seqlens) || rows <= 0) return HK_EINVAL;
+  if (!aligned16(k_out) || !aligned16(v_out) || !aligned4(ctx_lens) || !aligned4(cu_seqlens)) return HK_EINVAL;
+  const long long per_seq = (rows + 15ll) / hk::kPageTokens;
+  if (!fp8_warps(cu_seqlens ? rows / hk::kPageTokens + S + 1ll : S * per_seq, H_KV, &p.warps)) return HK_EINVAL;
+  DeviceState* st = nullptr;
+  DeviceScope scope;
+  if ((rc = scope.enter(device, &st)) != HK_OK) return rc;
+  p.c.status = st->status;
+  p.rows.cu = cu_seqlens;
+  p.rows.T = rows;
+  p.rows.fd_units = hk::FastDiv(static_cast<int>(per_seq));
+  p.ctx_lens = ctx_lens;
+  p.k_out = static_cast<__nv_bfloat16*>(k_out);
+  p.v_out = static_cast<__nv_bfloat16*>(v_out);
+  p.zero_tail = zero_tail;
+  p.fd_heads = hk::FastDiv(H_KV);
+  return launch_blocks(D == 128 ? hk::paged_kv_read_fp8_kernel<128> : hk::paged_kv_read_fp8_kernel<64>, p, cuda_stream);
+}
+
+size_t hk_attn_paged_decode_fp8_workspace_bytes(int S, int H, int D, int max_pages_per_seq, int page_size, int window, int sinks) {
+  return hk::decode_workspace_bytes(S, H, D, decode_fp8_span(max_pages_per_seq, window, sinks), page_size, true);
+}
+
+int hk_attn_paged_decode_fp8(const void* q, const void* k_pages, const void* v_pages, const float* k_scales, const float* v_scales,
+                             const int32_t* block_table, const int32_t* ctx_lens, void* o, float* lse, int S, int H, int H_KV, int D,
+                             int page_size, int max_pages_per_seq, int num_pages, int window, int sinks, float softmax_scale,
+                             void* workspace, size_t workspace_bytes, int device, void* cuda_stream) {
+  hk::Fp8Cache c = {};
+  int rc = fp8_cache(c, k_pages, v_pages, k_scales, v_scales, block_table, S, H_KV, D, page_size, max_pages_per_seq, num_pages);
+  if (rc != HK_OK) return rc;
+  if (!q || !ctx_lens || !o || !lse || H <= 0 || window < 0 || sinks < 0 || (window == 0 && sinks != 0)) return HK_EINVAL;
+  if (H % H_KV != 0) return HK_EINVAL;
+  if (H / H_KV > 8) return HK_EUNSUPPORTED;  // the heads of a group sit in the 8 columns of one product
+  if (!aligned16(q) || !aligned16(o) || !aligned4(ctx_lens) || !aligned4(lse)) return HK_EINVAL;
+  const int span = decode_fp8_span(max_pages_per_seq, window, sinks);
+  if (!hk::decode_shape_supported(S, H_KV, span)) {
+    snprintf(g_cuda_err, sizeof(g_cuda_err), "paged decode supports up to %d pages of a context (got %d)",
+             hk::kMaxCombineSplits * hk::kChunkPagesMin, span);
+    return HK_EUNSUPPORTED;
+  }
+  const size_t need = hk::decode_workspace_bytes(S, H, D, span, page_size, true);
+  if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255)) return HK_EWORKSPACE;
+  DeviceState* st = nullptr;
+  DeviceScope scope;
+  if ((rc = scope.enter(device, &st)) != HK_OK) return rc;
+  {
+    std::lock_guard<std::mutex> lock(st->mu);
+    if (!st->decode_fp8_ready) {
+      rc = hk::prepare_decode_fp8_kernels(g_cuda_err, sizeof(g_cuda_err), st->sm_count, &st->decode_fp8);
+      if (rc != HK_OK) return rc;
+      st->decode_fp8_ready = true;
+    }
+  }
+  hk::DecodeFp8Params p = {};
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.k_codes = c.k_pages, p.v_codes = c.v_pages;
+  p.k_scales = c.k_scales, p.v_scales = c.v_scales;
+  p.block_table = block_table;
+  p.ctx_lens = ctx_lens;
+  p.o = static_cast<__nv_bfloat16*>(o);
+  p.lse = lse;
+  p.S = S, p.H = H, p.H_KV = H_KV;
+  p.max_pages = max_pages_per_seq, p.num_pages = num_pages;
+  p.scale = softmax_scale > 0.f ? softmax_scale : 1.0f / std::sqrt(float(D));
+  p.scale_log2 = p.scale * 1.4426950408889634f;
+  p.workspace = workspace;
+  p.status = st->status;
+  const int capacity = max_pages_per_seq * hk::kPageTokens;  // no context is longer
+  p.window = window == 0 ? capacity : std::min(window, capacity);
+  p.sinks = std::min(sinks, capacity);
+  p.span_pages = span;
+  int launched = 0;
+  const cudaError_t e = hk::launch_paged_decode_fp8(p, D, st->decode_fp8, static_cast<cudaStream_t>(cuda_stream), &launched);
+  g_launches.fetch_add(launched, std::memory_order_relaxed);
+  if (e != cudaSuccess) return cuda_fail(e, "fp8 decode launch");
+  return HK_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,376 @@
+// The paged KV cache in 8 bits: appending new K/V tokens to it, and reading tokens back as bf16.
+//
+// A page holds 16 tokens of every K/V head as e4m3 codes; the 16 x D codes of one page and head are a block, with one fp32 scale for
+// K and one for V: value = code * scale. An append picks the smallest power of two that brings the block's largest magnitude to 448
+// (the largest e4m3 value) at most:
+//     amax = m * 2^e, 1 <= m < 2:  scale = 2^(e - 8) if m <= 1.75, else 2^(e - 7)        (448 = 1.75 * 2^8)
+// A code has an exponent of its own, so a power of two costs no relative precision against amax / 448, and where a later token needs a
+// larger scale the block's other tokens move by a power of two: their codes change exactly, but for those that become subnormal
+// (below 2^-14 of the block's largest value). With scales that are not powers of two every growth would round them once more.
+// The arithmetic is fp32 with one rounding, to e4m3; the rotation of K is part of it, so that a rotated token is rounded once and not
+// twice. Its products and sums are rounded one by one (no fused multiply-adds), the same in any order of evaluation.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "attn_fwd_sm100.cuh"
+#include "paged_decode_common.cuh"
+#include "sm100_ptx.cuh"
+
+namespace hk {
+
+constexpr int kFp8LeastExp = -120, kFp8MostExp = 119;  // exponents of the scales that an append picks
+
+struct Fp8Cache {
+  uint8_t *k_pages, *v_pages;   // [P, 16, H_KV, D] e4m3 codes
+  float *k_scales, *v_scales;   // [P, H_KV]
+  const int32_t* block_table;   // [S, max_pages]
+  int S, H_KV, max_pages, num_pages;
+  int* status;
+};
+
+// Where the tokens of sequence s are: [S, T, heads, D], or rows cu[s] .. cu[s + 1] - 1 of [T, heads, D] (T in all).
+struct Fp8Rows {
+  const int32_t* cu;  // [S + 1], or null
+  int T;
+  FastDiv fd_units;   // without cu: units of a sequence
+};
+
+namespace fp8 {
+
+// Units of 16 tokens of ragged sequences: sequence s has those from cu[s] / 16 + PER * s on, which is room for whole pages from its
+// first token on (PER = 1) or for pages that it enters and leaves in the middle (PER = 2).
+template <int PER>
+__device__ __forceinline__ int first_unit(const int32_t* cu, int s) { return (cu[s] >> 4) + PER * s; }
+// The last sequence of `n` that starts at or before `unit`. Whatever cu holds, it is one of them.
+template <int PER>
+__device__ __forceinline__ int sequence_of(const int32_t* cu, int n, int unit) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (first_unit<PER>(cu, mid) <= unit) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+// Rows [first, first + n) of sequence s, kept inside [0, total) whatever cu holds.
+__device__ __forceinline__ void ragged_rows(const int32_t* cu, int s, int total, int& first, int& n) {
+  first = min(max(cu[s], 0), total);
+  n = max(min(cu[s + 1], total) - first, 0);
+}
+// One block of threads looks the whole array over.
+__device__ __forceinline__ void check_cu(const int32_t* cu, int S, int total, int* status) {
+  for (int s = threadIdx.x; s < S; s += blockDim.x)
+    if (cu[s] < 0 || cu[s + 1] < cu[s] || cu[s + 1] > total) atomicCAS(status, 0, kStatusBadLen);
+}
+
+__device__ __forceinline__ float2 decode2(uint32_t codes) {  // the low 16 bits
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<unsigned short>(codes)));
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
+  unsigned short lo, hi;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
+  return lo | static_cast<uint32_t>(hi) << 16;
+}
+__device__ __forceinline__ float2 bf16x2(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+
+// Bits of the scale for a largest magnitude, given by its bits: NaN for NaN, which makes the whole block NaN for every reader.
+__device__ __forceinline__ uint32_t scale_bits(uint32_t amax) {
+  if (amax > 0x7f800000u) return 0x7fc00000u;
+  const int e = static_cast<int>(amax >> 23) - 127 - 8 + ((amax & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return static_cast<uint32_t>(min(max(e, kFp8LeastExp), kFp8MostExp) + 127) << 23;
+}
+// x / scale. Exact through the reciprocal of a power of two; a scale that another quantiser left behind divides.
+struct Divide {
+  float scale, inv;
+  bool power;
+  __device__ __forceinline__ explicit Divide(uint32_t bits) {
+    scale = __uint_as_float(bits);
+    const int e = static_cast<int>(bits >> 23);
+    power = (bits & 0x807fffffu) == 0 && e > 0 && e < 254;
+    inv = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+  }
+  __device__ __forceinline__ float operator()(float x) const { return power ? x * inv : __fdiv_rn(x, scale); }
+};
+
+}  // namespace fp8
+
+struct AppendFp8Params {
+  Fp8Cache c;
+  Fp8Rows rows;
+  const __nv_bfloat16 *k_new, *v_new;
+  long long k_stride[3], v_stride[3];  // sequence, token, head; elements
+  const int32_t* start_pos;            // [S] position of the first new token of each sequence
+  const void *cos, *sin;               // [table_rows, R / 2] bf16 or fp32
+  int R, table_rows;
+  int warps;                           // units x H_KV x 2
+  FastDiv fd_heads2, fd_heads;         // 2 * H_KV, H_KV
+};
+
+enum Fp8Rotation : int { kFp8Plain = 0, kFp8TableBf16 = 1, kFp8TableF32 = 2 };
+
+// A warp has one block: a page's new tokens of one head, of K or of V, all requested before the first is looked at (8 x 16 bytes a
+// lane at D = 128). It finds their largest magnitude, settles the scale, and writes the codes; if the page had tokens already and the
+// scale grows, it reads and rounds anew the rows that get none. Nothing else touches that block, so there is nothing to order.
+// The heads of a page, and K and V, are neighbouring warps: they share its rows of the tables in L1, and lines of the page.
+// Bound by HBM (3 bytes a value); a token for each sequence is a launch and two dependent loads.
+template <int D, int ROT>
+__global__ void __launch_bounds__(256) paged_kv_append_fp8_kernel(const __grid_constant__ AppendFp8Params p) {
+  ptx::grid_dep_wait();
+  ptx::grid_dep_launch();
+  const Fp8Cache& c = p.c;
+  const int32_t* const cu = p.rows.cu;
+  if (cu && blockIdx.x == 0) fp8::check_cu(cu, c.S, p.rows.T, c.status);
+  const int w = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (w >= p.warps) return;
+  int unit, rem, head, is_v;
+  p.fd_heads2.divmod(w, unit, rem);
+  p.fd_heads.divmod(rem, is_v, head);
+  int s, block, n = p.rows.T, first = 0;
+  if (cu) {
+    s = fp8::sequence_of<2>(cu, c.S, unit);
+    block = unit - fp8::first_unit<2>(cu, s);
+    fp8::ragged_rows(cu, s, p.rows.T, first, n);
+  } else {
+    p.rows.fd_units.divmod(unit, s, block);
+  }
+  const long long start = p.start_pos[s], slot = (start >> 4) + block, base = slot * kPageTokens - start;  // row r has token base + r
+  const int r0 = static_cast<int>(max(-base, 0ll));
+  int r1 = static_cast<int>(min(n - base, static_cast<long long>(kPageTokens)));
+  if (block < 0 || r1 <= r0) return;
+  if (slot < 0 || slot >= c.max_pages) {
+    if (lane == 0) atomicCAS(c.status, 0, kStatusBadPage);
+    return;
+  }
+  const int id = c.block_table[static_cast<size_t>(s) * c.max_pages + slot];
+  if (id < 0 || id >= c.num_pages) {  // never write through an id outside the pool
+    if (lane == 0) atomicCAS(c.status, 0, kStatusBadPage);
+    return;
+  }
+  if constexpr (ROT != kFp8Plain) {
+    if (slot * kPageTokens + r1 > p.table_rows) {  // tokens behind the tables are not written
+      if (lane == 0) atomicCAS(c.status, 0, kStatusBadPos);
+      r1 = static_cast<int>(p.table_rows - slot * kPageTokens);
+      if (r1 <= r0) return;
+    }
+  }
+
+  constexpr int kLanes = D / 8, kRows = 32 / kLanes, kSteps = kPageTokens / kRows;  // lanes of a row, rows of a step
+  const int col = (lane % kLanes) * 8, row0 = lane / kLanes;
+  const long long* const stride = is_v ? p.v_stride : p.k_stride;
+  const __nv_bfloat16* const src = (is_v ? p.v_new : p.k_new) + s * stride[0] + (first + base) * stride[1] + head * stride[2] + col;
+  uint4 x[kSteps];
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    const int r = row0 + i * kRows;
+    x[i] = make_uint4(0, 0, 0, 0);
+    if (r >= r0 && r < r1) x[i] = __ldcs(reinterpret_cast<const uint4*>(src + r * stride[1]));
+  }
+  float* const scale_at = (is_v ? c.v_scales : c.k_scales) + static_cast<size_t>(id) * c.H_KV + head;
+  const uint32_t before = r0 > 0 ? __float_as_uint(*scale_at) : 0u;  // a page that starts anew has no scale yet
+
+  [[maybe_unused]] float y[ROT != kFp8Plain ? kSteps : 1][8];
+  uint32_t amax = 0;
+  if constexpr (ROT != kFp8Plain) {
+    const int half = p.R / 2, at = col < half ? col : col - half;  // pairs are (i, i + R / 2)
+    const bool turned = !is_v && col < p.R;
+    const int partner = lane + (col < half ? half / 8 : -half / 8);
+    const float sign = col < half ? -1.f : 1.f;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      const int r = row0 + i * kRows;
+      const uint32_t xw[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+      float cs[8], sn[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) cs[j] = 1.f, sn[j] = 0.f;
+      if (turned && r >= r0 && r < r1) {
+        const size_t t = static_cast<size_t>(slot * kPageTokens + r) * half + at;
+        if constexpr (ROT == kFp8TableF32) {
+          const float4 *const c4 = reinterpret_cast<const float4*>(static_cast<const float*>(p.cos) + t),
+                       *const s4 = reinterpret_cast<const float4*>(static_cast<const float*>(p.sin) + t);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float4 a = c4[j], b = s4[j];
+            cs[4 * j] = a.x, cs[4 * j + 1] = a.y, cs[4 * j + 2] = a.z, cs[4 * j + 3] = a.w;
+            sn[4 * j] = b.x, sn[4 * j + 1] = b.y, sn[4 * j + 2] = b.z, sn[4 * j + 3] = b.w;
+          }
+        } else {
+          const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.cos) + t),
+                      b = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.sin) + t);
+          const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 ca = fp8::bf16x2(aw[j]), sa = fp8::bf16x2(bw[j]);
+            cs[2 * j] = ca.x, cs[2 * j + 1] = ca.y, sn[2 * j] = sa.x, sn[2 * j + 1] = sa.y;
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 own = fp8::bf16x2(xw[j]), other = fp8::bf16x2(__shfl_sync(0xffffffffu, xw[j], partner & 31));
+        if (turned) {  // a cos - b sin, or b cos + a sin
+          y[i][2 * j] = __fadd_rn(__fmul_rn(own.x, cs[2 * j]), sign * __fmul_rn(other.x, sn[2 * j]));
+          y[i][2 * j + 1] = __fadd_rn(__fmul_rn(own.y, cs[2 * j + 1]), sign * __fmul_rn(other.y, sn[2 * j + 1]));
+        } else {
+          y[i][2 * j] = own.x, y[i][2 * j + 1] = own.y;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) amax = max(amax, __float_as_uint(y[i][j]) & 0x7fffffffu);
+    }
+  } else {
+    uint32_t two = 0;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i)
+      for (uint32_t v : {x[i].x, x[i].y, x[i].z, x[i].w}) two = __vmaxu2(two, v & 0x7fff7fffu);
+    amax = max(two & 0xffff0000u, two << 16);
+  }
+  amax = __reduce_max_sync(0xffffffffu, amax);
+  uint32_t bits = fp8::scale_bits(amax);
+  if (r0 > 0) {
+    if ((before & 0x7fffffffu) > 0x7f800000u) bits = 0x7fc00000u;
+    else if (static_cast<int>(before) > static_cast<int>(bits)) bits = before;  // of floats above zero
+  }
+  const fp8::Divide divide(bits);
+  const size_t row_bytes = static_cast<size_t>(c.H_KV) * D;
+  uint8_t* const page = (is_v ? c.v_pages : c.k_pages) + static_cast<size_t>(id) * kPageTokens * row_bytes + head * D + col;
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    const int r = row0 + i * kRows;
+    if (r < r0 || r >= r1) continue;
+    uint2 out;
+    if constexpr (ROT != kFp8Plain) {
+      out.x = fp8::encode4(divide(y[i][0]), divide(y[i][1]), divide(y[i][2]), divide(y[i][3]));
+      out.y = fp8::encode4(divide(y[i][4]), divide(y[i][5]), divide(y[i][6]), divide(y[i][7]));
+    } else {
+      const float2 a = fp8::bf16x2(x[i].x), b = fp8::bf16x2(x[i].y), d = fp8::bf16x2(x[i].z), e = fp8::bf16x2(x[i].w);
+      out.x = fp8::encode4(divide(a.x), divide(a.y), divide(b.x), divide(b.y));
+      out.y = fp8::encode4(divide(d.x), divide(d.y), divide(e.x), divide(e.y));
+    }
+    *reinterpret_cast<uint2*>(page + r * row_bytes) = out;
+  }
+  if (r0 > 0 && bits == before) return;
+  if (r0 > 0) {
+    const float old = __uint_as_float(before);
+#pragma unroll 1
+    for (int i = 0; i < kSteps; ++i) {
+      const int r = row0 + i * kRows;
+      if (r >= r0 && r < r1) continue;
+      uint2 v = *reinterpret_cast<const uint2*>(page + r * row_bytes);
+      auto anew = [&](uint32_t codes) {
+        const float2 a = fp8::decode2(codes), b = fp8::decode2(codes >> 16);
+        return fp8::encode4(divide(a.x * old), divide(a.y * old), divide(b.x * old), divide(b.y * old));
+      };
+      v.x = anew(v.x), v.y = anew(v.y);
+      *reinterpret_cast<uint2*>(page + r * row_bytes) = v;
+    }
+  }
+  if (lane == 0) *scale_at = __uint_as_float(bits);
+}
+
+struct ReadFp8Params {
+  Fp8Cache c;
+  Fp8Rows rows;
+  const int32_t* ctx_lens;        // [S], without rows.cu
+  __nv_bfloat16 *k_out, *v_out;   // contiguous
+  int zero_tail;                  // with rows.cu: rows behind the last sequence become zeros
+  int warps;                      // units x H_KV
+  FastDiv fd_heads;
+};
+
+// A warp has 16 tokens of one head, K and V: all of their codes are requested before the first is used (8 x 16 bytes a lane at D =
+// 128), scaled in fp32 and rounded once. Bound by HBM: 3 bytes a value.
+template <int D>
+__global__ void __launch_bounds__(256) paged_kv_read_fp8_kernel(const __grid_constant__ ReadFp8Params p) {
+  ptx::grid_dep_wait();
+  ptx::grid_dep_launch();
+  const Fp8Cache& c = p.c;
+  const int32_t* const cu = p.rows.cu;
+  if (cu && blockIdx.x == 0) fp8::check_cu(cu, c.S, p.rows.T, c.status);
+  const int w = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (w >= p.warps) return;
+  int unit, head, s, block;
+  p.fd_heads.divmod(w, unit, head);
+  int len, there;       // tokens of the sequence, rows of this unit that are written
+  long long out_row;
+  if (cu) {
+    s = fp8::sequence_of<1>(cu, c.S + 1, unit);
+    block = unit - fp8::first_unit<1>(cu, s);
+    if (block < 0) return;
+    int first;
+    if (s < c.S) {
+      fp8::ragged_rows(cu, s, p.rows.T, first, len);
+      there = len - block * kPageTokens;
+    } else {
+      if (!p.zero_tail) return;
+      first = min(max(cu[s], 0), p.rows.T);
+      len = 0;
+      there = p.rows.T - first - block * kPageTokens;
+    }
+    out_row = first + block * kPageTokens;
+  } else {
+    p.rows.fd_units.divmod(unit, s, block);
+    len = p.ctx_lens[s];
+    there = p.rows.T - block * kPageTokens;
+    out_row = static_cast<long long>(s) * p.rows.T + block * kPageTokens;
+  }
+  there = min(there, kPageTokens);
+  if (there <= 0) return;
+  if (len > static_cast<long long>(c.max_pages) * kPageTokens || (!cu && len > p.rows.T)) {
+    if (lane == 0) atomicCAS(c.status, 0, kStatusBadLen);
+    len = static_cast<int>(min(static_cast<long long>(len), static_cast<long long>(c.max_pages) * kPageTokens));
+  }
+  int valid = min(len - block * kPageTokens, there);  // what lies behind them comes back as zeros
+  int id = 0;
+  if (valid > 0) {
+    id = c.block_table[static_cast<size_t>(s) * c.max_pages + block];
+    if (id < 0 || id >= c.num_pages) {
+      if (lane == 0) atomicCAS(c.status, 0, kStatusBadPage);
+      id = valid = 0;
+    }
+  }
+  constexpr int kLanes = D / 16, kRows = 32 / kLanes, kSteps = kPageTokens / kRows;
+  const int col = (lane % kLanes) * 16, row0 = lane / kLanes;
+  const size_t row_bytes = static_cast<size_t>(c.H_KV) * D, at = static_cast<size_t>(id) * kPageTokens * row_bytes + head * D + col;
+  uint4 x[2][kSteps];
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      const int r = row0 + i * kRows;
+      x[kv][i] = make_uint4(0, 0, 0, 0);
+      if (r < valid) x[kv][i] = __ldcs(reinterpret_cast<const uint4*>((kv ? c.v_pages : c.k_pages) + at + r * row_bytes));
+    }
+  const size_t scale_at = static_cast<size_t>(id) * c.H_KV + head;
+  const float scales[2] = {valid > 0 ? c.k_scales[scale_at] : 0.f, valid > 0 ? c.v_scales[scale_at] : 0.f};
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      const int r = row0 + i * kRows;
+      if (r >= there) continue;
+      const uint32_t words[4] = {x[kv][i].x, x[kv][i].y, x[kv][i].z, x[kv][i].w};
+      uint32_t o[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 a = fp8::decode2(words[j]), b = fp8::decode2(words[j] >> 16);
+        o[2 * j] = ptx::pack_bf16x2(a.x * scales[kv], a.y * scales[kv]);
+        o[2 * j + 1] = ptx::pack_bf16x2(b.x * scales[kv], b.y * scales[kv]);
+      }
+      if (r >= valid)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] = 0;  // and not a NaN of the block's scale
+      uint4* const dst = reinterpret_cast<uint4*>((kv ? p.v_out : p.k_out) + ((out_row + r) * c.H_KV + head) * D + col);
+      dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
+      dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
+    }
+}
+
+}  // namespace hk

@@ -27,7 +27,7 @@
 #include <stdint.h>
 
 #include "attn_fwd_sm100.cuh"
-#include "paged_decode_sm100.cuh"
+#include "paged_decode_common.cuh"
 #include "sm100_ptx.cuh"
 
 namespace hk {

@@ -483,6 +483,152 @@ PyObject* paged_kv_append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
+// An 8-bit paged cache: k_pages, v_pages, k_scales, v_scales, block_table.
+struct Fp8Cache {
+  const Tensor *kp, *vp, *ks, *vs, *table;
+  int64_t s, pool, page, hkv, d, max_pages;
+  void *k_pages, *v_pages;
+  float *k_scales, *v_scales;
+  const int32_t* table_ptr;
+  int device;
+  bool take(PyObject* const* a) {
+    kp = plain(a[0]), vp = plain(a[1]), ks = plain(a[2]), vs = plain(a[3]), table = plain(a[4]);
+    if (!dense(kp, at::kFloat8_e4m3fn, 4) || !dense(vp, at::kFloat8_e4m3fn, 4) || !dense(ks, at::kFloat, 2) || !dense(vs, at::kFloat, 2) ||
+        !dense(table, at::kInt, 2))
+      return false;
+    pool = kp->size(0), page = kp->size(1), hkv = kp->size(2), d = kp->size(3), s = table->size(0), max_pages = table->size(1);
+    const std::initializer_list<int64_t> scales = {pool, hkv};
+    return vp->sizes() == kp->sizes() && ks->sizes() == at::IntArrayRef(scales) && vs->sizes() == at::IntArrayRef(scales) &&
+           same_device(*kp, {vp, ks, vs, table}) && fits({pool, page, hkv, d, s, max_pages}) && kp->numel() && table->numel();
+  }
+  void read() {
+    k_pages = ptr(*kp), v_pages = ptr(*vp), k_scales = ptr<float>(*ks), v_scales = ptr<float>(*vs), table_ptr = ptr<int32_t>(*table);
+    device = kp->device().index();
+  }
+  // int32 [n] beside it, or null for None; false: neither
+  bool ints(PyObject* o, int64_t n, const Tensor*& t) const {
+    t = nullptr;
+    if (o == Py_None) return true;
+    t = plain(o);
+    return dense(t, at::kInt, 1) && t->size(0) == n && t->device() == kp->device();
+  }
+};
+
+// paged_kv_append_fp8(k_new, v_new, k_pages, v_pages, k_scales, v_scales, block_table, start_pos, cos, sin, cu_seqlens): 0 when launched
+PyObject* paged_kv_append_fp8(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  Fp8Cache c;
+  const Tensor *start, *cu;
+  if (n_args != 11 || !c.take(a + 2) || a[7] == Py_None || !c.ints(a[7], c.s, start) || !c.ints(a[10], c.s + 1, cu)) Py_RETURN_NONE;
+  const int dims = cu ? 3 : 4;
+  const Tensor* x[2] = {plain(a[0]), plain(a[1])};
+  long long st[2][3];
+  for (int i = 0; i < 2; ++i) {
+    const Tensor* t = x[i];
+    if (!is(t, at::kBFloat16, dims) || !t->numel() || t->size(dims - 2) != c.hkv || t->size(dims - 1) != c.d ||
+        (!cu && t->size(0) != c.s) || t->device() != c.kp->device() || t->stride(dims - 1) != 1 || t->sizes() != x[0]->sizes())
+      Py_RETURN_NONE;
+    st[i][0] = 0;
+    for (int k = cu ? 1 : 0; k < 3; ++k) {
+      st[i][k] = t->stride(cu ? k - 1 : k);
+      if (st[i][k] <= 0 || st[i][k] % 8 != 0) Py_RETURN_NONE;
+    }
+  }
+  const int64_t tokens = x[0]->size(dims - 3);
+  const Tensor *cos = nullptr, *sin = nullptr;
+  int flags = 0;
+  if (a[8] != Py_None || a[9] != Py_None) {
+    cos = plain(a[8]), sin = plain(a[9]);
+    if (!(dense(cos, at::kBFloat16, 2) && dense(sin, at::kBFloat16, 2))) {
+      if (!(dense(cos, at::kFloat, 2) && dense(sin, at::kFloat, 2))) Py_RETURN_NONE;
+      flags = HK_FP8_TABLE_F32;
+    }
+    if (cos->sizes() != sin->sizes() || !same_device(*c.kp, {cos, sin}) || !fits({cos->size(0), 2 * cos->size(1)})) Py_RETURN_NONE;
+  }
+  if (!fits({tokens})) Py_RETURN_NONE;
+  void* stream = stream_of(*c.kp);
+  c.read();
+  const void *kn = ptr(*x[0]), *vn = ptr(*x[1]), *cosp = cos ? ptr(*cos) : nullptr, *sinp = cos ? ptr(*sin) : nullptr;
+  const int rows = cos ? i32(cos->size(0)) : 0, rotary_dim = cos ? i32(2 * cos->size(1)) : 0;
+  const int32_t *startp = ptr<int32_t>(*start), *cup = cu ? ptr<int32_t>(*cu) : nullptr;
+  const int rc = unlocked([&] {
+    return hk_paged_kv_append_fp8(kn, vn, c.k_pages, c.v_pages, c.k_scales, c.v_scales, c.table_ptr, startp, cup, sinp, cosp, i32(c.s),
+                                  i32(tokens), i32(c.hkv), i32(c.d), st[0], st[1], rotary_dim, rows, flags, i32(c.page),
+                                  i32(c.max_pages), i32(c.pool), c.device, stream);
+  });
+  return PyLong_FromLong(rc);
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_kv_read_fp8(k_pages, v_pages, k_scales, v_scales, block_table, rows, ctx_lens, cu_seqlens, k_out, v_out)
+PyObject* paged_kv_read_fp8(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  Fp8Cache c;
+  const Tensor *lens, *cu;
+  if (n_args != 10 || !c.take(a) || !PyLong_CheckExact(a[5]) || !c.ints(a[6], c.s, lens) || !c.ints(a[7], c.s + 1, cu) || !lens == !cu ||
+      (a[8] == Py_None) != (a[9] == Py_None))
+    Py_RETURN_NONE;
+  int overflow = 0;
+  const long rows = PyLong_AsLongAndOverflow(a[5], &overflow);
+  if (overflow || rows <= 0 || !fits({rows})) Py_RETURN_NONE;
+  Tensor out[2];
+  for (int i = 0; i < 2; ++i)
+    if (!(cu ? output(a[8 + i], *c.kp, {rows, c.hkv, c.d}, at::kBFloat16, out[i])
+             : output(a[8 + i], *c.kp, {c.s, rows, c.hkv, c.d}, at::kBFloat16, out[i])))
+      Py_RETURN_NONE;
+  void* stream = stream_of(*c.kp);
+  c.read();
+  void *ko = ptr(out[0]), *vo = ptr(out[1]);
+  const int32_t *lensp = lens ? ptr<int32_t>(*lens) : nullptr, *cup = cu ? ptr<int32_t>(*cu) : nullptr;
+  const int zero_tail = a[8] == Py_None;
+  const int rc = unlocked([&] {
+    return hk_paged_kv_read_fp8(c.k_pages, c.v_pages, c.k_scales, c.v_scales, c.table_ptr, lensp, cup, ko, vo, i32(c.s), i32(rows),
+                                i32(c.hkv), i32(c.d), zero_tail, i32(c.page), i32(c.max_pages), i32(c.pool), c.device, stream);
+  });
+  return result(rc, out[0], out[1]);
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_decode_fp8(q, k_pages, v_pages, k_scales, v_scales, block_table, ctx_lens, softmax_scale, out, lse, workspace, window or 0, sinks)
+PyObject* paged_decode_fp8(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  Fp8Cache c;
+  float scale;
+  const Tensor* lens;
+  if (n_args != 13 || !c.take(a + 1) || a[6] == Py_None || !c.ints(a[6], c.s, lens) || !number(a[7], scale)) Py_RETURN_NONE;
+  int window = 0, sinks = 0;
+  if (!PyLong_CheckExact(a[11]) || (PyObject_IsTrue(a[11]) && !window_args(a, n_args, 11, window, sinks))) Py_RETURN_NONE;
+  const Tensor* q = plain(a[0]);
+  if (!dense(q, at::kBFloat16, 4) || q->size(0) != c.s || q->size(1) != 1 || q->size(3) != c.d || q->device() != c.kp->device() ||
+      !fits({q->size(2)}))
+    Py_RETURN_NONE;
+  const int64_t h = q->size(2);
+  const size_t need = hk_attn_paged_decode_fp8_workspace_bytes(i32(c.s), i32(h), i32(c.d), i32(c.max_pages), i32(c.page), window, sinks);
+  Tensor out, lse, ws;
+  if (need == 0 || !output(a[8], *q, q->sizes(), at::kBFloat16, out) || !output(a[9], *q, {c.s, h, 1, 1}, at::kFloat, lse))
+    Py_RETURN_NONE;
+  if (a[10] == Py_None) {
+    if (!output(Py_None, *q, {int64_t(need < 256 ? 256 : need)}, at::kByte, ws)) Py_RETURN_NONE;
+  } else {
+    const Tensor* t = plain(a[10]);
+    if (!dense(t, at::kByte, 1) || t->device() != q->device()) Py_RETURN_NONE;
+    ws = *t;
+  }
+  void* stream = stream_of(*q);
+  c.read();
+  void *qp = ptr(*q), *outp = ptr(out), *wsp = ptr(ws);
+  float* lsep = ptr<float>(lse);
+  const int32_t* lensp = ptr<int32_t>(*lens);
+  const size_t ws_bytes = size_t(ws.numel());
+  const int rc = unlocked([&] {
+    return hk_attn_paged_decode_fp8(qp, c.k_pages, c.v_pages, c.k_scales, c.v_scales, c.table_ptr, lensp, outp, lsep, i32(c.s), i32(h),
+                                    i32(c.hkv), i32(c.d), i32(c.page), i32(c.max_pages), i32(c.pool), window, sinks, scale, wsp,
+                                    ws_bytes, c.device, stream);
+  });
+  return result(rc, out, lse);
+  END_HANDLE_TH_ERRORS
+}
+
 // ---- autograd. A step through the Python functions behind these spends about 55 us on them, in the caller's thread and in the
 // engine's, which has to have the interpreter for its part; small steps are made of little else.
 
@@ -794,6 +940,7 @@ PyObject* captured_backward(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
 PyMethodDef methods[] = {HK_METHOD(attn_fwd),       HK_METHOD(attn_bwd_strided), HK_METHOD(rotary_bnhd),
                          HK_METHOD(paged_decode),   HK_METHOD(attn_fwd_paged),   HK_METHOD(paged_kv_append),
                          HK_METHOD(qk_norm_rotary), HK_METHOD(qk_norm_rotary_bwd),
+                         HK_METHOD(paged_kv_append_fp8), HK_METHOD(paged_kv_read_fp8), HK_METHOD(paged_decode_fp8),
                          HK_METHOD(packed_attention), HK_METHOD(norm_rotary), HK_METHOD(captured_backward),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_front", "Native tensor front ends of hipkittens_b200", -1, methods,

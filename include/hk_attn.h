@@ -317,6 +317,50 @@ int hk_paged_kv_append_rotary(const void* k_new, const void* v_new, void* k_page
                               int S, int T, int H_KV, int D, int rotary_dim, int cos_rows, int page_size,
                               int max_pages_per_seq, int num_pages, int device, void* cuda_stream);
 
+/* ---- The paged cache in 8 bits: pages of e4m3 codes [num_pages, 16, H_KV, D] and an fp32 scale for each page and head, K and V
+ * [num_pages, H_KV] each; value = code * scale, where scales are finite and above zero. No counterpart in the reference, whose cache
+ * is bf16 (training/llama/llama/models/mha.py:16-42). D = 64 or 128, page_size 16, S <= 65535; pages 16-byte aligned.
+ *
+ * hk_paged_kv_append_fp8 writes new tokens, K rotated on the way if tables are given (pairs (i, i + rotary_dim / 2), row = position).
+ *   k_new, v_new : bf16 [S, T, H_KV, D] through element strides of the sequence, token and head (positive multiples of 8; the last
+ *                  dimension is contiguous), token t of sequence s at position start_pos[s] + t; or, with cu_seqlens [S + 1], [T, H_KV,
+ *                  D] through the last two strides, where sequence s has the rows cu_seqlens[s] .. cu_seqlens[s + 1] - 1 (T in all)
+ *   sin, cos     : [table_rows, rotary_dim / 2] bf16, or fp32 with HK_FP8_TABLE_F32; or NULL both. rotary_dim <= 0 selects D
+ * A block is what one page holds of one head. Its scale becomes the smallest power of two (2^-120 to 2^119) that brings its new tokens to
+ * 448 at most. If a block's first row is among the new tokens it starts anew: its other rows keep their codes, which stand for nothing.
+ * Otherwise its scale does not shrink, and if it grows the other rows are rounded anew under it. All is computed in fp32 and rounded once.
+ * Infinities become the block's largest value; a NaN makes the block's scale NaN, and with it all of the block for every reader.
+ * The tokens of one block have to come from one sequence of a call: a page that two sequences share takes no new tokens.
+ * Positions outside the block table and page ids outside the pool are skipped (HK_EBADPAGE), positions behind the tables too
+ * (HK_EBADPOS); a cu_seqlens that does not rise from 0 to at most T is reported as HK_EBADLEN, and its rows are kept inside [0, T). */
+#define HK_FP8_TABLE_F32 1
+int hk_paged_kv_append_fp8(const void* k_new, const void* v_new, void* k_pages, void* v_pages, float* k_scales, float* v_scales,
+                           const int32_t* block_table, const int32_t* start_pos, const int32_t* cu_seqlens, const void* sin,
+                           const void* cos, int S, int T, int H_KV, int D, const long long* k_strides, const long long* v_strides,
+                           int rotary_dim, int table_rows, int flags, int page_size, int max_pages_per_seq, int num_pages,
+                           int device, void* cuda_stream);
+
+/* Reads tokens back as bf16 (fp32 product, rounded once), for instance as keys and values of the attention of a chunk.
+ *   ctx_lens   : int32 [S]; k_out, v_out [S, rows, H_KV, D] get tokens 0 .. ctx_lens[s] - 1 of each sequence and zeros behind them
+ *   cu_seqlens : int32 [S + 1], instead of ctx_lens; k_out, v_out [rows, H_KV, D] get the first cu_seqlens[s + 1] - cu_seqlens[s]
+ *                tokens of sequence s from row cu_seqlens[s] on. Rows behind the last sequence are left as they are, or zeros with
+ *                `zero_tail`.
+ * Tokens behind the block table are zeros, and a length above `rows` is cut (HK_EBADLEN both); those of a page id outside the pool are
+ * zeros (HK_EBADPAGE). */
+int hk_paged_kv_read_fp8(const void* k_pages, const void* v_pages, const float* k_scales, const float* v_scales,
+                         const int32_t* block_table, const int32_t* ctx_lens, const int32_t* cu_seqlens, void* k_out, void* v_out,
+                         int S, int rows, int H_KV, int D, int zero_tail, int page_size, int max_pages_per_seq, int num_pages,
+                         int device, void* cuda_stream);
+
+/* hk_attn_paged_decode (window = 0 and sinks = 0) and hk_attn_paged_decode_window (window > 0) against such a cache. H / H_KV from 1 to 8;
+ * the pages of a context, or those of a window and its sinks, at most 8192. The products take q, whose values over the power of two of
+ * their row's largest become fp16, and P, which becomes bf16 after its page's scale; sums and statistics are fp32. */
+size_t hk_attn_paged_decode_fp8_workspace_bytes(int S, int H, int D, int max_pages_per_seq, int page_size, int window, int sinks);
+int hk_attn_paged_decode_fp8(const void* q, const void* k_pages, const void* v_pages, const float* k_scales, const float* v_scales,
+                             const int32_t* block_table, const int32_t* ctx_lens, void* o, float* lse, int S, int H, int H_KV, int D,
+                             int page_size, int max_pages_per_seq, int num_pages, int window, int sinks, float softmax_scale,
+                             void* workspace, size_t workspace_bytes, int device, void* cuda_stream);
+
 /* Paged-KV decode for callers that cannot allocate device memory. No counterpart in the reference.
  *
  * Who needs it: a serving engine that hands all of HBM to its own block allocator at start-up leaves nothing
