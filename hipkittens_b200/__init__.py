@@ -9,6 +9,8 @@ Public surface
 * ``attn_fwd(q, k, v, causal=False, ...) -> (O, L)``, ``attn_bwd_prep`` / ``attn_bwd`` / ``dq_shuffle`` (the
   backward pass), ``paged_decode(...) -> (O, L)`` and ``paged_kv_append(...)``: torch-tensor front ends over
   the C ABI (ctypes).
+* ``attn_fwd_ragged(...)`` and ``attn_bwd_ragged(...)``: the same over sequences of different lengths one after the other, without padding;
+  ``HipRaggedAttention`` in :mod:`hipkittens_b200.attention` is the module.
 * ``paged_kv_append_fp8(...)``, ``paged_kv_read_fp8(...)`` and ``paged_decode_fp8(...)``: the paged cache in 8 bits, with a scale for
   each page and head.
 * ``qk_norm_rotary(...)`` and ``qk_norm_rotary_bwd(...)``: RMS norm of every head of q and k with the rotation of its position.
@@ -25,7 +27,9 @@ from ._native import (  # noqa: F401
     HkError,
     attn_bwd,
     attn_bwd_prep,
+    attn_bwd_ragged,
     attn_fwd,
+    attn_fwd_ragged,
     capi,
     dq_shuffle,
     kernel_launch_count,
@@ -56,7 +60,9 @@ __all__ = [
     "HkError",
     "attn_bwd",
     "attn_bwd_prep",
+    "attn_bwd_ragged",
     "attn_fwd",
+    "attn_fwd_ragged",
     "capi",
     "dq_shuffle",
     "kernel_launch_count",

@@ -76,7 +76,7 @@ def nvcc_path() -> str:
 
 
 # the library's translation units, compiled side by side
-LIB_UNITS = ["hk_attn_api.cu", "hk_kv8_api.cu"]
+LIB_UNITS = ["hk_attn_api.cu", "hk_kv8_api.cu", "hk_ragged_api.cu"]
 OBJ_DIR = os.path.join(PKG, "build")
 
 

@@ -49,6 +49,10 @@ EXPORTED_SYMBOLS = (
     "hk_attn_paged_decode_window",
     "hk_attn_paged_decode_static",
     "hk_paged_kv_append",
+    "hk_attn_fwd_ragged_workspace_bytes",
+    "hk_attn_fwd_ragged",
+    "hk_attn_bwd_ragged_workspace_bytes",
+    "hk_attn_bwd_ragged",
     "hk_paged_kv_append_fp8",
     "hk_paged_kv_read_fp8",
     "hk_attn_paged_decode_fp8_workspace_bytes",
@@ -155,6 +159,15 @@ def capi() -> ctypes.CDLL:
     lib.hk_attn_paged_decode_static.restype = ci
     lib.hk_paged_kv_append.argtypes = [vp, vp, vp, vp, vp, vp, ci, ci, ci, ci, ci, ci, ci, ci, vp]
     lib.hk_paged_kv_append.restype = ci
+    size = ctypes.c_size_t
+    lib.hk_attn_fwd_ragged_workspace_bytes.argtypes = [ci] * 2
+    lib.hk_attn_fwd_ragged_workspace_bytes.restype = size
+    lib.hk_attn_fwd_ragged.argtypes = [vp] * 7 + [ci] * 6 + [ll3] * 3 + [ci, cf, ci, vp, size, ci, vp]
+    lib.hk_attn_fwd_ragged.restype = ci
+    lib.hk_attn_bwd_ragged_workspace_bytes.argtypes = [ci] * 3
+    lib.hk_attn_bwd_ragged_workspace_bytes.restype = size
+    lib.hk_attn_bwd_ragged.argtypes = [vp] * 12 + [ci] * 6 + [ll3] * 6 + [ci, cf, ci, vp, size, ci, vp]
+    lib.hk_attn_bwd_ragged.restype = ci
     lib.hk_paged_kv_append_fp8.argtypes = [vp] * 11 + [ci] * 4 + [ll3] * 2 + [ci] * 7 + [vp]
     lib.hk_paged_kv_append_fp8.restype = ci
     lib.hk_paged_kv_read_fp8.argtypes = [vp] * 9 + [ci] * 9 + [vp]
@@ -975,6 +988,137 @@ def paged_kv_append_rotary(
                                           s_n, t_n, hkv, d, 2 * cos.shape[1], cos.shape[0], page, block_table.shape[1],
                                           p_n, k_new.device.index, st.cuda_stream)
     _check(rc, "hk_paged_kv_append_rotary")
+
+
+def _ragged_strides(t: torch.Tensor):
+    # a dimension of size 1 has no stride that matters: give it one the library takes
+    return (ctypes.c_longlong * 3)(*(st if n > 1 else t.shape[2] for st, n in zip(t.stride()[:2], t.shape[:2])), 0)
+
+
+def _check_ragged(q, k, v, cu_seqlens_q, cu_seqlens_k):
+    """What both directions ask of their inputs; returns cu_seqlens_k, which is that of q where it is None."""
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if not isinstance(t, torch.Tensor) or t.device.type != "cuda" or t.dim() != 3:
+            raise RuntimeError(f"{name} must be a 3-D CUDA tensor, [rows, heads, D]")
+        if t.dtype != torch.bfloat16:
+            raise RuntimeError(f"{name} must be torch.bfloat16")
+        if t.numel() and (t.stride(2) != 1 or any(st <= 0 or st % 8 for st, n in zip(t.stride()[:2], t.shape) if n > 1)):
+            raise RuntimeError(f"{name}: the last dimension must be contiguous and the other strides positive multiples of 8 elements")
+    if k.shape != v.shape or k.shape[2] != q.shape[2]:
+        raise RuntimeError("k/v must be [rows, H_KV, D] with q's head dimension")
+    if cu_seqlens_k is None:
+        if k.shape[0] != q.shape[0]:
+            raise RuntimeError("without cu_seqlens_k, k and v have q's rows")
+        cu_seqlens_k = cu_seqlens_q
+    for name, t in (("cu_seqlens_q", cu_seqlens_q), ("cu_seqlens_k", cu_seqlens_k)):
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] < 2 or not t.is_contiguous():
+            raise RuntimeError(f"{name} must be a contiguous int32 tensor [S + 1] with S >= 1")
+    if cu_seqlens_q.shape != cu_seqlens_k.shape:
+        raise RuntimeError("cu_seqlens_q and cu_seqlens_k must have the same shape")
+    _require_same_device(q, k=k, v=v, cu_seqlens_q=cu_seqlens_q, cu_seqlens_k=cu_seqlens_k)
+    return cu_seqlens_k
+
+
+def attn_fwd_ragged(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    cu_seqlens_k: Optional[torch.Tensor] = None,
+    causal: bool = True,
+    softmax_scale: Optional[float] = None,
+    out: Optional[torch.Tensor] = None,
+    lse: Optional[torch.Tensor] = None,
+    stream: Optional[torch.cuda.Stream] = None,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """`attn_fwd` over sequences of different lengths that lie one after the other, without padding.
+
+    q [T,H,D] bf16, k/v [Tk,H_KV,D] bf16, contiguous or views with a contiguous last dimension (slices of a packed projection). Sequence s
+    has rows cu_seqlens_q[s] .. cu_seqlens_q[s+1]-1 of q and, by `cu_seqlens_k` (None: those of q), of k and v; both int32 [S+1], rising,
+    on the device. A sequence may have fewer queries than keys (a chunk behind what is cached), more, or none. With `causal` the last query
+    of a sequence is at its last key, and a row that sees no key has O = 0 and L = -inf. Returns O [T,H,D] bf16 and L [H,T] fp32; rows
+    that belong to no sequence are zeros and -inf in new outputs, and left as they are in `out` and `lse`. Offsets that fall or lie outside
+    the rows are reported by the device status (HK_EBADLEN), and nothing is written. Asynchronous on `stream`."""
+    if stream is None:
+        r = _front().attn_fwd_ragged(q, k, v, cu_seqlens_q, cu_seqlens_k, bool(causal), softmax_scale, out, lse)
+        if r is not None:
+            return _done(r, "hk_attn_fwd_ragged")
+    cu_seqlens_k = _check_ragged(q, k, v, cu_seqlens_q, cu_seqlens_k)
+    t_n, h, d = q.shape
+    if (out is None) != (lse is None):
+        raise RuntimeError("out and lse belong together")
+    fill_rest = out is None
+    if fill_rest:
+        out, lse = _new(q.shape, q.dtype, q.device, stream), _new((h, t_n), torch.float32, q.device, stream)
+    if not isinstance(out, torch.Tensor) or out.shape != q.shape or out.dtype != torch.bfloat16 or not out.is_contiguous():
+        raise RuntimeError("out must be a contiguous bf16 tensor of q's shape")
+    if not isinstance(lse, torch.Tensor) or lse.shape != (h, t_n) or lse.dtype != torch.float32 or not lse.is_contiguous():
+        raise RuntimeError("lse must be a contiguous fp32 tensor [H, T]")
+    _require_same_device(q, out=out, lse=lse)
+    s_n = cu_seqlens_q.shape[0] - 1
+    need = int(capi().hk_attn_fwd_ragged_workspace_bytes(s_n, t_n))
+    ws = _new(need, torch.uint8, q.device, stream)
+    st = stream if stream is not None else torch.cuda.current_stream(q.device)
+    _check(capi().hk_attn_fwd_ragged(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), cu_seqlens_q.data_ptr(),
+                                     cu_seqlens_k.data_ptr(), s_n, t_n, k.shape[0], h, k.shape[1], d, _ragged_strides(q),
+                                     _ragged_strides(k), _ragged_strides(v), int(bool(causal)), float(softmax_scale or 0.0),
+                                     int(fill_rest), ws.data_ptr(), need, q.device.index, st.cuda_stream), "hk_attn_fwd_ragged")
+    return out, lse
+
+
+def attn_bwd_ragged(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    o: torch.Tensor,
+    d_o: torch.Tensor,
+    lse: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    cu_seqlens_k: Optional[torch.Tensor] = None,
+    causal: bool = True,
+    softmax_scale: Optional[float] = None,
+    dq: Optional[torch.Tensor] = None,
+    dk: Optional[torch.Tensor] = None,
+    dv: Optional[torch.Tensor] = None,
+    stream: Optional[torch.cuda.Stream] = None,
+) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """dQ, dK and dV of `attn_fwd_ragged`, whose inputs and outputs these are; o and d_o [T,H,D] bf16 are contiguous. `dq`, `dk` and `dv`
+    may be views as q, k and v may (slices of the gradient of a packed projection); rows that belong to no sequence are zeros in new
+    gradients, and left as they are in given ones. The same from run to run."""
+    if stream is None:
+        r = _front().attn_bwd_ragged(q, k, v, o, d_o, lse, cu_seqlens_q, cu_seqlens_k, bool(causal), softmax_scale, dq, dk, dv)
+        if r is not None:
+            return _done(r, "hk_attn_bwd_ragged")
+    cu_seqlens_k = _check_ragged(q, k, v, cu_seqlens_q, cu_seqlens_k)
+    t_n, h, d = q.shape
+    for name, t in (("o", o), ("d_o", d_o)):
+        if not isinstance(t, torch.Tensor) or t.shape != q.shape or t.dtype != torch.bfloat16 or not t.is_contiguous():
+            raise RuntimeError(f"{name} must be a contiguous bf16 tensor of q's shape")
+    if not isinstance(lse, torch.Tensor) or lse.shape != (h, t_n) or lse.dtype != torch.float32 or not lse.is_contiguous():
+        raise RuntimeError("lse must be a contiguous fp32 tensor [H, T]")
+    if len({t is None for t in (dq, dk, dv)}) > 1:
+        raise RuntimeError("dq, dk and dv belong together")
+    fill_rest = dq is None
+    if fill_rest:
+        dq, dk, dv = (_new(t.shape, t.dtype, t.device, stream) for t in (q, k, v))
+    for name, t, like in (("dq", dq, q), ("dk", dk, k), ("dv", dv, v)):
+        if not isinstance(t, torch.Tensor) or t.shape != like.shape or t.dtype != torch.bfloat16:
+            raise RuntimeError(f"{name} must be a bf16 tensor of its input's shape")
+        if t.numel() and (t.stride(2) != 1 or any(st <= 0 or st % 8 for st, n in zip(t.stride()[:2], t.shape) if n > 1)):
+            raise RuntimeError(f"{name}: the last dimension must be contiguous and the other strides positive multiples of 8 elements")
+    _require_same_device(q, o=o, d_o=d_o, lse=lse, dq=dq, dk=dk, dv=dv)
+    s_n = cu_seqlens_q.shape[0] - 1
+    need = int(capi().hk_attn_bwd_ragged_workspace_bytes(s_n, t_n, k.shape[0]))
+    ws = _new(need, torch.uint8, q.device, stream)
+    delta = _new(lse.shape, torch.float32, q.device, stream)
+    st = stream if stream is not None else torch.cuda.current_stream(q.device)
+    _check(capi().hk_attn_bwd_ragged(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), d_o.data_ptr(), lse.data_ptr(),
+                                     delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), cu_seqlens_q.data_ptr(),
+                                     cu_seqlens_k.data_ptr(), s_n, t_n, k.shape[0], h, k.shape[1], d,
+                                     *(_ragged_strides(t) for t in (q, k, v, dq, dk, dv)), int(bool(causal)),
+                                     float(softmax_scale or 0.0), int(fill_rest), ws.data_ptr(), need, q.device.index, st.cuda_stream),
+           "hk_attn_bwd_ragged")
+    return dq, dk, dv
 
 
 HK_FP8_TABLE_F32 = 1

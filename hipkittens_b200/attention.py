@@ -25,7 +25,18 @@ import torch.nn as nn
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
-from ._native import _check_window, _front, attn_bwd_strided, attn_fwd, device_status, key_padding_lens, qk_norm_rotary, qk_norm_rotary_bwd
+from ._native import (
+    _check_window,
+    _front,
+    attn_bwd_ragged,
+    attn_bwd_strided,
+    attn_fwd,
+    attn_fwd_ragged,
+    device_status,
+    key_padding_lens,
+    qk_norm_rotary,
+    qk_norm_rotary_bwd,
+)
 
 
 def _tma_viewable(t: torch.Tensor) -> bool:
@@ -237,6 +248,55 @@ class HipCrossAttention(nn.Module):
         causal = self.causal if causal is None else causal
         assert kv.shape[0] == batch_size and kv.shape[4] == q.shape[3]
         return _attend(q, kv, causal, self.softmax_scale, key_padding_mask, self.window, self.sinks)
+
+
+class RaggedAttnFunction(Function):
+    """``attn_fwd_ragged`` with gradients of q [T,H,D] and the packed kv [Tk,2,H_KV,D], bf16. Asynchronous in both directions, as the
+    call itself is."""
+
+    @classmethod
+    def apply(cls, q, kv, cu_seqlens_q, cu_seqlens_k=None, causal=True, softmax_scale=None):
+        out = _front().ragged_attention(q, kv, cu_seqlens_q, cu_seqlens_k, bool(causal), softmax_scale)
+        if out is not None:
+            return out
+        return super().apply(q, kv, cu_seqlens_q, cu_seqlens_k, causal, softmax_scale)
+
+    @staticmethod
+    def forward(ctx, q, kv, cu_seqlens_q, cu_seqlens_k, causal, softmax_scale):
+        if kv.dim() != 4 or kv.shape[1] != 2:
+            raise RuntimeError("kv must be [Tk, 2, H_KV, D]")
+        O, L = attn_fwd_ragged(q, *kv.unbind(1), cu_seqlens_q, cu_seqlens_k, causal, softmax_scale)
+        ctx.save_for_backward(q, kv, O, L, cu_seqlens_q, cu_seqlens_k)
+        ctx.rest = causal, softmax_scale
+        return O
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dO):
+        q, kv, O, L, cu_q, cu_k = ctx.saved_tensors
+        _front().captured_backward(dO)
+        # saved-tensor hooks may have given them back in other layouts
+        q, kv = (t if t.stride(-1) == 1 and all(st % 8 == 0 and st > 0 for st in t.stride()[:-1]) else t.contiguous() for t in (q, kv))
+        dq, dk, dv = attn_bwd_ragged(q, *kv.unbind(1), O.contiguous(), dO.to(torch.bfloat16).contiguous(), L.contiguous(), cu_q, cu_k,
+                                     *ctx.rest)
+        return dq, torch.stack((dk, dv), 1), None, None, None, None
+
+
+class HipRaggedAttention(nn.Module):
+    """HipCrossAttention over a ragged batch: q [T, H, D], kv [Tk, 2, H_KV, D] bf16 -> [T, H, D], the sequences one after the other as
+    ``attn_fwd_ragged`` says (`cu_seqlens_k` None: queries and keys are the same tokens). The reference's modules pad instead
+    (hipkittens.py:122-202). A call does not synchronise: what the device has to say of offsets that fall is in its status."""
+
+    def __init__(self, causal=False, softmax_scale=None, attention_dropout=0.0, deterministic=False):
+        super().__init__()
+        self.causal = causal
+        self.softmax_scale = softmax_scale
+        self.drop = nn.Dropout(attention_dropout)
+        self.deterministic = deterministic
+
+    def forward(self, q, kv, cu_seqlens_q, cu_seqlens_k=None, causal=None):
+        causal = self.causal if causal is None else causal
+        return RaggedAttnFunction.apply(q, kv, cu_seqlens_q, cu_seqlens_k, causal, self.softmax_scale)
 
 
 class QkNormRotaryFunction(Function):

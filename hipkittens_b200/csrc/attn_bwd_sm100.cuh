@@ -95,6 +95,11 @@ struct BwdParams {
 #ifdef HK_TRACE
   long long* trace;     // [4 roles][4096] clock stamps of CTA 0 (debug builds only)
 #endif
+  // kMaskRagged: as in FwdParams; the places are key blocks in the dK/dV kernel (x K/V heads) and query tiles in the dQ kernel (x heads)
+  const int* plan_count;
+  const int4* plan;
+  int per_place, causal;
+  FastDiv fd_per_place;
 };
 
 __device__ __forceinline__ __nv_bfloat16* dk_row(const BwdParams& p, int b, int key, int kvh) {
@@ -490,6 +495,37 @@ struct DkdvItem {
   int g_first, i_first;  // head and query tile of the first
   int rank;
 };
+// Ragged: as RaggedItem of the forward. A sequence's last query tile is loaded with rows of the next one behind it: their probabilities
+// and dS are masked, and the rows of Q and dO zeroed in shared memory before the products that sum over them.
+struct DkdvRaggedItem : DkdvItem {
+  int q0, n_q, k0;
+};
+template <int MASK>
+using DkdvItemOf = std::conditional_t<MASK == kMaskRagged, DkdvRaggedItem, DkdvItem>;
+__device__ __forceinline__ int first_query(const DkdvItem&) { return 0; }
+__device__ __forceinline__ int first_query(const DkdvRaggedItem& w) { return w.q0; }
+__device__ __forceinline__ int queries(const BwdParams& p, const DkdvItem&) { return p.N; }
+__device__ __forceinline__ int queries(const BwdParams&, const DkdvRaggedItem& w) { return w.n_q; }
+__device__ __forceinline__ int first_of_keys(const DkdvItem&) { return 0; }
+__device__ __forceinline__ int first_of_keys(const DkdvRaggedItem& w) { return w.k0; }
+__device__ __forceinline__ int stored_keys(const BwdParams& p, const DkdvItem&) { return p.NK; }  // those that have gradients
+__device__ __forceinline__ int stored_keys(const BwdParams&, const DkdvRaggedItem& w) { return w.kv_len; }
+__device__ __forceinline__ size_t stats_row(const BwdParams& p, const DkdvItem& w, int head) {
+  return (static_cast<size_t>(w.b) * p.H + head) * p.N;
+}
+__device__ __forceinline__ size_t stats_row(const BwdParams& p, const DkdvRaggedItem& w, int head) {
+  return static_cast<size_t>(head) * p.N + w.q0;
+}
+// Rows [from, 128) of a tile in shared memory become zeros, by the threads of the element-wise warps, for the products issued behind
+// their next arrival.
+template <int D>
+__device__ __forceinline__ void zero_rows(uint8_t* tile, int from, int tid, int threads) {
+  constexpr int kUnits = D / 8;  // 16 bytes each
+  for (int i = from * kUnits + tid; i < kBlockM * kUnits; i += threads) {
+    const int r = i / kUnits, u = i % kUnits;
+    *reinterpret_cast<uint4*>(tile + (u >> 3) * BwdSmem<D>::kSubTileBytes + r * 128 + (u & 7) * 16) = make_uint4(0, 0, 0, 0);
+  }
+}
 
 // First pair of rank r's share of n pairs.
 __device__ __forceinline__ int dkdv_share(int r, int ranks, int n) { return r * n / ranks; }
@@ -528,15 +564,26 @@ __device__ __forceinline__ int dkdv_item_for_round(const BwdParams& p, int round
 }
 
 template <int MASK, bool SPLIT>
-__device__ __forceinline__ DkdvItem decode_dkdv_item(const BwdParams& p, int idx) {
+__device__ __forceinline__ DkdvItemOf<MASK> decode_dkdv_item(const BwdParams& p, int idx) {
   constexpr bool CAUSAL = MASK != kMaskNone;
-  DkdvItem w;
-  const int NBQ = (p.N + kBlockM - 1) / kBlockM;   // query tiles
-  int unit;
-  p.fd_unit.divmod(idx, unit, w.j);
-  p.fd_hkv.divmod(unit, w.b, w.kvh);
-  w.kv_len = p.kv_lens ? min(max(p.kv_lens[w.b], 1), p.NK) : p.NK;
-  w.off = w.kv_len - p.N;
+  DkdvItemOf<MASK> w;
+  int NBQ = (p.N + kBlockM - 1) / kBlockM;   // query tiles
+  if constexpr (MASK == kMaskRagged) {
+    int place;
+    p.fd_per_place.divmod(idx, place, w.kvh);
+    const int4 seq = p.plan[2 * place];
+    w.j = p.plan[2 * place + 1].x;
+    w.b = 0;
+    w.q0 = seq.x, w.n_q = seq.y, w.k0 = seq.z, w.kv_len = seq.w;
+    w.off = p.causal ? w.kv_len - w.n_q : w.kv_len;  // not causal: as if every row were behind all keys
+    NBQ = (w.n_q + kBlockM - 1) / kBlockM;
+  } else {
+    int unit;
+    p.fd_unit.divmod(idx, unit, w.j);
+    p.fd_hkv.divmod(unit, w.b, w.kvh);
+    w.kv_len = p.kv_lens ? min(max(p.kv_lens[w.b], 1), p.NK) : p.NK;
+    w.off = w.kv_len - p.N;
+  }
   // causal: key c is seen by query rows r >= c - off; the first key of the block, j*128, is the one seen by most
   w.i_min = CAUSAL ? max(w.j * kBlockN - w.off, 0) / kBlockM : 0;
   [[maybe_unused]] int share = 0, of = 1;
@@ -587,7 +634,7 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
                      const BwdParams p) {
   using namespace ptx;
   constexpr int MASK = static_cast<int>(KIND);
-  constexpr bool CAUSAL = MASK != kMaskNone, WINDOW = MASK == kMaskWindow;
+  constexpr bool CAUSAL = MASK != kMaskNone, WINDOW = MASK == kMaskWindow, RAGGED = MASK == kMaskRagged;
   using SM = BwdSmem<D>;
   constexpr int kTile = SM::kTileBytes;
   constexpr int kSub = SM::kSubTileBytes;
@@ -657,6 +704,23 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   volatile uint32_t* abortp = abort_word;
   grid_dep_wait();
   grid_dep_launch();
+  [[maybe_unused]] int n_planned = 0, n_rounds = 0;
+  if constexpr (RAGGED) {
+    n_planned = *p.plan_count * p.per_place;
+    n_rounds = (n_planned + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
+  }
+  auto rounds = [&]() -> int {
+    if constexpr (RAGGED && !SPLIT) return n_rounds;
+    else return p.total_rounds;
+  };
+  auto item_of_round = [&](int round) -> int {
+    if constexpr (RAGGED) {
+      if constexpr (SPLIT) return planned_item(n_planned, round, p.fd_split.div(blockIdx.x), p.n_items);
+      else return planned_item(n_planned, round, blockIdx.x, gridDim.x);
+    } else {
+      return dkdv_item_for_round<MASK, SPLIT>(p, round);
+    }
+  };
   const int G = p.G;
   // TMEM columns: X [0,128) takes the two score-shaped products in turn, S^T(n) then dP^T(n), each free again as soon
   // as the element-wise warps hold it in registers; Y [128,256) holds the two bf16 operands, P^T in [128,192) and dS^T
@@ -691,10 +755,10 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     int trace_n = 0;
 #endif
     for (int round = 0; ok; ++round) {
-      if (round >= p.total_rounds) break;
-      const int idx = dkdv_item_for_round<MASK, SPLIT>(p, round);
+      if (round >= rounds()) break;
+      const int idx = item_of_round(round);
       if (idx < 0) continue;  // a partial round leaves some CTAs without an item
-      const DkdvItem w = decode_dkdv_item<MASK, SPLIT>(p, idx);
+      const DkdvItemOf<MASK> w = decode_dkdv_item<MASK, SPLIT>(p, idx);
       const bool pad_row = w.j * kBlockN + row >= w.kv_len;  // this key is padding (or lies beyond NK)
       const bool pad_block = (w.j + 1) * kBlockN > w.kv_len;  // uniform over the CTA: only such a block has padded keys
       if (w.n_iter == 0) {
@@ -702,9 +766,9 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         if (WINDOW && w.j < p.shared_blocks) continue;  // whoever adds the shares up writes them
         // nobody sees this key block (padding, or causal with every query before it): its gradients are zero and no
         // product was issued for it
-        if (w.j * kBlockN + row < p.NK) {
-          __nv_bfloat16* const dk = dk_row(p, w.b, w.j * kBlockN + row, w.kvh) + part * (D / kBwdParts);
-          __nv_bfloat16* const dv = dv_row(p, w.b, w.j * kBlockN + row, w.kvh) + part * (D / kBwdParts);
+        if (w.j * kBlockN + row < stored_keys(p, w)) {
+          __nv_bfloat16* const dk = dk_row(p, w.b, first_of_keys(w) + w.j * kBlockN + row, w.kvh) + part * (D / kBwdParts);
+          __nv_bfloat16* const dv = dv_row(p, w.b, first_of_keys(w) + w.j * kBlockN + row, w.kvh) + part * (D / kBwdParts);
 #pragma unroll
           for (int v = 0; v < D / kBwdParts / 8; ++v) {
             reinterpret_cast<uint4*>(dk)[v] = make_uint4(0, 0, 0, 0);
@@ -786,6 +850,12 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
 #pragma unroll
             for (int col = 0; col < kBwdPC; ++col) su[col] = (part * kBwdPC + col) < lim ? 0u : su[col];
           }
+          if constexpr (RAGGED) {
+            if (int rest = w.n_q - i_t * kBlockM - part * kBwdPC; rest < kBwdPC) {  // queries behind the sequence's last
+#pragma unroll
+              for (int col = 0; col < kBwdPC; ++col) su[col] = col < rest ? su[col] : 0u;
+            }
+          }
           if (pad_block) {
             // a padded key is seen by nobody: P^T and dS^T rows are zero, so are its dK and dV rows
 #pragma unroll
@@ -805,6 +875,16 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bars + DP_FREE);
+        if constexpr (RAGGED) {
+          if (const int rest = w.n_q - i_t * kBlockM; rest < kBlockM) {
+#pragma unroll
+            for (int col = 0; col < kBwdPC; ++col) du[col] = col < rest - part * kBwdPC ? du[col] : 0u;
+            // S^T and dP^T of the pair, which read the tiles, are complete; dV and dK are issued behind the arrivals below
+            zero_rows<D>(sQ + (it % RA) * kTile, rest, tid, 32 * kBwdCW);
+            zero_rows<D>(sDO + (it % RB) * kTile, rest, tid, 32 * kBwdCW);
+            fence_proxy_async();
+          }
+        }
         // ---- Y is free once dV and dK of the previous pair have consumed their operands (first pair ever: at once)
         ok = mbar_wait(bars + Y_FREE, (it & 1) ^ 1, abortp, kWaitLimitCycles);
         ok = __all_sync(0xffffffffu, ok);
@@ -876,8 +956,9 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         tc_fence_before();
         continue;
       }
-      const bool row_exists = w.j * kBlockN + row < p.NK;  // keys of a partial last block beyond NK are computed, not stored
-      const int key = w.j * kBlockN + row;
+      // keys of a partial last block beyond NK are computed, not stored
+      const bool row_exists = w.j * kBlockN + row < stored_keys(p, w);
+      const int key = first_of_keys(w) + w.j * kBlockN + row;
       bwd_store_part_row<D>(tmem + lane_addr + cDK + part * (D / kBwdParts),
                             dk_row(p, w.b, key, w.kvh) + part * (D / kBwdParts), p.scale, row_exists);
       bwd_store_part_row<D>(tmem + lane_addr + cDV + part * (D / kBwdParts),
@@ -888,9 +969,9 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       __syncwarp();
       cluster_arrive();
       cluster_wait();
-      if (ok) {
+      if (ok && (!RAGGED || item_of_round(0) >= 0)) {
         // every n-th row of the key block is added up here
-        const DkdvItem w = decode_dkdv_item<MASK, SPLIT>(p, dkdv_item_for_round<MASK, SPLIT>(p, 0));
+        const DkdvItemOf<MASK> w = decode_dkdv_item<MASK, SPLIT>(p, item_of_round(0));
         constexpr int kUnits = 2 * (D / 8);         // 8 columns each: dK, then dV
         for (int u = tid; w.n_iter > 0; u += 32 * kBwdCW) {
           const int r_row = w.rank + (u / kUnits) * p.split, unit = u % kUnits;
@@ -910,8 +991,8 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
               acc[h * 4 + 3] += x.w;
             }
           }
-          const int key = w.j * kBlockN + r_row;
-          if (key < p.NK) {
+          const int key = first_of_keys(w) + w.j * kBlockN + r_row;
+          if (w.j * kBlockN + r_row < stored_keys(p, w)) {
             __nv_bfloat16* const dst = (is_dv ? dv_row(p, w.b, key, w.kvh) : dk_row(p, w.b, key, w.kvh)) + c8 * 8;
             *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3]),
                                                         pack_bf16x2(acc[4], acc[5]), pack_bf16x2(acc[6], acc[7]));
@@ -935,10 +1016,10 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       uint32_t qa_par = 0, rb_par = 0;
       bool ok = true;
       for (int round = 0; ok; ++round) {
-        if (round >= p.total_rounds) break;
-        const int idx = dkdv_item_for_round<MASK, SPLIT>(p, round);
+        if (round >= rounds()) break;
+        const int idx = item_of_round(round);
         if (idx < 0) continue;  // a partial round leaves some CTAs without an item
-        const DkdvItem w = decode_dkdv_item<MASK, SPLIT>(p, idx);
+        const DkdvItemOf<MASK> w = decode_dkdv_item<MASK, SPLIT>(p, idx);
         if (w.n_first == w.n_end) continue;  // key block wholly beyond this batch element's length: nothing to do
         ok = mbar_wait(bars + KV_EMPTY, (item_cnt & 1) ^ 1, abortp, kWaitLimitCycles);
         if (!ok) break;
@@ -946,8 +1027,8 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
         mbar_expect_tx(bars + KV_FULL, 2 * kTile);
 #pragma unroll
         for (int ch = 0; ch < kChunks; ++ch) {
-          tma_load_4d(sK + ch * kSub, &tmap_k, bars + KV_FULL, ch * 64, w.kvh, w.j * kBlockN, w.b);
-          tma_load_4d(sV + ch * kSub, &tmap_v, bars + KV_FULL, ch * 64, w.kvh, w.j * kBlockN, w.b);
+          tma_load_4d(sK + ch * kSub, &tmap_k, bars + KV_FULL, ch * 64, w.kvh, first_of_keys(w) + w.j * kBlockN, w.b);
+          tma_load_4d(sV + ch * kSub, &tmap_v, bars + KV_FULL, ch * 64, w.kvh, first_of_keys(w) + w.j * kBlockN, w.b);
         }
         for (int n = w.n_first, g_rel = w.g_first, i_rel = w.i_first; n < w.n_end && ok; ++n) {
           const int head = w.kvh * G + g_rel;  // n / cnt_i and n % cnt_i, counted instead of divided
@@ -961,7 +1042,7 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
           mbar_expect_tx(bars + QA_FULL + qa, kTile);
 #pragma unroll
           for (int ch = 0; ch < kChunks; ++ch)
-            tma_load_4d(sQ + qa * kTile + ch * kSub, &tmap_q, bars + QA_FULL + qa, ch * 64, head, i * kBlockM, w.b);
+            tma_load_4d(sQ + qa * kTile + ch * kSub, &tmap_q, bars + QA_FULL + qa, ch * 64, head, first_query(w) + i * kBlockM, w.b);
           if (++qa == RA) {
             qa = 0;
             qa_par ^= 1;
@@ -971,7 +1052,7 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
           mbar_expect_tx(bars + RB_FULL + rb, kTile);
 #pragma unroll
           for (int ch = 0; ch < kChunks; ++ch)
-            tma_load_4d(sDO + rb * kTile + ch * kSub, &tmap_do, bars + RB_FULL + rb, ch * 64, head, i * kBlockM, w.b);
+            tma_load_4d(sDO + rb * kTile + ch * kSub, &tmap_do, bars + RB_FULL + rb, ch * 64, head, first_query(w) + i * kBlockM, w.b);
           if (++rb == RB) {
             rb = 0;
             rb_par ^= 1;
@@ -997,10 +1078,10 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       int trace_n = 0;
 #endif
       for (int round = 0; ok; ++round) {
-        if (round >= p.total_rounds) break;
-        const int idx = dkdv_item_for_round<MASK, SPLIT>(p, round);
+        if (round >= rounds()) break;
+        const int idx = item_of_round(round);
         if (idx < 0) continue;  // a partial round leaves some CTAs without an item
-        const DkdvItem w = decode_dkdv_item<MASK, SPLIT>(p, idx);
+        const DkdvItemOf<MASK> w = decode_dkdv_item<MASK, SPLIT>(p, idx);
         if (w.n_first == w.n_end) continue;  // key block wholly beyond this batch element's length: nothing to do
         ok = iss_wait(bars + KV_FULL, item_cnt & 1, abortp, kWaitLimitCycles);
         if (!ok) break;
@@ -1058,10 +1139,10 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       int trace_n = 0;
 #endif
       for (int round = 0; ok; ++round) {
-        if (round >= p.total_rounds) break;
-        const int idx = dkdv_item_for_round<MASK, SPLIT>(p, round);
+        if (round >= rounds()) break;
+        const int idx = item_of_round(round);
         if (idx < 0) continue;  // a partial round leaves some CTAs without an item
-        const DkdvItem w = decode_dkdv_item<MASK, SPLIT>(p, idx);
+        const DkdvItemOf<MASK> w = decode_dkdv_item<MASK, SPLIT>(p, idx);
         if (w.n_first == w.n_end) continue;  // key block wholly beyond this batch element's length: nothing to do
         for (int n = w.n_first; n < w.n_end && ok; ++n, ++it) {
           ok = iss_wait(bars + P_FULL, it & 1, abortp, kWaitLimitCycles) &&
@@ -1114,24 +1195,24 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       uint32_t it = 0;
       bool ok = true;
       float lv[kBlockM / 32], dv_[kBlockM / 32];
-      auto fetch = [&](const DkdvItem& w, int n) {
+      auto fetch = [&](const DkdvItemOf<MASK>& w, int n) {
         const int head = w.kvh * G + n / w.cnt_i;
         const int i = w.i_min + n % w.cnt_i;
-        const size_t base = (static_cast<size_t>(w.b) * p.H + head) * p.N;
+        const size_t base = stats_row(p, w, head);
 #pragma unroll
         for (int t = 0; t < kBlockM / 32; ++t) {
           const int pos = i * kBlockM + t * 32 + lane;
-          const bool in = pos < p.N;
+          const bool in = pos < queries(p, w);
           // stored ready for use: -L * log2(e) is the addend of the exponent, -delta the addend of dP
           lv[t] = in ? p.lse[base + pos] * -1.4426950408889634f : 0.f;
           dv_[t] = in ? -p.delta[base + pos] : 0.f;
         }
       };
       for (int round = 0; ok; ++round) {
-        if (round >= p.total_rounds) break;
-        const int idx = dkdv_item_for_round<MASK, SPLIT>(p, round);
+        if (round >= rounds()) break;
+        const int idx = item_of_round(round);
         if (idx < 0) continue;  // a partial round leaves some CTAs without an item
-        const DkdvItem w = decode_dkdv_item<MASK, SPLIT>(p, idx);
+        const DkdvItemOf<MASK> w = decode_dkdv_item<MASK, SPLIT>(p, idx);
         if (w.n_first == w.n_end) continue;  // key block wholly beyond this batch element's length: nothing to do
         fetch(w, w.n_first);
         for (int n = w.n_first; n < w.n_end && ok; ++n, ++it) {
@@ -1216,8 +1297,19 @@ struct DqItem {
 struct DqWindowItem : DqItem {
   int sink_tiles, skip;
 };
+// Ragged: as RaggedItem of the forward. A sequence's last tile of keys is loaded with rows of the next one behind them: their dS is masked,
+// and K's rows are zeroed in shared memory before the product that sums over them.
+struct DqRaggedItem : DqItem {
+  int q0, n_q, k0;
+};
 template <int MASK>
-using DqItemOf = std::conditional_t<MASK == kMaskWindow, DqWindowItem, DqItem>;
+using DqItemOf = std::conditional_t<MASK == kMaskWindow, DqWindowItem, std::conditional_t<MASK == kMaskRagged, DqRaggedItem, DqItem>>;
+__device__ __forceinline__ int dq_queries(const BwdParams& p, const DqItem&) { return p.N; }
+__device__ __forceinline__ int dq_queries(const BwdParams&, const DqRaggedItem& w) { return w.n_q; }
+__device__ __forceinline__ int dq_query0(const DqItem&) { return 0; }
+__device__ __forceinline__ int dq_query0(const DqRaggedItem& w) { return w.q0; }
+__device__ __forceinline__ int dq_key0(const DqItem&) { return 0; }
+__device__ __forceinline__ int dq_key0(const DqRaggedItem& w) { return w.k0; }
 __device__ __forceinline__ int dq_tile(const DqItem&, int n) { return n; }
 __device__ __forceinline__ int dq_tile(const DqWindowItem& w, int n) { return n >= w.sink_tiles ? n + w.skip : n; }
 
@@ -1230,7 +1322,16 @@ __device__ __forceinline__ DqItemOf<MASK> decode_dq_item(const BwdParams& p, int
   const int NB = (p.N + kBlockM - 1) / kBlockM;  // the last tile may be partial
   const int G = p.G;
   int unit, g;
-  if (MASK == kMaskCausal || (MASK == kMaskWindow && p.longest_first)) {
+  if constexpr (MASK == kMaskRagged) {
+    int place;
+    p.fd_per_place.divmod(idx, place, w.h);
+    const int4 seq = ptx::ld_gpu(p.plan + 2 * place);
+    w.i = ptx::ld_gpu(p.plan + 2 * place + 1).x;
+    w.b = unit = g = 0;
+    w.kvh = p.fd_inner.div(w.h);
+    w.q0 = seq.x, w.n_q = seq.y, w.k0 = seq.z, w.kv_len = seq.w;
+    w.off = p.causal ? w.kv_len - w.n_q : w.kv_len;
+  } else if (MASK == kMaskCausal || (MASK == kMaskWindow && p.longest_first)) {
     const int grp = min(p.fd_group.div(idx), p.last_group);
     const int within = idx - grp * p.group_items;
     int qd, rem;
@@ -1245,10 +1346,12 @@ __device__ __forceinline__ DqItemOf<MASK> decode_dq_item(const BwdParams& p, int
     p.fd_unit.divmod(idx, unit, rem);
     p.fd_inner.divmod(rem, g, w.i);
   }
-  p.fd_hkv.divmod(unit, w.b, w.kvh);
-  w.h = w.kvh * G + g;
-  w.kv_len = p.kv_lens ? min(max(ptx::ld_gpu(p.kv_lens + w.b), 1), p.NK) : p.NK;
-  w.off = w.kv_len - p.N;
+  if constexpr (MASK != kMaskRagged) {
+    p.fd_hkv.divmod(unit, w.b, w.kvh);
+    w.h = w.kvh * G + g;
+    w.kv_len = p.kv_lens ? min(max(ptx::ld_gpu(p.kv_lens + w.b), 1), p.NK) : p.NK;
+    w.off = w.kv_len - p.N;
+  }
   const int n_kv = (w.kv_len + kBlockN - 1) / kBlockN;
   // causal: the last row of the tile sees keys up to i*128 + 127 + off
   w.n_iter = CAUSAL ? min(max((w.i * kBlockM + kBlockM + w.off + kBlockN - 1) / kBlockN, 0), n_kv) : n_kv;
@@ -1268,7 +1371,7 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
                    const BwdParams p) {
   using namespace ptx;
   constexpr int MASK = static_cast<int>(KIND);
-  constexpr bool CAUSAL = MASK != kMaskNone, WINDOW = MASK == kMaskWindow;
+  constexpr bool CAUSAL = MASK != kMaskNone, WINDOW = MASK == kMaskWindow, RAGGED = MASK == kMaskRagged;
   using SM = BwdSmem<D>;
   constexpr int kTile = SM::kTileBytes;
   constexpr int kSub = SM::kSubTileBytes;
@@ -1332,6 +1435,19 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
   // The wait for the dK/dV kernel is the last thing a CTA does, so that who waits for this kernel waits for both.
   if (p.dq_waits) grid_dep_wait();
   grid_dep_launch();
+  [[maybe_unused]] int n_planned = 0, n_rounds = 0;
+  if constexpr (RAGGED) {
+    n_planned = ld_gpu(p.plan_count) * p.per_place;
+    n_rounds = (n_planned + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
+  }
+  auto rounds = [&]() -> int {
+    if constexpr (RAGGED) return n_rounds;
+    else return p.total_rounds;
+  };
+  auto item_of_round = [&](int round) -> int {
+    if constexpr (RAGGED) return planned_item(n_planned, round, blockIdx.x, gridDim.x);
+    else return item_for_round(p, round, blockIdx.x, gridDim.x);
+  };
   // TMEM columns: S [0,128)  dP [128,256)  dQ [256,256+D)  dS (bf16, 64 packed columns) [384,448).
   // Nothing aliases: S and dP are free for the next tile as soon as they are in registers.
   constexpr uint32_t cS = 0, cDP = 128, cDQ = 256, cDS = 384;
@@ -1353,16 +1469,16 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
     int trace_n = 0;
 #endif
     for (int round = 0; ok; ++round) {
-      if (round >= p.total_rounds) break;
-      const int idx = item_for_round(p, round, blockIdx.x, gridDim.x);
+      if (round >= rounds()) break;
+      const int idx = item_of_round(round);
       if (idx < 0) continue;  // a partial round leaves some CTAs without an item
       const DqItemOf<MASK> w = decode_dq_item<MASK>(p, idx);
-      const size_t srow = (static_cast<size_t>(w.b) * p.H + w.h) * p.N + static_cast<size_t>(w.i) * kBlockM + row;
-      const bool row_exists = w.i * kBlockM + row < p.N;  // rows of a partial last tile beyond N: zero statistics
+      const size_t srow = (static_cast<size_t>(w.b) * p.H + w.h) * p.N + dq_query0(w) + static_cast<size_t>(w.i) * kBlockM + row;
+      const bool row_exists = w.i * kBlockM + row < dq_queries(p, w);  // rows of a partial last tile beyond N: zero statistics
       if (w.n_iter == 0) {
         // causal with more queries than kept keys: no row of this tile sees a key, dQ = 0 and no product is issued
         if (row_exists) {
-          __nv_bfloat16* dst0 = p.dq + w.b * p.dq_stride_b + (static_cast<long long>(w.i) * kBlockM + row) * p.dq_stride_n +
+          __nv_bfloat16* dst0 = p.dq + w.b * p.dq_stride_b + (dq_query0(w) + static_cast<long long>(w.i) * kBlockM + row) * p.dq_stride_n +
                                 w.h * p.dq_stride_h + part * (D / kBwdParts);
 #pragma unroll
           for (int v = 0; v < D / kBwdParts / 8; ++v) reinterpret_cast<uint4*>(dst0)[v] = make_uint4(0, 0, 0, 0);
@@ -1447,6 +1563,14 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(bars + DP_FREE);  // issuer B may overwrite dP with the next tile's
+          if constexpr (RAGGED) {
+            if (const int rest = w.kv_len - kv * kBlockN; rest < kBlockN) {  // keys behind the sequence's last
+#pragma unroll
+              for (int col = 0; col < kBwdPC; ++col) du[col] = col < rest - part * kBwdPC ? du[col] : 0u;
+              zero_rows<D>(sK + (it % RA) * kTile, rest, tid, 32 * kBwdCW);  // S, which read the tile, is complete
+              fence_proxy_async();
+            }
+          }
           const uint64_t ndl2 = pack2(-dl, -dl);
 #pragma unroll
           for (int i = 0; i < kBwdPC / 2; ++i) {
@@ -1476,7 +1600,7 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       if (!ok) break;
       ++dq_cnt;
       tc_fence_after();
-      __nv_bfloat16* dst = p.dq + w.b * p.dq_stride_b + (static_cast<long long>(w.i) * kBlockM + row) * p.dq_stride_n +
+      __nv_bfloat16* dst = p.dq + w.b * p.dq_stride_b + (dq_query0(w) + static_cast<long long>(w.i) * kBlockM + row) * p.dq_stride_n +
                            w.h * p.dq_stride_h + part * (D / kBwdParts);
       bwd_store_part_row<D>(tmem + lane_addr + cDQ + part * (D / kBwdParts), dst, p.scale, row_exists);
       tc_fence_before();  // orders these reads before the next item's first dQ product (published through DS_FULL)
@@ -1494,8 +1618,8 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       uint32_t ka_par = 0, vb_par = 0;
       bool ok = true;
       for (int round = 0; ok; ++round) {
-        if (round >= p.total_rounds) break;
-        const int idx = item_for_round(p, round, blockIdx.x, gridDim.x);
+        if (round >= rounds()) break;
+        const int idx = item_of_round(round);
         if (idx < 0) continue;  // a partial round leaves some CTAs without an item
         const DqItemOf<MASK> w = decode_dq_item<MASK>(p, idx);
         if (w.n_iter == 0) continue;  // no row of this tile sees a key: nothing is loaded or issued
@@ -1505,8 +1629,8 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         mbar_expect_tx(bars + QDO_FULL, 2 * kTile);
 #pragma unroll
         for (int ch = 0; ch < kChunks; ++ch) {
-          tma_load_4d(sQ + ch * kSub, &tmap_q, bars + QDO_FULL, ch * 64, w.h, w.i * kBlockM, w.b);
-          tma_load_4d(sDO + ch * kSub, &tmap_do, bars + QDO_FULL, ch * 64, w.h, w.i * kBlockM, w.b);
+          tma_load_4d(sQ + ch * kSub, &tmap_q, bars + QDO_FULL, ch * 64, w.h, dq_query0(w) + w.i * kBlockM, w.b);
+          tma_load_4d(sDO + ch * kSub, &tmap_do, bars + QDO_FULL, ch * 64, w.h, dq_query0(w) + w.i * kBlockM, w.b);
         }
         for (int n = 0; n < w.n_iter && ok; ++n) {
           ok = mbar_wait(bars + KA_EMPTY + ka, ka_par ^ 1, abortp, kWaitLimitCycles);
@@ -1514,7 +1638,7 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           mbar_expect_tx(bars + KA_FULL + ka, kTile);
 #pragma unroll
           for (int ch = 0; ch < kChunks; ++ch)
-            tma_load_4d(sK + ka * kTile + ch * kSub, &tmap_k, bars + KA_FULL + ka, ch * 64, w.kvh, dq_tile(w, n) * kBlockN, w.b);
+            tma_load_4d(sK + ka * kTile + ch * kSub, &tmap_k, bars + KA_FULL + ka, ch * 64, w.kvh, dq_key0(w) + dq_tile(w, n) * kBlockN, w.b);
           if (++ka == RA) {
             ka = 0;
             ka_par ^= 1;
@@ -1524,7 +1648,7 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
           mbar_expect_tx(bars + VB_FULL + vb, kTile);
 #pragma unroll
           for (int ch = 0; ch < kChunks; ++ch)
-            tma_load_4d(sV + vb * kTile + ch * kSub, &tmap_v, bars + VB_FULL + vb, ch * 64, w.kvh, dq_tile(w, n) * kBlockN, w.b);
+            tma_load_4d(sV + vb * kTile + ch * kSub, &tmap_v, bars + VB_FULL + vb, ch * 64, w.kvh, dq_key0(w) + dq_tile(w, n) * kBlockN, w.b);
           if (++vb == RB) {
             vb = 0;
             vb_par ^= 1;
@@ -1547,8 +1671,8 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
       int trace_n = 0;
 #endif
       for (int round = 0; ok; ++round) {
-        if (round >= p.total_rounds) break;
-        const int idx = item_for_round(p, round, blockIdx.x, gridDim.x);
+        if (round >= rounds()) break;
+        const int idx = item_of_round(round);
         if (idx < 0) continue;  // a partial round leaves some CTAs without an item
         const DqItemOf<MASK> w = decode_dq_item<MASK>(p, idx);
         if (w.n_iter == 0) continue;  // no row of this tile sees a key: nothing is loaded or issued
@@ -1606,8 +1730,8 @@ attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_cons
         return true;
       };
       for (int round = 0; ok; ++round) {
-        if (round >= p.total_rounds) break;
-        const int idx = item_for_round(p, round, blockIdx.x, gridDim.x);
+        if (round >= rounds()) break;
+        const int idx = item_of_round(round);
         if (idx < 0) continue;  // a partial round leaves some CTAs without an item
         const DqItemOf<MASK> w = decode_dq_item<MASK>(p, idx);
         if (w.n_iter == 0) continue;  // no row of this tile sees a key: nothing is loaded or issued

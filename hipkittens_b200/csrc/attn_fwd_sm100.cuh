@@ -84,8 +84,10 @@ constexpr uint64_t kWaitLimitCycles = 8000ull * 1000 * 1000;  // SM cycles, > 4 
 enum : int { kStatusOk = 0, kStatusTimeout = 1, kStatusFwdBadPage = 2 };  // 2 = the decode kernels' kStatusBadPage
 
 // What a query row sees: every key, those up to its own position, or of those the last `window` and the first `sinks`.
-// Where a template takes `auto KIND` it is false, true or kMaskWindow: whether a call is causal, which a call with a window is too.
-enum Mask : int { kMaskNone = 0, kMaskCausal = 1, kMaskWindow = 2 };
+// Where a template takes `auto KIND` it is false, true, kMaskWindow or kMaskRagged: whether a call is causal, which a call with a window is
+// too.
+// A ragged call has its batch elements one after the other, each with lengths of its own, causal or not (see RaggedItem).
+enum Mask : int { kMaskNone = 0, kMaskCausal = 1, kMaskWindow = 2, kMaskRagged = 3 };
 
 // Division of a non-negative int below 2^31 by a divisor fixed at launch: a multiply-high and a shift instead of the
 // ~40 dependent instructions of a 32-bit division. The work-item decode below divides ten times per item, on the
@@ -148,6 +150,12 @@ struct FwdParams {
 #ifdef HK_TRACE
   long long* trace;     // [3 roles][4096] clock stamps of CTA 0 (debug builds only)
 #endif
+  // kMaskRagged: B = 1, N and NK are the rows of q and of k in all; what the plan kernel of the call has listed, and the items of a place
+  // in that list: K/V heads x slot pairs inside a group
+  const int* plan_count;
+  const int4* plan;
+  int per_place, causal;
+  FastDiv fd_per_place;
 };
 
 template <int D, bool CAUSAL>
@@ -178,8 +186,30 @@ struct WindowItem : WorkItem {
   int sink_tiles, skip;
   int first_key;  // of the item's windows
 };
+// Ragged: the sequence that an item belongs to has the rows q0 ... of q and k0 ... of k, and tiles are counted from there. Tiles that run
+// over its end are loaded with rows of the next one, whatever these hold: products' rows of queries behind the end are not stored; keys
+// behind it are masked, and V's rows there are zeroed in shared memory before their product, since 0 times a NaN is one.
+struct RaggedItem : WorkItem {
+  int q0, n_q, k0;
+};
 template <int MASK>
-using ItemOf = std::conditional_t<MASK == kMaskWindow, WindowItem, WorkItem>;
+using ItemOf = std::conditional_t<MASK == kMaskWindow, WindowItem, std::conditional_t<MASK == kMaskRagged, RaggedItem, WorkItem>>;
+__device__ __forceinline__ int query_rows(const FwdParams& p, const WorkItem&) { return p.N; }
+__device__ __forceinline__ int query_rows(const FwdParams&, const RaggedItem& w) { return w.n_q; }
+// The row of q and O that a row of the item's sequence is, and its place in L.
+__device__ __forceinline__ size_t query_row(const FwdParams& p, const WorkItem& w, int row) { return static_cast<size_t>(w.b) * p.N + row; }
+__device__ __forceinline__ size_t query_row(const FwdParams&, const RaggedItem& w, int row) { return static_cast<size_t>(w.q0) + row; }
+__device__ __forceinline__ size_t lse_place(const FwdParams& p, const WorkItem& w, int head, int row) {
+  return (static_cast<size_t>(w.b) * p.H + head) * p.N + row;
+}
+__device__ __forceinline__ size_t lse_place(const FwdParams& p, const RaggedItem& w, int head, int row) {
+  return static_cast<size_t>(head) * p.N + w.q0 + row;
+}
+// Row coordinates of tiles.
+__device__ __forceinline__ int q_coord(const WorkItem&, int qb) { return qb * kBlockM; }
+__device__ __forceinline__ int q_coord(const RaggedItem& w, int qb) { return w.q0 + qb * kBlockM; }
+__device__ __forceinline__ int k_coord(const WorkItem&, int tile) { return tile * kBlockN; }
+__device__ __forceinline__ int k_coord(const RaggedItem& w, int tile) { return w.k0 + tile * kBlockN; }
 // The tile of keys at place j of a slot's list.
 __device__ __forceinline__ int kv_tile(const WorkItem&, int j) { return j; }
 __device__ __forceinline__ int kv_tile(const WindowItem& w, int j) { return j >= w.sink_tiles ? j + w.skip : j; }
@@ -197,12 +227,22 @@ __device__ __forceinline__ ItemOf<MASK> decode_item(const FwdParams& p, int idx)
   constexpr bool CAUSAL = MASK != kMaskNone;
   ItemOf<MASK> w;
   const int G = p.G;
-  const int NQB = p.nqb;  // the last block may be partial
+  int NQB = p.nqb;  // the last block may be partial
   // an item is (unit, q position, pair inside the group); a q position is a q tile (two heads per item) or a pair
   // of q tiles (one head per item), of which there are nq per unit
   const int nq = p.pair_heads ? NQB : (NQB + 1) / 2;
   int unit, qx, hx;
-  if (MASK == kMaskCausal || (MASK == kMaskWindow && p.longest_first)) {
+  if constexpr (MASK == kMaskRagged) {
+    int place, rem;
+    p.fd_per_place.divmod(idx, place, rem);
+    const int4 seq = p.plan[2 * place];
+    qx = p.plan[2 * place + 1].x;
+    p.fd_inner.divmod(rem, w.kvh, hx);
+    w.b = unit = 0;
+    w.q0 = seq.x, w.n_q = seq.y, w.k0 = seq.z, w.kv_len = seq.w;
+    w.off = p.causal ? w.kv_len - w.n_q : w.kv_len;  // not causal: as if every row were behind all keys
+    NQB = (w.n_q + kBlockM - 1) / kBlockM;
+  } else if (MASK == kMaskCausal || (MASK == kMaskWindow && p.longest_first)) {
     const int grp = min(p.fd_group_items.div(idx), p.last_group);
     const int within = idx - grp * p.group_items;
     int qd, rem;
@@ -227,14 +267,16 @@ __device__ __forceinline__ ItemOf<MASK> decode_item(const FwdParams& p, int idx)
     qb1 = 2 * qx + 1;
     h0 = h1 = hx;
   }
-  p.fd_hkv.divmod(unit, w.b, w.kvh);
+  if constexpr (MASK != kMaskRagged) p.fd_hkv.divmod(unit, w.b, w.kvh);
   w.head[0] = w.kvh * G + h0;
   w.head[1] = w.kvh * G + h1;
   w.qb[0] = qb0;
   w.qb[1] = qb1;
   // key-padding lengths: tiles beyond the batch element's own length are never loaded
-  w.kv_len = p.kv_lens ? min(max(p.kv_lens[w.b], 1), p.NK) : p.NK;
-  w.off = w.kv_len - p.N;
+  if constexpr (MASK != kMaskRagged) {
+    w.kv_len = p.kv_lens ? min(max(p.kv_lens[w.b], 1), p.NK) : p.NK;
+    w.off = w.kv_len - p.N;
+  }
   const int n_kv = (w.kv_len + kBlockN - 1) / kBlockN;
   // causal: the last row of query block qb sees keys up to qb*128 + 127 + off; a block none of whose rows sees a
   // key gets no tiles (its rows are written as O = 0, L = -inf by the softmax warps)
@@ -266,6 +308,12 @@ __device__ __forceinline__ int item_for_round(const Params& p, int round, int ct
   const int first = grp * p.group_items;
   const int in_grp = r * n_cta + (((r + grp) & 1) ? (n_cta - 1 - cta) : cta);
   return (in_grp < min(p.group_items, p.n_items - first)) ? first + in_grp : -1;
+}
+
+// The same for the `n` items that a plan kernel has listed, the longest first.
+__device__ __forceinline__ int planned_item(int n, int round, int cta, int n_cta) {
+  const int idx = round * n_cta + ((round & 1) ? n_cta - 1 - cta : cta);
+  return idx < n ? idx : -1;
 }
 
 // Host side: fills the fields the item decode reads. Call after B, N, H, H_KV, pair_heads, group_units, group_items
@@ -330,7 +378,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
                 const FwdParams p) {
   using namespace ptx;
   constexpr int MASK = static_cast<int>(KIND);
-  constexpr bool CAUSAL = MASK != kMaskNone, WINDOW = MASK == kMaskWindow;
+  constexpr bool CAUSAL = MASK != kMaskNone, WINDOW = MASK == kMaskWindow, RAGGED = MASK == kMaskRagged;
   using SM = FwdSmem<D, CAUSAL>;
   constexpr int kStages = SM::kStages;
   constexpr int kTile = SM::kTileBytes;
@@ -348,7 +396,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
   constexpr int kOtherRegs = (D == 64 && !CAUSAL) ? 72 : 88;
   static_assert(8 * kSoftmaxRegs + 4 * kOtherRegs == 12 * kFwdRegsAtLaunch, "registers taken = registers released");
   constexpr int kEmuMod = (D == 64 && !CAUSAL) ? HK_EMU_MOD_D64_NONCAUSAL : HK_EMU_MOD;
-  constexpr int kEmuCnt = WINDOW ? 0 : (D == 64) ? (CAUSAL ? HK_EMU_CNT_D64 : HK_EMU_CNT_D64_NONCAUSAL) : HK_EMU_CNT_D128;
+  constexpr int kEmuCnt = WINDOW || RAGGED ? 0 : (D == 64) ? (CAUSAL ? HK_EMU_CNT_D64 : HK_EMU_CNT_D64_NONCAUSAL) : HK_EMU_CNT_D128;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -412,6 +460,24 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
     grid_dep_wait();
     grid_dep_launch();
   }
+  // Ragged: the planned items and their rounds. In shared memory, and the items looked up again where an epilogue needs them, because the
+  // softmax warps have no registers left for what lives through an item's loop.
+  __shared__ int planned[RAGGED ? 2 : 1];
+  if constexpr (RAGGED) {
+    if (tid == 0) {
+      planned[0] = *p.plan_count * p.per_place;
+      planned[1] = (planned[0] + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
+    }
+    __syncthreads();
+  }
+  auto rounds = [&]() -> int {
+    if constexpr (RAGGED) return *static_cast<volatile int*>(&planned[1]);
+    else return p.total_rounds;
+  };
+  auto item_of_round = [&](int round) -> int {
+    if constexpr (RAGGED) return planned_item(*static_cast<volatile int*>(&planned[0]), round, blockIdx.x, gridDim.x);
+    else return item_for_round(p, round, blockIdx.x, gridDim.x);
+  };
 
   if (warp < 8) {
     // ------------------------------------------------------------------ softmax warpgroups
@@ -424,6 +490,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
     const uint32_t tP = kSepP ? tmem + lane_addr + 384 + slot * 64 : tS;  // bf16 P: 64 packed columns
     const float c = p.scale_log2;
     uint32_t s_cnt = 0, o_cnt = 0, pv_cnt = 0;
+    [[maybe_unused]] uint32_t kv_pos = 0;  // ragged: ring tiles of the items before this one
     // Staging buffer of this slot and the number of times it has been used before the current item. With one
     // buffer for both slots its uses are ordered: item by item, and inside an item the slot with fewer K/V tiles
     // (which finishes first) before the other; both slots and the store warp derive that order from the item.
@@ -433,8 +500,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
     int trace_n = 0;
 #endif
     for (int round = 0; ok; ++round) {
-      if (round >= p.total_rounds) break;
-      const int idx = item_for_round(p, round, blockIdx.x, gridDim.x);
+      if (round >= rounds()) break;
+      const int idx = item_of_round(round);
       if (idx < 0) continue;  // a partial round leaves some CTAs without an item
       const ItemOf<MASK> w = decode_item<MASK>(p, idx);
       const int nkv = w.n[slot];
@@ -463,18 +530,21 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
         select([&](int base) { return seen_bits(base, lo, hi, p.sinks - first); });
       };
       if (nkv == 0) {
-        if (CAUSAL && w.qb[slot] * kBlockM < p.N) {
+        if (CAUSAL && w.qb[slot] * kBlockM < query_rows(p, w)) {
           // a query block that sees no key at all (more queries than keys): defined output, no products
           const int qrow = w.qb[slot] * kBlockM + row;
-          if (qrow < p.N) {
-            uint4* dst = reinterpret_cast<uint4*>(p.o + ((static_cast<size_t>(w.b) * p.N + qrow) * p.H + w.head[slot]) * D);
+          if (qrow < query_rows(p, w)) {
+            uint4* dst = reinterpret_cast<uint4*>(p.o + (query_row(p, w, qrow) * p.H + w.head[slot]) * D);
 #pragma unroll
             for (int v4 = 0; v4 < D / 8; ++v4) dst[v4] = make_uint4(0u, 0u, 0u, 0u);
-            p.lse[(static_cast<size_t>(w.b) * p.H + w.head[slot]) * p.N + qrow] = -INFINITY;
+            p.lse[lse_place(p, w, w.head[slot], qrow)] = -INFINITY;
           }
         }
+        if constexpr (RAGGED) kv_pos += 2 * max(w.n[0], w.n[1]);
         continue;
       }
+      // V's rows from here on become zeros, by the first slot whose product reads their tile (the other's is issued behind it)
+      [[maybe_unused]] const int zeros_from = slot == 0 || nkv > w.n[0] ? w.kv_len : 0x7fffffff;
       float m = 0.f, l = 0.f;
       for (int j = 0; j < nkv && ok; ++j) {
         HK_STAMP2(slot, 0);
@@ -738,6 +808,18 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
 #undef HK_S
         }
         HK_STAMP2(slot, 4);
+        if constexpr (RAGGED) {
+          if ((j + 1) * kBlockN > zeros_from) {
+            const uint32_t at = kv_pos + 2 * j + 1;
+            ok = mbar_wait(&kv_full[at % kStages], (at / kStages) & 1, abortp, kWaitLimitCycles);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            uint8_t* const v_tile = sKV + (at % kStages) * kTile;
+            for (int r = zeros_from - j * kBlockN + (warp & 3); r < kBlockN; r += 4)
+              if (lane < D / 8) *reinterpret_cast<uint4*>(v_tile + (lane >> 3) * kSub + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+            fence_proxy_async();  // visible to the product that reads the tile
+          }
+        }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -745,6 +827,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
         HK_STAMP(slot, 5);
       }
       if (!ok) break;
+      if constexpr (RAGGED) kv_pos += 2 * max(w.n[0], w.n[1]);
       // ---- epilogue of this slot: O / l -> bf16, L = m*scale + ln(l)
       ok = mbar_wait(&o_full[slot], o_cnt & 1, abortp, kWaitLimitCycles);
       ok = __all_sync(0xffffffffu, ok);
@@ -752,9 +835,14 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
       ++o_cnt;
       tc_fence_after();
       const float inv_l = (CAUSAL && l == 0.f) ? 0.f : 1.0f / l;  // l = 0: a row that sees no key gets O = 0, L = -inf
-      const int qrow = w.qb[slot] * kBlockM + row;
-      const int head = w.head[slot];
-      const bool row_exists = qrow < p.N;  // rows of a partial last block beyond N are computed but not stored
+      auto again = [&]() -> decltype(auto) {
+        if constexpr (RAGGED) return decode_item<MASK>(p, item_of_round(round));
+        else return (w);
+      };
+      const auto& e = again();
+      const int qrow = e.qb[slot] * kBlockM + row;
+      const int head = e.head[slot];
+      const bool row_exists = qrow < query_rows(p, e);  // rows of a partial last block beyond N are computed but not stored
       // O leaves through shared memory: a thread's row goes into the staging tile in the 128-byte-swizzled layout
       // (conflict-free 16-byte stores) and the store warp sends the tile to global memory as TMA boxes, which write
       // whole 128-byte lines and clip the rows beyond N. (Storing from registers, each thread its own row, touched
@@ -798,7 +886,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
         }
       } else if constexpr (!kTmaOut) {
         // straight from registers, 32 bytes per store where the tensor allows it
-        __nv_bfloat16* orow = p.o + ((static_cast<size_t>(w.b) * p.N + qrow) * p.H + head) * D;
+        __nv_bfloat16* orow = p.o + (query_row(p, e, qrow) * p.H + head) * D;
         const bool wide = (reinterpret_cast<uintptr_t>(p.o) & 31) == 0;  // rows are multiples of 128 bytes apart
 #pragma unroll
         for (int cc = 0; cc < D / 32; ++cc) {
@@ -850,7 +938,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
         if (lane == 0) mbar_arrive(&so_full[slot]);
       }
       if (row_exists)
-        p.lse[(static_cast<size_t>(w.b) * p.H + head) * p.N + qrow] =
+        p.lse[lse_place(p, e, head, qrow)] =
             (CAUSAL && l == 0.f) ? -INFINITY : m * p.scale + __logf(l);
       // order this slot's TMEM reads before the next item's PV (published through p_full)
       tc_fence_before();
@@ -874,7 +962,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
         int ring_st = 0;        // next ring stage to fill
         uint32_t ring_par = 0;  // its phase parity
         bool ok = true;
-        auto push_kv = [&](const CUtensorMap* tm, int b, int kvh, int tile, int kv_len, [[maybe_unused]] int first_key) -> bool {
+        auto push_kv = [&](const CUtensorMap* tm, int b, int kvh, int row, int tile, int kv_len, [[maybe_unused]] int first_key) -> bool {
           const int st = ring_st;
           bool good = true;
           if (lane == 0) {
@@ -887,7 +975,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
           if (!kPaged) {
 #pragma unroll
             for (int ch = 0; ch < kChunks; ++ch)
-              tma_load_4d(dst + ch * kSub, tm, &kv_full[st], ch * 64, kvh, tile * kBlockN, b);
+              tma_load_4d(dst + ch * kSub, tm, &kv_full[st], ch * 64, kvh, row, b);
           } else if (lane < kBlockN / 16) {
             // the tile's 128 keys are 8 pages of 16, one lane and one 16-row box each. Pages beyond the context
             // repeat its last page, so that every row of the tile holds cache contents (those keys are masked; their
@@ -915,14 +1003,14 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
           return true;
         };
         for (int round = 0; ok; ++round) {
-          if (round >= p.total_rounds) break;
-          const int idx = item_for_round(p, round, blockIdx.x, gridDim.x);
+          if (round >= rounds()) break;
+          const int idx = item_of_round(round);
           if (idx < 0) continue;
           const ItemOf<MASK> w = decode_item<MASK>(p, idx);
           const int nmax = max(w.n[0], w.n[1]);
           // the first K tile is requested before the Q tiles: the stage it goes to is free two K/V tiles before the
           // previous item ends, the Q tiles only when that item's last Q K^T has been issued
-          if (nmax > 0) ok = push_kv(&tmap_k, w.b, w.kvh, kv_tile(w, 0), w.kv_len, first_key(w));
+          if (nmax > 0) ok = push_kv(&tmap_k, w.b, w.kvh, k_coord(w, kv_tile(w, 0)), kv_tile(w, 0), w.kv_len, first_key(w));
           if (!kQThread && lane == 0 && ok) {
             for (int s = 0; s < 2 && ok; ++s) {
               if (w.n[s] == 0) continue;
@@ -932,14 +1020,14 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
               mbar_expect_tx(&q_full[s], kTile);
 #pragma unroll
               for (int ch = 0; ch < kChunks; ++ch)
-                tma_load_4d(sQ + s * kTile + ch * kSub, &tmap_q, &q_full[s], ch * 64, w.head[s], w.qb[s] * kBlockM,
+                tma_load_4d(sQ + s * kTile + ch * kSub, &tmap_q, &q_full[s], ch * 64, w.head[s], q_coord(w, w.qb[s]),
                             w.b);
             }
           }
           if (kPaged) ok = __shfl_sync(0xffffffffu, ok, 0);
           for (int j = 0; j < nmax && ok; ++j) {
-            ok = push_kv(&tmap_v, w.b, w.kvh, kv_tile(w, j), w.kv_len, first_key(w));
-            if (ok && j + 1 < nmax) ok = push_kv(&tmap_k, w.b, w.kvh, kv_tile(w, j + 1), w.kv_len, first_key(w));
+            ok = push_kv(&tmap_v, w.b, w.kvh, k_coord(w, kv_tile(w, j)), kv_tile(w, j), w.kv_len, first_key(w));
+            if (ok && j + 1 < nmax) ok = push_kv(&tmap_k, w.b, w.kvh, k_coord(w, kv_tile(w, j + 1)), kv_tile(w, j + 1), w.kv_len, first_key(w));
           }
         }
       };
@@ -962,8 +1050,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
       uint32_t q_par[2] = {0, 0}, cnt[2] = {0, 0};  // cnt: products issued so far per slot
       bool ok = true;
       for (int round = 0; ok; ++round) {
-        if (round >= p.total_rounds) break;
-        const int idx = item_for_round(p, round, blockIdx.x, gridDim.x);
+        if (round >= rounds()) break;
+        const int idx = item_of_round(round);
         if (idx < 0) continue;
         const ItemOf<MASK> w = decode_item<MASK>(p, idx);
         const int nmax = max(w.n[0], w.n[1]);
@@ -1062,12 +1150,12 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
       // Q K^T, where this thread has nothing to issue until slot 0's next P arrives.
       // The first valid round at or after `from` (rounds in which this CTA has no item are skipped), or total_rounds.
       auto next_round = [&](int from, int& idx) {
-        for (int r = from; r < p.total_rounds; ++r) {
-          idx = item_for_round(p, r, blockIdx.x, gridDim.x);
+        for (int r = from; r < rounds(); ++r) {
+          idx = item_of_round(r);
           if (idx >= 0) return r;
         }
         idx = -1;
-        return p.total_rounds;
+        return rounds();
       };
       // At the end of an item this thread would wait for slot 1's last P before it could turn to the next item, and
       // slot 0's softmax warps, done with their epilogue, would wait some 2 500 clocks for their first S. So when
@@ -1092,7 +1180,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
       int round = next_round(0, idx), nround = 0;
       ItemOf<MASK> w, wn;
       if (idx >= 0) w = decode_item<MASK>(p, idx);
-      for (; ok && round < p.total_rounds; round = nround, w = wn) {
+      for (; ok && round < rounds(); round = nround, w = wn) {
         // the item after this one, for the early issue of its first products
         nround = next_round(round + 1, nidx);
         wn.n[0] = wn.n[1] = 0;
@@ -1205,8 +1293,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
       uint32_t q_cnt0 = 0, q_cnt1 = 0;
       bool ok = true;
       for (int round = 0; ok; ++round) {
-        if (round >= p.total_rounds) break;
-        const int idx = item_for_round(p, round, blockIdx.x, gridDim.x);
+        if (round >= rounds()) break;
+        const int idx = item_of_round(round);
         if (idx < 0) continue;
         const ItemOf<MASK> w = decode_item<MASK>(p, idx);
         if (w.n[0] > 0) {
@@ -1228,16 +1316,17 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
             tma_load_4d(sQ + kTile + ch * kSub, &tmap_q, &q_full[1], ch * 64, w.head[1], w.qb[1] * kBlockM, w.b);
         }
       }
-    } else if (kTmaOut && warp == 11 && lane == 0) {
+    } else if (kTmaOut && warp == 11 && (RAGGED || lane == 0)) {
       // ---------------- store thread: gives the staging tile to one slot at a time and sends what the slot wrote
       // there to global memory. Order of the turns: item by item and, inside an item, the slot with fewer K/V tiles
-      // (which finishes first) before the other.
-      prefetch_tmap(&tmap_o);
+      // (which finishes first) before the other. Ragged: the warp stores the tiles that a sequence ends in row by row, since behind
+      // them are another one's rows.
+      if (lane == 0) prefetch_tmap(&tmap_o);
       uint32_t full_cnt0 = 0, full_cnt1 = 0;  // tiles sent so far, per slot
       bool ok = true;
       for (int round = 0; ok; ++round) {
-        if (round >= p.total_rounds) break;
-        const int idx = item_for_round(p, round, blockIdx.x, gridDim.x);
+        if (round >= rounds()) break;
+        const int idx = item_of_round(round);
         if (idx < 0) continue;
         const ItemOf<MASK> w = decode_item<MASK>(p, idx);
         const int first = (w.n[1] < w.n[0]) ? 1 : 0;
@@ -1246,19 +1335,35 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constan
           // selects, not indexing with s: the item stays in registers
           const int n_s = s ? w.n[1] : w.n[0], head_s = s ? w.head[1] : w.head[0], qb_s = s ? w.qb[1] : w.qb[0];
           if (n_s == 0) continue;
-          mbar_arrive(&so_turn[s]);
+          if (lane == 0) mbar_arrive(&so_turn[s]);
           ok = mbar_wait_parked(&so_full[s], (s ? full_cnt1 : full_cnt0) & 1, abortp, kWaitLimitCycles);
+          if constexpr (RAGGED) ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           full_cnt0 += s ? 0u : 1u;
           full_cnt1 += s ? 1u : 0u;
+          if constexpr (RAGGED) {
+            const int rows = w.n_q - qb_s * kBlockM;
+            if (rows < kBlockM) {
+              constexpr int kUnits = D / 8;  // 16 bytes each
+              __nv_bfloat16* const dst = p.o + (query_row(p, w, qb_s * kBlockM) * p.H + head_s) * D;
+              for (int i = lane; i < rows * kUnits; i += 32) {
+                const int r = i / kUnits, u = i % kUnits;
+                const uint4 val = *reinterpret_cast<const uint4*>(sOut + (u >> 3) * kSub + r * 128 + (((u & 7) ^ (r & 7)) << 4));
+                *reinterpret_cast<uint4*>(dst + static_cast<size_t>(r) * p.H * D + u * 8) = val;
+              }
+              __syncwarp();
+              continue;
+            }
+            if (lane != 0) continue;
+          }
 #pragma unroll
           for (int ch = 0; ch < kChunks; ++ch)
-            tma_store_4d(&tmap_o, sOut + ch * kSub, ch * 64, head_s, qb_s * kBlockM, w.b);
+            tma_store_4d(&tmap_o, sOut + ch * kSub, ch * 64, head_s, q_coord(w, qb_s), w.b);
           bulk_commit_group();
           bulk_wait_group_read0();  // the tile may be overwritten
         }
       }
-      bulk_wait_group0();  // the last boxes have reached global memory
+      if (lane == 0) bulk_wait_group0();  // the last boxes have reached global memory
     }
   }
 

@@ -475,6 +475,19 @@ int launch_bwd_window(const CUtensorMap& tq, const CUtensorMap& tk, const CUtens
 
 }  // namespace
 
+int hk_host::prep_launch(const void* o, const void* d_o, float* delta, int B, int N, int H, int D, cudaStream_t stream) {
+  const long long rows = static_cast<long long>(B) * N * H;
+  if (rows > 0x7fffffffll) return HK_EINVAL;  // rows are indexed with int
+  const int rows_per_block = hk::row_pass_rows(D / 8);
+  const unsigned blocks = unsigned((rows + rows_per_block - 1) / rows_per_block);
+  const auto* po = static_cast<const __nv_bfloat16*>(o);
+  const auto* pd = static_cast<const __nv_bfloat16*>(d_o);
+  auto* fn = D == 128 ? hk::attn_bwd_prep_kernel<128> : hk::attn_bwd_prep_kernel<64>;
+  HK_CUDA(hk::launch_dependent(true, fn, blocks, 256, 0, stream, po, pd, delta, int(rows), N, H, hk::FastDiv(H), hk::FastDiv(N)));
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  return HK_OK;
+}
+
 extern "C" {
 
 #ifdef HK_TRACE
@@ -668,19 +681,6 @@ int hk_attn_fwd_paged_window(const void* q, const void* k_pages, const void* v_p
   if (window <= 0 || sinks < 0) return HK_EINVAL;
   return fwd_paged(q, k_pages, v_pages, block_table, ctx_lens, o, lse, S, T, H, H_KV, D, page_size, max_pages_per_seq,
                    num_pages, hk::kMaskWindow, window, sinks, softmax_scale, device, cuda_stream);
-}
-
-static int prep_launch(const void* o, const void* d_o, float* delta, int B, int N, int H, int D, cudaStream_t stream) {
-  const long long rows = static_cast<long long>(B) * N * H;
-  if (rows > 0x7fffffffll) return HK_EINVAL;  // rows are indexed with int
-  const int rows_per_block = hk::row_pass_rows(D / 8);
-  const unsigned blocks = unsigned((rows + rows_per_block - 1) / rows_per_block);
-  const auto* po = static_cast<const __nv_bfloat16*>(o);
-  const auto* pd = static_cast<const __nv_bfloat16*>(d_o);
-  auto* fn = D == 128 ? hk::attn_bwd_prep_kernel<128> : hk::attn_bwd_prep_kernel<64>;
-  HK_CUDA(hk::launch_dependent(true, fn, blocks, 256, 0, stream, po, pd, delta, int(rows), N, H, hk::FastDiv(H), hk::FastDiv(N)));
-  g_launches.fetch_add(1, std::memory_order_relaxed);
-  return HK_OK;
 }
 
 int hk_attn_bwd_prep(const void* o, const void* d_o, float* delta, int B, int N, int H, int D, int device,

@@ -58,6 +58,7 @@ struct DeviceState {
   hk::DecodeLimits decode;
   bool decode_fp8_ready = false;  // the decode over 8-bit pages, set up by its first call
   hk::DecodeLimits decode_fp8;
+  bool ragged_ready = false;  // the kernels of ragged batches, as well
   int bwd_clusters[hk::kMaxDkdvSplit + 1] = {};  // clusters of so many dK/dV CTAs that the device holds at once
   int* status = nullptr;       // the status word, device address (kernels write it only when something went wrong)
   int* status_host = nullptr;  // ... and host address: mapped memory, so that reading it needs no copy
@@ -67,6 +68,8 @@ inline DeviceState g_dev[kMaxDevices];
 // The first call on a device, and the first with a window there (hk_attn_api.cu).
 int init_device(int device);
 int init_windows();
+// delta of a backward (hk_attn_api.cu).
+int prep_launch(const void* o, const void* d_o, float* delta, int B, int N, int H, int D, cudaStream_t stream);
 
 template <int D, auto KIND, bool DEP>
 int prepare_fwd_kernel() {
@@ -115,7 +118,7 @@ template <int D, auto KIND>
 int prepare_bwd_kernels() {
   int rc = prepare_bwd_kernel(hk::attn_bwd_dkdv_kernel<D, KIND, false>, hk::BwdSmem<D>::kDynBytes, "attn_bwd_dkdv_kernel");
   if (rc != HK_OK) return rc;
-  if constexpr (int(KIND) != hk::kMaskWindow) {
+  if constexpr (int(KIND) != hk::kMaskWindow && int(KIND) != hk::kMaskRagged) {
     rc = prepare_bwd_kernel(hk::attn_bwd_dkdv_kernel<D, KIND, true>, hk::BwdSmem<D>::kDynBytes, "attn_bwd_dkdv_kernel");
     if (rc != HK_OK) return rc;
   }

@@ -629,6 +629,103 @@ PyObject* paged_decode_fp8(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
+// A ragged batch: q, k, v, cu_seqlens_q, cu_seqlens_k or None.
+struct Ragged {
+  const Tensor *q, *k, *v, *cu_q, *cu_k;
+  long long qs[2], ks[2], vs[2];
+  int s, tq, tk, h, hkv, d, device;
+  static bool strides(const Tensor& t, long long* st) {  // [rows, heads, D]
+    for (int i = 0; i < 2; ++i) {
+      st[i] = t.stride(i);
+      if (st[i] <= 0 || st[i] % 8 != 0) return false;
+    }
+    return t.stride(2) == 1;
+  }
+  bool take(PyObject* const* a) { return take(plain(a[0]), plain(a[1]), plain(a[2]), plain(a[3]), a[4] == Py_None ? plain(a[3]) : plain(a[4])); }
+  bool take(const Tensor* q_, const Tensor* k_, const Tensor* v_, const Tensor* cu_q_, const Tensor* cu_k_) {
+    q = q_, k = k_, v = v_, cu_q = cu_q_, cu_k = cu_k_;
+    for (const Tensor* t : {q, k, v})
+      if (!is(t, at::kBFloat16, 3) || !t->numel()) return false;
+    if (!dense(cu_q, at::kInt, 1) || !dense(cu_k, at::kInt, 1) || cu_q->size(0) < 2 || cu_k->size(0) != cu_q->size(0)) return false;
+    if (k->sizes() != v->sizes() || k->size(2) != q->size(2) || (cu_k == cu_q && k->size(0) != q->size(0)) ||
+        !same_device(*q, {k, v, cu_q, cu_k}) || !fits({q->size(0), k->size(0), q->size(1), k->size(1), cu_q->size(0)}))
+      return false;
+    s = i32(cu_q->size(0) - 1), tq = i32(q->size(0)), tk = i32(k->size(0)), h = i32(q->size(1)), hkv = i32(k->size(1)), d = i32(q->size(2));
+    device = q->device().index();
+    return strides(*q, qs) && strides(*k, ks) && strides(*v, vs);
+  }
+};
+
+// attn_fwd_ragged(q, k, v, cu_seqlens_q, cu_seqlens_k, causal, softmax_scale, out, lse)
+PyObject* attn_fwd_ragged(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  Ragged r;
+  float scale;
+  if (n_args != 9 || !PyBool_Check(a[5]) || !number(a[6], scale) || !r.take(a) || (a[7] == Py_None) != (a[8] == Py_None)) Py_RETURN_NONE;
+  Tensor out, lse, ws;
+  const size_t need = hk_attn_fwd_ragged_workspace_bytes(r.s, r.tq);
+  if (!output(a[7], *r.q, r.q->sizes(), at::kBFloat16, out) || !output(a[8], *r.q, {r.h, r.tq}, at::kFloat, lse) ||
+      !output(Py_None, *r.q, {int64_t(need)}, at::kByte, ws))
+    Py_RETURN_NONE;
+  void* st = stream_of(*r.q);
+  const void *qp = ptr(*r.q), *kp = ptr(*r.k), *vp = ptr(*r.v);
+  void *op = ptr(out), *wsp = ptr(ws);
+  float* lp = ptr<float>(lse);
+  const int32_t *cq = ptr<int32_t>(*r.cu_q), *ck = ptr<int32_t>(*r.cu_k);
+  const int causal = a[5] == Py_True, fill = a[7] == Py_None;
+  const int rc = unlocked([&] {
+    return hk_attn_fwd_ragged(qp, kp, vp, op, lp, cq, ck, r.s, r.tq, r.tk, r.h, r.hkv, r.d, r.qs, r.ks, r.vs, causal, scale, fill, wsp, need,
+                              r.device, st);
+  });
+  return result(rc, out, lse);
+  END_HANDLE_TH_ERRORS
+}
+
+// attn_bwd_ragged(q, k, v, o, d_o, lse, cu_seqlens_q, cu_seqlens_k, causal, softmax_scale, dq, dk, dv)
+PyObject* attn_bwd_ragged(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  Ragged r;
+  float scale;
+  if (n_args != 13) Py_RETURN_NONE;
+  const Tensor *cu = plain(a[6]), *o = plain(a[3]), *d_o = plain(a[4]), *lse = plain(a[5]);
+  if (!PyBool_Check(a[8]) || !number(a[9], scale) || !r.take(plain(a[0]), plain(a[1]), plain(a[2]), cu, a[7] == Py_None ? cu : plain(a[7])))
+    Py_RETURN_NONE;
+  if (!dense(o, at::kBFloat16, 3) || !dense(d_o, at::kBFloat16, 3) || !dense(lse, at::kFloat, 2) || o->sizes() != r.q->sizes() ||
+      d_o->sizes() != r.q->sizes() || lse->size(0) != r.h || lse->size(1) != r.tq || !same_device(*r.q, {o, d_o, lse}))
+    Py_RETURN_NONE;
+  const int fill = a[10] == Py_None;
+  Tensor grad[3], ws, delta;
+  long long st[3][2];
+  for (int i = 0; i < 3; ++i) {
+    const Tensor& like = i ? *r.k : *r.q;
+    if ((a[10 + i] == Py_None) != (fill != 0)) Py_RETURN_NONE;
+    if (fill) {
+      if (!output(Py_None, *r.q, like.sizes(), at::kBFloat16, grad[i])) Py_RETURN_NONE;
+    } else {
+      const Tensor* t = plain(a[10 + i]);
+      if (!is(t, at::kBFloat16, 3) || t->sizes() != like.sizes() || t->device() != r.q->device()) Py_RETURN_NONE;
+      grad[i] = *t;
+    }
+    if (!Ragged::strides(grad[i], st[i])) Py_RETURN_NONE;
+  }
+  const size_t need = hk_attn_bwd_ragged_workspace_bytes(r.s, r.tq, r.tk);
+  if (!output(Py_None, *r.q, {int64_t(need)}, at::kByte, ws) || !output(Py_None, *r.q, lse->sizes(), at::kFloat, delta)) Py_RETURN_NONE;
+  void* stream = stream_of(*r.q);
+  const void *qp = ptr(*r.q), *kp = ptr(*r.k), *vp = ptr(*r.v), *op = ptr(*o), *dop = ptr(*d_o);
+  const float* lp = ptr<float>(*lse);
+  float* dp = ptr<float>(delta);
+  void *gp[3] = {ptr(grad[0]), ptr(grad[1]), ptr(grad[2])}, *wsp = ptr(ws);
+  const int32_t *cq = ptr<int32_t>(*r.cu_q), *ck = ptr<int32_t>(*r.cu_k);
+  const int causal = a[8] == Py_True;
+  const int rc = unlocked([&] {
+    return hk_attn_bwd_ragged(qp, kp, vp, op, dop, lp, dp, gp[0], gp[1], gp[2], cq, ck, r.s, r.tq, r.tk, r.h, r.hkv, r.d, r.qs, r.ks, r.vs,
+                              st[0], st[1], st[2], causal, scale, fill, wsp, need, r.device, stream);
+  });
+  if (rc != HK_OK) return PyLong_FromLong(rc);
+  return Py_BuildValue("(NNN)", THPVariable_Wrap(grad[0]), THPVariable_Wrap(grad[1]), THPVariable_Wrap(grad[2]));
+  END_HANDLE_TH_ERRORS
+}
+
 // ---- autograd. A step through the Python functions behind these spends about 55 us on them, in the caller's thread and in the
 // engine's, which has to have the interpreter for its part; small steps are made of little else.
 
@@ -926,6 +1023,89 @@ PyObject* norm_rotary(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
+// Attention over a ragged batch, q [T, H, D] with a packed kv [Tk, 2, H_KV, D].
+class RaggedAttention : public torch::autograd::Function<RaggedAttention> {
+ public:
+  // K and V of a packed projection, or of its gradient: [Tk, H_KV, D] each
+  static Tensor part(const Tensor& kv, int i) { return kv.select(1, i); }
+
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& kv, const Tensor& cu_q, const std::optional<Tensor>& cu_k_or_none,
+                        bool causal, double scale) {
+    const Tensor cu_k = cu_k_or_none.value_or(cu_q), k = part(kv, 0), v = part(kv, 1);
+    Ragged r;
+    if (!r.take(&q, &k, &v, &cu_q, cu_k_or_none ? &cu_k : &cu_q)) throw Refused();
+    const auto options = q.options().requires_grad(false);
+    const Tensor o = at::empty(q.sizes(), options.memory_format(at::MemoryFormat::Contiguous));
+    const Tensor lse = at::empty({r.h, r.tq}, options.dtype(at::kFloat));
+    const size_t need = hk_attn_fwd_ragged_workspace_bytes(r.s, r.tq);
+    const Tensor ws = at::empty({int64_t(need)}, options.dtype(at::kByte));
+    const void *qp = ptr(q), *kp = ptr(k), *vp = ptr(v);
+    void *op = ptr(o), *wsp = ptr(ws), *stream = stream_of(q);
+    float* lp = ptr<float>(lse);
+    const int32_t *cq = ptr<int32_t>(cu_q), *ck = ptr<int32_t>(cu_k);
+    const int rc = unlocked([&] {
+      return hk_attn_fwd_ragged(qp, kp, vp, op, lp, cq, ck, r.s, r.tq, r.tk, r.h, r.hkv, r.d, r.qs, r.ks, r.vs, causal,
+                                static_cast<float>(scale), 1, wsp, need, r.device, stream);
+    });
+    if (rc != HK_OK) throw Refused();
+    ctx->save_for_backward({q, kv, o, lse, cu_q, cu_k_or_none.value_or(Tensor())});
+    ctx->saved_data["causal"] = causal;
+    ctx->saved_data["scale"] = scale;
+    return o;
+  }
+
+  // In a thread of the engine, without the interpreter.
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list s = ctx->get_saved_variables();
+    check_next_streams(static_cast<cudaStream_t>(stream_of(s[0])));
+    // saved-tensor hooks may have given them back in a layout that the kernels do not read
+    Tensor q = s[0], kv = s[1];
+    const Tensor o = s[2].contiguous(), lse = s[3].contiguous(), cu_q = s[4].contiguous(),
+                 cu_k = s[5].defined() ? s[5].contiguous() : cu_q;
+    TORCH_CHECK(grads[0].defined() && grads[0].sizes() == o.sizes(), "dO shape mismatch: expected ", o.sizes());
+    TORCH_CHECK(grads[0].device() == o.device(), "dO must be on correct CUDA device");
+    const Tensor d_o = grads[0].to(at::kBFloat16).contiguous();
+    long long st[2];
+    if (!Ragged::strides(q, st)) q = q.contiguous();
+    if (!Ragged::strides(part(kv, 0), st) || kv.stride(1) % 8 != 0) kv = kv.contiguous();
+    const Tensor k = part(kv, 0), v = part(kv, 1);
+    Ragged r;
+    TORCH_CHECK(r.take(&q, &k, &v, &cu_q, s[5].defined() ? &cu_k : &cu_q), "ragged attention: saved tensors of another shape");
+    const auto options = q.options().requires_grad(false);
+    const Tensor dq = at::empty(q.sizes(), options.memory_format(at::MemoryFormat::Contiguous));
+    const Tensor dkv = at::empty(kv.sizes(), options.memory_format(at::MemoryFormat::Contiguous));
+    const Tensor delta = at::empty(lse.sizes(), options.dtype(at::kFloat));
+    const size_t need = hk_attn_bwd_ragged_workspace_bytes(r.s, r.tq, r.tk);
+    const Tensor ws = at::empty({int64_t(need)}, options.dtype(at::kByte));
+    const Tensor dk = part(dkv, 0), dv = part(dkv, 1);
+    const long long dqs[2] = {dq.stride(0), dq.stride(1)}, dks[2] = {dk.stride(0), dk.stride(1)};
+    const int rc = hk_attn_bwd_ragged(ptr(q), ptr(k), ptr(v), ptr(o), ptr(d_o), ptr<float>(lse), ptr<float>(delta), ptr(dq), ptr(dk), ptr(dv),
+                                      ptr<int32_t>(cu_q), ptr<int32_t>(cu_k), r.s, r.tq, r.tk, r.h, r.hkv, r.d, r.qs, r.ks, r.vs, dqs, dks,
+                                      dks, ctx->saved_data["causal"].toBool(), static_cast<float>(ctx->saved_data["scale"].toDouble()), 1,
+                                      ptr(ws), need, r.device, stream_of(q));
+    if (rc != HK_OK) fail("hk_attn_bwd_ragged", rc);
+    return without_a_second({dq, dkv}, 6);
+  }
+};
+
+// ragged_attention(q, kv, cu_seqlens_q, cu_seqlens_k or None, causal, softmax_scale): O, or None
+PyObject* ragged_attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  float scale;
+  if (n_args != 6 || !PyBool_Check(a[4]) || !number(a[5], scale)) Py_RETURN_NONE;
+  const Tensor *q = plain(a[0]), *kv = plain(a[1]), *cu_q = plain(a[2]), *cu_k = a[3] == Py_None ? nullptr : plain(a[3]);
+  if (!is(q, at::kBFloat16, 3) || !is(kv, at::kBFloat16, 4) || kv->size(1) != 2 || !dense(cu_q, at::kInt, 1) ||
+      (a[3] != Py_None && !dense(cu_k, at::kInt, 1)) || !q->numel() || !kv->numel())
+    Py_RETURN_NONE;
+  try {
+    return THPVariable_Wrap(RaggedAttention::apply(*q, *kv, *cu_q, cu_k ? std::optional<Tensor>(*cu_k) : std::nullopt, a[4] == Py_True,
+                                                   static_cast<double>(scale)));
+  } catch (const Refused&) {
+    Py_RETURN_NONE;
+  }
+  END_HANDLE_TH_ERRORS
+}
+
 // captured_backward(tensor): raises what the backward of `norm_rotary` does, for a Python function whose backward is running on the
 // tensor's device
 PyObject* captured_backward(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
@@ -941,6 +1121,7 @@ PyMethodDef methods[] = {HK_METHOD(attn_fwd),       HK_METHOD(attn_bwd_strided),
                          HK_METHOD(paged_decode),   HK_METHOD(attn_fwd_paged),   HK_METHOD(paged_kv_append),
                          HK_METHOD(qk_norm_rotary), HK_METHOD(qk_norm_rotary_bwd),
                          HK_METHOD(paged_kv_append_fp8), HK_METHOD(paged_kv_read_fp8), HK_METHOD(paged_decode_fp8),
+                         HK_METHOD(attn_fwd_ragged), HK_METHOD(attn_bwd_ragged), HK_METHOD(ragged_attention),
                          HK_METHOD(packed_attention), HK_METHOD(norm_rotary), HK_METHOD(captured_backward),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_front", "Native tensor front ends of hipkittens_b200", -1, methods,

@@ -317,6 +317,32 @@ int hk_paged_kv_append_rotary(const void* k_new, const void* v_new, void* k_page
                               int S, int T, int H_KV, int D, int rotary_dim, int cos_rows, int page_size,
                               int max_pages_per_seq, int num_pages, int device, void* cuda_stream);
 
+/* ---- Attention over a ragged batch: sequences of different lengths one after the other, without padding. The reference pads
+ * (training/llama/llama/models/attentions/base.py:88-116).
+ *   q, o : [q_rows, H, D] bf16, sequence s has the rows cu_seqlens_q[s] .. cu_seqlens_q[s + 1] - 1 (int32 [S + 1], rising, inside [0, q_rows])
+ *   k, v : [k_rows, H_KV, D] bf16, with cu_seqlens_k; a sequence may have fewer queries than keys, or more, or none of either
+ *   lse  : [H, q_rows] fp32
+ * q, k, v and the gradients through element strides of the row and the head (positive multiples of 8, the last dimension contiguous);
+ * o and d_o are contiguous. With `causal` query r of a sequence sees its keys up to r + (keys - queries), as in hk_attn_fwd_cross; a row
+ * that sees none has O = 0 and L = -inf. Rows that belong to no sequence are left as they are, or with `fill_rest` become O = 0, L =
+ * -inf and zero gradients. What a sequence's neighbours hold, NaN and infinities too, does not reach it.
+ * D = 64 or 128, S <= 65535, rows <= 2^30. cu_seqlens that fall or lie outside are reported as HK_EBADLEN, and the call writes nothing.
+ * workspace: device scratch, 256-byte aligned, of at least the bytes that the functions say (0: such sizes are refused). Nothing is added
+ * up with atomics: results are the same from run to run. Asynchronous on `cuda_stream`.
+ * The backward writes delta [H, q_rows] (rowsum(O * dO)), dq, dk and dv. dq may not share memory with another output. */
+size_t hk_attn_fwd_ragged_workspace_bytes(int S, int q_rows);
+int hk_attn_fwd_ragged(const void* q, const void* k, const void* v, void* o, float* lse, const int32_t* cu_seqlens_q,
+                       const int32_t* cu_seqlens_k, int S, int q_rows, int k_rows, int H, int H_KV, int D, const long long* q_strides,
+                       const long long* k_strides, const long long* v_strides, int causal, float softmax_scale, int fill_rest,
+                       void* workspace, size_t workspace_bytes, int device, void* cuda_stream);
+size_t hk_attn_bwd_ragged_workspace_bytes(int S, int q_rows, int k_rows);
+int hk_attn_bwd_ragged(const void* q, const void* k, const void* v, const void* o, const void* d_o, const float* lse, float* delta,
+                       void* dq, void* dk, void* dv, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int S, int q_rows,
+                       int k_rows, int H, int H_KV, int D, const long long* q_strides, const long long* k_strides,
+                       const long long* v_strides, const long long* dq_strides, const long long* dk_strides, const long long* dv_strides,
+                       int causal, float softmax_scale, int fill_rest, void* workspace, size_t workspace_bytes, int device,
+                       void* cuda_stream);
+
 /* ---- The paged cache in 8 bits: pages of e4m3 codes [num_pages, 16, H_KV, D] and an fp32 scale for each page and head, K and V
  * [num_pages, H_KV] each; value = code * scale, where scales are finite and above zero. No counterpart in the reference, whose cache
  * is bf16 (training/llama/llama/models/mha.py:16-42). D = 64 or 128, page_size 16, S <= 65535; pages 16-byte aligned.
