@@ -187,27 +187,15 @@ inline int status_to_code(int word) {
   }
 }
 
-// 4-D map over a contiguous bf16 [B, N, heads, D] tensor, box = 64 columns x 1 head x 128 rows,
-// 128-byte swizzle (rows of the box are 128 B, the layout tcgen05 descriptors expect).
-// `st` = element strides of the batch, sequence and head dimensions (the D dimension is contiguous); every
-// stride must be a multiple of 8 elements (16 bytes), which TMA requires.
-inline int make_bnhd_map(CUtensorMap* map, const void* base, int B, int N, int heads, int D, const long long* st,
-                  int box_rows = hk::kBlockM) {
+// A tensor map by `encode`, called with the driver's function.
+template <typename Encode>
+int make_map(const Encode& encode) {
   EncodeTiledFn enc = get_encode();
   if (!enc) {
     snprintf(g_cuda_err, sizeof(g_cuda_err), "cuTensorMapEncodeTiled not available from the driver");
     return HK_ECUDA;
   }
-  cuuint64_t dims[4] = {cuuint64_t(D), cuuint64_t(heads), cuuint64_t(N), cuuint64_t(B)};
-  cuuint64_t strides[3] = {cuuint64_t(st[2]) * 2, cuuint64_t(st[1]) * 2, cuuint64_t(st[0]) * 2};
-  cuuint32_t box[4] = {64, 1, cuuint32_t(box_rows), 1};
-  cuuint32_t estr[4] = {1, 1, 1, 1};
-  auto encode = [&] {
-    return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
-               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  };
-  CUresult r = encode();
+  CUresult r = encode(enc);
   if (r == CUDA_ERROR_INVALID_CONTEXT) {
     // a thread that has made no runtime call yet (autograd's) has no current context: let the runtime bind the
     // device's own and try again. cudaSetDevice does that and, unlike cudaFree(nullptr), leaves a graph alone that
@@ -215,13 +203,44 @@ inline int make_bnhd_map(CUtensorMap* map, const void* base, int B, int N, int h
     int device = 0;
     HK_CUDA(cudaGetDevice(&device));
     HK_CUDA(cudaSetDevice(device));
-    r = encode();
+    r = encode(enc);
   }
   if (r != CUDA_SUCCESS) {
     snprintf(g_cuda_err, sizeof(g_cuda_err), "cuTensorMapEncodeTiled failed with CUresult %d", int(r));
     return HK_ECUDA;
   }
   return HK_OK;
+}
+
+// 4-D map over a contiguous bf16 [B, N, heads, D] tensor, box = 64 columns x 1 head x 128 rows,
+// 128-byte swizzle (rows of the box are 128 B, the layout tcgen05 descriptors expect).
+// `st` = element strides of the batch, sequence and head dimensions (the D dimension is contiguous); every
+// stride must be a multiple of 8 elements (16 bytes), which TMA requires.
+inline int make_bnhd_map(CUtensorMap* map, const void* base, int B, int N, int heads, int D, const long long* st,
+                  int box_rows = hk::kBlockM) {
+  cuuint64_t dims[4] = {cuuint64_t(D), cuuint64_t(heads), cuuint64_t(N), cuuint64_t(B)};
+  cuuint64_t strides[3] = {cuuint64_t(st[2]) * 2, cuuint64_t(st[1]) * 2, cuuint64_t(st[0]) * 2};
+  cuuint32_t box[4] = {64, 1, cuuint32_t(box_rows), 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  return make_map([&](EncodeTiledFn enc) {
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  });
+}
+
+// 3-D map over the codes of a pool of 8-bit pages, [num_pages * 16 rows, heads, D] bytes, box = one page of one head, its rows of 64 or
+// 128 bytes swizzled over as many.
+inline int make_code_map(CUtensorMap* map, const void* base, int num_pages, int heads, int D) {
+  cuuint64_t dims[3] = {cuuint64_t(D), cuuint64_t(heads), cuuint64_t(num_pages) * hk::kPageTokens};
+  cuuint64_t strides[2] = {cuuint64_t(D), cuuint64_t(heads) * D};
+  cuuint32_t box[3] = {cuuint32_t(D), 1, hk::kPageTokens};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return make_map([&](EncodeTiledFn enc) {
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  });
 }
 
 // Whether an attention kernel is launched so that it may start under the tail of the one before it: up to 100 tiles per CTA

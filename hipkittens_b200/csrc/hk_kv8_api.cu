@@ -18,7 +18,7 @@ int fp8_cache(hk::Fp8Cache& c, const void* k_pages, const void* v_pages, const f
   if (!k_pages || !v_pages || !k_scales || !v_scales || !block_table) return HK_EINVAL;
   if (S <= 0 || H_KV <= 0 || D <= 0 || max_pages <= 0 || num_pages <= 0) return HK_EINVAL;
   if (page_size != hk::kPageTokens || (D != 64 && D != 128)) return HK_EUNSUPPORTED;
-  if (S > 65535 || H_KV > 65535 || max_pages > 0x7fffffff / hk::kPageTokens) return HK_EINVAL;
+  if (S > 65535 || H_KV > 65535 || max_pages > 0x7fffffff / hk::kPageTokens || num_pages > 0x7fffffff / hk::kPageTokens) return HK_EINVAL;
   if (!aligned16(k_pages) || !aligned16(v_pages) || !aligned4(k_scales) || !aligned4(v_scales) || !aligned4(block_table)) return HK_EINVAL;
   c.k_pages = static_cast<uint8_t*>(const_cast<void*>(k_pages));
   c.v_pages = static_cast<uint8_t*>(const_cast<void*>(v_pages));
@@ -160,9 +160,11 @@ int hk_attn_paged_decode_fp8(const void* q, const void* k_pages, const void* v_p
       st->decode_fp8_ready = true;
     }
   }
+  CUtensorMap tk, tv;
+  if ((rc = make_code_map(&tk, k_pages, num_pages, H_KV, D)) != HK_OK) return rc;
+  if ((rc = make_code_map(&tv, v_pages, num_pages, H_KV, D)) != HK_OK) return rc;
   hk::DecodeFp8Params p = {};
   p.q = static_cast<const __nv_bfloat16*>(q);
-  p.k_codes = c.k_pages, p.v_codes = c.v_pages;
   p.k_scales = c.k_scales, p.v_scales = c.v_scales;
   p.block_table = block_table;
   p.ctx_lens = ctx_lens;
@@ -179,7 +181,7 @@ int hk_attn_paged_decode_fp8(const void* q, const void* k_pages, const void* v_p
   p.sinks = std::min(sinks, capacity);
   p.span_pages = span;
   int launched = 0;
-  const cudaError_t e = hk::launch_paged_decode_fp8(p, D, st->decode_fp8, static_cast<cudaStream_t>(cuda_stream), &launched);
+  const cudaError_t e = hk::launch_paged_decode_fp8(tk, tv, p, D, st->decode_fp8, static_cast<cudaStream_t>(cuda_stream), &launched);
   g_launches.fetch_add(launched, std::memory_order_relaxed);
   if (e != cudaSuccess) return cuda_fail(e, "fp8 decode launch");
   return HK_OK;

@@ -18,6 +18,7 @@
 // shared memory.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_fp16.h>
 
 #include "attn_fwd_sm100.cuh"
@@ -33,10 +34,11 @@ struct DecodeFp8Ring {
   static constexpr int kSlabBytes = kPageTokens * D;    // one page of one head: 2 KB at D = 128
   static constexpr int kStageBytes = 2 * kSlabBytes;    // K and V
 };
-constexpr int decode_fp8_smem_bytes(int warps) { return warps * DecodeFp8Ring<128>::kStages * DecodeFp8Ring<128>::kStageBytes; }
+// The ring of every warp, and a barrier for each stage.
+__host__ __device__ constexpr int decode_fp8_ring_bytes(int warps) { return warps * DecodeFp8Ring<128>::kStages * DecodeFp8Ring<128>::kStageBytes; }
+constexpr int decode_fp8_smem_bytes(int warps) { return decode_fp8_ring_bytes(warps) + warps * DecodeFp8Ring<64>::kStages * 8 + 8; }
 
 struct DecodeFp8Params : DecodeParams {  // k_pages and v_pages are not used; a call without a window has one that hides nothing
-  const uint8_t *k_codes, *v_codes;
   const float *k_scales, *v_scales;      // [P, H_KV]
 };
 
@@ -67,12 +69,25 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 // grid = (max_splits, H_KV, S), or (cluster size, H_KV, S) in clusters along x; block = 32 W threads, dynamic smem =
 // decode_fp8_smem_bytes(W).
 template <bool CLUSTER, int W, int D>
-__global__ void __launch_bounds__(W * 32, 16 / W) paged_decode_fp8_split_kernel(const __grid_constant__ DecodeFp8Params p) {
+__global__ void __launch_bounds__(W * 32, 16 / W)
+paged_decode_fp8_split_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
+                              const __grid_constant__ DecodeFp8Params p) {
   using namespace dec;
   using Ring = DecodeFp8Ring<D>;
   constexpr int kStages = Ring::kStages, kSlabBytes = Ring::kSlabBytes, kStageBytes = Ring::kStageBytes, kRowBytes = Ring::kRowBytes;
   constexpr int kChunks = D / 16;  // 16-byte chunks of a token, of 16 dimensions
-  extern __shared__ __align__(128) uint8_t dsmem[];
+  extern __shared__ __align__(1024) uint8_t dsmem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint64_t* const full = reinterpret_cast<uint64_t*>(dsmem + decode_fp8_ring_bytes(W)) + warp * kStages;
+  uint32_t* const abort_word = reinterpret_cast<uint32_t*>(dsmem + decode_fp8_ring_bytes(W) + W * DecodeFp8Ring<64>::kStages * 8);
+  if (lane == 0) {
+    for (int s = 0; s < kStages; ++s) ptx::mbar_init(full + s, 1);
+    if (warp == 0) *abort_word = 0;
+    ptx::fence_mbar_init();
+    ptx::prefetch_tmap(&tmap_k);
+    ptx::prefetch_tmap(&tmap_v);
+  }
+  __syncthreads();
   ptx::grid_dep_wait();
   ptx::grid_dep_launch();
   const int split = blockIdx.x, kvh = blockIdx.y, seq = blockIdx.z;
@@ -82,7 +97,6 @@ __global__ void __launch_bounds__(W * 32, 16 / W) paged_decode_fp8_split_kernel(
     ctx = p.max_pages * kPageTokens;
     if (threadIdx.x == 0) atomicCAS(p.status, 0, kStatusBadLen);
   }
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const LivePages live(ctx, p.window, p.sinks);
   // this warp's pages: page_first, page_first + page_step, ... below page_end, of the live ones
@@ -126,29 +140,23 @@ __global__ void __launch_bounds__(W * 32, 16 / W) paged_decode_fp8_split_kernel(
   };
   look_up(0);
 
-  const uint32_t ring = ptx::smem_u32(dsmem) + warp * (kStages * kStageBytes);
-  const size_t row_bytes = size_t(p.H_KV) * D;
+  uint8_t* const ring = dsmem + warp * (kStages * kStageBytes);
   auto sees = [&](int key) { return key < ctx && (key >= live.first_key || key < p.sinks); };
-  // a chunk lies where ldmatrix finds the chunks of 8 consecutive tokens in 8 different groups of banks
-  auto place = [](int tok, int ch) { return tok * kRowBytes + ((ch ^ (D == 128 ? tok & 7 : (tok >> 1) & 3)) << 4); };
+  // A page's tokens of this head are one box of the pool, swizzled so that ldmatrix finds a chunk of 8 consecutive tokens in 8 different
+  // groups of banks. All 16 come, whether the query sees them or not: masked scores do not look at K, and p = 0 meets a finite V, since
+  // the products take no code for a NaN.
   auto fetch = [&](int i) {
     if (page_first + i * page_step < page_end) {
       if (i > 0 && (i & 31) == 0) look_up(i);
       const int id = __shfl_sync(0xffffffffu, my_id, i & 31);
-      const size_t base = size_t(id) * kPageTokens * row_bytes + size_t(kvh) * D;
-      const int tok_base = live.page(page_first + i * page_step) * kPageTokens;
-      const uint32_t st = ring + (i % kStages) * kStageBytes;
-#pragma unroll
-      for (int r = 0; r < kChunks / 2; ++r) {
-        const int ch_lin = r * 32 + lane, tok = ch_lin / kChunks, ch = ch_lin % kChunks;
-        const size_t src = base + size_t(tok) * row_bytes + ch * 16;
-        // keys that the query does not see are not read, and are zeros: whatever the cache holds there meets p = 0
-        const bool seen = sees(tok_base + tok);
-        cp_async16_if(st + place(tok, ch), p.k_codes + src, seen);
-        cp_async16_if(st + kSlabBytes + place(tok, ch), p.v_codes + src, seen);
+      if (lane == 0) {
+        uint64_t* const bar = full + i % kStages;
+        uint8_t* const st = ring + (i % kStages) * kStageBytes;
+        ptx::mbar_expect_tx(bar, kStageBytes);
+        ptx::tma_load_3d(st, &tmap_k, bar, 0, kvh, id * kPageTokens);
+        ptx::tma_load_3d(st + kSlabBytes, &tmap_v, bar, 0, kvh, id * kPageTokens);
       }
     }
-    cp_async_commit();
   };
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) fetch(i);
@@ -187,6 +195,10 @@ __global__ void __launch_bounds__(W * 32, 16 / W) paged_decode_fp8_split_kernel(
   for (int j = 0; j < kChunks; ++j) oacc[j][0] = oacc[j][1] = oacc[j][2] = oacc[j][3] = 0.f;
   float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
   float my_ks = 0.f, my_w = 0.f, most_vs = 0.f;
+  const uint32_t ring_at = ptx::smem_u32(ring);
+  // where this lane's row of ldmatrix begins: tokens 0-7 and 8-15, of a chunk and the one behind it
+  const int row = (lane & 7) + ((lane >> 3) & 1) * 8;
+  const uint32_t mine = row * kRowBytes + (((lane >> 4) ^ (D == 128 ? row & 7 : (row >> 1) & 3)) << 4);
   constexpr float kUp = 5192296858534827628530496329220096.f;  // 2^112
 
   for (int i = 0, page = page_first; page < page_end; ++i, page += page_step) {
@@ -208,27 +220,27 @@ __global__ void __launch_bounds__(W * 32, 16 / W) paged_decode_fp8_split_kernel(
       my_w = most_vs > 0.f ? next_vs / most_vs * kUp : next_vs * kUp;  // all zero, or NaN
     }
     fetch(i + kStages - 1);
-    cp_async_wait<kStages - 1>();
-    __syncwarp();
-    const uint32_t sK = ring + (i % kStages) * kStageBytes, sV = sK + kSlabBytes;
+    if (!__all_sync(0xffffffffu, ptx::mbar_wait(full + i % kStages, (i / kStages) & 1, abort_word, kWaitLimitCycles))) break;
+    const uint32_t sK = ring_at + (i % kStages) * kStageBytes, sV = sK + kSlabBytes;
     const float ks = __shfl_sync(0xffffffffu, my_ks, i & 31), wv = __shfl_sync(0xffffffffu, my_w, i & 31);
-    const int mi = lane >> 3, tok = (lane & 7) + 8 * (mi & 1);
 
     // ---- S^T[16 tokens x 8 heads] = K Q^T, even and odd chunks apart: one accumulator's products wait for one another
     float sc[4] = {0.f, 0.f, 0.f, 0.f}, sd[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int ch = 0; ch < kChunks; ch += 2) {
       uint32_t r0, r1, r2, r3;
-      ldmatrix_x4(sK + place(tok, ch + (mi >> 1)), r0, r1, r2, r3);
+      ldmatrix_x4((sK + mine) ^ (ch << 4), r0, r1, r2, r3);
       fp8::mma_f16(sc, fp8::widen(r0), fp8::widen(r1), fp8::widen(r0 >> 16), fp8::widen(r1 >> 16), qb[ch][0], qb[ch][1]);
       fp8::mma_f16(sd, fp8::widen(r2), fp8::widen(r3), fp8::widen(r2 >> 16), fp8::widen(r3 >> 16), qb[ch + 1][0], qb[ch + 1][1]);
     }
     const float f0 = ks * qs0, f1 = ks * qs1;
     float sv[4] = {(sc[0] + sd[0]) * f0, (sc[1] + sd[1]) * f1, (sc[2] + sd[2]) * f0, (sc[3] + sd[3]) * f1};
     // ---- online softmax over tokens g and g + 8 of this page, heads 2 t and 2 t + 1
-    const int key = live.page(page) * kPageTokens + g;
-    if (!sees(key)) sv[0] = sv[1] = -INFINITY;
-    if (!sees(key + 8)) sv[2] = sv[3] = -INFINITY;
+    const int key = live.page(page) * kPageTokens;
+    if (key + kPageTokens > ctx || (key < live.first_key && key + kPageTokens > p.sinks)) {  // a page that is not seen whole
+      if (!sees(key + g)) sv[0] = sv[1] = -INFINITY;
+      if (!sees(key + g + 8)) sv[2] = sv[3] = -INFINITY;
+    }
     // The maximum is looked for only where some score is far above the one that the head has (the first page's is -inf)
     float pm0 = fmaxf(sv[0], sv[2]), pm1 = fmaxf(sv[1], sv[3]);
     if (__any_sync(0xffffffffu, (pm0 - m0) * c > kRescaleThresholdLog2 || (pm1 - m1) * c > kRescaleThresholdLog2)) {
@@ -253,21 +265,27 @@ __global__ void __launch_bounds__(W * 32, 16 / W) paged_decode_fp8_split_kernel(
 #pragma unroll
     for (int ch = 0; ch < kChunks; ch += 2) {
       uint32_t r0, r1, r2, r3;
-      ldmatrix_x4_trans(sV + place(tok, ch + (mi >> 1)), r0, r1, r2, r3);
+      ldmatrix_x4_trans((sV + mine) ^ (ch << 4), r0, r1, r2, r3);
       mma_16816(oacc[ch], fp8::even_bf16(r0), fp8::odd_bf16(r0), fp8::even_bf16(r1), fp8::odd_bf16(r1), b0, b1);
       mma_16816(oacc[ch + 1], fp8::even_bf16(r2), fp8::odd_bf16(r2), fp8::even_bf16(r3), fp8::odd_bf16(r3), b0, b1);
     }
     __syncwarp();
   }
-  cp_async_wait<0>();
+  __syncthreads();  // the ring is idle now, or a wait has run out
+  if (*static_cast<volatile uint32_t*>(abort_word) != 0) {
+    // copies that are still in flight get time to land before the shared memory goes away
+    const uint64_t t0 = ptx::globaltimer_ns();
+    while (ptx::globaltimer_ns() - t0 < 2000000ull) {
+    }
+    if (threadIdx.x == 0) atomicCAS(p.status, kStatusOk, kStatusTimeout);
+  }
 #pragma unroll
   for (int off = 4; off < 32; off <<= 1) {
     l0 += __shfl_xor_sync(0xffffffffu, l0, off);
     l1 += __shfl_xor_sync(0xffffffffu, l1, off);
   }
 
-  // ---- merge the W warps through shared memory (the ring is idle now)
-  __syncthreads();
+  // ---- merge the W warps through shared memory
   float* sm_o = reinterpret_cast<float*>(dsmem);  // [W][8][D]
   float* sm_m = sm_o + W * 8 * D;                // [W][8]
   float* sm_l = sm_m + W * 8;                     // [W][8]
@@ -400,18 +418,19 @@ inline DecodeShape decode_pick_fp8_shape(int S, int H_KV, int span, const Decode
 }
 
 template <int D>
-cudaError_t launch_decode_fp8(DecodeFp8Params p, DecodeShape shape, int chunk_pages, cudaStream_t stream, int* launched) {
+cudaError_t launch_decode_fp8(const CUtensorMap& tk, const CUtensorMap& tv, DecodeFp8Params p, DecodeShape shape, int chunk_pages,
+                              cudaStream_t stream, int* launched) {
   p.chunk_pages = chunk_pages;
   const int splits = (p.span_pages + p.chunk_pages - 1) / p.chunk_pages;
   if (splits > kMaxCombineSplits) return cudaErrorInvalidValue;
   const dim3 grid(shape.cluster ? shape.cluster : splits, p.H_KV, p.S);
   cudaError_t e;
   if (shape.cluster == 0) {
-    e = launch_dependent(true, paged_decode_fp8_split_kernel<false, 4, D>, grid, 128, decode_fp8_smem_bytes(4), stream, p);
+    e = launch_dependent(true, paged_decode_fp8_split_kernel<false, 4, D>, grid, 128, decode_fp8_smem_bytes(4), stream, tk, tv, p);
   } else {
     auto* fn = shape.warps == 8 ? paged_decode_fp8_split_kernel<true, 8, D> : paged_decode_fp8_split_kernel<true, 4, D>;
     e = launch_dependent(true, fn, grid, shape.warps * 32, decode_fp8_smem_bytes(shape.warps), stream,
-                         ClusterX{unsigned(shape.cluster)}, p);
+                         ClusterX{unsigned(shape.cluster)}, tk, tv, p);
   }
   *launched += 1;
   if (e != cudaSuccess || shape.cluster) return e;
@@ -420,11 +439,11 @@ cudaError_t launch_decode_fp8(DecodeFp8Params p, DecodeShape shape, int chunk_pa
   return e;
 }
 
-inline cudaError_t launch_paged_decode_fp8(const DecodeFp8Params& p, int D, const DecodeLimits& lim, cudaStream_t stream,
+inline cudaError_t launch_paged_decode_fp8(const CUtensorMap& tk, const CUtensorMap& tv, const DecodeFp8Params& p, int D, const DecodeLimits& lim, cudaStream_t stream,
                                            int* launched) {
   const DecodeShape shape = decode_pick_fp8_shape(p.S, p.H_KV, p.span_pages, lim);
   const int chunk_pages = decode_pick_chunk_pages(p.S, p.H_KV, p.span_pages, lim.sm_count);
-  return (D == 64 ? launch_decode_fp8<64> : launch_decode_fp8<128>)(p, shape, chunk_pages, stream, launched);
+  return (D == 64 ? launch_decode_fp8<64> : launch_decode_fp8<128>)(tk, tv, p, shape, chunk_pages, stream, launched);
 }
 
 }  // namespace hk

@@ -87,18 +87,38 @@ __device__ __forceinline__ uint32_t scale_bits(uint32_t amax) {
   const int e = static_cast<int>(amax >> 23) - 127 - 8 + ((amax & 0x7fffffu) > 0x600000u ? 1 : 0);
   return static_cast<uint32_t>(min(max(e, kFp8LeastExp), kFp8MostExp) + 127) << 23;
 }
-// x / scale. Exact through the reciprocal of a power of two; a scale that another quantiser left behind divides.
-struct Divide {
-  float scale, inv;
-  bool power;
-  __device__ __forceinline__ explicit Divide(uint32_t bits) {
-    scale = __uint_as_float(bits);
-    const int e = static_cast<int>(bits >> 23);
-    power = (bits & 0x807fffffu) == 0 && e > 0 && e < 254;
-    inv = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+// The larger of two magnitudes and a, NaN if one of them is.
+__device__ __forceinline__ float max_size(float a, float x, float y) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(fabsf(x)), "f"(fabsf(y)));
+  return d;
+}
+// x / scale for four values at a time, as codes. Exact through the reciprocal of a power of two; a scale that another quantiser left
+// behind divides.
+struct ByPower {
+  uint64_t inv2;
+  __device__ __forceinline__ uint32_t operator()(float a, float b, float c, float d) const {
+    ptx::unpack2(ptx::mul2(ptx::pack2(a, b), inv2), a, b);
+    ptx::unpack2(ptx::mul2(ptx::pack2(c, d), inv2), c, d);
+    return encode4(a, b, c, d);
   }
-  __device__ __forceinline__ float operator()(float x) const { return power ? x * inv : __fdiv_rn(x, scale); }
 };
+struct ByDivision {
+  float scale;
+  __device__ __forceinline__ uint32_t operator()(float a, float b, float c, float d) const {
+    return encode4(__fdiv_rn(a, scale), __fdiv_rn(b, scale), __fdiv_rn(c, scale), __fdiv_rn(d, scale));
+  }
+};
+template <typename Fn>
+__device__ __forceinline__ void with_divisor(uint32_t bits, const Fn& fn) {
+  const int e = static_cast<int>(bits >> 23);
+  if ((bits & 0x807fffffu) == 0 && e > 0 && e < 254) {
+    const float inv = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+    fn(ByPower{ptx::pack2(inv, inv)});
+  } else {
+    fn(ByDivision{__uint_as_float(bits)});
+  }
+}
 
 }  // namespace fp8
 
@@ -176,20 +196,63 @@ __global__ void __launch_bounds__(256) paged_kv_append_fp8_kernel(const __grid_c
   float* const scale_at = (is_v ? c.v_scales : c.k_scales) + static_cast<size_t>(id) * c.H_KV + head;
   const uint32_t before = r0 > 0 ? __float_as_uint(*scale_at) : 0u;  // a page that starts anew has no scale yet
 
-  [[maybe_unused]] float y[ROT != kFp8Plain ? kSteps : 1][8];
-  uint32_t amax = 0;
-  if constexpr (ROT != kFp8Plain) {
-    const int half = p.R / 2, at = col < half ? col : col - half;  // pairs are (i, i + R / 2)
-    const bool turned = !is_v && col < p.R;
-    const int partner = lane + (col < half ? half / 8 : -half / 8);
-    const float sign = col < half ? -1.f : 1.f;
+  const size_t row_bytes = static_cast<size_t>(c.H_KV) * D;
+  uint8_t* const page = (is_v ? c.v_pages : c.k_pages) + static_cast<size_t>(id) * kPageTokens * row_bytes + head * D + col;
+  // From the largest magnitude on: the scale, the codes of the new rows (`row(i, divide)`: those of a lane's 8 values in step i), and where
+  // the scale has grown the other rows'.
+  auto finish = [&](uint32_t amax, auto&& row) {
+    uint32_t bits = fp8::scale_bits(__reduce_max_sync(0xffffffffu, amax));
+    if (r0 > 0) {
+      if ((before & 0x7fffffffu) > 0x7f800000u) bits = 0x7fc00000u;
+      else if (static_cast<int>(before) > static_cast<int>(bits)) bits = before;  // of floats above zero
+    }
+    fp8::with_divisor(bits, [&](auto divide) {
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        const int r = row0 + i * kRows;
+        if (r >= r0 && r < r1) *reinterpret_cast<uint2*>(page + r * row_bytes) = row(i, divide);
+      }
+      if (r0 > 0 && bits != before) {
+        const float old = __uint_as_float(before);
+#pragma unroll 1
+        for (int r = row0; r < kPageTokens; r += kRows) {
+          if (r >= r0 && r < r1) continue;
+          const uint2 v = *reinterpret_cast<const uint2*>(page + r * row_bytes);
+          auto anew = [&](uint32_t codes) {
+            const float2 a = fp8::decode2(codes), b = fp8::decode2(codes >> 16);
+            return divide(a.x * old, a.y * old, b.x * old, b.y * old);
+          };
+          *reinterpret_cast<uint2*>(page + r * row_bytes) = make_uint2(anew(v.x), anew(v.y));
+        }
+      }
+    });
+    if (lane == 0 && (r0 == 0 || bits != before)) *scale_at = __uint_as_float(bits);
+  };
+
+  if (ROT == kFp8Plain || is_v) {
+    uint32_t two = 0;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i)
+      for (uint32_t v : {x[i].x, x[i].y, x[i].z, x[i].w}) two = __vmaxu2(two, v & 0x7fff7fffu);
+    finish(max(two & 0xffff0000u, two << 16), [&](int i, auto divide) {
+      const float2 a = fp8::bf16x2(x[i].x), b = fp8::bf16x2(x[i].y), d = fp8::bf16x2(x[i].z), e = fp8::bf16x2(x[i].w);
+      return make_uint2(divide(a.x, a.y, b.x, b.y), divide(d.x, d.y, e.x, e.y));
+    });
+  } else if constexpr (ROT != kFp8Plain) {
+    // pairs are (i, i + R / 2): a cos - b sin for the lanes that have a, b cos + a sin for those that have b, which send -b
+    const int half = p.R / 2;
+    const bool first_half = col < half, turned = col < p.R;
+    const int partner = (lane + (first_half ? half / 8 : -half / 8)) & 31, at = first_half ? col : col - half;
+    const uint32_t flip = first_half ? 0u : 0x80008000u;
+    uint64_t y[kSteps][4];
+    float amax = 0.f;
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
       const int r = row0 + i * kRows;
       const uint32_t xw[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-      float cs[8], sn[8];
+      uint64_t cs[4], sn[4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) cs[j] = 1.f, sn[j] = 0.f;
+      for (int j = 0; j < 4; ++j) cs[j] = ptx::pack2(1.f, 1.f), sn[j] = ptx::pack2(0.f, 0.f);
       if (turned && r >= r0 && r < r1) {
         const size_t t = static_cast<size_t>(slot * kPageTokens + r) * half + at;
         if constexpr (ROT == kFp8TableF32) {
@@ -198,8 +261,8 @@ __global__ void __launch_bounds__(256) paged_kv_append_fp8_kernel(const __grid_c
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const float4 a = c4[j], b = s4[j];
-            cs[4 * j] = a.x, cs[4 * j + 1] = a.y, cs[4 * j + 2] = a.z, cs[4 * j + 3] = a.w;
-            sn[4 * j] = b.x, sn[4 * j + 1] = b.y, sn[4 * j + 2] = b.z, sn[4 * j + 3] = b.w;
+            cs[2 * j] = ptx::pack2(a.x, a.y), cs[2 * j + 1] = ptx::pack2(a.z, a.w);
+            sn[2 * j] = ptx::pack2(b.x, b.y), sn[2 * j + 1] = ptx::pack2(b.z, b.w);
           }
         } else {
           const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.cos) + t),
@@ -208,71 +271,27 @@ __global__ void __launch_bounds__(256) paged_kv_append_fp8_kernel(const __grid_c
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float2 ca = fp8::bf16x2(aw[j]), sa = fp8::bf16x2(bw[j]);
-            cs[2 * j] = ca.x, cs[2 * j + 1] = ca.y, sn[2 * j] = sa.x, sn[2 * j + 1] = sa.y;
+            cs[j] = ptx::pack2(ca.x, ca.y), sn[j] = ptx::pack2(sa.x, sa.y);
           }
         }
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float2 own = fp8::bf16x2(xw[j]), other = fp8::bf16x2(__shfl_sync(0xffffffffu, xw[j], partner & 31));
-        if (turned) {  // a cos - b sin, or b cos + a sin
-          y[i][2 * j] = __fadd_rn(__fmul_rn(own.x, cs[2 * j]), sign * __fmul_rn(other.x, sn[2 * j]));
-          y[i][2 * j + 1] = __fadd_rn(__fmul_rn(own.y, cs[2 * j + 1]), sign * __fmul_rn(other.y, sn[2 * j + 1]));
-        } else {
-          y[i][2 * j] = own.x, y[i][2 * j + 1] = own.y;
-        }
+        const float2 own = fp8::bf16x2(xw[j]), other = fp8::bf16x2(__shfl_sync(0xffffffffu, xw[j] ^ flip, partner));
+        const uint64_t own2 = ptx::pack2(own.x, own.y);
+        y[i][j] = turned ? ptx::add2(ptx::mul2(own2, cs[j]), ptx::mul2(ptx::pack2(other.x, other.y), sn[j])) : own2;
+        float lo, hi;
+        ptx::unpack2(y[i][j], lo, hi);
+        amax = fp8::max_size(amax, lo, hi);
       }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) amax = max(amax, __float_as_uint(y[i][j]) & 0x7fffffffu);
     }
-  } else {
-    uint32_t two = 0;
+    finish(__float_as_uint(amax), [&](int i, auto divide) {
+      float v[8];
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i)
-      for (uint32_t v : {x[i].x, x[i].y, x[i].z, x[i].w}) two = __vmaxu2(two, v & 0x7fff7fffu);
-    amax = max(two & 0xffff0000u, two << 16);
+      for (int j = 0; j < 4; ++j) ptx::unpack2(y[i][j], v[2 * j], v[2 * j + 1]);
+      return make_uint2(divide(v[0], v[1], v[2], v[3]), divide(v[4], v[5], v[6], v[7]));
+    });
   }
-  amax = __reduce_max_sync(0xffffffffu, amax);
-  uint32_t bits = fp8::scale_bits(amax);
-  if (r0 > 0) {
-    if ((before & 0x7fffffffu) > 0x7f800000u) bits = 0x7fc00000u;
-    else if (static_cast<int>(before) > static_cast<int>(bits)) bits = before;  // of floats above zero
-  }
-  const fp8::Divide divide(bits);
-  const size_t row_bytes = static_cast<size_t>(c.H_KV) * D;
-  uint8_t* const page = (is_v ? c.v_pages : c.k_pages) + static_cast<size_t>(id) * kPageTokens * row_bytes + head * D + col;
-#pragma unroll
-  for (int i = 0; i < kSteps; ++i) {
-    const int r = row0 + i * kRows;
-    if (r < r0 || r >= r1) continue;
-    uint2 out;
-    if constexpr (ROT != kFp8Plain) {
-      out.x = fp8::encode4(divide(y[i][0]), divide(y[i][1]), divide(y[i][2]), divide(y[i][3]));
-      out.y = fp8::encode4(divide(y[i][4]), divide(y[i][5]), divide(y[i][6]), divide(y[i][7]));
-    } else {
-      const float2 a = fp8::bf16x2(x[i].x), b = fp8::bf16x2(x[i].y), d = fp8::bf16x2(x[i].z), e = fp8::bf16x2(x[i].w);
-      out.x = fp8::encode4(divide(a.x), divide(a.y), divide(b.x), divide(b.y));
-      out.y = fp8::encode4(divide(d.x), divide(d.y), divide(e.x), divide(e.y));
-    }
-    *reinterpret_cast<uint2*>(page + r * row_bytes) = out;
-  }
-  if (r0 > 0 && bits == before) return;
-  if (r0 > 0) {
-    const float old = __uint_as_float(before);
-#pragma unroll 1
-    for (int i = 0; i < kSteps; ++i) {
-      const int r = row0 + i * kRows;
-      if (r >= r0 && r < r1) continue;
-      uint2 v = *reinterpret_cast<const uint2*>(page + r * row_bytes);
-      auto anew = [&](uint32_t codes) {
-        const float2 a = fp8::decode2(codes), b = fp8::decode2(codes >> 16);
-        return fp8::encode4(divide(a.x * old), divide(a.y * old), divide(b.x * old), divide(b.y * old));
-      };
-      v.x = anew(v.x), v.y = anew(v.y);
-      *reinterpret_cast<uint2*>(page + r * row_bytes) = v;
-    }
-  }
-  if (lane == 0) *scale_at = __uint_as_float(bits);
 }
 
 struct ReadFp8Params {
@@ -348,6 +367,7 @@ __global__ void __launch_bounds__(256) paged_kv_read_fp8_kernel(const __grid_con
       x[kv][i] = make_uint4(0, 0, 0, 0);
       if (r < valid) x[kv][i] = __ldcs(reinterpret_cast<const uint4*>((kv ? c.v_pages : c.k_pages) + at + r * row_bytes));
     }
+  const bool wide[2] = {(reinterpret_cast<uintptr_t>(p.k_out) & 31) == 0, (reinterpret_cast<uintptr_t>(p.v_out) & 31) == 0};
   const size_t scale_at = static_cast<size_t>(id) * c.H_KV + head;
   const float scales[2] = {valid > 0 ? c.k_scales[scale_at] : 0.f, valid > 0 ? c.v_scales[scale_at] : 0.f};
 #pragma unroll
@@ -368,8 +388,12 @@ __global__ void __launch_bounds__(256) paged_kv_read_fp8_kernel(const __grid_con
 #pragma unroll
         for (int j = 0; j < 8; ++j) o[j] = 0;  // and not a NaN of the block's scale
       uint4* const dst = reinterpret_cast<uint4*>((kv ? p.v_out : p.k_out) + ((out_row + r) * c.H_KV + head) * D + col);
-      dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
-      dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
+      if (wide[kv]) {
+        ptx::st_global_v8(dst, o);
+      } else {
+        dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
+        dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
+      }
     }
 }
 

@@ -47,7 +47,7 @@ def decode(**change):
 CACHE = [(dict(kp=None), "EINVAL"), (dict(vp=None), "EINVAL"), (dict(ks=None), "EINVAL"), (dict(vs=None), "EINVAL"),
          (dict(table=None), "EINVAL"), (dict(kp=4104), "EINVAL"), (dict(vp=4097), "EINVAL"), (dict(ks=4098), "EINVAL"),
          (dict(vs=4097), "EINVAL"), (dict(table=4098), "EINVAL"), (dict(s=0), "EINVAL"), (dict(hkv=0), "EINVAL"), (dict(max_pages=0), "EINVAL"),
-         (dict(pool=0), "EINVAL"), (dict(s=65536), "EINVAL"), (dict(max_pages=2 ** 27), "EINVAL"), (dict(d=96), "EUNSUPPORTED"),
+         (dict(pool=0), "EINVAL"), (dict(s=65536), "EINVAL"), (dict(max_pages=2 ** 27), "EINVAL"), (dict(pool=2 ** 27), "EINVAL"), (dict(d=96), "EUNSUPPORTED"),
          (dict(d=256), "EUNSUPPORTED"), (dict(page=32), "EUNSUPPORTED")]
 
 
