@@ -172,7 +172,7 @@ def capi() -> ctypes.CDLL:
     lib.hk_paged_kv_append_fp8.restype = ci
     lib.hk_paged_kv_read_fp8.argtypes = [vp] * 9 + [ci] * 9 + [vp]
     lib.hk_paged_kv_read_fp8.restype = ci
-    lib.hk_attn_paged_decode_fp8_workspace_bytes.argtypes = [ci] * 7
+    lib.hk_attn_paged_decode_fp8_workspace_bytes.argtypes = [ci] * 3
     lib.hk_attn_paged_decode_fp8_workspace_bytes.restype = ctypes.c_size_t
     lib.hk_attn_paged_decode_fp8.argtypes = [vp] * 9 + [ci] * 9 + [cf, vp, ctypes.c_size_t, ci, vp]
     lib.hk_attn_paged_decode_fp8.restype = ci
@@ -1273,10 +1273,8 @@ def paged_kv_read_fp8(
     return outs[0], outs[1]
 
 
-def paged_decode_fp8_workspace_bytes(s: int, h: int, d: int, max_pages: int, page_size: int = 16, window: Optional[int] = None,
-                                     sinks: int = 0) -> int:
-    _check_window(window, sinks)
-    return int(capi().hk_attn_paged_decode_fp8_workspace_bytes(s, h, d, max_pages, page_size, window or 0, sinks))
+def paged_decode_fp8_workspace_bytes(s: int, hkv: int, d: int) -> int:
+    return int(capi().hk_attn_paged_decode_fp8_workspace_bytes(s, hkv, d))
 
 
 def paged_decode_fp8(
@@ -1320,13 +1318,11 @@ def paged_decode_fp8(
         raise RuntimeError("out must be a contiguous bf16 tensor of q's shape")
     if not isinstance(lse, torch.Tensor) or lse.shape != (s_n, h, 1, 1) or lse.dtype != torch.float32 or not lse.is_contiguous():
         raise RuntimeError("lse must be a contiguous fp32 tensor [S, H, 1, 1]")
-    need = paged_decode_fp8_workspace_bytes(s_n, h, d, max_pages, k_pages.shape[1], window, sinks)
+    need = paged_decode_fp8_workspace_bytes(s_n, hkv, d)
     if need == 0:
-        raise HkError(HK_EUNSUPPORTED, "hk_attn_paged_decode_fp8",
-                      "shape outside the decode kernels' limits (D = 64 or 128, 16-token pages, 1 <= S <= 65535, max_pages, or pages of "
-                      "a window and its sinks, <= 8192)")
+        raise HkError(HK_EUNSUPPORTED, "hk_attn_paged_decode_fp8", "shape outside the decode kernels' limits (D = 64 or 128, 1 <= S <= 65535)")
     if workspace is None:
-        workspace = _new(max(need, 256), torch.uint8, q.device, stream)  # it goes back to the stream that uses it
+        workspace = _new(need, torch.uint8, q.device, stream)  # it goes back to the stream that uses it
     if not isinstance(workspace, torch.Tensor) or not workspace.is_contiguous():
         raise RuntimeError("workspace must be a contiguous tensor")
     _require_same_device(k_pages, q=q, out=out, lse=lse, workspace=workspace)

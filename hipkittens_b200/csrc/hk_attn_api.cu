@@ -23,11 +23,6 @@
 
 using namespace hk_host;
 
-cudaError_t hk::launch_window_combine(const DecodeParams& p, int D, cudaStream_t stream) {
-  return launch_dependent(true, D == 128 ? paged_decode_combine_kernel<128, true> : paged_decode_combine_kernel<64, true>,
-                          dim3(p.H, p.S), D, 0, stream, p);
-}
-
 int hk_host::init_device(int device) {
   DeviceState& st = g_dev[device];
   cudaDeviceProp prop;

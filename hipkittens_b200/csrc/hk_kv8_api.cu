@@ -43,11 +43,6 @@ int launch_blocks(void (*fn)(Params), const Params& p, void* cuda_stream) {
   return HK_OK;
 }
 
-int decode_fp8_span(int max_pages, int window, int sinks) {
-  if (window < 0 || sinks < 0 || max_pages <= 0 || max_pages > 0x7fffffff / hk::kPageTokens) return 0;
-  return window == 0 ? max_pages : hk::decode_span_pages(max_pages, window, sinks);
-}
-
 }  // namespace
 
 extern "C" {
@@ -126,8 +121,9 @@ int hk_paged_kv_read_fp8(const void* k_pages, const void* v_pages, const float* 
   return launch_blocks(D == 128 ? hk::paged_kv_read_fp8_kernel<128> : hk::paged_kv_read_fp8_kernel<64>, p, cuda_stream);
 }
 
-size_t hk_attn_paged_decode_fp8_workspace_bytes(int S, int H, int D, int max_pages_per_seq, int page_size, int window, int sinks) {
-  return hk::decode_workspace_bytes(S, H, D, decode_fp8_span(max_pages_per_seq, window, sinks), page_size, true);
+size_t hk_attn_paged_decode_fp8_workspace_bytes(int S, int H_KV, int D) {
+  if (S <= 0 || S > 65535 || H_KV <= 0 || H_KV > 65535 || 1ll * S * H_KV > 0x3fffffff || (D != 64 && D != 128)) return 0;
+  return hk::decode_fp8_workspace_bytes(S, H_KV, D);
 }
 
 int hk_attn_paged_decode_fp8(const void* q, const void* k_pages, const void* v_pages, const float* k_scales, const float* v_scales,
@@ -141,13 +137,8 @@ int hk_attn_paged_decode_fp8(const void* q, const void* k_pages, const void* v_p
   if (H % H_KV != 0) return HK_EINVAL;
   if (H / H_KV > 8) return HK_EUNSUPPORTED;  // the heads of a group sit in the 8 columns of one product
   if (!aligned16(q) || !aligned16(o) || !aligned4(ctx_lens) || !aligned4(lse)) return HK_EINVAL;
-  const int span = decode_fp8_span(max_pages_per_seq, window, sinks);
-  if (!hk::decode_shape_supported(S, H_KV, span)) {
-    snprintf(g_cuda_err, sizeof(g_cuda_err), "paged decode supports up to %d pages of a context (got %d)",
-             hk::kMaxCombineSplits * hk::kChunkPagesMin, span);
-    return HK_EUNSUPPORTED;
-  }
-  const size_t need = hk::decode_workspace_bytes(S, H, D, span, page_size, true);
+  const size_t need = hk_attn_paged_decode_fp8_workspace_bytes(S, H_KV, D);
+  if (need == 0) return HK_EINVAL;
   if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255)) return HK_EWORKSPACE;
   DeviceState* st = nullptr;
   DeviceScope scope;
@@ -179,9 +170,9 @@ int hk_attn_paged_decode_fp8(const void* q, const void* k_pages, const void* v_p
   const int capacity = max_pages_per_seq * hk::kPageTokens;  // no context is longer
   p.window = window == 0 ? capacity : std::min(window, capacity);
   p.sinks = std::min(sinks, capacity);
-  p.span_pages = span;
+  p.span_pages = window == 0 ? max_pages_per_seq : hk::decode_span_pages(max_pages_per_seq, window, sinks);
   int launched = 0;
-  const cudaError_t e = hk::launch_paged_decode_fp8(tk, tv, p, D, st->decode_fp8, static_cast<cudaStream_t>(cuda_stream), &launched);
+  const cudaError_t e = hk::launch_paged_decode_fp8(tk, tv, p, D, window != 0, st->decode_fp8, static_cast<cudaStream_t>(cuda_stream), &launched);
   g_launches.fetch_add(launched, std::memory_order_relaxed);
   if (e != cudaSuccess) return cuda_fail(e, "fp8 decode launch");
   return HK_OK;

@@ -214,7 +214,4 @@ using ptx::mma_16816;
 
 }  // namespace dec
 
-// Merges the per-chunk partials that a split kernel with a window left in the workspace (hk_attn_api.cu).
-cudaError_t launch_window_combine(const DecodeParams& p, int D, cudaStream_t stream);
-
 }  // namespace hk

@@ -603,12 +603,12 @@ PyObject* paged_decode_fp8(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
       !fits({q->size(2)}))
     Py_RETURN_NONE;
   const int64_t h = q->size(2);
-  const size_t need = hk_attn_paged_decode_fp8_workspace_bytes(i32(c.s), i32(h), i32(c.d), i32(c.max_pages), i32(c.page), window, sinks);
+  const size_t need = hk_attn_paged_decode_fp8_workspace_bytes(i32(c.s), i32(c.hkv), i32(c.d));
   Tensor out, lse, ws;
   if (need == 0 || !output(a[8], *q, q->sizes(), at::kBFloat16, out) || !output(a[9], *q, {c.s, h, 1, 1}, at::kFloat, lse))
     Py_RETURN_NONE;
   if (a[10] == Py_None) {
-    if (!output(Py_None, *q, {int64_t(need < 256 ? 256 : need)}, at::kByte, ws)) Py_RETURN_NONE;
+    if (!output(Py_None, *q, {int64_t(need)}, at::kByte, ws)) Py_RETURN_NONE;
   } else {
     const Tensor* t = plain(a[10]);
     if (!dense(t, at::kByte, 1) || t->device() != q->device()) Py_RETURN_NONE;

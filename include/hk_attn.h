@@ -378,10 +378,10 @@ int hk_paged_kv_read_fp8(const void* k_pages, const void* v_pages, const float* 
                          int S, int rows, int H_KV, int D, int zero_tail, int page_size, int max_pages_per_seq, int num_pages,
                          int device, void* cuda_stream);
 
-/* hk_attn_paged_decode (window = 0 and sinks = 0) and hk_attn_paged_decode_window (window > 0) against such a cache. H / H_KV from 1 to 8;
- * the pages of a context, or those of a window and its sinks, at most 8192. The products take q, whose values over the power of two of
+/* hk_attn_paged_decode (window = 0 and sinks = 0) and hk_attn_paged_decode_window (window > 0) against such a cache. H / H_KV from 1 to 8,
+ * contexts of any length. The products take q, whose values over the power of two of
  * their row's largest become fp16, and P, which becomes bf16 after its page's scale; sums and statistics are fp32. */
-size_t hk_attn_paged_decode_fp8_workspace_bytes(int S, int H, int D, int max_pages_per_seq, int page_size, int window, int sinks);
+size_t hk_attn_paged_decode_fp8_workspace_bytes(int S, int H_KV, int D);
 int hk_attn_paged_decode_fp8(const void* q, const void* k_pages, const void* v_pages, const float* k_scales, const float* v_scales,
                              const int32_t* block_table, const int32_t* ctx_lens, void* o, float* lse, int S, int H, int H_KV, int D,
                              int page_size, int max_pages_per_seq, int num_pages, int window, int sinks, float softmax_scale,

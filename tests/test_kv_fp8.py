@@ -74,7 +74,7 @@ def test_read_refusals(native_built, change, code):
     (dict(q=None), "EINVAL"), (dict(lens=None), "EINVAL"), (dict(o=None), "EINVAL"), (dict(lse=None), "EINVAL"), (dict(q=4100), "EINVAL"),
     (dict(o=4104), "EINVAL"), (dict(lens=4097), "EINVAL"), (dict(lse=4098), "EINVAL"), (dict(h=0), "EINVAL"), (dict(hkv=3), "EINVAL"),
     (dict(window=-1), "EINVAL"), (dict(sinks=-1, window=5), "EINVAL"), (dict(sinks=1), "EINVAL"), (dict(h=18), "EUNSUPPORTED"),
-    (dict(max_pages=8193), "EUNSUPPORTED"), (dict(max_pages=10000, window=8192 * 16 + 2), "EUNSUPPORTED"),
+    (dict(s=65535, h=65535, hkv=65535), "EINVAL"),
     (dict(ws=None), "EWORKSPACE"), (dict(ws=4112), "EWORKSPACE"), (dict(ws_bytes=100), "EWORKSPACE"),
 ])
 def test_decode_refusals(native_built, change, code):
@@ -82,12 +82,10 @@ def test_decode_refusals(native_built, change, code):
 
 
 def test_workspace(native_built):
-    full = hk.paged_decode_fp8_workspace_bytes(4, 8, 128, 8192)
-    assert hk.paged_decode_fp8_workspace_bytes(4, 8, 128, 8192, window=100000000) == full
-    small = hk.paged_decode_fp8_workspace_bytes(4, 8, 64, 100000, window=500, sinks=4)
-    assert 0 < small < full
-    for bad in (dict(d=96), dict(page_size=8), dict(max_pages=8193), dict(s=0)):
-        assert hk.paged_decode_fp8_workspace_bytes(**(dict(s=4, h=8, d=128, max_pages=8, page_size=16) | bad)) == 0
+    # two parts of up to 8 heads for each warp of the GPU, in fp32
+    assert 0 < hk.paged_decode_fp8_workspace_bytes(4, 8, 64) < hk.paged_decode_fp8_workspace_bytes(4, 8, 128) < 1 << 25
+    for bad in (dict(d=96), dict(hkv=0), dict(s=0), dict(s=65536)):
+        assert hk.paged_decode_fp8_workspace_bytes(**(dict(s=4, hkv=8, d=128) | bad)) == 0
 
 
 def test_python_refuses_what_is_not_on_the_gpu(native_built):
