@@ -29,18 +29,11 @@ int fp8_cache(hk::Fp8Cache& c, const void* k_pages, const void* v_pages, const f
   return HK_OK;
 }
 
-// The units of 16 tokens of a call and with them its warps, `per_unit` each; false if there are too many for an int.
-bool fp8_warps(long long units, int per_unit, int* warps) {
+// The units of 16 tokens of a call, times what each takes; false if that is too many for an int.
+bool fp8_units(long long units, int per_unit, int* count) {
   const long long n = units * per_unit;
-  *warps = static_cast<int>(n);
+  *count = static_cast<int>(n);
   return n <= 0x7ffffff0ll;
-}
-
-template <typename Params>
-int launch_blocks(void (*fn)(Params), const Params& p, void* cuda_stream) {
-  HK_CUDA(hk::launch_dependent(true, fn, unsigned((p.warps + 7ll) / 8), 256, 0, static_cast<cudaStream_t>(cuda_stream), p));
-  g_launches.fetch_add(1, std::memory_order_relaxed);
-  return HK_OK;
 }
 
 }  // namespace
@@ -68,10 +61,17 @@ int hk_paged_kv_append_fp8(const void* k_new, const void* v_new, void* k_pages, 
     if (table_rows <= 0) return HK_EINVAL;
   }
   const long long units = cu_seqlens ? T / hk::kPageTokens + 2ll * S : S * ((T + 30ll) / hk::kPageTokens);
-  if (!fp8_warps(units, 2 * H_KV, &p.warps)) return HK_EINVAL;
+  const int warps = std::min(hk::kFp8AppendWarps, H_KV);
+  int blocks;  // with a head a warp
+  if (!fp8_units(units, 2 * ((H_KV + warps - 1) / warps), &blocks)) return HK_EINVAL;
   DeviceState* st = nullptr;
   DeviceScope scope;
   if ((rc = scope.enter(device, &st)) != HK_OK) return rc;
+  // Two heads a warp where there is more than the device holds at once: the next head's tokens come in meanwhile, and a page's tables
+  // serve twice as many. Prompts of 29,000 tokens, H_KV = 8, D = 128: 33.8 us, against 40.6; a token for each of 64 sequences: 4.4,
+  // against 3.6.
+  p.turns = blocks > 4 * st->sm_count ? 2 : 1;
+  const int groups = (H_KV + p.turns * warps - 1) / (p.turns * warps);
   p.c.status = st->status;
   p.rows.cu = cu_seqlens;
   p.rows.T = T;
@@ -83,16 +83,14 @@ int hk_paged_kv_append_fp8(const void* k_new, const void* v_new, void* k_pages, 
   p.start_pos = start_pos;
   p.cos = cos, p.sin = sin;
   p.R = rotary_dim, p.table_rows = table_rows;
-  p.fd_heads2 = hk::FastDiv(2 * H_KV);
-  p.fd_heads = hk::FastDiv(H_KV);
-  const int rot = !sin ? hk::kFp8Plain : flags & HK_FP8_TABLE_F32 ? hk::kFp8TableF32 : hk::kFp8TableBf16;
-  auto pick = [&](auto d) {
-    constexpr int kD = decltype(d)::value;
-    return rot == hk::kFp8Plain       ? hk::paged_kv_append_fp8_kernel<kD, hk::kFp8Plain>
-           : rot == hk::kFp8TableBf16 ? hk::paged_kv_append_fp8_kernel<kD, hk::kFp8TableBf16>
-                                      : hk::paged_kv_append_fp8_kernel<kD, hk::kFp8TableF32>;
-  };
-  return launch_blocks(D == 128 ? pick(std::integral_constant<int, 128>{}) : pick(std::integral_constant<int, 64>{}), p, cuda_stream);
+  p.fd_groups2 = hk::FastDiv(2 * groups);
+  p.fd_groups = hk::FastDiv(groups);
+  p.rotation = !sin ? hk::kFp8Plain : flags & HK_FP8_TABLE_F32 ? hk::kFp8TableF32 : hk::kFp8TableBf16;
+  auto* fn = D == 128 ? sin ? hk::paged_kv_append_fp8_kernel<128, true> : hk::paged_kv_append_fp8_kernel<128, false>
+                      : sin ? hk::paged_kv_append_fp8_kernel<64, true> : hk::paged_kv_append_fp8_kernel<64, false>;
+  HK_CUDA(hk::launch_dependent(true, fn, unsigned(units * 2 * groups), warps * 32, 0, static_cast<cudaStream_t>(cuda_stream), p));
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  return HK_OK;
 }
 
 int hk_paged_kv_read_fp8(const void* k_pages, const void* v_pages, const float* k_scales, const float* v_scales,
@@ -105,7 +103,7 @@ int hk_paged_kv_read_fp8(const void* k_pages, const void* v_pages, const float* 
   if (!k_out || !v_out || (!ctx_lens) == (!cu_seqlens) || rows <= 0) return HK_EINVAL;
   if (!aligned16(k_out) || !aligned16(v_out) || !aligned4(ctx_lens) || !aligned4(cu_seqlens)) return HK_EINVAL;
   const long long per_seq = (rows + 15ll) / hk::kPageTokens;
-  if (!fp8_warps(cu_seqlens ? rows / hk::kPageTokens + S + 1ll : S * per_seq, H_KV, &p.warps)) return HK_EINVAL;
+  if (!fp8_units(cu_seqlens ? rows / hk::kPageTokens + S + 1ll : S * per_seq, H_KV, &p.warps)) return HK_EINVAL;
   DeviceState* st = nullptr;
   DeviceScope scope;
   if ((rc = scope.enter(device, &st)) != HK_OK) return rc;
@@ -118,7 +116,10 @@ int hk_paged_kv_read_fp8(const void* k_pages, const void* v_pages, const float* 
   p.v_out = static_cast<__nv_bfloat16*>(v_out);
   p.zero_tail = zero_tail;
   p.fd_heads = hk::FastDiv(H_KV);
-  return launch_blocks(D == 128 ? hk::paged_kv_read_fp8_kernel<128> : hk::paged_kv_read_fp8_kernel<64>, p, cuda_stream);
+  auto* fn = D == 128 ? hk::paged_kv_read_fp8_kernel<128> : hk::paged_kv_read_fp8_kernel<64>;
+  HK_CUDA(hk::launch_dependent(true, fn, unsigned((p.warps + 7ll) / 8), 256, 0, static_cast<cudaStream_t>(cuda_stream), p));
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  return HK_OK;
 }
 
 size_t hk_attn_paged_decode_fp8_workspace_bytes(int S, int H_KV, int D) {

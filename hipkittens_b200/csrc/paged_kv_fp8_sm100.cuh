@@ -15,6 +15,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "attn_fwd_sm100.cuh"
 #include "paged_decode_common.cuh"
 #include "sm100_ptx.cuh"
@@ -44,14 +46,17 @@ namespace fp8 {
 // first token on (PER = 1) or for pages that it enters and leaves in the middle (PER = 2).
 template <int PER>
 __device__ __forceinline__ int first_unit(const int32_t* cu, int s) { return (cu[s] >> 4) + PER * s; }
-// The last sequence of `n` that starts at or before `unit`. Whatever cu holds, it is one of them.
+// The last sequence of `n` that starts at or before `unit`; all lanes of a warp look, at 32 sequences a turn. Whatever cu holds, it is
+// one of them.
 template <int PER>
 __device__ __forceinline__ int sequence_of(const int32_t* cu, int n, int unit) {
-  int lo = 0, hi = n - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (first_unit<PER>(cu, mid) <= unit) lo = mid;
-    else hi = mid - 1;
+  int lo = 0;
+  while (n > 1) {
+    const int step = (n + 31) >> 5, at = static_cast<int>(threadIdx.x & 31) * step;
+    const uint32_t before = __ballot_sync(0xffffffffu, at < n && first_unit<PER>(cu, lo + at) <= unit) | 1u;
+    const int skip = (31 - __clz(before)) * step;
+    lo += skip;
+    n = min(step, n - skip);
   }
   return lo;
 }
@@ -81,6 +86,16 @@ __device__ __forceinline__ float2 bf16x2(uint32_t w) {
   return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 
+// Loads from shared memory that stay where they are: moved up, eight rows of them would not fit in the registers.
+__device__ __forceinline__ uint2 lds2(uint32_t at) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ void lds4(uint32_t at, uint64_t (&v)[2]) {
+  asm volatile("ld.shared.v2.u64 {%0, %1}, [%2];" : "=l"(v[0]), "=l"(v[1]) : "r"(at) : "memory");
+}
+
 // Bits of the scale for a largest magnitude, given by its bits: NaN for NaN, which makes the whole block NaN for every reader.
 __device__ __forceinline__ uint32_t scale_bits(uint32_t amax) {
   if (amax > 0x7f800000u) return 0x7fc00000u;
@@ -93,13 +108,21 @@ __device__ __forceinline__ float max_size(float a, float x, float y) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(fabsf(x)), "f"(fabsf(y)));
   return d;
 }
-// x / scale for four values at a time, as codes. Exact through the reciprocal of a power of two; a scale that another quantiser left
-// behind divides.
+// x / scale for four values at a time, as codes. Exact through the reciprocal of a power of two (an append's own scales are powers, or
+// NaN); a scale that another quantiser left behind divides.
 struct ByPower {
   uint64_t inv2;
+  __device__ __forceinline__ explicit ByPower(uint32_t bits) {
+    const float inv = __uint_as_float(bits > 0x7f800000u ? bits : (254u << 23) - bits);
+    inv2 = ptx::pack2(inv, inv);
+  }
   __device__ __forceinline__ uint32_t operator()(float a, float b, float c, float d) const {
-    ptx::unpack2(ptx::mul2(ptx::pack2(a, b), inv2), a, b);
-    ptx::unpack2(ptx::mul2(ptx::pack2(c, d), inv2), c, d);
+    return (*this)(ptx::pack2(a, b), ptx::pack2(c, d));
+  }
+  __device__ __forceinline__ uint32_t operator()(uint64_t ab, uint64_t cd) const {
+    float a, b, c, d;
+    ptx::unpack2(ptx::mul2(ab, inv2), a, b);
+    ptx::unpack2(ptx::mul2(cd, inv2), c, d);
     return encode4(a, b, c, d);
   }
 };
@@ -108,19 +131,23 @@ struct ByDivision {
   __device__ __forceinline__ uint32_t operator()(float a, float b, float c, float d) const {
     return encode4(__fdiv_rn(a, scale), __fdiv_rn(b, scale), __fdiv_rn(c, scale), __fdiv_rn(d, scale));
   }
+  __device__ __forceinline__ uint32_t operator()(uint64_t ab, uint64_t cd) const {
+    float a, b, c, d;
+    ptx::unpack2(ab, a, b);
+    ptx::unpack2(cd, c, d);
+    return (*this)(a, b, c, d);
+  }
 };
 template <typename Fn>
 __device__ __forceinline__ void with_divisor(uint32_t bits, const Fn& fn) {
   const int e = static_cast<int>(bits >> 23);
-  if ((bits & 0x807fffffu) == 0 && e > 0 && e < 254) {
-    const float inv = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
-    fn(ByPower{ptx::pack2(inv, inv)});
-  } else {
-    fn(ByDivision{__uint_as_float(bits)});
-  }
+  if ((bits & 0x807fffffu) == 0 && e > 0 && e < 254) fn(ByPower(bits));
+  else fn(ByDivision{__uint_as_float(bits)});
 }
 
 }  // namespace fp8
+
+enum Fp8Rotation : int { kFp8Plain = 0, kFp8TableBf16 = 1, kFp8TableF32 = 2 };
 
 struct AppendFp8Params {
   Fp8Cache c;
@@ -129,30 +156,38 @@ struct AppendFp8Params {
   long long k_stride[3], v_stride[3];  // sequence, token, head; elements
   const int32_t* start_pos;            // [S] position of the first new token of each sequence
   const void *cos, *sin;               // [table_rows, R / 2] bf16 or fp32
+  int rotation;                        // Fp8Rotation
   int R, table_rows;
-  int warps;                           // units x H_KV x 2
-  FastDiv fd_heads2, fd_heads;         // 2 * H_KV, H_KV
+  int turns;                           // heads of a warp
+  FastDiv fd_groups2, fd_groups;       // 2 * groups, groups of kFp8AppendWarps x turns heads
 };
 
-enum Fp8Rotation : int { kFp8Plain = 0, kFp8TableBf16 = 1, kFp8TableF32 = 2 };
+constexpr int kFp8AppendWarps = 4, kFp8AppendStages = 2;
 
-// A warp has one block: a page's new tokens of one head, of K or of V, all requested before the first is looked at (8 x 16 bytes a
-// lane at D = 128). It finds their largest magnitude, settles the scale, and writes the codes; if the page had tokens already and the
-// scale grows, it reads and rounds anew the rows that get none. Nothing else touches that block, so there is nothing to order.
-// The heads of a page, and K and V, are neighbouring warps: they share its rows of the tables in L1, and lines of the page.
-// Bound by HBM (3 bytes a value); a token for each sequence is a launch and two dependent loads.
-template <int D, int ROT>
-__global__ void __launch_bounds__(256) paged_kv_append_fp8_kernel(const __grid_constant__ AppendFp8Params p) {
+// A CTA has new tokens of a page, of K or of V, and its warps have a block at a time: a head's tokens of the page, and those of the
+// next head already on their way. A warp finds the block's largest magnitude, settles the scale, and writes the codes; if the page had
+// tokens already and the scale grows, it reads and rounds anew the rows that get none. Nothing else touches that block, so there is
+// nothing to order. The rows of the tables that the page's tokens need are brought in once, as fp32, for all of the CTA's heads: with
+// them read from L1 by every warp, and a warp's tokens in its registers from the start, prompts of 29,000 tokens at H_KV = 8 and D = 128
+// took 66 us.
+// Bound by HBM (3 bytes a value): those take 34 us, 80% of the copy rate, and 30 without a rotation; a token for each sequence is a
+// launch and three dependent loads.
+// grid = units x 2 x groups of heads; block = 32 * min(kFp8AppendWarps, H_KV).
+template <int D, bool ROT>
+__global__ void __launch_bounds__(kFp8AppendWarps * 32, ROT ? 4 : 5) paged_kv_append_fp8_kernel(const __grid_constant__ AppendFp8Params p) {
+  constexpr int kLanes = D / 8, kRows = 32 / kLanes, kSteps = kPageTokens / kRows;  // lanes of a row, rows of a step
+  constexpr int kTile = kPageTokens * D * 2;
+  __shared__ __align__(16) uint8_t rings[kFp8AppendWarps][kFp8AppendStages * kTile];
+  __shared__ __align__(16) float tables[ROT ? 2 : 1][ROT ? kPageTokens * D / 2 : 1];  // cos, sin: [16, R / 2]
   ptx::grid_dep_wait();
   ptx::grid_dep_launch();
   const Fp8Cache& c = p.c;
   const int32_t* const cu = p.rows.cu;
   if (cu && blockIdx.x == 0) fp8::check_cu(cu, c.S, p.rows.T, c.status);
-  const int w = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (w >= p.warps) return;
-  int unit, rem, head, is_v;
-  p.fd_heads2.divmod(w, unit, rem);
-  p.fd_heads.divmod(rem, is_v, head);
+  const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+  int unit, rem, group, is_v;
+  p.fd_groups2.divmod(blockIdx.x, unit, rem);
+  p.fd_groups.divmod(rem, is_v, group);
   int s, block, n = p.rows.T, first = 0;
   if (cu) {
     s = fp8::sequence_of<2>(cu, c.S, unit);
@@ -166,131 +201,179 @@ __global__ void __launch_bounds__(256) paged_kv_append_fp8_kernel(const __grid_c
   int r1 = static_cast<int>(min(n - base, static_cast<long long>(kPageTokens)));
   if (block < 0 || r1 <= r0) return;
   if (slot < 0 || slot >= c.max_pages) {
-    if (lane == 0) atomicCAS(c.status, 0, kStatusBadPage);
+    if (threadIdx.x == 0) atomicCAS(c.status, 0, kStatusBadPage);
     return;
   }
   const int id = c.block_table[static_cast<size_t>(s) * c.max_pages + slot];
+  if (ROT && slot * kPageTokens + r1 > p.table_rows) {  // tokens behind the tables are not written
+    if (threadIdx.x == 0) atomicCAS(c.status, 0, kStatusBadPos);
+    r1 = static_cast<int>(p.table_rows - slot * kPageTokens);
+    if (r1 <= r0) return;
+  }
+
+  const int row0 = lane / kLanes, col = (lane % kLanes) * 8;
+  const int head0 = group * p.turns * warps + warp, heads = min(p.turns, (c.H_KV - head0 + warps - 1) / warps);  // every warps-th from head0 on
+  const long long* const stride = is_v ? p.v_stride : p.k_stride;
+  const __nv_bfloat16* const src = (is_v ? p.v_new : p.k_new) + s * stride[0] + (first + base + row0) * stride[1] + col;
+  uint8_t* const ring = rings[warp];
+  const uint32_t ring_u32 = ptx::smem_u32(ring) + (row0 * D + col) * 2;
+  auto request = [&](int turn) {  // rows that are not new become zeros
+    const __nv_bfloat16* at = src + (head0 + turn * warps) * stride[2];
+    uint32_t to = ring_u32 + (turn % kFp8AppendStages) * kTile;
+#pragma unroll
+    for (int r = row0; r < kPageTokens; r += kRows, at += kRows * stride[1], to += kRows * D * 2)
+      dec::cp_async16_if(to, at, r >= r0 && r < r1);
+    dec::cp_async_commit();
+  };
+  if (heads > 0) request(0);
+  if (ROT && !is_v) {
+    const int quads = p.R / 8;  // of a row
+    for (int i = r0 * quads + threadIdx.x; i < r1 * quads; i += blockDim.x) {
+      const size_t at = static_cast<size_t>(slot) * kPageTokens * quads + i;
+      float4 cs, sn;
+      if (p.rotation == kFp8TableF32) {
+        cs = static_cast<const float4*>(p.cos)[at], sn = static_cast<const float4*>(p.sin)[at];
+      } else {
+        const uint2 a = static_cast<const uint2*>(p.cos)[at], b = static_cast<const uint2*>(p.sin)[at];
+        const float2 a0 = fp8::bf16x2(a.x), a1 = fp8::bf16x2(a.y), b0 = fp8::bf16x2(b.x), b1 = fp8::bf16x2(b.y);
+        cs = make_float4(a0.x, a0.y, a1.x, a1.y), sn = make_float4(b0.x, b0.y, b1.x, b1.y);
+      }
+      reinterpret_cast<float4*>(tables[0])[i] = cs;
+      reinterpret_cast<float4*>(tables[ROT ? 1 : 0])[i] = sn;
+    }
+    __syncthreads();
+  }
   if (id < 0 || id >= c.num_pages) {  // never write through an id outside the pool
-    if (lane == 0) atomicCAS(c.status, 0, kStatusBadPage);
+    if (threadIdx.x == 0) atomicCAS(c.status, 0, kStatusBadPage);
+    dec::cp_async_wait<0>();
     return;
   }
-  if constexpr (ROT != kFp8Plain) {
-    if (slot * kPageTokens + r1 > p.table_rows) {  // tokens behind the tables are not written
-      if (lane == 0) atomicCAS(c.status, 0, kStatusBadPos);
-      r1 = static_cast<int>(p.table_rows - slot * kPageTokens);
-      if (r1 <= r0) return;
-    }
-  }
-
-  constexpr int kLanes = D / 8, kRows = 32 / kLanes, kSteps = kPageTokens / kRows;  // lanes of a row, rows of a step
-  const int col = (lane % kLanes) * 8, row0 = lane / kLanes;
-  const long long* const stride = is_v ? p.v_stride : p.k_stride;
-  const __nv_bfloat16* const src = (is_v ? p.v_new : p.k_new) + s * stride[0] + (first + base) * stride[1] + head * stride[2] + col;
-  uint4 x[kSteps];
-#pragma unroll
-  for (int i = 0; i < kSteps; ++i) {
-    const int r = row0 + i * kRows;
-    x[i] = make_uint4(0, 0, 0, 0);
-    if (r >= r0 && r < r1) x[i] = __ldcs(reinterpret_cast<const uint4*>(src + r * stride[1]));
-  }
-  float* const scale_at = (is_v ? c.v_scales : c.k_scales) + static_cast<size_t>(id) * c.H_KV + head;
-  const uint32_t before = r0 > 0 ? __float_as_uint(*scale_at) : 0u;  // a page that starts anew has no scale yet
 
   const size_t row_bytes = static_cast<size_t>(c.H_KV) * D;
-  uint8_t* const page = (is_v ? c.v_pages : c.k_pages) + static_cast<size_t>(id) * kPageTokens * row_bytes + head * D + col;
-  // From the largest magnitude on: the scale, the codes of the new rows (`row(i, divide)`: those of a lane's 8 values in step i), and where
-  // the scale has grown the other rows'.
-  auto finish = [&](uint32_t amax, auto&& row) {
-    uint32_t bits = fp8::scale_bits(__reduce_max_sync(0xffffffffu, amax));
-    if (r0 > 0) {
-      if ((before & 0x7fffffffu) > 0x7f800000u) bits = 0x7fc00000u;
-      else if (static_cast<int>(before) > static_cast<int>(bits)) bits = before;  // of floats above zero
-    }
-    fp8::with_divisor(bits, [&](auto divide) {
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        const int r = row0 + i * kRows;
-        if (r >= r0 && r < r1) *reinterpret_cast<uint2*>(page + r * row_bytes) = row(i, divide);
-      }
-      if (r0 > 0 && bits != before) {
-        const float old = __uint_as_float(before);
+  // FULL: all of the page's rows are new. TURN: these heads are rotated.
+  auto work = [&](auto full_c, auto turn_c) {
+    constexpr bool FULL = decltype(full_c)::value, TURN = decltype(turn_c)::value;
+    // A lane has 8 neighbouring values of a row, or where they are turned 4 and their 4 partners, half the rotated columns further on.
+    const bool turned = TURN && col < p.R;
+    const int col0 = turned ? col / 2 : col, col1 = turned ? (col + p.R) / 2 : col + 4;
+    auto is_new = [&](int i) { return FULL || (row0 + i * kRows >= r0 && row0 + i * kRows < r1); };
 #pragma unroll 1
-        for (int r = row0; r < kPageTokens; r += kRows) {
-          if (r >= r0 && r < r1) continue;
-          const uint2 v = *reinterpret_cast<const uint2*>(page + r * row_bytes);
-          auto anew = [&](uint32_t codes) {
-            const float2 a = fp8::decode2(codes), b = fp8::decode2(codes >> 16);
-            return divide(a.x * old, a.y * old, b.x * old, b.y * old);
-          };
-          *reinterpret_cast<uint2*>(page + r * row_bytes) = make_uint2(anew(v.x), anew(v.y));
-        }
-      }
-    });
-    if (lane == 0 && (r0 == 0 || bits != before)) *scale_at = __uint_as_float(bits);
-  };
-
-  if (ROT == kFp8Plain || is_v) {
-    uint32_t two = 0;
+    for (int turn = 0; turn < heads; ++turn) {
+      const int head = head0 + turn * warps;
+      float* const scale_at = (is_v ? c.v_scales : c.k_scales) + static_cast<size_t>(id) * c.H_KV + head;
+      uint8_t* const page = (is_v ? c.v_pages : c.k_pages) + static_cast<size_t>(id) * kPageTokens * row_bytes + head * D;
+      const uint32_t before = !FULL && r0 > 0 ? __float_as_uint(*scale_at) : 0u;  // a page that starts anew has no scale yet
+      // From the largest magnitude on: the scale, the codes of the new rows (`row(i, divide)`: those of a lane's 8 values in step i), and
+      // where the scale has grown the other rows'.
+      auto finish = [&](uint32_t amax, auto&& row) {
+        uint32_t bits = fp8::scale_bits(__reduce_max_sync(0xffffffffu, amax));
+        auto write = [&](auto divide) {
+          uint8_t* at = page + row0 * row_bytes;
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i)
-      for (uint32_t v : {x[i].x, x[i].y, x[i].z, x[i].w}) two = __vmaxu2(two, v & 0x7fff7fffu);
-    finish(max(two & 0xffff0000u, two << 16), [&](int i, auto divide) {
-      const float2 a = fp8::bf16x2(x[i].x), b = fp8::bf16x2(x[i].y), d = fp8::bf16x2(x[i].z), e = fp8::bf16x2(x[i].w);
-      return make_uint2(divide(a.x, a.y, b.x, b.y), divide(d.x, d.y, e.x, e.y));
-    });
-  } else if constexpr (ROT != kFp8Plain) {
-    // pairs are (i, i + R / 2): a cos - b sin for the lanes that have a, b cos + a sin for those that have b, which send -b
-    const int half = p.R / 2;
-    const bool first_half = col < half, turned = col < p.R;
-    const int partner = (lane + (first_half ? half / 8 : -half / 8)) & 31, at = first_half ? col : col - half;
-    const uint32_t flip = first_half ? 0u : 0x80008000u;
-    uint64_t y[kSteps][4];
-    float amax = 0.f;
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-      const int r = row0 + i * kRows;
-      const uint32_t xw[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-      uint64_t cs[4], sn[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) cs[j] = ptx::pack2(1.f, 1.f), sn[j] = ptx::pack2(0.f, 0.f);
-      if (turned && r >= r0 && r < r1) {
-        const size_t t = static_cast<size_t>(slot * kPageTokens + r) * half + at;
-        if constexpr (ROT == kFp8TableF32) {
-          const float4 *const c4 = reinterpret_cast<const float4*>(static_cast<const float*>(p.cos) + t),
-                       *const s4 = reinterpret_cast<const float4*>(static_cast<const float*>(p.sin) + t);
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float4 a = c4[j], b = s4[j];
-            cs[2 * j] = ptx::pack2(a.x, a.y), cs[2 * j + 1] = ptx::pack2(a.z, a.w);
-            sn[2 * j] = ptx::pack2(b.x, b.y), sn[2 * j + 1] = ptx::pack2(b.z, b.w);
+          for (int i = 0; i < kSteps; ++i, at += kRows * row_bytes) {
+            if (!is_new(i)) continue;
+            const uint2 codes = row(i, divide);
+            if constexpr (TURN) {
+              *reinterpret_cast<uint32_t*>(at + col0) = codes.x;
+              *reinterpret_cast<uint32_t*>(at + col1) = codes.y;
+            } else {
+              *reinterpret_cast<uint2*>(at + col) = codes;
+            }
           }
-        } else {
-          const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.cos) + t),
-                      b = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.sin) + t);
-          const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+        };
+        if (FULL) {
+          write(fp8::ByPower(bits));
+          if (lane == 0) *scale_at = __uint_as_float(bits);
+          return;
+        }
+        if (r0 > 0) {
+          if ((before & 0x7fffffffu) > 0x7f800000u) bits = 0x7fc00000u;
+          else if (static_cast<int>(before) > static_cast<int>(bits)) bits = before;  // of floats above zero
+        }
+        fp8::with_divisor(bits, [&](auto divide) {
+          write(divide);
+          if (r0 > 0 && bits != before) {
+            const float old = __uint_as_float(before);
+#pragma unroll 1
+            for (int r = row0; r < kPageTokens; r += kRows) {
+              if (r >= r0 && r < r1) continue;
+              uint2* const at = reinterpret_cast<uint2*>(page + r * row_bytes + col);
+              const uint2 v = *at;
+              auto anew = [&](uint32_t codes) {
+                const float2 a = fp8::decode2(codes), b = fp8::decode2(codes >> 16);
+                return divide(a.x * old, a.y * old, b.x * old, b.y * old);
+              };
+              *at = make_uint2(anew(v.x), anew(v.y));
+            }
+          }
+        });
+        if (lane == 0 && (r0 == 0 || bits != before)) *scale_at = __uint_as_float(bits);
+      };
+
+      __syncwarp();  // the tile that the next tokens go to has been read
+      if (turn + 1 < heads) {
+        request(turn + 1);
+        dec::cp_async_wait<1>();
+      } else {
+        dec::cp_async_wait<0>();
+      }
+      __syncwarp();
+      const uint8_t* const tile = ring + (turn % kFp8AppendStages) * kTile + row0 * D * 2;
+      if constexpr (!TURN) {
+        auto values = [&](int i) { return *reinterpret_cast<const uint4*>(tile + (i * kRows * D + col) * 2); };
+        uint32_t two = 0;
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+          const uint4 x = values(i);
+          for (uint32_t v : {x.x, x.y, x.z, x.w}) two = __vmaxu2(two, v & 0x7fff7fffu);
+        }
+        finish(max(two & 0xffff0000u, two << 16), [&](int i, auto divide) {
+          const uint4 x = values(i);
+          const float2 a = fp8::bf16x2(x.x), b = fp8::bf16x2(x.y), d = fp8::bf16x2(x.z), e = fp8::bf16x2(x.w);
+          return make_uint2(divide(ptx::pack2(a.x, a.y), ptx::pack2(b.x, b.y)), divide(ptx::pack2(d.x, d.y), ptx::pack2(e.x, e.y)));
+        });
+      } else {
+        // a pair (i, i + R / 2) becomes (a cos - b sin, b cos + a sin)
+        uint64_t y[kSteps][4];
+        float amax = 0.f;
+        const float* const cs_at = tables[0] + row0 * (p.R / 2) + col0;
+        const uint32_t at0 = ptx::smem_u32(cs_at), step = kRows * (p.R / 2) * 4, x0 = ptx::smem_u32(tile);
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+          const uint2 xa = fp8::lds2(x0 + (i * kRows * D + col0) * 2), xb = fp8::lds2(x0 + (i * kRows * D + col1) * 2);
+          const uint32_t words[4] = {xa.x, xa.y, xb.x, xb.y};
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const float2 ca = fp8::bf16x2(aw[j]), sa = fp8::bf16x2(bw[j]);
-            cs[j] = ptx::pack2(ca.x, ca.y), sn[j] = ptx::pack2(sa.x, sa.y);
+            const float2 v = fp8::bf16x2(words[j]);
+            y[i][j] = ptx::pack2(v.x, v.y);
+          }
+          if (turned && is_new(i)) {
+            uint64_t cs[2], sn[2];
+            fp8::lds4(at0 + i * step, cs);
+            fp8::lds4(at0 + i * step + static_cast<uint32_t>(sizeof(tables[0])), sn);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const uint64_t a2 = y[i][j], b2 = y[i][j + 2];
+              y[i][j] = ptx::fma2(ptx::mul2(b2, sn[j]), ptx::pack2(-1.f, -1.f), ptx::mul2(a2, cs[j]));
+              y[i][j + 2] = ptx::add2(ptx::mul2(b2, cs[j]), ptx::mul2(a2, sn[j]));
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float lo, hi;
+            ptx::unpack2(y[i][j], lo, hi);
+            amax = fp8::max_size(amax, lo, hi);
           }
         }
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 own = fp8::bf16x2(xw[j]), other = fp8::bf16x2(__shfl_sync(0xffffffffu, xw[j] ^ flip, partner));
-        const uint64_t own2 = ptx::pack2(own.x, own.y);
-        y[i][j] = turned ? ptx::add2(ptx::mul2(own2, cs[j]), ptx::mul2(ptx::pack2(other.x, other.y), sn[j])) : own2;
-        float lo, hi;
-        ptx::unpack2(y[i][j], lo, hi);
-        amax = fp8::max_size(amax, lo, hi);
+        finish(__float_as_uint(amax), [&](int i, auto divide) { return make_uint2(divide(y[i][0], y[i][1]), divide(y[i][2], y[i][3])); });
       }
     }
-    finish(__float_as_uint(amax), [&](int i, auto divide) {
-      float v[8];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) ptx::unpack2(y[i][j], v[2 * j], v[2 * j + 1]);
-      return make_uint2(divide(v[0], v[1], v[2], v[3]), divide(v[4], v[5], v[6], v[7]));
-    });
+  };
+  const bool full = r0 == 0 && r1 == kPageTokens;
+  if (!ROT || is_v) {
+    full ? work(std::true_type{}, std::false_type{}) : work(std::false_type{}, std::false_type{});
+  } else if constexpr (ROT) {
+    full ? work(std::true_type{}, std::true_type{}) : work(std::false_type{}, std::true_type{});
   }
 }
 

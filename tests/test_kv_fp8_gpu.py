@@ -170,6 +170,28 @@ def test_append_rotates(dev, hkv, d, rot, n, start, dtype):
     assert status() == _native.HK_OK
 
 
+@pytest.mark.parametrize("hkv,d,rot", [(13, 128, 128), (8, 64, 32), (5, 128, 0), (1, 64, 64)])
+def test_many_pages_and_heads_are_as_one_sequence_at_a_time(dev, hkv, d, rot):
+    """More of them than are worked on at once, where a warp takes two heads: bit for bit what a call for each sequence leaves."""
+    s, width = 40, 26
+    cache, other = (Cache(dev, s * width, hkv, d, s, width, seed=17) for _ in range(2))
+    gen = torch.Generator().manual_seed(18)
+    lens = [390, 0, 1] + torch.randint(100, 390, (s - 3,), generator=gen).tolist()
+    start = torch.randint(0, 20, (s,), generator=gen).tolist()
+    cu = [sum(lens[:i]) for i in range(s + 1)]
+    x = torch.randn(cu[-1], 2, hkv, d, generator=gen).to(torch.bfloat16).to(dev)
+    angle = torch.arange(416)[:, None] / 100.0 ** (torch.arange(0, rot, 2) / max(rot, 1))
+    turn = dict(cos=angle.cos().to(dev), sin=angle.sin().to(dev)) if rot else {}
+    hk.paged_kv_append_fp8(x[:, 0], x[:, 1], *cache.gpu, int32(dev, start), cu_seqlens=int32(dev, cu), **turn)
+    for i in range(s):
+        if lens[i]:
+            rows = x[None, cu[i]:cu[i + 1]]
+            hk.paged_kv_append_fp8(rows[:, :, 0], rows[:, :, 1], *other.gpu[:4], other.gpu[4][i:i + 1], int32(dev, start[i:i + 1]), **turn)
+    for got, want in zip(cache.gpu, other.gpu):
+        assert torch.equal(got.view(torch.uint8), want.view(torch.uint8))
+    assert status() == _native.HK_OK
+
+
 def test_values_at_the_ends(dev):
     """Zeros, infinities, NaN, the smallest and largest bf16 values: each in a block of its own, beside one that it does not touch."""
     hkv, d = 2, 64
