@@ -635,6 +635,7 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   using namespace ptx;
   constexpr int MASK = static_cast<int>(KIND);
   constexpr bool CAUSAL = MASK != kMaskNone, WINDOW = MASK == kMaskWindow, RAGGED = MASK == kMaskRagged;
+  static_assert(!(RAGGED && SPLIT));
   using SM = BwdSmem<D>;
   constexpr int kTile = SM::kTileBytes;
   constexpr int kSub = SM::kSubTileBytes;
@@ -710,16 +711,12 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     n_rounds = (n_planned + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
   }
   auto rounds = [&]() -> int {
-    if constexpr (RAGGED && !SPLIT) return n_rounds;
+    if constexpr (RAGGED) return n_rounds;
     else return p.total_rounds;
   };
   auto item_of_round = [&](int round) -> int {
-    if constexpr (RAGGED) {
-      if constexpr (SPLIT) return planned_item(n_planned, round, p.fd_split.div(blockIdx.x), p.n_items);
-      else return planned_item(n_planned, round, blockIdx.x, gridDim.x);
-    } else {
-      return dkdv_item_for_round<MASK, SPLIT>(p, round);
-    }
+    if constexpr (RAGGED) return planned_item(n_planned, round, blockIdx.x, gridDim.x);
+    else return dkdv_item_for_round<MASK, SPLIT>(p, round);
   };
   const int G = p.G;
   // TMEM columns: X [0,128) takes the two score-shaped products in turn, S^T(n) then dP^T(n), each free again as soon
@@ -969,7 +966,7 @@ attn_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       __syncwarp();
       cluster_arrive();
       cluster_wait();
-      if (ok && (!RAGGED || item_of_round(0) >= 0)) {
+      if (ok) {
         // every n-th row of the key block is added up here
         const DkdvItemOf<MASK> w = decode_dkdv_item<MASK, SPLIT>(p, item_of_round(0));
         constexpr int kUnits = 2 * (D / 8);         // 8 columns each: dK, then dV

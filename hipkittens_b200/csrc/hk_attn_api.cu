@@ -470,7 +470,7 @@ int launch_bwd_window(const CUtensorMap& tq, const CUtensorMap& tk, const CUtens
 
 }  // namespace
 
-int hk_host::prep_launch(const void* o, const void* d_o, float* delta, int B, int N, int H, int D, cudaStream_t stream) {
+static int prep_launch(const void* o, const void* d_o, float* delta, int B, int N, int H, int D, cudaStream_t stream) {
   const long long rows = static_cast<long long>(B) * N * H;
   if (rows > 0x7fffffffll) return HK_EINVAL;  // rows are indexed with int
   const int rows_per_block = hk::row_pass_rows(D / 8);

@@ -68,8 +68,6 @@ inline DeviceState g_dev[kMaxDevices];
 // The first call on a device, and the first with a window there (hk_attn_api.cu).
 int init_device(int device);
 int init_windows();
-// delta of a backward (hk_attn_api.cu).
-int prep_launch(const void* o, const void* d_o, float* delta, int B, int N, int H, int D, cudaStream_t stream);
 
 template <int D, auto KIND, bool DEP>
 int prepare_fwd_kernel() {

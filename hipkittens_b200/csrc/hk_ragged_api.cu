@@ -28,13 +28,6 @@ int init_ragged(DeviceState* st) {
   return HK_OK;
 }
 
-int launch_plan(const hk::RaggedPlanParams& p, cudaStream_t stream) {
-  const int grid = p.lists + (p.rests ? hk::kPlanRestBlocks : 0);
-  HK_CUDA(hk::launch_dependent(true, hk::ragged_plan_kernel, unsigned(grid), hk::kPlanThreads, 0, stream, p));
-  g_launches.fetch_add(1, std::memory_order_relaxed);
-  return HK_OK;
-}
-
 // What both directions ask of their arguments. Rows may be none, and pointers to none null.
 int check_ragged(std::initializer_list<const void*> q_rows, std::initializer_list<const void*> k_rows, const int32_t* cu_q, const int32_t* cu_k,
                  const float* lse, int S, int Tq, int Tk, int H, int H_KV, int D, std::initializer_list<const long long*> strides) {
@@ -107,7 +100,8 @@ int hk_attn_fwd_ragged(const void* q, const void* k, const void* v, void* o, flo
     plan.rest[1] = {lse, 1, q_rows, H, q_rows, 0, 0};
   }
   plan.status = st->status;
-  if ((rc = launch_plan(plan, stream)) != HK_OK) return rc;
+  const int plan_grid = plan.lists + (plan.rests ? hk::kPlanRestThreads / hk::kPlanThreads : 0);
+  HK_CUDA(hk::launch_dependent(true, hk::ragged_plan_kernel, unsigned(plan_grid), hk::kPlanThreads, 0, stream, plan));
   p.o = static_cast<__nv_bfloat16*>(o);
   p.lse = lse;
   p.B = 1, p.N = q_rows, p.NK = k_rows, p.H = H, p.H_KV = H_KV;
@@ -126,7 +120,7 @@ int hk_attn_fwd_ragged(const void* q, const void* k, const void* v, void* o, flo
   auto* fn = D == 128 ? hk::attn_fwd_kernel<128, hk::kMaskRagged, true> : hk::attn_fwd_kernel<64, hk::kMaskRagged, true>;
   const int smem = D == 128 ? hk::FwdSmem<128, true>::kDynBytes : hk::FwdSmem<64, true>::kDynBytes;
   HK_CUDA(hk::launch_dependent(true, fn, unsigned(grid), hk::kFwdThreads, smem, stream, tq, tk, tv, to, p));
-  g_launches.fetch_add(1, std::memory_order_relaxed);
+  g_launches.fetch_add(2, std::memory_order_relaxed);
   return HK_OK;
 }
 
@@ -145,6 +139,7 @@ int hk_attn_bwd_ragged(const void* q, const void* k, const void* v, const void* 
                         {q_strides, k_strides, v_strides, dq_strides, dk_strides, dv_strides});
   if (rc != HK_OK) return rc;
   if ((q_rows > 0 && !delta) || !aligned4(delta)) return HK_EINVAL;
+  if (1ll * q_rows * H > 0x7fffffffll) return HK_EINVAL;  // rows are indexed with int
   if (!workspace || workspace_bytes < hk_attn_bwd_ragged_workspace_bytes(S, q_rows, k_rows) || (reinterpret_cast<uintptr_t>(workspace) & 255))
     return HK_EWORKSPACE;
   if (q_rows == 0 && k_rows == 0) return HK_OK;
@@ -162,7 +157,8 @@ int hk_attn_bwd_ragged(const void* q, const void* k, const void* v, const void* 
   if (q_rows == 0) tq = tdo = tk;  // of no rows nothing is loaded
   if (k_rows == 0) tk = tv = tq;
   cudaStream_t stream = static_cast<cudaStream_t>(cuda_stream);
-  hk::RaggedPlanParams plan = {};
+  hk::RaggedPrepParams prep = {};
+  hk::RaggedPlanParams& plan = prep.plan;
   plan.cu_q = cu_seqlens_q, plan.cu_k = cu_seqlens_k;
   plan.S = S, plan.q_rows = q_rows, plan.k_rows = k_rows, plan.causal = causal != 0;
   plan.lists = 2;
@@ -178,8 +174,6 @@ int hk_attn_bwd_ragged(const void* q, const void* k, const void* v, const void* 
     plan.rest[2] = {dv, dvs.st[1], dvs.st[2], H_KV, k_rows, D / 8, 1};
   }
   plan.status = st->status;
-  if ((rc = launch_plan(plan, stream)) != HK_OK) return rc;
-  if (q_rows > 0 && (rc = prep_launch(o, d_o, delta, 1, q_rows, H, D, stream)) != HK_OK) return rc;
   hk::BwdParams p = {};
   p.lse = lse;
   p.delta = delta;
@@ -197,6 +191,22 @@ int hk_attn_bwd_ragged(const void* q, const void* k, const void* v, const void* 
   p.causal = causal != 0;
   p.status = st->status;
   const bool d128 = D == 128;
+  prep.q = static_cast<const __nv_bfloat16*>(q), prep.k = static_cast<const __nv_bfloat16*>(k), prep.v = static_cast<const __nv_bfloat16*>(v);
+  prep.o = static_cast<const __nv_bfloat16*>(o), prep.d_o = static_cast<const __nv_bfloat16*>(d_o);
+  prep.lse = lse, prep.delta = delta;
+  for (int i = 0; i < 2; ++i) prep.q_stride[i] = qs.st[i + 1], prep.k_stride[i] = ks.st[i + 1], prep.v_stride[i] = vs.st[i + 1];
+  prep.H = H, prep.rows = q_rows * H;
+  prep.scale_log2 = p.scale_log2;
+  prep.fd_h = hk::FastDiv(H), prep.fd_h2 = hk::FastDiv(2 * H), prep.fd_g = hk::FastDiv(p.G);
+  const int per_block = hk::row_pass_rows(D / 8);
+  if (q_rows > 0) {
+    prep.few_blocks = int((2ll * S * H + 7) / 8);
+    prep.row_blocks = int((1ll * q_rows * H + per_block - 1) / per_block);
+  }
+  const long long prep_grid = plan.lists + 1ll * prep.few_blocks + prep.row_blocks + (plan.rests ? hk::kPlanRestThreads / hk::kPrepThreads : 0);
+  HK_CUDA(hk::launch_dependent(true, d128 ? hk::ragged_prep_kernel<128> : hk::ragged_prep_kernel<64>, unsigned(prep_grid), hk::kPrepThreads,
+                               0, stream, prep));
+  g_launches.fetch_add(1, std::memory_order_relaxed);
   const int smem = d128 ? hk::BwdSmem<128>::kDynBytes : hk::BwdSmem<64>::kDynBytes;
   if (k_rows > 0) {
     p.plan_count = plan.count[0], p.plan = plan.places[0];

@@ -86,6 +86,56 @@ def test_longer_batches(dev, lens, d):
     assert status() == _native.HK_OK
 
 
+@pytest.mark.parametrize("n,most", [(257, 40), (1025, 20), (2100, 9)])
+def test_more_sequences_than_a_plan_takes_at_a_time(dev, n, most):
+    gen = torch.Generator().manual_seed(n)
+    lens_q = torch.randint(0, most, (n,), generator=gen).tolist()
+    lens_k = torch.randint(0, most, (n,), generator=gen).tolist()
+    lens_q[n // 2], lens_k[n // 2] = 700, 900  # one that is not like the others
+    q, kv, cu_q, cu_k, d_o = make(lens_q, lens_k, 2, 1, 64, seed=n, behind=3)
+    k, v = kv.unbind(1)
+    want = ref.attention(q, k, v, cu_q, cu_k, True, d_o=d_o)
+    o, l = hk.attn_fwd_ragged(q, k, v, cu_q, cu_k)
+    ref.close(o, want[0], "O")
+    ref.close(l, want[1], "L")
+    for got, pair, what in zip(hk.attn_bwd_ragged(q, k, v, o, d_o, l, cu_q, cu_k), want[2:], ("dQ", "dK", "dV")):
+        ref.close(got, pair, what)
+    assert status() == _native.HK_OK
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("causal", [True, False])
+def test_dq_of_rows_with_few_keys(dev, d, causal):
+    """Where a row has few keys, delta is what P dP adds up to in fp32, and not a product with the rounded O: what is left in dS is its
+    own rounding to bf16 (2^-8), the exponential's 2^-13 in it and in delta's terms, and the scores' and dP's sums in fp32."""
+    lens_q = [1, 2, 3, 17, 31, 32, 33, 60, 5, 40, 16]
+    lens_k = [1, 2, 3, 17, 31, 32, 33, 60, 29, 12, 0] if causal else [1, 2, 3, 4, 24, 23, 8, 9, 16, 5, 0]
+    h, hkv = 3, 1
+    q, kv, cu_q, cu_k, d_o = make(lens_q, lens_k, h, hkv, d, seed=d, first=2, behind=1)
+    k, v = kv.unbind(1)
+    o, l = hk.attn_fwd_ragged(q, k, v, cu_q, cu_k, causal=causal)
+    dq = hk.attn_bwd_ragged(q, k, v, o, d_o, l, cu_q, cu_k, causal=causal)[0].double()
+    c = d ** -0.5
+    for rq, rk in ref.sequences(cu_q, cu_k):
+        n, m = rq.stop - rq.start, rk.stop - rk.start
+        pos = torch.arange(n, device=dev)[:, None] + (m - n)
+        see = torch.arange(m, device=dev)[None, :] <= pos if causal else torch.ones(n, m, dtype=torch.bool, device=dev)
+        few = ((pos >= 0) & (pos < 32))[:, 0] if causal else torch.ones(n, dtype=torch.bool, device=dev)
+        for j in range(h):
+            if m == 0 or not few.any():
+                continue
+            qj, kj, vj, gj = q[rq, j].double()[few], k[rk, 0].double(), v[rk, 0].double(), d_o[rq, j].double()[few]
+            p = torch.softmax((qj @ kj.T * c).masked_fill(~see[few], -math.inf), 1)
+            dp, sizes = gj @ vj.T, qj.abs() @ kj.abs().T * c
+            ds = p * (dp - (p * dp).sum(1, keepdim=True)) * c
+            fp32 = d * 2 ** -23 * (gj.abs() @ vj.abs().T)
+            terms = (p * (dp.abs() * (2 ** -13 + sizes * d * 2 ** -23) + fp32)).sum(1, keepdim=True)
+            err = ds.abs() * (2 ** -8 + 2 ** -13 + sizes * d * 2 ** -23) + p * c * (terms + fp32)
+            want = ds @ kj
+            assert ((dq[rq, j][few] - want).abs() <= err @ kj.abs() + want.abs() * 2 ** -8 + 1e-30).all()
+    assert status() == _native.HK_OK
+
+
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("fill", [math.nan, math.inf, 3e38])
