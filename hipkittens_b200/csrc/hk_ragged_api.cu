@@ -197,10 +197,10 @@ int hk_attn_bwd_ragged(const void* q, const void* k, const void* v, const void* 
   for (int i = 0; i < 2; ++i) prep.q_stride[i] = qs.st[i + 1], prep.k_stride[i] = ks.st[i + 1], prep.v_stride[i] = vs.st[i + 1];
   prep.H = H, prep.rows = q_rows * H;
   prep.scale_log2 = p.scale_log2;
-  prep.fd_h = hk::FastDiv(H), prep.fd_h2 = hk::FastDiv(2 * H), prep.fd_g = hk::FastDiv(p.G);
+  prep.fd_h = hk::FastDiv(H), prep.fd_g = hk::FastDiv(p.G);
   const int per_block = hk::row_pass_rows(D / 8);
   if (q_rows > 0) {
-    prep.few_blocks = int((2ll * S * H + 7) / 8);
+    prep.few_blocks = int((hk::ragged_few_tiles(S, q_rows, causal != 0) * H + 7) / 8);
     prep.row_blocks = int((1ll * q_rows * H + per_block - 1) / per_block);
   }
   const long long prep_grid = plan.lists + 1ll * prep.few_blocks + prep.row_blocks + (plan.rests ? hk::kPlanRestThreads / hk::kPrepThreads : 0);

@@ -13,10 +13,13 @@
 //    included). V's codes are fetched transposed in pairs of neighbouring columns, and the two halves of such a pair are two
 //    shifts and masks apart, where `cvt` would first have to bring the tokens of one column together. bf16, because P takes the
 //    page's scale with it, which may be anything: p s_V / r with r the largest s_V so far keeps 8 bits whatever the scales, as 2^112
-//    times that; the accumulators are O / (2^-8 ...) in fp32 until the end.
+//    times that; the accumulators are 2^-8 O l / r in fp32 until the end.
 // How contexts are spread (decode_pick_fp8_cluster): with few (sequence, K/V head) units a cluster of CTAs shares each, as in the bf16 kernel
 // (paged_decode_common.cuh). Otherwise the pages of all units are one row of work, of which every warp of the GPU takes an equal run,
 // whatever the contexts' lengths, and a second kernel joins the units that more than one warp had a part of.
+// Bound by HBM where contexts are many: 64 of 512 to 8192 tokens, H64/8 D128, in a loop 71.6 us, 70% of the copy rate; the row kernel
+// takes 64 of them and is at 94% of it for equal contexts, the join the rest. One context of 12,006 tokens (H32/8) 14 us, of which its 25 MB
+// are 3.8: a launch, three dependent loads and the cluster's barriers are the rest. At D = 64 a TMA row is 64 bytes and their rate the bound.
 #pragma once
 
 #include <cuda.h>
@@ -435,7 +438,7 @@ paged_decode_fp8_cluster_kernel(const __grid_constant__ CUtensorMap tmap_k, cons
 // ------------------------------------------------------------------------------------ all pages as one row
 // The live pages of sequence after sequence; group w of n has the places [T w / n, T (w + 1) / n), each of its H_KV warps for a head of its
 // own. (With the heads' pages one head after the other, what the GPU reads at a time is 128 or 64 bytes here and there: 64 contexts of 4096
-// tokens of H_KV 8 D128 155 us, against 101.)
+// tokens of H_KV 8 D128 155 us, against 148, when the kernel was slower in other ways.)
 struct DecodeFp8Row {
   long long total = 0;  // T
   int groups = 0;       // n
@@ -673,9 +676,9 @@ inline int prepare_decode_fp8_kernels(char* err, size_t err_len, int sm_count, D
 //    34.8 / 36.9 (4), 32 of them 42.9 / 61.4 (3).
 //  * Many units, each a CTA of its own while the longest a context can be does not hold up the rest: 64 of 300 to 1000 tokens 30.7 / 26.6
 //    (1); windows, which most contexts fill: 64 of 2048 61.4 / 57.3 (1), 33 of H48/8 D64 500 20.4 / 14.3 (1). Otherwise the row: 64 of
-//    512 to 8192 77.9 / 131 (1), 92 (4); of 4096 each 100.3 / 98.3 (1), 111 (4); D64 53.2 / 94 (1), 65.6 (2); 256 of 200 to 2000 of H32/4 53.2 /
-//    55.3 (1). Chunks of 64 pages and a
-//    combining kernel, as in the bf16 decode, took as long for 64 of 512 to 8192, and leave a tail that the row does not have: D64 53.2 / 60.
+//    512 to 8192 77.9 / 131 (1), 92 (4); of 4096 each 100.3 / 98.3 (1), 111 (4); D64 53.2 / 94 (1), 65.6 (2); 256 of 200 to 2000 of
+//    H32/4 53.2 / 55.3 (1). Chunks of 64 pages and a combining kernel, as in the bf16 decode, took as long for 64 of 512 to 8192, and
+//    leave a tail that the row does not have: D64 53.2 / 60.
 inline int decode_pick_fp8_cluster(int S, int H_KV, int span, bool window, const DecodeLimits& lim) {
   const long long units = 1ll * S * H_KV;
   int cluster = kMaxCluster;

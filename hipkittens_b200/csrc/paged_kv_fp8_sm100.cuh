@@ -388,7 +388,8 @@ struct ReadFp8Params {
 };
 
 // A warp has 16 tokens of one head, K and V: all of their codes are requested before the first is used (8 x 16 bytes a lane at D =
-// 128), scaled in fp32 and rounded once. Bound by HBM: 3 bytes a value.
+// 128), scaled in fp32 and rounded once. Bound by HBM, 3 bytes a value: 4 sequences of 4,096 to 8,192 tokens, H_KV 8 D128, 31 us in a
+// loop, 87% of the copy rate; 32-byte stores, where the output allows them, are one a lane in place of two.
 template <int D>
 __global__ void __launch_bounds__(256) paged_kv_read_fp8_kernel(const __grid_constant__ ReadFp8Params p) {
   ptx::grid_dep_wait();

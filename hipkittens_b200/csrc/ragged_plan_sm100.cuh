@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(kPlanThreads) ragged_plan_kernel(const __grid_
 // sum of P dP over these, from the scores, as in attn_bwd_prep_window_kernel and for its reasons: those at the first kFewRows positions of
 // a sequence under the causal rule, and without it all rows of sequences of up to kFewKeys keys. (With delta from O alone in all rows, dQ
 // over 23 sequences of up to 400 tokens was off by 2.6e-3 of its size, D = 64; so by 2.4e-3, of which 2.35e-3 are the roundings of dS and
-// of dQ itself.) 16,000 tokens of 32 heads of 128 take 35 us from cold caches; the plan and attn_bwd_prep_kernel one
+// of dQ itself.) 12,100 tokens of 32 heads of 128 take 35 us from cold caches; the plan and attn_bwd_prep_kernel one
 // after the other took 41.
 struct RaggedPrepParams {
   RaggedPlanParams plan;
@@ -220,10 +220,27 @@ struct RaggedPrepParams {
   float* delta;                                     // [H, q_rows]
   long long q_stride[2], k_stride[2], v_stride[2];  // row, head; elements
   int H, rows;                                      // heads, rows of all heads
-  int few_blocks, row_blocks;
+  int few_blocks, row_blocks;                       // few_blocks: 8 of ragged_few_tiles x H warps
   float scale_log2;
-  FastDiv fd_h, fd_h2, fd_g;                        // H, 2 * H, H / H_KV
+  FastDiv fd_h, fd_g;                               // H, H / H_KV
 };
+
+// Tiles of 16 rows that may be of few keys: causal, two of each sequence; otherwise sequence s has those from cu[s] / 16 + s on.
+inline long long ragged_few_tiles(int S, int q_rows, bool causal) { return causal ? 2ll * S : q_rows / 16 + 1ll * S; }
+
+// The last sequence whose `key` is not above `value`; all lanes of a warp look. Keys do not fall; whatever they do, it is one of them.
+template <typename Key>
+__device__ __forceinline__ int ragged_sequence_at(int S, int value, const Key& key) {
+  int s = 0;
+  for (int n = S; n > 1;) {
+    const int step = (n + 31) >> 5, at = static_cast<int>(threadIdx.x & 31) * step;
+    const uint32_t there = __ballot_sync(0xffffffffu, at < n && key(s + at) <= value) | 1u;
+    const int skip = (31 - __clz(there)) * step;
+    s += skip;
+    n = min(step, n - skip);
+  }
+  return s;
+}
 
 // Is delta of the row at this position of a sequence taken from the scores?
 __device__ __forceinline__ bool ragged_few(const RaggedSequence& x, bool causal, int row) {
@@ -231,19 +248,28 @@ __device__ __forceinline__ bool ragged_few(const RaggedSequence& x, bool causal,
   return causal ? pos >= 0 && pos < kFewRows : x.n_k <= kFewKeys;
 }
 
-// Rows of few keys of one sequence and head, every second 16 of them from `tile` on.
+// One of those tiles, one head.
 template <int D>
-__device__ void ragged_few_rows(const RaggedPrepParams& p, int s, int h, int tile) {
-  const RaggedSequence x(p.plan, s);
+__device__ void ragged_few_rows(const RaggedPrepParams& p, int tile, int h) {
   const bool causal = p.plan.causal;
-  if (x.is_bad(p.plan) || x.n_q == 0 || (!causal && x.n_k > kFewKeys)) return;
+  int s = tile >> 1;
+  if (causal) {
+    if (s >= p.plan.S) return;
+    tile &= 1;
+  } else {
+    auto first_tile = [&](int at) { return (p.plan.cu_q[at] >> 4) + at; };
+    s = ragged_sequence_at(p.plan.S, tile, first_tile);
+    tile -= first_tile(s);
+  }
+  const RaggedSequence x(p.plan, s);
+  if (x.is_bad(p.plan) || tile < 0 || (!causal && x.n_k > kFewKeys)) return;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, kvh = p.fd_g.div(h);
   const int behind = causal ? x.n_k - x.n_q : 0;  // a row's position less its number
   const int rows = causal ? min(kFewRows - behind, x.n_q) : x.n_q;
   const __nv_bfloat16 *const k = p.k + x.k0 * p.k_stride[0] + kvh * p.k_stride[1] + t * 8,
                       *const v = p.v + x.k0 * p.v_stride[0] + kvh * p.v_stride[1] + t * 8;
   auto load = [](const __nv_bfloat16* at) { return *reinterpret_cast<const uint4*>(at); };
-  for (int first = max(-behind, 0) + tile * 16; first < rows; first += 32) {
+  if (const int first = max(-behind, 0) + tile * 16; first < rows) {
     const __nv_bfloat16 *q[2], *grad[2];  // rows g and g + 8
     float nl[2], sum[2] = {0.f, 0.f};
 #pragma unroll
@@ -285,7 +311,7 @@ __device__ void ragged_few_rows(const RaggedPrepParams& p, int s, int h, int til
   }
 }
 
-// grid = lists, few_blocks (a warp each: sequence, head, one of two), row_blocks, and the rest's; block = kPrepThreads.
+// grid = lists, few_blocks, row_blocks, and the rest's; block = kPrepThreads.
 template <int D>
 __global__ void __launch_bounds__(kPrepThreads, 4) ragged_prep_kernel(const __grid_constant__ RaggedPrepParams p) {
   __shared__ RaggedPlanSmem<kPrepThreads> smem;
@@ -296,10 +322,9 @@ __global__ void __launch_bounds__(kPrepThreads, 4) ragged_prep_kernel(const __gr
   block -= p.plan.lists;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (block < p.few_blocks) {
-    int s, rem;
-    p.fd_h2.divmod(block * 8 + warp, s, rem);
-    if (s < p.plan.S) ragged_few_rows<D>(p, s, rem >> 1, rem & 1);
-    return;
+    int tile, h;
+    p.fd_h.divmod(block * 8 + warp, tile, h);
+    return ragged_few_rows<D>(p, tile, h);
   }
   block -= p.few_blocks;
   if (block >= p.row_blocks) {
@@ -316,14 +341,7 @@ __global__ void __launch_bounds__(kPrepThreads, 4) ragged_prep_kernel(const __gr
     b[u] = __ldcs(reinterpret_cast<const uint4*>(p.d_o + static_cast<size_t>(row) * D) + sub);
   }
   // the sequence of the warp's first row, while they come in; the others' are its or next ones
-  int s = 0;
-  for (int n = p.plan.S; n > 1;) {
-    const int step = (n + 31) >> 5, at = lane * step;
-    const uint32_t there = __ballot_sync(0xffffffffu, at < n && p.plan.cu_q[s + at] <= p.fd_h.div(min(warp0, p.rows - 1))) | 1u;
-    const int skip = (31 - __clz(there)) * step;
-    s += skip;
-    n = min(step, n - skip);
-  }
+  int s = ragged_sequence_at(p.plan.S, p.fd_h.div(min(warp0, p.rows - 1)), [&](int at) { return p.plan.cu_q[at]; });
   RaggedSequence x(p.plan, s);
 #pragma unroll
   for (int u = 0; u < kRowPassUnroll; ++u) {

@@ -329,7 +329,8 @@ int hk_paged_kv_append_rotary(const void* k_new, const void* v_new, void* k_page
  * D = 64 or 128, S <= 65535, rows <= 2^30. cu_seqlens that fall or lie outside are reported as HK_EBADLEN, and the call writes nothing.
  * workspace: device scratch, 256-byte aligned, of at least the bytes that the functions say (0: such sizes are refused). Nothing is added
  * up with atomics: results are the same from run to run. Asynchronous on `cuda_stream`.
- * The backward writes delta [H, q_rows] (rowsum(O * dO)), dq, dk and dv. dq may not share memory with another output. */
+ * The backward writes delta [H, q_rows] (rowsum(O * dO); of rows of few keys, the sum of P dP over these), dq, dk and dv. dq may not share
+ * memory with another output. */
 size_t hk_attn_fwd_ragged_workspace_bytes(int S, int q_rows);
 int hk_attn_fwd_ragged(const void* q, const void* k, const void* v, void* o, float* lse, const int32_t* cu_seqlens_q,
                        const int32_t* cu_seqlens_k, int S, int q_rows, int k_rows, int H, int H_KV, int D, const long long* q_strides,
