@@ -61,16 +61,22 @@ int hk_paged_kv_append_fp8(const void* k_new, const void* v_new, void* k_pages, 
     if (table_rows <= 0) return HK_EINVAL;
   }
   const long long units = cu_seqlens ? T / hk::kPageTokens + 2ll * S : S * ((T + 30ll) / hk::kPageTokens);
-  const int warps = std::min(hk::kFp8AppendWarps, H_KV);
+  int warps = std::min(hk::kFp8AppendWarps, H_KV);
   int blocks;  // with a head a warp
   if (!fp8_units(units, 2 * ((H_KV + warps - 1) / warps), &blocks)) return HK_EINVAL;
   DeviceState* st = nullptr;
   DeviceScope scope;
   if ((rc = scope.enter(device, &st)) != HK_OK) return rc;
-  // Two heads a warp where there is more than the device holds at once: the next head's tokens come in meanwhile, and a page's tables
-  // serve twice as many. Prompts of 29,000 tokens, H_KV = 8, D = 128: 33.8 us, against 40.6; a token for each of 64 sequences: 4.4,
-  // against 3.6.
-  p.turns = blocks > 4 * st->sm_count ? 2 : 1;
+  // Several heads a warp where there is more than the device holds at once: the next head's tokens come in meanwhile, and a page's tables
+  // serve as many. us, 1 / 2 / 4 heads of a warp, rotated prompts of as many bytes as 29,000 tokens of H_KV 8 D128: H_KV 8 D128 40.6 / 33.7 /
+  // 38, H_KV 4 D128 40.2 / 35.4 / 41, H_KV 8 D64 - / 41 / 37, H_KV 4 D64 56 / 42 / 38; a token for each of 64 sequences, H_KV 8 D128: 3.6 /
+  // 4.4. One head of 128 takes 52.
+  if (blocks > 4 * st->sm_count) {
+    p.turns = std::min(hk::fp8_append_turns(D), H_KV);
+    warps = std::min(hk::kFp8AppendWarps, (H_KV + p.turns - 1) / p.turns);
+  } else {
+    p.turns = 1;
+  }
   const int groups = (H_KV + p.turns * warps - 1) / (p.turns * warps);
   p.c.status = st->status;
   p.rows.cu = cu_seqlens;
@@ -88,7 +94,8 @@ int hk_paged_kv_append_fp8(const void* k_new, const void* v_new, void* k_pages, 
   p.rotation = !sin ? hk::kFp8Plain : flags & HK_FP8_TABLE_F32 ? hk::kFp8TableF32 : hk::kFp8TableBf16;
   auto* fn = D == 128 ? sin ? hk::paged_kv_append_fp8_kernel<128, true> : hk::paged_kv_append_fp8_kernel<128, false>
                       : sin ? hk::paged_kv_append_fp8_kernel<64, true> : hk::paged_kv_append_fp8_kernel<64, false>;
-  HK_CUDA(hk::launch_dependent(true, fn, unsigned(units * 2 * groups), warps * 32, 0, static_cast<cudaStream_t>(cuda_stream), p));
+  const int smem = hk::fp8_append_smem(D, sin, warps, p.turns);
+  HK_CUDA(hk::launch_dependent(true, fn, unsigned(units * 2 * groups), warps * 32, smem, static_cast<cudaStream_t>(cuda_stream), p));
   g_launches.fetch_add(1, std::memory_order_relaxed);
   return HK_OK;
 }

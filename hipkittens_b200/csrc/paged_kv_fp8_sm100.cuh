@@ -159,10 +159,16 @@ struct AppendFp8Params {
   int rotation;                        // Fp8Rotation
   int R, table_rows;
   int turns;                           // heads of a warp
-  FastDiv fd_groups2, fd_groups;       // 2 * groups, groups of kFp8AppendWarps x turns heads
+  FastDiv fd_groups2, fd_groups;       // 2 * groups, groups of a CTA's warps x turns heads
 };
 
-constexpr int kFp8AppendWarps = 4, kFp8AppendStages = 2;
+constexpr int kFp8AppendWarps = 4;  // at most
+constexpr int fp8_append_turns(int D) { return 256 / D; }  // at most: 8 KB of tokens a warp
+// Dynamic shared memory: cos and sin [16, D / 2], then the tokens of each warp's turns.
+constexpr int fp8_append_smem(int D, bool rotates, int warps, int turns) {
+  return (rotates ? 2 * kPageTokens * (D / 2) * 4 : 0) + warps * turns * kPageTokens * D * 2;
+}
+static_assert(fp8_append_smem(128, true, kFp8AppendWarps, fp8_append_turns(128)) <= 48 * 1024, "what a kernel has without asking");
 
 // A CTA has new tokens of a page, of K or of V, and its warps have a block at a time: a head's tokens of the page, and those of the
 // next head already on their way. A warp finds the block's largest magnitude, settles the scale, and writes the codes; if the page had
@@ -172,13 +178,14 @@ constexpr int kFp8AppendWarps = 4, kFp8AppendStages = 2;
 // took 66 us.
 // Bound by HBM (3 bytes a value): those take 34 us, 80% of the copy rate, and 30 without a rotation; a token for each sequence is a
 // launch and three dependent loads.
-// grid = units x 2 x groups of heads; block = 32 * min(kFp8AppendWarps, H_KV).
+// grid = units x 2 x groups of heads; block = up to 32 * kFp8AppendWarps, dynamic smem = fp8_append_smem.
 template <int D, bool ROT>
 __global__ void __launch_bounds__(kFp8AppendWarps * 32, ROT ? 4 : 5) paged_kv_append_fp8_kernel(const __grid_constant__ AppendFp8Params p) {
   constexpr int kLanes = D / 8, kRows = 32 / kLanes, kSteps = kPageTokens / kRows;  // lanes of a row, rows of a step
   constexpr int kTile = kPageTokens * D * 2;
-  __shared__ __align__(16) uint8_t rings[kFp8AppendWarps][kFp8AppendStages * kTile];
-  __shared__ __align__(16) float tables[ROT ? 2 : 1][ROT ? kPageTokens * D / 2 : 1];  // cos, sin: [16, R / 2]
+  constexpr int kTable = ROT ? kPageTokens * D / 2 : 0;  // values: [16, R / 2]
+  extern __shared__ __align__(16) uint8_t append_smem[];
+  float* const tables = reinterpret_cast<float*>(append_smem);  // cos, sin
   ptx::grid_dep_wait();
   ptx::grid_dep_launch();
   const Fp8Cache& c = p.c;
@@ -215,11 +222,11 @@ __global__ void __launch_bounds__(kFp8AppendWarps * 32, ROT ? 4 : 5) paged_kv_ap
   const int head0 = group * p.turns * warps + warp, heads = min(p.turns, (c.H_KV - head0 + warps - 1) / warps);  // every warps-th from head0 on
   const long long* const stride = is_v ? p.v_stride : p.k_stride;
   const __nv_bfloat16* const src = (is_v ? p.v_new : p.k_new) + s * stride[0] + (first + base + row0) * stride[1] + col;
-  uint8_t* const ring = rings[warp];
+  uint8_t* const ring = append_smem + 2 * kTable * sizeof(float) + warp * p.turns * kTile;
   const uint32_t ring_u32 = ptx::smem_u32(ring) + (row0 * D + col) * 2;
   auto request = [&](int turn) {  // rows that are not new become zeros
     const __nv_bfloat16* at = src + (head0 + turn * warps) * stride[2];
-    uint32_t to = ring_u32 + (turn % kFp8AppendStages) * kTile;
+    uint32_t to = ring_u32 + turn * kTile;
 #pragma unroll
     for (int r = row0; r < kPageTokens; r += kRows, at += kRows * stride[1], to += kRows * D * 2)
       dec::cp_async16_if(to, at, r >= r0 && r < r1);
@@ -238,8 +245,8 @@ __global__ void __launch_bounds__(kFp8AppendWarps * 32, ROT ? 4 : 5) paged_kv_ap
         const float2 a0 = fp8::bf16x2(a.x), a1 = fp8::bf16x2(a.y), b0 = fp8::bf16x2(b.x), b1 = fp8::bf16x2(b.y);
         cs = make_float4(a0.x, a0.y, a1.x, a1.y), sn = make_float4(b0.x, b0.y, b1.x, b1.y);
       }
-      reinterpret_cast<float4*>(tables[0])[i] = cs;
-      reinterpret_cast<float4*>(tables[ROT ? 1 : 0])[i] = sn;
+      reinterpret_cast<float4*>(tables)[i] = cs;
+      reinterpret_cast<float4*>(tables + kTable)[i] = sn;
     }
     __syncthreads();
   }
@@ -310,7 +317,6 @@ __global__ void __launch_bounds__(kFp8AppendWarps * 32, ROT ? 4 : 5) paged_kv_ap
         if (lane == 0 && (r0 == 0 || bits != before)) *scale_at = __uint_as_float(bits);
       };
 
-      __syncwarp();  // the tile that the next tokens go to has been read
       if (turn + 1 < heads) {
         request(turn + 1);
         dec::cp_async_wait<1>();
@@ -318,7 +324,7 @@ __global__ void __launch_bounds__(kFp8AppendWarps * 32, ROT ? 4 : 5) paged_kv_ap
         dec::cp_async_wait<0>();
       }
       __syncwarp();
-      const uint8_t* const tile = ring + (turn % kFp8AppendStages) * kTile + row0 * D * 2;
+      const uint8_t* const tile = ring + turn * kTile + row0 * D * 2;
       if constexpr (!TURN) {
         auto values = [&](int i) { return *reinterpret_cast<const uint4*>(tile + (i * kRows * D + col) * 2); };
         uint32_t two = 0;
@@ -336,7 +342,7 @@ __global__ void __launch_bounds__(kFp8AppendWarps * 32, ROT ? 4 : 5) paged_kv_ap
         // a pair (i, i + R / 2) becomes (a cos - b sin, b cos + a sin)
         uint64_t y[kSteps][4];
         float amax = 0.f;
-        const float* const cs_at = tables[0] + row0 * (p.R / 2) + col0;
+        const float* const cs_at = tables + row0 * (p.R / 2) + col0;
         const uint32_t at0 = ptx::smem_u32(cs_at), step = kRows * (p.R / 2) * 4, x0 = ptx::smem_u32(tile);
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
@@ -350,7 +356,7 @@ __global__ void __launch_bounds__(kFp8AppendWarps * 32, ROT ? 4 : 5) paged_kv_ap
           if (turned && is_new(i)) {
             uint64_t cs[2], sn[2];
             fp8::lds4(at0 + i * step, cs);
-            fp8::lds4(at0 + i * step + static_cast<uint32_t>(sizeof(tables[0])), sn);
+            fp8::lds4(at0 + i * step + kTable * 4, sn);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               const uint64_t a2 = y[i][j], b2 = y[i][j + 2];

@@ -99,3 +99,68 @@ def test_conversations(h, hkv, d, dtype):
         graph.replay()
         check()
     assert _native.device_status(0) == _native.HK_OK
+
+
+def test_two_streams_at_once_and_shared_pages():
+    """Two servers on one GPU, each with a stream, a cache and a graph of its own, replayed side by side; inside a cache two sequences that
+    share the pages of a prefix. What they leave is what each leaves alone."""
+    h, hkv, d, s, width = 8, 2, 128, 6, 40
+
+    class Server:
+        def __init__(self, seed):
+            gen = torch.Generator().manual_seed(seed)
+            self.stream = torch.cuda.Stream()
+            pool = s * width
+            self.pages = [torch.randint(0, 126, (pool, 16, hkv, d), generator=gen, dtype=torch.uint8).cuda().view(torch.float8_e4m3fn) for _ in range(2)]
+            self.scales = [torch.exp2(torch.randint(-12, -8, (pool, hkv), generator=gen).float()).cuda() for _ in range(2)]
+            self.table = torch.randperm(pool, generator=gen).reshape(s, width).to(torch.int32).cuda()
+            self.table[1, :20] = self.table[0, :20]
+            self.start = torch.tensor([330, 400, 15, 600, 0, 77], dtype=torch.int32, device="cuda")
+            self.x = torch.randn(s, 1, h + 2 * hkv, d, generator=gen).to(torch.bfloat16).cuda()
+            self.cu = offsets([200, 1, 130, 64])
+            self.q, self.kv = (torch.randn(395, n, d, generator=gen).to(torch.bfloat16).cuda() for n in (h, 2 * hkv))
+            self.out = []
+
+        def step(self):
+            q, k, v = self.x.split([h, hkv, hkv], 2)
+            hk.paged_kv_append_fp8(k, v, *self.pages, *self.scales, self.table, self.start)
+            self.out = [*hk.paged_decode_fp8(q.contiguous(), *self.pages, *self.scales, self.table, self.start + 1),
+                        *hk.attn_fwd_ragged(self.q, self.kv[:, :hkv], self.kv[:, hkv:], self.cu)]
+            self.out += hk.attn_bwd_ragged(self.q, self.kv[:, :hkv], self.kv[:, hkv:], self.out[2], self.q, self.out[3], self.cu)
+            self.start += 1
+            self.x.neg_()
+
+        def capture(self):
+            with torch.cuda.stream(self.stream):
+                self.step()
+                self.graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(self.graph, stream=self.stream):
+                    self.step()
+
+        def state(self):
+            return [t.clone() for t in (*(c.view(torch.uint8) for c in self.pages), *self.scales, *self.out)]
+
+    def run(servers, together):
+        torch.cuda.synchronize()
+        for server in servers:
+            server.capture()
+            torch.cuda.synchronize()
+        for _ in range(20):
+            for server in servers:
+                with torch.cuda.stream(server.stream):
+                    server.graph.replay()
+                if not together:
+                    torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        return [server.state() for server in servers]
+
+    alone, beside = run([Server(1), Server(2)], False), run([Server(1), Server(2)], True)
+    for a, b in zip(alone, beside):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+    server = Server(3)
+    q = server.x[:, :, :h].contiguous()
+    lens = int32([320, 400, 16, 600, 0, 77])
+    got = hk.paged_decode_fp8(q, *server.pages, *server.scales, server.table, lens)
+    want = kv_ref.decode(q, *server.pages, *server.scales, server.table, lens)
+    assert ((got[0].cpu().double() - want[0]).abs() <= want[1]).all()
+    assert _native.device_status(0) == _native.HK_OK

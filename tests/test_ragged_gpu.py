@@ -342,6 +342,27 @@ def test_streams_and_views(dev):
     assert status() == _native.HK_OK
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_strides_behind_32_bits(dev, d):
+    """Rows 2^24 elements apart: the last lies 5 * 10^9 elements behind the first."""
+    lens, h, hkv = [130, 1, 20, 149], 4, 2
+    q, kv, cu, _, d_o = make(lens, lens, h, hkv, d, seed=9)
+    k, v = kv.unbind(1)
+    o, l = hk.attn_fwd_ragged(q, k, v, cu)
+    want = hk.attn_bwd_ragged(q, k, v, o, d_o, l, cu)
+    rows, step = q.shape[0], 1 << 24
+    room = torch.empty(rows * step, dtype=torch.bfloat16, device=dev)
+    far = [room.as_strided((rows, n, d), (step, d, 1), 4096 * i) for i, n in enumerate((h, hkv, hkv, h, hkv, hkv))]
+    for x, y in zip(far, (q, k, v)):
+        x.copy_(y)
+    got = hk.attn_fwd_ragged(*far[:3], cu)
+    assert torch.equal(got[0], o) and torch.equal(got[1], l)
+    hk.attn_bwd_ragged(*far[:3], o, d_o, l, cu, dq=far[3], dk=far[4], dv=far[5])
+    for x, y in zip(far[3:], want):
+        assert torch.equal(x, y)
+    assert status() == _native.HK_OK
+
+
 def test_refusals(dev):
     gen = torch.Generator().manual_seed(6)
     q, kv, cu = rand(gen, 20, 4, 64), rand(gen, 20, 2, 2, 64), offsets([20])
