@@ -50,7 +50,9 @@ struct DecodeFp8Params : DecodeParams {  // k_pages and v_pages are not used; a 
 // A warp leaves at most two parts of units that it does not have whole: its first and its last. Workspace: their O as fp32 [part][8][D], then
 // (m, l) pairs [part][8][2], then for each unit which parts it has (DecodeFp8Parts).
 constexpr int kRowWarps = 16 * 148;  // what a B200 holds at once
-constexpr int kRowPages = 2;         // no warp takes fewer pages, unless there are no more
+// No warp takes fewer pages, unless there are no more: what it leaves has to be joined. us, 2 / 4 / 8 / 16, a read of 256 MB before each: one
+// context of 100,000 tokens H8/1 D128 44 / 38 / 30 / 30, of 40,000 30 / 24 / 22 / 28, of H32/8 30 / 30 / 30 / 32.
+constexpr int kRowPages = 8;
 inline int decode_fp8_row_groups(int H_KV, int warps = kRowWarps) { return H_KV < warps ? warps / H_KV : 1; }
 struct __align__(16) DecodeFp8Parts {
   int first, group, last_group, unused;  // the part of its first group, that group and the last one; the same: none, the rows are finished
@@ -584,11 +586,11 @@ paged_decode_fp8_row_kernel(const __grid_constant__ CUtensorMap tmap_k, const __
   decode_fp8_check_waits(a.abort_word, p.status);
 }
 
-// grid = (H_KV x ceil(G / heads), S), block = 256: a block has `heads` (8, 4, 2 or 1) heads of a unit, 8 / heads warps for each, every warp so
-// many-th parts, and a lane D / 32 columns.
-template <int D>
-__global__ void __launch_bounds__(256) paged_decode_fp8_join_kernel(const __grid_constant__ DecodeFp8Params p, int heads) {
-  constexpr int kCols = D / 32, kWarps = 8;
+// grid = (H_KV x ceil(G / heads), S), block = 32 W, W = 8 or 32: a block has `heads` (8, 4, 2 or 1) heads of a unit, W / heads warps for each,
+// every warp so many-th parts, and a lane D / 32 columns.
+template <int D, int W>
+__global__ void __launch_bounds__(W * 32) paged_decode_fp8_join_kernel(const __grid_constant__ DecodeFp8Params p, int heads) {
+  constexpr int kCols = D / 32, kWarps = W;
   __shared__ float s_m[kWarps], s_l[kWarps], s_o[kWarps][D];
   ptx::grid_dep_wait();  // from here on the parts are visible
   ptx::grid_dep_launch();
@@ -706,7 +708,10 @@ cudaError_t launch_decode_fp8(const CUtensorMap& tk, const CUtensorMap& tv, Deco
   const int G = p.H / p.H_KV;
   int heads = 1;
   while (heads < G && 1ll * p.S * p.H_KV * ((G + heads - 1) / heads) > 16ll * sm_count) heads *= 2;
-  return launch_dependent(true, paged_decode_fp8_join_kernel<D>, dim3(p.H_KV * ((G + heads - 1) / heads), p.S), 256, 0, stream, p, heads);
+  // many parts to a unit: 32 warps (one context of 100,000 tokens H8/1 D128 107 / 44, of H32/8 54 / 46)
+  const bool many = heads == 1 && p.row_groups > 16 * p.S;
+  return launch_dependent(true, many ? paged_decode_fp8_join_kernel<D, 32> : paged_decode_fp8_join_kernel<D, 8>,
+                          dim3(p.H_KV * ((G + heads - 1) / heads), p.S), many ? 1024 : 256, 0, stream, p, heads);
 }
 
 inline cudaError_t launch_paged_decode_fp8(const CUtensorMap& tk, const CUtensorMap& tv, const DecodeFp8Params& p, int D, bool window,
