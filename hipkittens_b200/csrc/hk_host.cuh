@@ -246,9 +246,9 @@ inline int make_code_map(CUtensorMap* map, const void* base, int num_pages, int 
 // The tiles are counted as if nothing were masked. A causal call has about half of them, and a paged one those of its
 // contexts, which the host does not know, and not of its block table's width: such calls are launched the ordinary way
 // from half the time on, or earlier.
-// us per call in a loop, dependent / ordinary, at 28, 62, 111, 221 and 443 tiles per CTA (H32/8 D128, B1 N2048, N3072, N4096,
-// B2 and B4 N4096): non-causal 65.8 / 67.9, 134.8 / 136.8, 232.0 / 233.7, 415.7 / 417.0, 830.7 / 830.1; causal
-// 39.0 / 40.3, 77.2 / 79.4, 117.7 / 120.4, 230.7 / 229.8, 456.6 / 452.8. Append and paged chunk, 8 x 512 tokens on contexts
+// us per call in a loop, dependent / ordinary, at 28, 111, 221 and 443 tiles per CTA (H32/8 D128, B1 N2048, N4096,
+// B2 and B4 N4096): non-causal 65.8 / 67.9, 232.0 / 233.7, 415.7 / 417.0, 830.7 / 830.1; causal
+// 39.0 / 40.3, 117.7 / 120.4, 230.7 / 229.8, 456.6 / 452.8. Append and paged chunk, 8 x 512 tokens on contexts
 // of 4096 (221 tiles): 487.8 / 479.2, and so the line is no higher.
 inline bool short_kernel(long long tiles, int grid) { return tiles <= 100ll * grid; }
 

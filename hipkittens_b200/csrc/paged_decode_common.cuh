@@ -96,7 +96,7 @@ struct DecodeLimits {
 //    would spread it over the GPU. The lines are where that costs the one long context about as much as batches of equal
 //    lengths gain. us, chunks / this, one context as long as the table beside others of 100 tokens, then all that long, then
 //    all a quarter of that:
-//    CTAs of 4 warps in clusters, 64 pages each: 8 x 3072 tokens of H_KV 8 (48 pages each) 10.8 / 10.4, 22.3 / 16.6, 11.7 / 6.7; 8 x
+//    CTAs of 4 warps in clusters, 64 pages each: 8 x 48 pages of H_KV 8 10.8 / 10.4, 22.3 / 16.6, 11.7 / 6.7; 8 x
 //    4096 10.8 / 12.4, 30.5 / 25.3, 11.9 / 7.2; 64 x 4096 of H_KV 1 9.8 / 11.9, 30.2 / 25.1, 12.3 / 7.3; behind the line 8 x 8192
 //    12.3 / 19.8, 53.7 / 45.2, 14.0 / 10.0.
 //    CTAs of their own of 8 warps (units for more than a wave in clusters of 3), 96 pages: 16 x 1408 10.8 / 10.7, 20.1 /
