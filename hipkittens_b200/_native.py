@@ -63,6 +63,7 @@ EXPORTED_SYMBOLS = (
     "hk_selftest_dkdv_in_pairs",
     "hk_selftest_bwd_dealing",
     "hk_selftest_decode_shape",
+    "hk_selftest_decode_fp8_parts",
     "hk_kernel_launch_count",
     "hk_strerror",
     "hk_last_cuda_error",
@@ -188,6 +189,8 @@ def capi() -> ctypes.CDLL:
     lib.hk_selftest_bwd_dealing.restype = ci
     lib.hk_selftest_decode_shape.argtypes = [ci] * 4 + [ctypes.POINTER(ci), ci, ctypes.POINTER(ci)]
     lib.hk_selftest_decode_shape.restype = ci
+    lib.hk_selftest_decode_fp8_parts.argtypes = [ci] * 5
+    lib.hk_selftest_decode_fp8_parts.restype = ci
     lib.hk_kernel_launch_count.argtypes = []
     lib.hk_kernel_launch_count.restype = ctypes.c_ulonglong
     lib.hk_strerror.argtypes = [ci]

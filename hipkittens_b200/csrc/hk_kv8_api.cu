@@ -186,4 +186,9 @@ int hk_attn_paged_decode_fp8(const void* q, const void* k_pages, const void* v_p
   return HK_OK;
 }
 
+int hk_selftest_decode_fp8_parts(int first, int group, int last_group, int row_groups, int H_KV) {
+  if (row_groups <= 0 || H_KV <= 0 || H_KV > 65535 || 1ll * row_groups * H_KV > 0x3fffffff) return HK_EINVAL;
+  return hk::decode_fp8_parts_valid({first, group, last_group, 0}, row_groups, H_KV) ? 1 : 0;
+}
+
 }  // extern "C"

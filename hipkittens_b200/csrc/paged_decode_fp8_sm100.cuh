@@ -57,6 +57,11 @@ inline int decode_fp8_row_groups(int H_KV, int warps = kRowWarps) { return H_KV 
 struct __align__(16) DecodeFp8Parts {
   int first, group, last_group, unused;  // the part of its first group, that group and the last one; the same: none, the rows are finished
 };
+// Whether these lie in the workspace. The row kernel leaves them for every context that is not empty, unless a wait of its has run out: then
+// the join finds whatever was there before.
+__host__ __device__ inline bool decode_fp8_parts_valid(const DecodeFp8Parts& x, int row_groups, int H_KV) {
+  return x.group >= 0 && x.group <= x.last_group && x.last_group < row_groups && x.first >= 0 && x.first < 2 * row_groups * H_KV;
+}
 inline size_t decode_fp8_workspace_bytes(int S, int H_KV, int D) {
   return size_t(decode_fp8_row_groups(H_KV)) * H_KV * 2 * 8 * (D + 2) * sizeof(float) + size_t(S) * H_KV * sizeof(DecodeFp8Parts);
 }
@@ -607,6 +612,10 @@ __global__ void __launch_bounds__(W * 32) paged_decode_fp8_join_kernel(const __g
     return;
   }
   if (ctx > p.max_pages * kPageTokens && threadIdx.x == 0) atomicCAS(p.status, 0, kStatusBadLen);
+  if (!decode_fp8_parts_valid(parts, p.row_groups, p.H_KV)) {
+    if (threadIdx.x == 0) atomicCAS(p.status, kStatusOk, kStatusTimeout);
+    return;
+  }
   if (parts.group == parts.last_group) return;
   const int n = h < G ? parts.last_group - parts.group + 1 : 0;
   auto part = [&](int i) { return i == 0 ? parts.first : 2 * ((parts.group + i) * p.H_KV + kvh); };

@@ -453,6 +453,11 @@ int hk_selftest_bwd_dealing(int B, int Nq, int Nk, int H, int H_KV, int D, int c
 int hk_selftest_decode_shape(int S, int H_KV, int max_pages_per_seq, int sm_count, const int* clusters, int clusters8,
                              int* warps);
 
+/* Host-only self-test: 1 if the kernel that joins the parts of an 8-bit decode follows such a description of a unit's parts (the part of
+ * its first group, that group and the last one, of row_groups groups of H_KV warps, which leave two parts each), 0 if it reports
+ * HK_ETIMEOUT instead, since nothing but a wait that has run out leaves it. */
+int hk_selftest_decode_fp8_parts(int first, int group, int last_group, int row_groups, int H_KV);
+
 /* Number of kernels this library has launched in the calling process (all devices). */
 unsigned long long hk_kernel_launch_count(void);
 
