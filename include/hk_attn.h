@@ -345,8 +345,8 @@ int hk_attn_bwd_ragged(const void* q, const void* k, const void* v, const void* 
                        void* cuda_stream);
 
 /* ---- The paged cache in 8 bits: pages of e4m3 codes [num_pages, 16, H_KV, D] and an fp32 scale for each page and head, K and V
- * [num_pages, H_KV] each; value = code * scale, where scales are finite and above zero. No counterpart in the reference, whose cache
- * is bf16 (training/llama/llama/models/mha.py:16-42). D = 64 or 128, page_size 16, S <= 65535; pages 16-byte aligned.
+ * [num_pages, H_KV] each; value = code * scale, where scales are finite and above zero, or NaN, as codes may be (0x7f and 0xff). No
+ * counterpart in the reference, whose cache is bf16 (training/llama/llama/models/mha.py:16-42). D = 64 or 128, page_size 16, S <= 65535; pages 16-byte aligned.
  *
  * hk_paged_kv_append_fp8 writes new tokens, K rotated on the way if tables are given (pairs (i, i + rotary_dim / 2), row = position).
  *   k_new, v_new : bf16 [S, T, H_KV, D] through element strides of the sequence, token and head (positive multiples of 8; the last
