@@ -12,9 +12,10 @@
 //  * V in bf16: an e4m3 code's exponent and mantissa moved behind its sign are the bf16 of 2^-120 times its value (subnormals
 //    included). V's codes are fetched transposed in pairs of neighbouring columns, and the two halves of such a pair are two
 //    shifts and masks apart, where `cvt` would first have to bring the tokens of one column together. A code that is NaN comes out as 480 and
-//    is found beside that, by the largest size of a page's codes (one context of 12,006 tokens 15.1 us, 14.4 without). bf16, because P takes the
-//    page's scale with it, which may be anything: p s_V / r with r the largest s_V so far keeps 8 bits whatever the scales, as 2^112
-//    times that; the accumulators are 2^-8 O l / r in fp32 until the end.
+//    is found beside that, by the largest size of a page's codes (one context of 12,006 tokens 0.6 of 15 us). bf16, because P takes the
+//    page's scale with it, which may be anything: p s_V / r, with r the power of two of the unit's largest s_V so far, keeps 8 bits whatever
+//    the scales, as 2^117 times that, and the accumulators are 2^-3 O l / r in fp32 until the end. (What is 2^-146 of r is their smallest
+//    step: values so far below the largest that the same query sees are lost, and no others.)
 // How contexts are spread (decode_pick_fp8_cluster): with few (sequence, K/V head) units a cluster of CTAs shares each, as in the bf16 kernel
 // (paged_decode_common.cuh). Otherwise the pages of all units are one row of work, of which every warp of the GPU takes an equal run,
 // whatever the contexts' lengths, and a second kernel joins the units that more than one warp had a part of.
@@ -123,8 +124,9 @@ struct DecodeFp8Warp {
   uint32_t next_seen = 0;
   // ... of those that are worked on
   int my_unit = 0;
-  float my_ks = 0.f, my_w = 0.f, most_vs = 0.f;
+  float my_ks = 0.f, my_vs = 0.f;
   uint32_t my_seen = 0;
+  uint32_t ref = 0;  // r of the unit, by its bits; 0: it has no pages yet
   // Q^T as B operand: lane (g, t) has the values 16 c + 4 t ... + 3 of head g, which the products take as its four places of the sum
   // over the dimension; K's lanes have the same places
   uint32_t qb[kChunks][2];
@@ -210,26 +212,25 @@ struct DecodeFp8Warp {
 #pragma unroll
     for (int j = 0; j < kChunks; ++j) oacc[j][0] = oacc[j][1] = oacc[j][2] = oacc[j][3] = 0.f;
     m0 = m1 = -INFINITY, l0 = l1 = 0.f;
+    ref = 0;
   }
 
-  // The pages looked up last are those that are worked on from here. P takes s_V / r, r the largest so far.
-  __device__ __forceinline__ void take_pages(bool first) {
-    constexpr float kUp = 5192296858534827628530496329220096.f;  // 2^112
-    my_ks = next_ks, my_seen = next_seen, my_unit = next_unit;
-    float most = next_vs;
+  // The pages looked up last are those that are worked on from here.
+  __device__ __forceinline__ void take_pages() { my_ks = next_ks, my_vs = next_vs, my_seen = next_seen, my_unit = next_unit; }
+  // r, where a unit begins or goes on to these pages; of those of other units nothing is taken. Between 2^-10 and 2^126, so that 2^117 / r is
+  // a number.
+  __device__ __forceinline__ void refer(int unit) {
+    const uint32_t vs = __float_as_uint(my_vs);
+    const uint32_t most = __reduce_max_sync(0xffffffffu, my_unit == unit && vs <= 0x7f800000u ? vs & 0x7f800000u : 0u);
+    const uint32_t to = min(max(most, 117u << 23), 253u << 23);
+    if (to > ref) {
+      const float less = __uint_as_float(ref) * __uint_as_float((254u << 23) - to);
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
-    if (most > most_vs) {
-      if (!first) {
-        const float less = most_vs / most;
+      for (int j = 0; j < kChunks; ++j)
 #pragma unroll
-        for (int j = 0; j < kChunks; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) oacc[j][e] *= less;
-      }
-      most_vs = most;
+        for (int e = 0; e < 4; ++e) oacc[j][e] *= less;
+      ref = to;
     }
-    my_w = most_vs > 0.f ? next_vs / most_vs * kUp : next_vs * kUp;  // all zero, or NaN
   }
   __device__ __forceinline__ uint32_t seen_of(int i) const { return __shfl_sync(0xffffffffu, my_seen, i & 31); }
 
@@ -265,7 +266,7 @@ struct DecodeFp8Warp {
     using namespace dec;
     if (!__all_sync(0xffffffffu, ptx::mbar_wait(full + i % Ring::kStages, (i / Ring::kStages) & 1, abort_word, kWaitLimitCycles))) return false;
     const uint32_t sK = ring_at + (i % Ring::kStages) * Ring::kStageBytes, sV = sK + Ring::kSlabBytes;
-    const float ks = __shfl_sync(0xffffffffu, my_ks, i & 31), wv = __shfl_sync(0xffffffffu, my_w, i & 31);
+    const float ks = __shfl_sync(0xffffffffu, my_ks, i & 31), wv = __shfl_sync(0xffffffffu, my_vs, i & 31) * __uint_as_float((371u << 23) - ref);
     const float c = p.scale_log2;
     // ---- S^T[16 tokens x 8 heads] = K Q^T, even and odd chunks apart: one accumulator's products wait for one another
     float sc[4] = {0.f, 0.f, 0.f, 0.f}, sd[4] = {0.f, 0.f, 0.f, 0.f};
@@ -325,7 +326,7 @@ struct DecodeFp8Warp {
       l0 += __shfl_xor_sync(0xffffffffu, l0, off);
       l1 += __shfl_xor_sync(0xffffffffu, l1, off);
     }
-    return most_vs > 0.f ? most_vs * 256.f : 256.f;
+    return __uint_as_float(ref) * 8.f;
   }
 };
 
@@ -387,7 +388,10 @@ paged_decode_fp8_cluster_kernel(const __grid_constant__ CUtensorMap tmap_k, cons
   for (int i = 0; i < kStages - 1; ++i) fetch(i);
   a.begin_unit(seq * p.H_KV + kvh, G);
   for (int i = 0; page_first + i * page_step < total; ++i) {
-    if ((i & 31) == 0) a.take_pages(i == 0);
+    if ((i & 31) == 0) {
+      a.take_pages();
+      a.refer(seq * p.H_KV + kvh);
+    }
     fetch(i + kStages - 1);
     if (!a.page(i, a.seen_of(i))) break;
   }
@@ -589,7 +593,7 @@ paged_decode_fp8_row_kernel(const __grid_constant__ CUtensorMap tmap_k, const __
     bool fresh = true, begun = false;
     int part = 2 * w, unit_at = 0;
     for (int i = 0; i < n; ++i) {
-      if ((i & 31) == 0) a.take_pages(i == 0);
+      if ((i & 31) == 0) a.take_pages();
       const uint32_t seen = a.seen_of(i);
       const int unit = __shfl_sync(0xffffffffu, a.my_unit, i & 31);
       if (fresh) {
@@ -597,6 +601,7 @@ paged_decode_fp8_row_kernel(const __grid_constant__ CUtensorMap tmap_k, const __
         begun = seen & Warp::kBegins;
         unit_at = i;
       }
+      if (fresh || (i & 31) == 0) a.refer(unit);
       fetch(i + kStages - 1);
       if (!a.page(i, seen)) break;
       fresh = (seen & Warp::kEnds) || i == n - 1;

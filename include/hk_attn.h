@@ -381,7 +381,8 @@ int hk_paged_kv_read_fp8(const void* k_pages, const void* v_pages, const float* 
 
 /* hk_attn_paged_decode (window = 0 and sinks = 0) and hk_attn_paged_decode_window (window > 0) against such a cache. H / H_KV from 1 to 8,
  * contexts of any length. The products take q, whose values over the power of two of
- * their row's largest become fp16, and P, which becomes bf16 after its page's scale; sums and statistics are fp32. */
+ * their row's largest become fp16, and P, which becomes bf16 after its page's scale; sums and statistics are fp32. V's scales count from the
+ * largest that the same query sees, the other sequences' have no part in it. */
 size_t hk_attn_paged_decode_fp8_workspace_bytes(int S, int H_KV, int D);
 int hk_attn_paged_decode_fp8(const void* q, const void* k_pages, const void* v_pages, const float* k_scales, const float* v_scales,
                              const int32_t* block_table, const int32_t* ctx_lens, void* o, float* lse, int S, int H, int H_KV, int D,
