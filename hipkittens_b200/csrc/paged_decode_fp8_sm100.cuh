@@ -50,7 +50,7 @@ struct DecodeFp8Params : DecodeParams {  // k_pages and v_pages are not used; a 
   int row_groups;                        // groups of H_KV warps that share the row of all pages
 };
 // A warp leaves at most two parts of units that it does not have whole: its first and its last. Workspace: their O as fp32 [part][8][D], then
-// (m, l) pairs [part][8][2], then for each unit which parts it has (DecodeFp8Parts).
+// (m, l) pairs [part][8][2], l negative where O is 2^-64 times what it is, then for each unit which parts it has (DecodeFp8Parts).
 constexpr int kRowWarps = 16 * 148;  // what a B200 holds at once
 // No warp takes fewer pages, unless there are no more: what it leaves has to be joined. us, 2 / 4 / 8 / 16, a read of 256 MB before each: one
 // context of 100,000 tokens H8/1 D128 44 / 38 / 30 / 30, of 40,000 30 / 24 / 22 / 28, of H32/8 30 / 30 / 30 / 32.
@@ -102,6 +102,8 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 }
 
 }  // namespace fp8
+
+constexpr float kHugeScale = 5.421010862427522e-20f;  // 2^-64
 
 // One warp's state: its ring, up to 32 pages that are looked up ahead, and the attention of a unit's heads over the pages so far.
 template <int D>
@@ -223,14 +225,14 @@ struct DecodeFp8Warp {
     const uint32_t vs = __float_as_uint(my_vs);
     const uint32_t most = __reduce_max_sync(0xffffffffu, my_unit == unit && vs <= 0x7f800000u ? vs & 0x7f800000u : 0u);
     const uint32_t to = min(max(most, 117u << 23), 253u << 23);
-    if (to > ref) {
+    if (ref != 0 && to > ref) {
       const float less = __uint_as_float(ref) * __uint_as_float((254u << 23) - to);
 #pragma unroll
       for (int j = 0; j < kChunks; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) oacc[j][e] *= less;
-      ref = to;
     }
+    ref = max(ref, to);
   }
   __device__ __forceinline__ uint32_t seen_of(int i) const { return __shfl_sync(0xffffffffu, my_seen, i & 31); }
 
@@ -319,26 +321,33 @@ struct DecodeFp8Warp {
     return true;
   }
 
-  // Row sums over all tokens, and what O^T is times.
-  __device__ __forceinline__ float end_unit() {
+  // Row sums over all tokens.
+  __device__ __forceinline__ void end_unit() {
 #pragma unroll
     for (int off = 4; off < 32; off <<= 1) {
       l0 += __shfl_xor_sync(0xffffffffu, l0, off);
       l1 += __shfl_xor_sync(0xffffffffu, l1, off);
     }
-    return __uint_as_float(ref) * 8.f;
   }
+  // O^T as a mean of values, which is a number where they are, of a row sum 8 / inv.
+  __device__ __forceinline__ float mean(float acc, float inv) const { return acc * inv * __uint_as_float(ref); }
+  // What it is times as a sum. The sum of values near the end of fp32, as an infinity that was appended leaves one (448 x 2^119), is no
+  // number: those are 2^-64 of theirs, and who adds them up to others takes these times 2^-64 too.
+  __device__ __forceinline__ bool is_huge() const { return ref >= (127u + 64u) << 23; }
+  __device__ __forceinline__ float sum_scale(bool huge) const { return __uint_as_float(ref) * (huge ? 8.f * kHugeScale : 8.f); }
 };
 
 // Where a wait has run out, the status says so, and copies that are still in flight get time to land before the shared memory goes away.
-__device__ __forceinline__ void decode_fp8_check_waits(const volatile uint32_t* abort_word, int* status) {
-  __syncthreads();
+// Returns whether `flag` holds for any thread of the CTA.
+__device__ __forceinline__ bool decode_fp8_check_waits(const volatile uint32_t* abort_word, int* status, bool flag = false) {
+  flag = __syncthreads_or(flag);
   if (*abort_word != 0) {
     const uint64_t t0 = ptx::globaltimer_ns();
     while (ptx::globaltimer_ns() - t0 < 2000000ull) {
     }
     if (threadIdx.x == 0) atomicCAS(status, kStatusOk, kStatusTimeout);
   }
+  return flag;
 }
 
 // grid = (cluster size, H_KV, S) in clusters along x; block = 128, dynamic smem = kFp8SmemBytes.
@@ -395,10 +404,11 @@ paged_decode_fp8_cluster_kernel(const __grid_constant__ CUtensorMap tmap_k, cons
     fetch(i + kStages - 1);
     if (!a.page(i, a.seen_of(i))) break;
   }
-  decode_fp8_check_waits(a.abort_word, p.status);
+  const bool huge = decode_fp8_check_waits(a.abort_word, p.status, a.is_huge());
 
   // ---- merge the W warps through shared memory (the ring is idle now)
-  const float out_scale = a.end_unit();
+  a.end_unit();
+  const float out_scale = a.sum_scale(huge), up = huge ? 1.f / kHugeScale : 1.f;
   float* sm_o = reinterpret_cast<float*>(dsmem);  // [W][8][D]
   float* sm_m = sm_o + W * 8 * D;                // [W][8]
   float* sm_l = sm_m + W * 8;                     // [W][8]
@@ -438,7 +448,7 @@ paged_decode_fp8_cluster_kernel(const __grid_constant__ CUtensorMap tmap_k, cons
       const int h = i * kHalves + h0;
       if (h >= G) break;
       const size_t row = size_t(seq) * p.H + kvh * G + h;
-      p.o[row * D + d] = __float2bfloat16(acc[i] / L[i]);
+      p.o[row * D + d] = __float2bfloat16(acc[i] / L[i] * up);
       if (d == 0) p.lse[row] = M[i] * p.scale + __logf(L[i]);
     }
     return;
@@ -452,7 +462,7 @@ paged_decode_fp8_cluster_kernel(const __grid_constant__ CUtensorMap tmap_k, cons
     const int h = i * kHalves + h0;
     if (h >= G) break;
     cl_o[h * D + d] = acc[i];
-    if (d == 0) cl_ml[2 * h] = M[i], cl_ml[2 * h + 1] = L[i];
+    if (d == 0) cl_ml[2 * h] = M[i], cl_ml[2 * h + 1] = huge ? -L[i] : L[i];
   }
   ptx::cluster_arrive();
   ptx::cluster_wait();
@@ -471,8 +481,17 @@ paged_decode_fp8_cluster_kernel(const __grid_constant__ CUtensorMap tmap_k, cons
       }
     }
     float Mc = m_r[0];
+    uint32_t signs = __float_as_uint(l_r[0]);
 #pragma unroll
-    for (int r = 1; r < kMaxCluster; ++r) Mc = fmaxf(Mc, m_r[r]);
+    for (int r = 1; r < kMaxCluster; ++r) Mc = fmaxf(Mc, m_r[r]), signs |= __float_as_uint(l_r[r]);
+    const bool any_huge = signs >> 31;
+    if (any_huge) {
+#pragma unroll
+      for (int r = 0; r < kMaxCluster; ++r) {
+        if (!signbit(l_r[r])) o_r[r] *= kHugeScale;
+        l_r[r] = fabsf(l_r[r]);
+      }
+    }
     float sum = 0.f, out = 0.f;
 #pragma unroll
     for (int r = 0; r < kMaxCluster; ++r) {
@@ -481,7 +500,7 @@ paged_decode_fp8_cluster_kernel(const __grid_constant__ CUtensorMap tmap_k, cons
       out += wgt * o_r[r];
     }
     const size_t row = size_t(seq) * p.H + kvh * G + h;
-    p.o[row * D + d] = __float2bfloat16(out / sum);
+    p.o[row * D + d] = __float2bfloat16(out / sum * (any_huge ? 1.f / kHugeScale : 1.f));
     if (d == 0) p.lse[row] = Mc * p.scale + __logf(sum);
   }
   ptx::cluster_arrive();  // nobody leaves while its shared memory is being read
@@ -606,7 +625,7 @@ paged_decode_fp8_row_kernel(const __grid_constant__ CUtensorMap tmap_k, const __
       if (!a.page(i, seen)) break;
       fresh = (seen & Warp::kEnds) || i == n - 1;
       if (!fresh) continue;
-      const float out_scale = a.end_unit();
+      a.end_unit();
       const int h = 2 * a.t;
       const bool whole = begun && (seen & Warp::kEnds);
       if (begun) {
@@ -614,23 +633,28 @@ paged_decode_fp8_row_kernel(const __grid_constant__ CUtensorMap tmap_k, const __
         if (a.lane == 0) *parts_of(p, unit, D) = DecodeFp8Parts{part, group, last, 0};
       }
       if (whole) {
-        const float inv0 = out_scale / a.l0, inv1 = out_scale / a.l1;
+        const float inv0 = 8.f / a.l0, inv1 = 8.f / a.l1;
         __nv_bfloat16* const dst = p.o + (size_t(unit) * G + h) * D + 2 * a.g;
 #pragma unroll
         for (int j = 0; j < Warp::kChunks; ++j) {
-          if (h < G) *reinterpret_cast<uint32_t*>(dst + j * 16) = ptx::pack_bf16x2(a.oacc[j][0] * inv0, a.oacc[j][2] * inv0);
-          if (h + 1 < G) *reinterpret_cast<uint32_t*>(dst + D + j * 16) = ptx::pack_bf16x2(a.oacc[j][1] * inv1, a.oacc[j][3] * inv1);
+          if (h < G) *reinterpret_cast<uint32_t*>(dst + j * 16) = ptx::pack_bf16x2(a.mean(a.oacc[j][0], inv0), a.mean(a.oacc[j][2], inv0));
+          if (h + 1 < G) *reinterpret_cast<uint32_t*>(dst + D + j * 16) = ptx::pack_bf16x2(a.mean(a.oacc[j][1], inv1), a.mean(a.oacc[j][3], inv1));
         }
         if (a.g < 2 && h + a.g < G)
           p.lse[size_t(unit) * G + h + a.g] = a.g ? a.m1 * p.scale + __logf(a.l1) : a.m0 * p.scale + __logf(a.l0);
       } else {
+        const bool huge = a.is_huge();
+        const float out_scale = a.sum_scale(huge);
         float* const dst = part_o(p, part, D) + h * D + 2 * a.g;
 #pragma unroll
         for (int j = 0; j < Warp::kChunks; ++j) {
           if (h < G) *reinterpret_cast<float2*>(dst + j * 16) = make_float2(a.oacc[j][0] * out_scale, a.oacc[j][2] * out_scale);
           if (h + 1 < G) *reinterpret_cast<float2*>(dst + D + j * 16) = make_float2(a.oacc[j][1] * out_scale, a.oacc[j][3] * out_scale);
         }
-        if (a.g < 2) *reinterpret_cast<float2*>(part_ml(p, part, D) + 2 * (h + a.g)) = a.g ? make_float2(a.m1, a.l1) : make_float2(a.m0, a.l0);
+        if (a.g < 2) {
+          const float l = a.g ? a.l1 : a.l0;
+          *reinterpret_cast<float2*>(part_ml(p, part, D) + 2 * (h + a.g)) = make_float2(a.g ? a.m1 : a.m0, huge ? -l : l);
+        }
       }
       part = 2 * w + 1;  // what is behind the first unit and not whole is the last one
     }
@@ -666,7 +690,15 @@ __global__ void __launch_bounds__(W * 32) paged_decode_fp8_join_kernel(const __g
   if (parts.group == parts.last_group) return;
   const int n = h < G ? parts.last_group - parts.group + 1 : 0;
   auto part = [&](int i) { return i == 0 ? parts.first : 2 * ((parts.group + i) * p.H_KV + kvh); };
-  float m = -INFINITY, l = 0.f, acc[kCols] = {};
+  // of a negative row sum O is 2^-64 times what it is: so are the sums from there on
+  float m = -INFINITY, l = 0.f, acc[kCols] = {}, unit = 1.f;
+  auto huge_too = [&] {
+    if (unit == 1.f) {
+      unit = kHugeScale;
+#pragma unroll
+      for (int k = 0; k < kCols; ++k) acc[k] *= kHugeScale;
+    }
+  };
 #pragma unroll 4
   for (int i = sub; i < n; i += per_head) {
     const float2 ml = *reinterpret_cast<const float2*>(part_ml(p, part(i), D) + 2 * h);
@@ -675,30 +707,37 @@ __global__ void __launch_bounds__(W * 32) paged_decode_fp8_join_kernel(const __g
     if constexpr (kCols == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(src);
     else *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(src);
     const float top = fmaxf(m, ml.x), a = ptx::ex2_approx((m - top) * p.scale_log2), b = ptx::ex2_approx((ml.x - top) * p.scale_log2);
+    const bool huge = signbit(ml.y);
+    if (huge) huge_too();
+    const float b_o = huge ? b : b * unit;
     m = top;
-    l = l * a + ml.y * b;
+    l = l * a + fabsf(ml.y) * b;
 #pragma unroll
-    for (int k = 0; k < kCols; ++k) acc[k] = acc[k] * a + x[k] * b;
+    for (int k = 0; k < kCols; ++k) acc[k] = acc[k] * a + x[k] * b_o;
   }
   if (per_head > 1) {
-    if (lane == 0) s_m[warp] = m, s_l[warp] = l;
+    if (lane == 0) s_m[warp] = m, s_l[warp] = unit == 1.f ? l : -l;
 #pragma unroll
     for (int k = 0; k < kCols; ++k) s_o[warp][lane * kCols + k] = acc[k];
     __syncthreads();
     if (sub == 0) {
       for (int w = warp + 1; w < warp + per_head; ++w) {  // a warp without a part has l = 0 and m = -inf, and this one has one
         const float top = fmaxf(m, s_m[w]), a = ptx::ex2_approx((m - top) * p.scale_log2), b = ptx::ex2_approx((s_m[w] - top) * p.scale_log2);
+        const bool huge = signbit(s_l[w]);
+        if (huge) huge_too();
+        const float b_o = huge ? b : b * unit;
         m = top;
-        l = l * a + s_l[w] * b;
+        l = l * a + fabsf(s_l[w]) * b;
 #pragma unroll
-        for (int k = 0; k < kCols; ++k) acc[k] = acc[k] * a + s_o[w][lane * kCols + k] * b;
+        for (int k = 0; k < kCols; ++k) acc[k] = acc[k] * a + s_o[w][lane * kCols + k] * b_o;
       }
     }
   }
   if (h >= G || sub != 0) return;
+  const float up = unit == 1.f ? 1.f : 1.f / kHugeScale;
   uint32_t out[kCols / 2];
 #pragma unroll
-  for (int k = 0; k < kCols / 2; ++k) out[k] = ptx::pack_bf16x2(acc[2 * k] / l, acc[2 * k + 1] / l);
+  for (int k = 0; k < kCols / 2; ++k) out[k] = ptx::pack_bf16x2(acc[2 * k] / l * up, acc[2 * k + 1] / l * up);
   uint32_t* const dst = reinterpret_cast<uint32_t*>(p.o + (row + h) * D + lane * kCols);
 #pragma unroll
   for (int k = 0; k < kCols / 2; ++k) dst[k] = out[k];
