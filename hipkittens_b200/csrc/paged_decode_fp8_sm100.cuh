@@ -95,6 +95,12 @@ struct Bf16Codes {
 __device__ __forceinline__ bool has_nan(uint32_t top) { return ((top + 0x00100010u) & 0x08000800u) != 0; }
 // The high bit of each code that is NaN.
 __device__ __forceinline__ uint32_t nan_codes(uint32_t x) { return ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+// The largest number for what is above it (and above zero), so that a score of zero is one; NaN stays.
+__device__ __forceinline__ float finite(float x) {
+  float y;
+  asm("min.NaN.f32 %0, %1, 0f7F7FFFFF;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -279,7 +285,7 @@ struct DecodeFp8Warp {
       fp8::mma_f16(sc, fp8::widen(r0), fp8::widen(r1), fp8::widen(r0 >> 16), fp8::widen(r1 >> 16), qb[ch][0], qb[ch][1]);
       fp8::mma_f16(sd, fp8::widen(r2), fp8::widen(r3), fp8::widen(r2 >> 16), fp8::widen(r3 >> 16), qb[ch + 1][0], qb[ch + 1][1]);
     }
-    const float f0 = ks * qs0, f1 = ks * qs1;
+    const float f0 = fp8::finite(ks * qs0), f1 = fp8::finite(ks * qs1);
     float sv[4] = {(sc[0] + sd[0]) * f0, (sc[1] + sd[1]) * f1, (sc[2] + sd[2]) * f0, (sc[3] + sd[3]) * f1};
     // ---- online softmax over tokens g and g + 8 of this page, heads 2 t and 2 t + 1
     if ((seen & kAll) != kAll) {

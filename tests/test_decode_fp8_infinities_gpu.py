@@ -51,3 +51,21 @@ def test_values_of_another_quantiser_s_scales(dev):  # noqa: F811
     a[4].fill_(2.0 ** 126)
     for b in (a, wide(a, 2100)):
         check(b, hk.paged_decode_fp8(*b))
+
+
+@pytest.mark.parametrize("row", [False, True])
+def test_an_infinity_of_k(dev, row):  # noqa: F811
+    """In a column where q is zero: its page's scores are those of a page of zeros, also where q's largest value times the page's scale is
+    above fp32."""
+    a = make(dev, [100, 50], 4, 2, 128, seed=9)
+    at = a[5][0, 2].long()
+    a[0][0, 0, :, 7] = 0.0
+    a[0][0, 0, :, 1] = 1024.0
+    a[1][:, :, :, 1] = 0.0
+    a[1][at] = 0.0
+    zeros = [t.clone() for t in a]
+    a[1][at, 3, :, 7] = 448.0
+    a[3][at] = 2.0 ** 119
+    if row:
+        a = wide(a, 2100)
+    check(zeros, hk.paged_decode_fp8(*a))
