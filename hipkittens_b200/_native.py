@@ -1241,8 +1241,8 @@ def paged_kv_read_fp8(
 
     With `ctx_lens` (int32 [S]): [S,rows,H_KV,D], the first ctx_lens[s] tokens of each sequence and zeros behind them, as ``attn_fwd(...,
     kv_lens=ctx_lens)`` takes them. With `cu_seqlens` (int32 [S+1]): [rows,H_KV,D], the first cu_seqlens[s+1] - cu_seqlens[s] tokens
-    of sequence s from row cu_seqlens[s] on, as ``attn_fwd_ragged`` takes them; rows behind the last sequence are zeros in new outputs,
-    and left as they are in `k_out` and `v_out`."""
+    of sequence s from row cu_seqlens[s] on, as ``attn_fwd_ragged`` takes them; rows that belong to no sequence, in front of the first one or
+    behind the last, are zeros in new outputs, and left as they are in `k_out` and `v_out`."""
     if stream is None:
         r = _front().paged_kv_read_fp8(k_pages, v_pages, k_scales, v_scales, block_table, rows, ctx_lens, cu_seqlens, k_out, v_out)
         if r is not None:
@@ -1258,7 +1258,7 @@ def paged_kv_read_fp8(
         _check_int32("cu_seqlens", cu_seqlens, s_n + 1, k_pages)
     if (k_out is None) != (v_out is None):
         raise RuntimeError("k_out and v_out belong together")
-    zero_tail = k_out is None
+    zero_rest = k_out is None
     shape = (s_n, rows, hkv, d) if cu_seqlens is None else (rows, hkv, d)
     outs = []
     for name, t in (("k_out", k_out), ("v_out", v_out)):
@@ -1271,7 +1271,7 @@ def paged_kv_read_fp8(
         st = stream if stream is not None else torch.cuda.current_stream(k_pages.device)
         _check(capi().hk_paged_kv_read_fp8(
             k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), block_table.data_ptr(), _ptr(ctx_lens),
-            _ptr(cu_seqlens), outs[0].data_ptr(), outs[1].data_ptr(), s_n, rows, hkv, d, int(zero_tail), k_pages.shape[1],
+            _ptr(cu_seqlens), outs[0].data_ptr(), outs[1].data_ptr(), s_n, rows, hkv, d, int(zero_rest), k_pages.shape[1],
             block_table.shape[1], p_n, k_pages.device.index, st.cuda_stream), "hk_paged_kv_read_fp8")
     return outs[0], outs[1]
 

@@ -102,7 +102,7 @@ int hk_paged_kv_append_fp8(const void* k_new, const void* v_new, void* k_pages, 
 
 int hk_paged_kv_read_fp8(const void* k_pages, const void* v_pages, const float* k_scales, const float* v_scales,
                          const int32_t* block_table, const int32_t* ctx_lens, const int32_t* cu_seqlens, void* k_out, void* v_out,
-                         int S, int rows, int H_KV, int D, int zero_tail, int page_size, int max_pages_per_seq, int num_pages,
+                         int S, int rows, int H_KV, int D, int zero_rest, int page_size, int max_pages_per_seq, int num_pages,
                          int device, void* cuda_stream) {
   hk::ReadFp8Params p = {};
   int rc = fp8_cache(p.c, k_pages, v_pages, k_scales, v_scales, block_table, S, H_KV, D, page_size, max_pages_per_seq, num_pages);
@@ -121,7 +121,7 @@ int hk_paged_kv_read_fp8(const void* k_pages, const void* v_pages, const float* 
   p.ctx_lens = ctx_lens;
   p.k_out = static_cast<__nv_bfloat16*>(k_out);
   p.v_out = static_cast<__nv_bfloat16*>(v_out);
-  p.zero_tail = zero_tail;
+  p.zero_rest = zero_rest;
   p.fd_heads = hk::FastDiv(H_KV);
   auto* fn = D == 128 ? hk::paged_kv_read_fp8_kernel<128> : hk::paged_kv_read_fp8_kernel<64>;
   HK_CUDA(hk::launch_dependent(true, fn, unsigned((p.warps + 7ll) / 8), 256, 0, static_cast<cudaStream_t>(cuda_stream), p));

@@ -388,7 +388,7 @@ struct ReadFp8Params {
   Fp8Rows rows;
   const int32_t* ctx_lens;        // [S], without rows.cu
   __nv_bfloat16 *k_out, *v_out;   // contiguous
-  int zero_tail;                  // with rows.cu: rows behind the last sequence become zeros
+  int zero_rest;                  // with rows.cu: rows in front of the first sequence and behind the last one become zeros
   int warps;                      // units x H_KV
   FastDiv fd_heads;
 };
@@ -412,13 +412,20 @@ __global__ void __launch_bounds__(256) paged_kv_read_fp8_kernel(const __grid_con
   if (cu) {
     s = fp8::sequence_of<1>(cu, c.S + 1, unit);
     block = unit - fp8::first_unit<1>(cu, s);
+    if (s == 0 && block <= 0 && p.zero_rest) {  // the rows of this unit that are in front of the first sequence
+      const int row = unit * kPageTokens, n = min(min(max(cu[0], 0), p.rows.T) - row, kPageTokens);
+      for (int i = lane; i < n * (D / 8); i += 32) {
+        const size_t at = (static_cast<size_t>(row + i / (D / 8)) * c.H_KV + head) * D + i % (D / 8) * 8;
+        *reinterpret_cast<uint4*>(p.k_out + at) = *reinterpret_cast<uint4*>(p.v_out + at) = make_uint4(0, 0, 0, 0);
+      }
+    }
     if (block < 0) return;
     int first;
     if (s < c.S) {
       fp8::ragged_rows(cu, s, p.rows.T, first, len);
       there = len - block * kPageTokens;
     } else {
-      if (!p.zero_tail) return;
+      if (!p.zero_rest) return;
       first = min(max(cu[s], 0), p.rows.T);
       len = 0;
       there = p.rows.T - first - block * kPageTokens;

@@ -580,10 +580,10 @@ PyObject* paged_kv_read_fp8(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   c.read();
   void *ko = ptr(out[0]), *vo = ptr(out[1]);
   const int32_t *lensp = lens ? ptr<int32_t>(*lens) : nullptr, *cup = cu ? ptr<int32_t>(*cu) : nullptr;
-  const int zero_tail = a[8] == Py_None;
+  const int zero_rest = a[8] == Py_None;
   const int rc = unlocked([&] {
     return hk_paged_kv_read_fp8(c.k_pages, c.v_pages, c.k_scales, c.v_scales, c.table_ptr, lensp, cup, ko, vo, i32(c.s), i32(rows),
-                                i32(c.hkv), i32(c.d), zero_tail, i32(c.page), i32(c.max_pages), i32(c.pool), c.device, stream);
+                                i32(c.hkv), i32(c.d), zero_rest, i32(c.page), i32(c.max_pages), i32(c.pool), c.device, stream);
   });
   return result(rc, out[0], out[1]);
   END_HANDLE_TH_ERRORS

@@ -370,13 +370,13 @@ int hk_paged_kv_append_fp8(const void* k_new, const void* v_new, void* k_pages, 
 /* Reads tokens back as bf16 (fp32 product, rounded once), for instance as keys and values of the attention of a chunk.
  *   ctx_lens   : int32 [S]; k_out, v_out [S, rows, H_KV, D] get tokens 0 .. ctx_lens[s] - 1 of each sequence and zeros behind them
  *   cu_seqlens : int32 [S + 1], instead of ctx_lens; k_out, v_out [rows, H_KV, D] get the first cu_seqlens[s + 1] - cu_seqlens[s]
- *                tokens of sequence s from row cu_seqlens[s] on. Rows behind the last sequence are left as they are, or zeros with
- *                `zero_tail`.
+ *                tokens of sequence s from row cu_seqlens[s] on. Rows in front of the first sequence and behind the last one are left
+ *                as they are, or zeros with `zero_rest`.
  * Tokens behind the block table are zeros, and a length above `rows` is cut (HK_EBADLEN both); those of a page id outside the pool are
  * zeros (HK_EBADPAGE). */
 int hk_paged_kv_read_fp8(const void* k_pages, const void* v_pages, const float* k_scales, const float* v_scales,
                          const int32_t* block_table, const int32_t* ctx_lens, const int32_t* cu_seqlens, void* k_out, void* v_out,
-                         int S, int rows, int H_KV, int D, int zero_tail, int page_size, int max_pages_per_seq, int num_pages,
+                         int S, int rows, int H_KV, int D, int zero_rest, int page_size, int max_pages_per_seq, int num_pages,
                          int device, void* cuda_stream);
 
 /* hk_attn_paged_decode (window = 0 and sinks = 0) and hk_attn_paged_decode_window (window > 0) against such a cache. H / H_KV from 1 to 8,
