@@ -276,6 +276,15 @@ def _new(shape, dtype: torch.dtype, device: torch.device, stream) -> torch.Tenso
     return t
 
 
+def _scratch(shape, dtype: torch.dtype, device: torch.device, stream) -> torch.Tensor:
+    """What a call needs for itself, from the memory of the stream that uses it, and back there when the call returns: no other stream reads
+    it."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
 def _strides3(t):
     # a dimension of size 1 has no stride that matters: give it one the library takes
     return (ctypes.c_longlong * 3)(*(st if n > 1 else t.shape[3] for st, n in zip(t.stride()[:3], t.shape[:3])))
@@ -735,7 +744,7 @@ def qk_norm_rotary_bwd(
     need = int(capi().hk_qk_norm_rotary_bwd_workspace_bytes(d))
     dq, dk = (_new(t.shape, t.dtype, t.device, stream) for t in (q, k))
     dws = [_new(w.shape, w.dtype, w.device, stream) if weight_grads and w is not None else None for w in (q_weight, k_weight)]
-    ws = _new(need, torch.uint8, q.device, stream) if any(w is not None for w in dws) else None
+    ws = _scratch(need, torch.uint8, q.device, stream) if any(w is not None for w in dws) else None
     _check(capi().hk_qk_norm_rotary_bwd(q.data_ptr(), k.data_ptr(), _ptr(q_weight), _ptr(k_weight), cos.data_ptr(), sin.data_ptr(),
                                         dq_out.data_ptr(), dk_out.data_ptr(), dq.data_ptr(), dk.data_ptr(), _ptr(dws[0]),
                                         _ptr(dws[1]), b, n, h, k.shape[2], d, 2 * cos.shape[1], cos.shape[0], _strides3(q),
@@ -819,7 +828,7 @@ def paged_decode(
                       "max_pages, or pages of a window and its sinks, <= 8192)")
     st = stream if stream is not None else torch.cuda.current_stream(q.device)
     if workspace is None:
-        workspace = _new(max(need, 256), torch.uint8, q.device, stream)  # it goes back to the stream that uses it
+        workspace = _scratch(max(need, 256), torch.uint8, q.device, stream)
     _require_same_device(q, k_pages=k_pages, v_pages=v_pages, block_table=block_table, ctx_lens=ctx_lens, out=out,
                          lse=lse, workspace=workspace)
     if window is not None:
@@ -1060,7 +1069,7 @@ def attn_fwd_ragged(
     _require_same_device(q, out=out, lse=lse)
     s_n = cu_seqlens_q.shape[0] - 1
     need = int(capi().hk_attn_fwd_ragged_workspace_bytes(s_n, t_n))
-    ws = _new(need, torch.uint8, q.device, stream)
+    ws = _scratch(need, torch.uint8, q.device, stream)
     st = stream if stream is not None else torch.cuda.current_stream(q.device)
     _check(capi().hk_attn_fwd_ragged(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), cu_seqlens_q.data_ptr(),
                                      cu_seqlens_k.data_ptr(), s_n, t_n, k.shape[0], h, k.shape[1], d, _ragged_strides(q),
@@ -1112,8 +1121,8 @@ def attn_bwd_ragged(
     _require_same_device(q, o=o, d_o=d_o, lse=lse, dq=dq, dk=dk, dv=dv)
     s_n = cu_seqlens_q.shape[0] - 1
     need = int(capi().hk_attn_bwd_ragged_workspace_bytes(s_n, t_n, k.shape[0]))
-    ws = _new(need, torch.uint8, q.device, stream)
-    delta = _new(lse.shape, torch.float32, q.device, stream)
+    ws = _scratch(need, torch.uint8, q.device, stream)
+    delta = _scratch(lse.shape, torch.float32, q.device, stream)
     st = stream if stream is not None else torch.cuda.current_stream(q.device)
     _check(capi().hk_attn_bwd_ragged(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), d_o.data_ptr(), lse.data_ptr(),
                                      delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), cu_seqlens_q.data_ptr(),
@@ -1325,7 +1334,7 @@ def paged_decode_fp8(
     if need == 0:
         raise HkError(HK_EUNSUPPORTED, "hk_attn_paged_decode_fp8", "shape outside the decode kernels' limits (D = 64 or 128, 1 <= S <= 65535)")
     if workspace is None:
-        workspace = _new(need, torch.uint8, q.device, stream)  # it goes back to the stream that uses it
+        workspace = _scratch(need, torch.uint8, q.device, stream)
     if not isinstance(workspace, torch.Tensor) or not workspace.is_contiguous():
         raise RuntimeError("workspace must be a contiguous tensor")
     _require_same_device(k_pages, q=q, out=out, lse=lse, workspace=workspace)
