@@ -285,7 +285,8 @@ class RaggedAttnFunction(Function):
 class HipRaggedAttention(nn.Module):
     """HipCrossAttention over a ragged batch: q [T, H, D], kv [Tk, 2, H_KV, D] bf16 -> [T, H, D], the sequences one after the other as
     ``attn_fwd_ragged`` says (`cu_seqlens_k` None: queries and keys are the same tokens). The reference's modules pad instead
-    (hipkittens.py:122-202). A call does not synchronise: what the device has to say of offsets that fall is in its status."""
+    (hipkittens.py:122-202). A call does not synchronise: what the device has to say of offsets that fall is in its status. There is no dropout
+    of attention weights: in training, a module that was given a rate above zero refuses to run."""
 
     def __init__(self, causal=False, softmax_scale=None, attention_dropout=0.0, deterministic=False):
         super().__init__()
@@ -295,6 +296,8 @@ class HipRaggedAttention(nn.Module):
         self.deterministic = deterministic
 
     def forward(self, q, kv, cu_seqlens_q, cu_seqlens_k=None, causal=None):
+        if self.training and self.drop.p > 0:
+            raise RuntimeError("HipRaggedAttention has no dropout: attention_dropout must be 0 in training")
         causal = self.causal if causal is None else causal
         return RaggedAttnFunction.apply(q, kv, cu_seqlens_q, cu_seqlens_k, causal, self.softmax_scale)
 
