@@ -13,7 +13,7 @@
 //    included). V's codes are fetched transposed in pairs of neighbouring columns, and the two halves of such a pair are two
 //    shifts and masks apart, where `cvt` would first have to bring the tokens of one column together. A code that is NaN comes out as 480 and
 //    is found beside that, by the largest size of a page's codes (one context of 12,006 tokens 0.6 of 15 us). bf16, because P takes the
-//    page's scale with it, which may be anything: p s_V / r, with r the power of two of the unit's largest s_V so far, keeps 8 bits whatever
+//    page's scale with it, which may be anything: p s_V / r, with r the unit's largest s_V so far, keeps 8 bits whatever
 //    the scales, as 2^117 times that, and the accumulators are 2^-3 O l / r in fp32 until the end. (What is 2^-146 of r is their smallest
 //    step: values so far below the largest that the same query sees are lost, and no others.)
 // How contexts are spread (decode_pick_fp8_cluster): with few (sequence, K/V head) units a cluster of CTAs shares each, as in the bf16 kernel
@@ -134,7 +134,7 @@ struct DecodeFp8Warp {
   int my_unit = 0;
   float my_ks = 0.f, my_vs = 0.f;
   uint32_t my_seen = 0;
-  uint32_t ref = 0;  // r of the unit, by its bits; 0: it has no pages yet
+  float ref = 0.f;  // r of the unit; 0: it has no pages yet
   // Q^T as B operand: lane (g, t) has the values 16 c + 4 t ... + 3 of head g, which the products take as its four places of the sum
   // over the dimension; K's lanes have the same places
   uint32_t qb[kChunks][2];
@@ -220,25 +220,27 @@ struct DecodeFp8Warp {
 #pragma unroll
     for (int j = 0; j < kChunks; ++j) oacc[j][0] = oacc[j][1] = oacc[j][2] = oacc[j][3] = 0.f;
     m0 = m1 = -INFINITY, l0 = l1 = 0.f;
-    ref = 0;
+    ref = 0.f;
   }
 
   // The pages looked up last are those that are worked on from here.
   __device__ __forceinline__ void take_pages() { my_ks = next_ks, my_vs = next_vs, my_seen = next_seen, my_unit = next_unit; }
-  // r, where a unit begins or goes on to these pages; of those of other units nothing is taken. Between 2^-10 and 2^126, so that 2^117 / r is
-  // a number.
+  // r, where a unit begins or goes on to these pages, and what P takes of each of them: 2^117 s_V / r. Of pages of other units nothing is
+  // taken. r is a number, and 2^-10 at least, so that 2^117 / r is one.
   __device__ __forceinline__ void refer(int unit) {
+    constexpr float kUp = 166153499473114484112975882535043072.f;  // 2^117
     const uint32_t vs = __float_as_uint(my_vs);
-    const uint32_t most = __reduce_max_sync(0xffffffffu, my_unit == unit && vs <= 0x7f800000u ? vs & 0x7f800000u : 0u);
-    const uint32_t to = min(max(most, 117u << 23), 253u << 23);
-    if (ref != 0 && to > ref) {
-      const float less = __uint_as_float(ref) * __uint_as_float((254u << 23) - to);
+    const uint32_t most = __reduce_max_sync(0xffffffffu, my_unit == unit && vs <= 0x7f800000u ? min(max(vs, 117u << 23), 0x7f7fffffu) : 117u << 23);
+    const float to = fmaxf(ref, __uint_as_float(most));
+    if (ref != 0.f && to > ref) {
+      const float less = ref / to;
 #pragma unroll
       for (int j = 0; j < kChunks; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) oacc[j][e] *= less;
     }
-    ref = max(ref, to);
+    ref = to;
+    if (my_unit == unit) my_vs *= kUp / to;
   }
   __device__ __forceinline__ uint32_t seen_of(int i) const { return __shfl_sync(0xffffffffu, my_seen, i & 31); }
 
@@ -274,7 +276,7 @@ struct DecodeFp8Warp {
     using namespace dec;
     if (!__all_sync(0xffffffffu, ptx::mbar_wait(full + i % Ring::kStages, (i / Ring::kStages) & 1, abort_word, kWaitLimitCycles))) return false;
     const uint32_t sK = ring_at + (i % Ring::kStages) * Ring::kStageBytes, sV = sK + Ring::kSlabBytes;
-    const float ks = __shfl_sync(0xffffffffu, my_ks, i & 31), wv = __shfl_sync(0xffffffffu, my_vs, i & 31) * __uint_as_float((371u << 23) - ref);
+    const float ks = __shfl_sync(0xffffffffu, my_ks, i & 31), wv = __shfl_sync(0xffffffffu, my_vs, i & 31);
     const float c = p.scale_log2;
     // ---- S^T[16 tokens x 8 heads] = K Q^T, even and odd chunks apart: one accumulator's products wait for one another
     float sc[4] = {0.f, 0.f, 0.f, 0.f}, sd[4] = {0.f, 0.f, 0.f, 0.f};
@@ -336,11 +338,11 @@ struct DecodeFp8Warp {
     }
   }
   // O^T as a mean of values, which is a number where they are, of a row sum 8 / inv.
-  __device__ __forceinline__ float mean(float acc, float inv) const { return acc * inv * __uint_as_float(ref); }
+  __device__ __forceinline__ float mean(float acc, float inv) const { return acc * inv * ref; }
   // What it is times as a sum. The sum of values near the end of fp32, as an infinity that was appended leaves one (448 x 2^119), is no
   // number: those are 2^-64 of theirs, and who adds them up to others takes these times 2^-64 too.
-  __device__ __forceinline__ bool is_huge() const { return ref >= (127u + 64u) << 23; }
-  __device__ __forceinline__ float sum_scale(bool huge) const { return __uint_as_float(ref) * (huge ? 8.f * kHugeScale : 8.f); }
+  __device__ __forceinline__ bool is_huge() const { return ref >= 1.f / kHugeScale; }
+  __device__ __forceinline__ float sum_scale(bool huge) const { return ref * (huge ? 8.f * kHugeScale : 8.f); }
 };
 
 // Where a wait has run out, the status says so, and copies that are still in flight get time to land before the shared memory goes away.
