@@ -326,7 +326,8 @@ int hk_paged_kv_append_rotary(const void* k_new, const void* v_new, void* k_page
  * o and d_o are contiguous. With `causal` query r of a sequence sees its keys up to r + (keys - queries), as in hk_attn_fwd_cross; a row
  * that sees none has O = 0 and L = -inf. Rows that belong to no sequence are left as they are, or with `fill_rest` become O = 0, L =
  * -inf and zero gradients. What a sequence's neighbours hold, NaN and infinities too, does not reach it.
- * D = 64 or 128, S <= 65535, rows <= 2^30. cu_seqlens that fall or lie outside are reported as HK_EBADLEN, and the call writes nothing.
+ * D = 64 or 128, S <= 65535, rows <= 2^30. cu_seqlens that fall or lie outside are reported as HK_EBADLEN, and the call writes nothing
+ * (the backward nothing but delta).
  * workspace: device scratch, 256-byte aligned, of at least the bytes that the functions say (0: such sizes are refused). Nothing is added
  * up with atomics: results are the same from run to run. Asynchronous on `cuda_stream`.
  * The backward writes delta [H, q_rows] (rowsum(O * dO); of rows of few keys, the sum of P dP over these), dq, dk and dv. dq may not share
@@ -359,7 +360,8 @@ int hk_attn_bwd_ragged(const void* q, const void* k, const void* v, const void* 
  * Infinities become the block's largest value; a NaN makes the block's scale NaN, and with it all of the block for every reader.
  * The tokens of one block have to come from one sequence of a call: a page that two sequences share takes no new tokens.
  * Positions outside the block table and page ids outside the pool are skipped (HK_EBADPAGE), positions behind the tables too
- * (HK_EBADPOS); a cu_seqlens that does not rise from 0 to at most T is reported as HK_EBADLEN, and its rows are kept inside [0, T). */
+ * (HK_EBADPOS). Rows of k_new and v_new in front of cu_seqlens[0] or from cu_seqlens[S] on are no sequence's; a cu_seqlens that falls or
+ * leaves [0, T] is reported as HK_EBADLEN, and its rows are kept inside. */
 #define HK_FP8_TABLE_F32 1
 int hk_paged_kv_append_fp8(const void* k_new, const void* v_new, void* k_pages, void* v_pages, float* k_scales, float* v_scales,
                            const int32_t* block_table, const int32_t* start_pos, const int32_t* cu_seqlens, const void* sin,
@@ -373,7 +375,7 @@ int hk_paged_kv_append_fp8(const void* k_new, const void* v_new, void* k_pages, 
  *                tokens of sequence s from row cu_seqlens[s] on. Rows in front of the first sequence and behind the last one are left
  *                as they are, or zeros with `zero_rest`.
  * Tokens behind the block table are zeros, and a length above `rows` is cut (HK_EBADLEN both); those of a page id outside the pool are
- * zeros (HK_EBADPAGE). */
+ * zeros (HK_EBADPAGE). A cu_seqlens that falls or leaves [0, rows] is reported as HK_EBADLEN, and its rows are kept inside. */
 int hk_paged_kv_read_fp8(const void* k_pages, const void* v_pages, const float* k_scales, const float* v_scales,
                          const int32_t* block_table, const int32_t* ctx_lens, const int32_t* cu_seqlens, void* k_out, void* v_out,
                          int S, int rows, int H_KV, int D, int zero_rest, int page_size, int max_pages_per_seq, int num_pages,

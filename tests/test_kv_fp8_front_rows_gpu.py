@@ -1,4 +1,4 @@
-"""Reading ragged sequences back whose first does not begin at row 0: the rows in front of it are no sequence's."""
+"""Ragged sequences whose first does not begin at row 0, read back and appended: the rows in front of it are no sequence's."""
 import pytest
 import torch
 
@@ -34,4 +34,21 @@ def test_rows_in_front(dev, hkv, d, front, lens):  # noqa: F811
             if n:
                 want = ref.tokens(cache.ref[j], cache.ref[2 + j], cache.table[i], n).to(torch.bfloat16)
                 assert torch.equal(new[j][cu[i]:cu[i + 1]].cpu(), want) and torch.equal(given[j][cu[i]:cu[i + 1]].cpu(), want)
+    assert _native.device_status(0) == _native.HK_OK
+
+
+@pytest.mark.parametrize("front", [1, 16, 37])
+def test_an_append_from_a_later_row_on(dev, front):  # noqa: F811
+    hkv, d, lens, start = 2, 64, [20, 0, 33], [3, 0, 17]
+    cache = Cache(dev, 12, hkv, d, 3, 4, seed=front)
+    cu = [front + sum(lens[:i]) for i in range(4)]
+    x = torch.randn(cu[-1] + 11, hkv, d, generator=torch.Generator().manual_seed(front)).to(torch.bfloat16)
+    x[:front], x[cu[-1]:] = float("nan"), 1e30
+    hk.paged_kv_append_fp8(x.to(dev), x.to(dev), *cache.gpu, int32(dev, start), cu_seqlens=int32(dev, cu))
+    for i, n in enumerate(lens):
+        if n:
+            for j in (0, 1):
+                ref.append(cache.ref[j], cache.ref[2 + j], cache.table[i], start[i], x[cu[i]:cu[i + 1]])
+    for got, want in zip(cache.values(), cache.ref):
+        assert torch.equal(got, want)
     assert _native.device_status(0) == _native.HK_OK
