@@ -19,9 +19,9 @@
 // How contexts are spread (decode_pick_fp8_cluster): with few (sequence, K/V head) units a cluster of CTAs shares each, as in the bf16 kernel
 // (paged_decode_common.cuh). Otherwise the pages of all units are one row of work, of which every warp of the GPU takes an equal run,
 // whatever the contexts' lengths, and a second kernel joins the units that more than one warp had a part of.
-// Bound by HBM where contexts are many: 64 of 512 to 8192 tokens, H64/8 D128, in a loop 71.6 us, 70% of the copy rate; the row kernel
-// takes 64 of them and is at 94% of it for equal contexts, the join the rest. One context of 12,006 tokens (H32/8) 14 us, of which its 25 MB
-// are 3.8: a launch, three dependent loads and the cluster's barriers are the rest. At D = 64 a TMA row is 64 bytes and their rate the bound.
+// Bound by HBM where contexts are many: 64 of 512 to 8192 tokens, H64/8 D128, in a loop 70 us, 71% of the copy rate; the row kernel
+// takes 63 of them and is at 94% of it for equal contexts, the join the rest. One context of 12,006 tokens (H32/8) 14.7 us, of which its 25
+// MB are 3.8: a launch, three dependent loads and the cluster's barriers are the rest. At D = 64 a TMA row is 64 bytes and their rate the bound.
 #pragma once
 
 #include <cuda.h>
