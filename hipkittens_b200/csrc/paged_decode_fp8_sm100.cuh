@@ -337,10 +337,8 @@ struct DecodeFp8Warp {
       l1 += __shfl_xor_sync(0xffffffffu, l1, off);
     }
   }
-  // O^T as a mean of values, which is a number where they are, of a row sum 8 / inv.
-  __device__ __forceinline__ float mean(float acc, float inv) const { return acc * inv * ref; }
-  // What it is times as a sum. The sum of values near the end of fp32, as an infinity that was appended leaves one (448 x 2^119), is no
-  // number: those are 2^-64 of theirs, and who adds them up to others takes these times 2^-64 too.
+  // What O^T is times. The sum of values near the end of fp32, as an infinity that was appended leaves one (448 x 2^119), is no number:
+  // those are 2^-64 of theirs, and who adds them up to others takes these times 2^-64 too.
   __device__ __forceinline__ bool is_huge() const { return ref >= 1.f / kHugeScale; }
   __device__ __forceinline__ float sum_scale(bool huge) const { return ref * (huge ? 8.f * kHugeScale : 8.f); }
 };
@@ -641,12 +639,14 @@ paged_decode_fp8_row_kernel(const __grid_constant__ CUtensorMap tmap_k, const __
         if (a.lane == 0) *parts_of(p, unit, D) = DecodeFp8Parts{part, group, last, 0};
       }
       if (whole) {
-        const float inv0 = 8.f / a.l0, inv1 = 8.f / a.l1;
+        // a mean of values is a number where they are
+        const bool huge = a.is_huge();
+        const float out_scale = a.sum_scale(huge), up = huge ? 1.f / kHugeScale : 1.f, inv0 = out_scale / a.l0, inv1 = out_scale / a.l1;
         __nv_bfloat16* const dst = p.o + (size_t(unit) * G + h) * D + 2 * a.g;
 #pragma unroll
         for (int j = 0; j < Warp::kChunks; ++j) {
-          if (h < G) *reinterpret_cast<uint32_t*>(dst + j * 16) = ptx::pack_bf16x2(a.mean(a.oacc[j][0], inv0), a.mean(a.oacc[j][2], inv0));
-          if (h + 1 < G) *reinterpret_cast<uint32_t*>(dst + D + j * 16) = ptx::pack_bf16x2(a.mean(a.oacc[j][1], inv1), a.mean(a.oacc[j][3], inv1));
+          if (h < G) *reinterpret_cast<uint32_t*>(dst + j * 16) = ptx::pack_bf16x2(a.oacc[j][0] * inv0 * up, a.oacc[j][2] * inv0 * up);
+          if (h + 1 < G) *reinterpret_cast<uint32_t*>(dst + D + j * 16) = ptx::pack_bf16x2(a.oacc[j][1] * inv1 * up, a.oacc[j][3] * inv1 * up);
         }
         if (a.g < 2 && h + a.g < G)
           p.lse[size_t(unit) * G + h + a.g] = a.g ? a.m1 * p.scale + __logf(a.l1) : a.m0 * p.scale + __logf(a.l0);
