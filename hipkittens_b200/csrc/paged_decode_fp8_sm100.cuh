@@ -109,7 +109,7 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 
 }  // namespace fp8
 
-constexpr float kHugeScale = 5.421010862427522e-20f;  // 2^-64
+constexpr float kHugeScale = 0x1p-64f;
 
 // One warp's state: its ring, up to 32 pages that are looked up ahead, and the attention of a unit's heads over the pages so far.
 template <int D>
@@ -228,7 +228,7 @@ struct DecodeFp8Warp {
   // r, where a unit begins or goes on to these pages, and what P takes of each of them: 2^117 s_V / r. Of pages of other units nothing is
   // taken. r is a number, and 2^-10 at least, so that 2^117 / r is one.
   __device__ __forceinline__ void refer(int unit) {
-    constexpr float kUp = 166153499473114484112975882535043072.f;  // 2^117
+    constexpr float kUp = 0x1p117f;
     const uint32_t vs = __float_as_uint(my_vs);
     const uint32_t most = __reduce_max_sync(0xffffffffu, my_unit == unit && vs <= 0x7f800000u ? min(max(vs, 117u << 23), 0x7f7fffffu) : 117u << 23);
     const float to = fmaxf(ref, __uint_as_float(most));
